@@ -28,6 +28,7 @@ extern "C" {
 
 #define L3_DTYPE_F32 0   /* fp32 weights, activations, KV cache: token-identical mode */
 #define L3_DTYPE_BF16 1  /* bf16 weights / KV cache / GEMM operands, fp32 accumulation  */
+#define L3_DTYPE_F16 2   /* the operators on device buffers below only */
 
 /* ModelArgs (reference config.py:5-19) + the FFN width the reference infers from the
  * up_proj weight shape (llama3.py:86-95).  rope base is fixed at 10000 (llama3.py:31). */
@@ -375,6 +376,92 @@ int l3_op_recurrence(int device, const float* q, const float* k, const float* v,
                      float* state, int B, int L, int H, int DK, int DV, int ws_chunks, float* out);
 /* logits[:, -1, :].argmax(-1) (llama3.py:320): first maximum wins. */
 int l3_op_argmax(int device, const float* logits, int rows, int n, int64_t* out);
+
+/* -- operators on device buffers: a key / value cache in pages, and beam search -------------------------------------
+ * For programs that keep their own cache (no counterpart in the reference, whose cache is one array per layer, llama3.py:138-153).
+ * All pointers are device memory of `device` unless a comment says otherwise; a call enqueues its kernels on `stream` (a cudaStream_t;
+ * null: the default stream) and returns, can be captured into a graph, and leaves the calling thread's current device as it was.
+ * Workspaces belong to the call: two calls that can run at the same time need one each.  L3_EINVAL: nothing was enqueued; the
+ * message is l3_last_error(NULL). */
+/* A pool of pages: element (page, kv head, token of the page, dimension) at page * page_stride + head * head_stride + token *
+ * token_stride + dimension, strides in elements; every address a multiple of 16 bytes. */
+typedef struct L3PagePool {
+  void* data;
+  int64_t page_stride, head_stride, token_stride;
+} L3PagePool;
+/* Attention of one token per sequence: out[b, h] = sum_j softmax_j(scale q[b, h] . k_j) v_j over the tokens j < lengths[b], token j in
+ * page table[b, j / page_size] at place j % page_size; query head h reads kv head h / (heads / kv_heads).  Pages outside [0, pages) hold
+ * no tokens (theirs are left out); a length is cut to [0, max_pages * page_size]; with no token the result is 0 and its lse -infinity.
+ * With k_new / v_new the token lengths[b] - 1 is these rows, which are also written to its page (which no other sequence's lengths may
+ * reach in the same call). */
+typedef struct L3PagedAttention {
+  int32_t device;
+  int32_t batch, heads, kv_heads, head_dim;  /* head_dim 16, 32, 48, 64, 96, 128 */
+  int32_t pages, page_size, max_pages;       /* page_size: a power of two up to 65536 */
+  int32_t q_dtype, kv_dtype, out_dtype;      /* L3_DTYPE_*; q: the cache's type or fp32; out: q's type */
+  float scale;                               /* of q . k */
+  void* stream;
+  const void* q;                             /* [batch, heads, head_dim] */
+  int64_t q_batch_stride, q_head_stride;
+  L3PagePool k, v;
+  const int32_t* table;                      /* [batch, max_pages] */
+  int64_t table_stride;
+  const int32_t* lengths;                    /* [batch] */
+  const void *k_new, *v_new;                 /* null, or [batch, kv_heads, head_dim] of the cache's type */
+  int64_t k_new_batch_stride, k_new_head_stride, v_new_batch_stride, v_new_head_stride;
+  void* out;                                 /* [batch, heads, head_dim], contiguous */
+  float* lse;                                /* [batch, heads] or null: log of the softmax's denominator */
+  void* workspace;
+  int64_t workspace_bytes;
+} L3PagedAttention;
+/* bytes that l3_paged_attention wants as its workspace, for these heads, kv_heads and head_dim and any batch and length */
+int l3_paged_attention_workspace(int device, int heads, int kv_heads, int head_dim, int64_t* bytes);
+int l3_paged_attention(const L3PagedAttention* a);
+/* Writes tokens into their pages: token t < count[b] of sequence b goes to position start[b] + t.  Tokens beyond the table, at a
+ * negative position or of a page outside [0, pages) are dropped; two tokens of a call must not share a place. */
+typedef struct L3PagedWrite {
+  int32_t device;
+  int32_t batch, tokens, kv_heads, head_dim;
+  int32_t pages, page_size, max_pages, dtype;
+  void* stream;
+  const void *k, *v;                         /* [batch, tokens, kv_heads, head_dim], strides in elements */
+  int64_t k_batch_stride, k_token_stride, k_head_stride, v_batch_stride, v_token_stride, v_head_stride;
+  L3PagePool k_pool, v_pool;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t *start, *count;              /* [batch]; count null: all tokens are real */
+} L3PagedWrite;
+int l3_paged_write(const L3PagedWrite* a);
+/* A tensor as rows: row r is `outer` runs of `run` bytes, `outer_stride` apart, from base + r * row_stride on (bytes). */
+typedef struct L3Rows {
+  void* base;
+  int64_t rows, row_stride, outer, outer_stride, run;
+} L3Rows;
+/* Row dst[i] <- row src[i] of every tensor, i < n (src, dst on the device; `tensors` on the host).  Pairs with an entry outside [0, rows)
+ * are skipped.  No row may be a destination twice, nor both source and destination. */
+int l3_copy_rows(int device, void* stream, const L3Rows* tensors, int n_tensors, const int32_t* src, const int32_t* dst, int n);
+/* Row b * beams + j <- row b * beams + parents[b, j] of every tensor, in place, for any parents (a permutation, repetitions); a parent
+ * outside [0, beams) leaves the row as it is.  beams <= 256. */
+int l3_beam_reorder(int device, void* stream, const L3Rows* tensors, int n_tensors, const int32_t* parents, int batch, int beams);
+/* The `best` (at most 64) continuations of a sequence's beams: largest scores[b, k] + logits[b, k, v] - log sum_u exp(logits[b, k, u])
+ * first, equal ones by k * vocab + v.  A finished beam (done[b, k] != 0) has one continuation, the token eos at its own score.
+ * Candidates of score -infinity, +infinity or NaN are none; a place without candidate gets score -infinity, the token eos (0 without
+ * one), parent 0 and done.  out_done: the parent was done, or the token is eos (-1: no end token). */
+typedef struct L3BeamSelect {
+  int32_t device, batch, beams, vocab, best, eos, dtype, reserved;
+  void* stream;
+  const void* logits;                        /* [batch, beams, vocab], last dimension contiguous */
+  int64_t batch_stride, beam_stride;
+  const float* scores;                       /* [batch, beams] */
+  const uint8_t* done;                       /* [batch, beams] or null */
+  float* out_scores;                         /* [batch, best] */
+  int32_t *out_tokens, *out_parents;
+  uint8_t* out_done;
+  void* workspace;
+  int64_t workspace_bytes;
+} L3BeamSelect;
+int l3_beam_select_workspace(int device, int batch, int beams, int vocab, int best, int64_t* bytes);
+int l3_beam_select(const L3BeamSelect* a);
 
 /* How the model path cuts a tensor-core projection of `rows` rows in bf16 mode, or with fp32 != 0 one of up to 128 rows of the Llama
  * path's fp32 mode (epi 0: plain store, 1: added to the residual in place, 2: gated):

@@ -12,7 +12,7 @@ _VARIANT = os.environ.get("L3_LIB_VARIANT", "")
 LIB_PATH = os.path.join(_HERE, f"libllama3_b200_{_VARIANT}.so" if _VARIANT else "libllama3_b200.so")
 
 L3_OK, L3_EINVAL, L3_ECUDA, L3_ESTATE, L3_ENOMEM, L3_ENCCL = 0, -1, -2, -3, -4, -5
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 FLAG_NO_GRAPH, FLAG_NO_TENSORCORE, FLAG_NO_PDL, FLAG_NO_MEGA = 1, 2, 4, 8
 
 
@@ -67,6 +67,43 @@ class L3StackConfig(C.Structure):
                 ("norm_tanh", C.c_int32), ("dual_norm", C.c_int32), ("loop_x0", C.c_int32)]
 
 
+class L3PagePool(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+class L3PagedAttention(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("device", "batch", "heads", "kv_heads", "head_dim", "pages", "page_size", "max_pages",
+                                         "q_dtype", "kv_dtype", "out_dtype")] + [
+                ("scale", C.c_float), ("stream", C.c_void_p), ("q", C.c_void_p), ("q_batch_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("k", L3PagePool), ("v", L3PagePool), ("table", C.c_void_p),
+                ("table_stride", C.c_int64), ("lengths", C.c_void_p), ("k_new", C.c_void_p), ("v_new", C.c_void_p),
+                ("k_new_batch_stride", C.c_int64), ("k_new_head_stride", C.c_int64), ("v_new_batch_stride", C.c_int64),
+                ("v_new_head_stride", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+class L3PagedWrite(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("device", "batch", "tokens", "kv_heads", "head_dim", "pages", "page_size", "max_pages",
+                                         "dtype")] + [
+                ("stream", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p)] + [
+                (n, C.c_int64) for n in ("k_batch_stride", "k_token_stride", "k_head_stride", "v_batch_stride", "v_token_stride",
+                                         "v_head_stride")] + [
+                ("k_pool", L3PagePool), ("v_pool", L3PagePool), ("table", C.c_void_p), ("table_stride", C.c_int64),
+                ("start", C.c_void_p), ("count", C.c_void_p)]
+
+
+class L3Rows(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("rows", C.c_int64), ("row_stride", C.c_int64), ("outer", C.c_int64),
+                ("outer_stride", C.c_int64), ("run", C.c_int64)]
+
+
+class L3BeamSelect(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("device", "batch", "beams", "vocab", "best", "eos", "dtype", "reserved")] + [
+                ("stream", C.c_void_p), ("logits", C.c_void_p), ("batch_stride", C.c_int64), ("beam_stride", C.c_int64),
+                ("scores", C.c_void_p), ("done", C.c_void_p), ("out_scores", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("out_parents", C.c_void_p), ("out_done", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _F32P = C.POINTER(C.c_float)
@@ -114,6 +151,13 @@ SIGNATURES = {
     "l3_op_prompt_attention": (_I, [_I, _F32P, _F32P] + [_I] * 12 + [C.c_float, _F32P]),
     "l3_op_recurrence": (_I, [_I] + [_F32P] * 6 + [_I] * 6 + [_F32P]),
     "l3_op_argmax": (_I, [_I, _F32P, _I, _I, _I64P]),
+    "l3_paged_attention_workspace": (_I, [_I, _I, _I, _I, _I64P]),
+    "l3_paged_attention": (_I, [C.POINTER(L3PagedAttention)]),
+    "l3_paged_write": (_I, [C.POINTER(L3PagedWrite)]),
+    "l3_copy_rows": (_I, [_I, _P, C.POINTER(L3Rows), _I, _P, _P, _I]),
+    "l3_beam_reorder": (_I, [_I, _P, C.POINTER(L3Rows), _I, _P, _I, _I]),
+    "l3_beam_select_workspace": (_I, [_I, _I, _I, _I, _I, _I64P]),
+    "l3_beam_select": (_I, [C.POINTER(L3BeamSelect)]),
     "l3_debug_tc_timeline": (_I, [_I, _I, C.POINTER(C.c_uint64)]),
     "l3_sync": (_I, [_P]),
     "l3_timer_start": (_I, [_P]),

@@ -1,0 +1,230 @@
+"""A key / value cache in pages: operators on torch CUDA tensors, and `PagedCache`, the bookkeeping of its pages.
+
+The reference has one array per layer, [batch, positions, kv heads, head size], owned by its attention module
+(llama3.py:138-153, 184-187).  Here a cache is a pool of pages of a fixed number of tokens; a sequence is a row of a table that
+names its pages in order, so that sequences grow without moving and share what they have in common.
+
+Every operator enqueues its kernels on the current stream of the tensors' device and returns; it can be captured into a graph.
+Arguments that do not fit raise ValueError before anything is enqueued.  What is in device memory - lengths, tables - is not
+read by the host: a page number outside the pool names a page that holds no tokens.
+
+Pools have the dimensions [pages, kv heads, page size, head size] in any memory order whose last dimension is contiguous; a
+pool kept as [pages, page size, kv heads, head size] is passed as `pool.transpose(1, 2)`.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import heapq
+
+import torch
+
+from . import _cabi
+
+_KIND = {torch.float32: _cabi.DTYPE_F32, torch.bfloat16: _cabi.DTYPE_BF16, torch.float16: _cabi.DTYPE_F16}
+HEAD_DIMS = (16, 32, 48, 64, 96, 128)
+_workspace_bytes: dict = {}
+
+
+def _need(cond, text, *args):
+    if not cond:
+        raise ValueError(text % args if args else text)
+
+
+def _tensor(x, name, dims, dtypes=None):
+    _need(isinstance(x, torch.Tensor), "%s must be a tensor", name)
+    _need(x.dim() == dims, "%s must have %d dimensions, got %s", name, dims, tuple(x.shape))
+    if dtypes is not None:
+        _need(x.dtype in dtypes, "%s: type %s is not one of %s", name, x.dtype, ", ".join(str(d) for d in dtypes))
+    return x
+
+
+def _ints(x, name, shape):
+    _tensor(x, name, len(shape), (torch.int32,))
+    _need(tuple(x.shape) == tuple(shape), "%s must be %s, got %s", name, tuple(shape), tuple(x.shape))
+    _need(x.is_contiguous(), "%s must be contiguous", name)
+    return x
+
+
+def _one_device(named):
+    device = None
+    for name, x in named:
+        if x is None:
+            continue
+        _need(x.is_cuda, "%s must be on a CUDA device", name)
+        device = x.device if device is None else device
+        _need(x.device == device, "%s is on %s, the others on %s", name, x.device, device)
+    return device
+
+
+def _pool(k_pages, v_pages):
+    _tensor(k_pages, "k_pages", 4, tuple(_KIND))
+    _tensor(v_pages, "v_pages", 4, (k_pages.dtype,))
+    _need(k_pages.shape == v_pages.shape, "k_pages and v_pages differ: %s and %s", tuple(k_pages.shape), tuple(v_pages.shape))
+    pages, _, page, dim = k_pages.shape
+    _need(pages >= 1 and page >= 1 and page & (page - 1) == 0 and page <= 65536, "page size %d is not a power of two up to 65536", page)
+    for name, x in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _need(x.stride(3) == 1 or dim == 1, "%s: the last dimension must be contiguous", name)
+        _fits16(name, x)
+
+
+def _fits16(name, x):
+    size = x.element_size()
+    _need(x.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for n, s in zip(x.shape[:-1], x.stride()) if n > 1),
+          "%s: addresses must be multiples of 16 bytes", name)
+
+
+def _strides(x, *dims):
+    """Strides in elements; 0 where a dimension has one entry only (its stride may be anything)."""
+    return [x.stride(d) if x.shape[d] > 1 else 0 for d in dims]
+
+
+def _pool_arg(x):
+    return _cabi.L3PagePool(x.data_ptr(), *_strides(x, 0, 1, 2))
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_new=None, v_new=None, scale=None, return_lse=False, out=None):
+    """Attention of one token per sequence over the tokens of its pages.
+
+    q            [batch, heads, head size], the cache's type or fp32; query head h reads kv head h // (heads / kv heads)
+    k_pages, v_pages   the pools, fp32, bfloat16 or float16
+    page_table   [batch, max pages] int32; token j of a sequence is in page `page_table[b, j // page size]`
+    lengths      [batch] int32: tokens that the query sees.  0: the result is 0 (lse -inf)
+    k_new, v_new [batch, kv heads, head size]: the newest token, number lengths - 1; used here and written to its page, which no
+                 other sequence of the call may share
+    scale        of q . k; 1 / sqrt(head size) by default
+    Returns [batch, heads, head size] of q's type (written into `out` where given), and with `return_lse` also the log of the
+    softmax's denominator, [batch, heads] fp32.
+    """
+    _tensor(q, "q", 3, tuple(_KIND))
+    _pool(k_pages, v_pages)
+    batch, heads, dim = q.shape
+    pages, kv_heads, page, _ = k_pages.shape
+    _need(q.dtype in (k_pages.dtype, torch.float32), "q must have the cache's type or fp32, got %s over %s", q.dtype, k_pages.dtype)
+    _need(k_pages.shape[3] == dim and dim in HEAD_DIMS, "head size %d (cache: %d) is not one of %s", dim, k_pages.shape[3], HEAD_DIMS)
+    _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "%d heads over %d kv heads", heads, kv_heads)
+    _need(q.stride(2) == 1, "q: the last dimension must be contiguous")
+    _tensor(page_table, "page_table", 2, (torch.int32,))
+    _need(page_table.shape[0] == batch, "page_table has %d rows for %d sequences", page_table.shape[0], batch)
+    _need(page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
+    _ints(lengths, "lengths", (batch,))
+    _need((k_new is None) == (v_new is None), "k_new and v_new go together")
+    new = [None, None, 0, 0, 0, 0]
+    if k_new is not None:
+        for name, x in (("k_new", k_new), ("v_new", v_new)):
+            _tensor(x, name, 3, (k_pages.dtype,))
+            _need(tuple(x.shape) == (batch, kv_heads, dim), "%s must be %s, got %s", name, (batch, kv_heads, dim), tuple(x.shape))
+            _need(x.stride(2) == 1, "%s: the last dimension must be contiguous", name)
+            _fits16(name, x)
+        new = [k_new.data_ptr(), v_new.data_ptr(), *_strides(k_new, 0, 1), *_strides(v_new, 0, 1)]
+    if out is not None:
+        _tensor(out, "out", 3, (q.dtype,))
+        _need(out.shape == q.shape and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must be contiguous, of q's shape")
+    device = _one_device((("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("lengths", lengths),
+                          ("k_new", k_new), ("v_new", v_new), ("out", out)))
+    if out is None:
+        out = torch.empty((batch, heads, dim), dtype=q.dtype, device=device)
+    lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
+    if batch:
+        lib = _cabi.lib()
+        key = (device.index, heads, kv_heads, dim)
+        room = _workspace_bytes.get(key)
+        if room is None:
+            n = C.c_int64()
+            _cabi.check(lib.l3_paged_attention_workspace(*key, C.byref(n)))
+            room = _workspace_bytes[key] = n.value
+        ws = torch.empty(room, dtype=torch.uint8, device=device)   # of this call: a captured graph has one of its own
+        arg = _cabi.L3PagedAttention(
+            device.index, batch, heads, kv_heads, dim, pages, page, page_table.shape[1], _KIND[q.dtype], _KIND[k_pages.dtype],
+            _KIND[q.dtype], dim ** -0.5 if scale is None else float(scale), _stream(device), q.data_ptr(), *_strides(q, 0, 1),
+            _pool_arg(k_pages), _pool_arg(v_pages), page_table.data_ptr(), *_strides(page_table, 0), lengths.data_ptr(), *new,
+            out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr(), room)
+        _cabi.check(lib.l3_paged_attention(C.byref(arg)))
+    return (out, lse) if return_lse else out
+
+
+def paged_write(k, v, k_pages, v_pages, page_table, start, count=None):
+    """Writes keys and values of a padded batch into their pages.
+
+    k, v   [batch, tokens, kv heads, head size] of the pools' type; token t < count[b] of sequence b becomes its token start[b] + t
+    start, count   [batch] int32 (count None: every token is real)
+    Tokens that the table has no page for are dropped; what lies behind a sequence's last token stays as it was.
+    """
+    _pool(k_pages, v_pages)
+    pages, kv_heads, page, dim = k_pages.shape
+    for name, x in (("k", k), ("v", v)):
+        _tensor(x, name, 4, (k_pages.dtype,))
+        _need(x.shape == k.shape and tuple(x.shape[2:]) == (kv_heads, dim), "%s must be [batch, tokens, %d, %d], got %s", name, kv_heads,
+              dim, tuple(x.shape))
+        _need(x.stride(3) == 1 or dim == 1, "%s: the last dimension must be contiguous", name)
+        _fits16(name, x)
+    _need(dim * k.element_size() % 16 == 0, "head size %d: a head's row must be a multiple of 16 bytes", dim)
+    batch, tokens = k.shape[:2]
+    _need(batch <= 65535, "at most 65535 sequences a call")
+    _tensor(page_table, "page_table", 2, (torch.int32,))
+    _need(page_table.shape[0] == batch, "page_table has %d rows for %d sequences", page_table.shape[0], batch)
+    _need(page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
+    _ints(start, "start", (batch,))
+    if count is not None:
+        _ints(count, "count", (batch,))
+    device = _one_device((("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("start", start),
+                          ("count", count)))
+    if batch == 0 or tokens == 0:
+        return
+    arg = _cabi.L3PagedWrite(
+        device.index, batch, tokens, kv_heads, dim, pages, page, page_table.shape[1], _KIND[k.dtype], _stream(device), k.data_ptr(),
+        v.data_ptr(), *_strides(k, 0, 1, 2), *_strides(v, 0, 1, 2), _pool_arg(k_pages), _pool_arg(v_pages), page_table.data_ptr(),
+        *_strides(page_table, 0), start.data_ptr(), count.data_ptr() if count is not None else None)
+    _cabi.check(_cabi.lib().l3_paged_write(C.byref(arg)))
+
+
+def _rows(tensors, what):
+    """L3Rows of tensors whose first dimension counts rows; a row is a contiguous run, or equal runs at equal distances."""
+    _need(len(tensors) >= 1, "no %s", what)
+    out = (_cabi.L3Rows * len(tensors))()
+    for i, x in enumerate(tensors):
+        _need(isinstance(x, torch.Tensor) and x.dim() >= 1, "%s must be tensors with rows", what)
+        size = x.element_size()
+        dims = [(n, s) for n, s in zip(x.shape[1:], x.stride()[1:]) if n != 1]
+        if any(n == 0 for n, _ in dims):
+            dims = [(0, 1)]
+        run, outer, outer_stride = 1, 1, 0
+        while dims and dims[-1][1] == run:
+            run *= dims.pop()[0]
+        if dims:                                  # the next dimensions out, as far as they are one
+            outer, outer_stride = dims.pop()
+            while dims and dims[-1][1] == outer * outer_stride:
+                outer *= dims.pop()[0]
+        _need(not dims, "%s %d: a row of shape %s and strides %s is not a run, or equal runs at equal distances", what, i,
+              tuple(x.shape[1:]), tuple(x.stride()[1:]))
+        row = x.stride(0)
+        span = (outer - 1) * outer_stride + run if run and outer else 0
+        _need(outer <= 1 or outer_stride >= run, "%s %d overlaps itself", what, i)
+        _need(x.shape[0] <= 1 or row >= span or _interleaved(x, row, run, outer, outer_stride), "%s %d: rows overlap", what, i)
+        out[i] = _cabi.L3Rows(x.data_ptr(), x.shape[0], row * size, outer, outer_stride * size, run * size)
+    return out
+
+
+def _interleaved(x, row, run, outer, outer_stride):
+    """Rows that lie between one another's runs, as in a cache kept [heads, sequences, ...]."""
+    return run <= row and row * x.shape[0] <= outer_stride
+
+
+def copy_pages(pools, src, dst):
+    """Page dst[i] becomes a copy of page src[i] in every pool: pools a list of tensors [pages, ...], src and dst [n] int32.
+
+    Pairs with a number outside the pools are skipped.  No page may be a destination twice, nor both source and destination.
+    """
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    rows = _rows(pools, "pools")
+    for x in pools:
+        _need(x.shape[0] == pools[0].shape[0], "pools have %d and %d pages", pools[0].shape[0], x.shape[0])
+    _tensor(src, "src", 1)
+    _ints(src, "src", (src.shape[0],))
+    _ints(dst, "dst", (src.shape[0],))
+    device = _one_device([("src", src), ("dst", dst)] + [("pools", x) for x in pools])
+    if src.shape[0]:
+        _cabi.check(_cabi.lib().l3_copy_rows(device.index, _stream(device), rows, len(pools), src.data_ptr(), dst.data_ptr(), src.shape[0]))
