@@ -22,7 +22,6 @@ from . import _cabi
 
 _KIND = {torch.float32: _cabi.DTYPE_F32, torch.bfloat16: _cabi.DTYPE_BF16, torch.float16: _cabi.DTYPE_F16}
 HEAD_DIMS = (16, 32, 48, 64, 96, 128)
-_workspace_bytes: dict = {}
 
 
 def _need(cond, text, *args):
@@ -78,12 +77,69 @@ def _strides(x, *dims):
     return [x.stride(d) if x.shape[d] > 1 else 0 for d in dims]
 
 
-def _pool_arg(x):
-    return _cabi.L3PagePool(x.data_ptr(), *_strides(x, 0, 1, 2))
+def _stream(device_index):
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# A call's checks and the parts of its C struct that hang on shapes, strides, types and the device alone are made once per such
+# form: they take several times as long as the kernels of a small call.  Addresses and values are never kept.
+_MOST_PLANS = 4096
+
+
+def _form(x):
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
+
+
+def _planned(plans, key, make, *args):
+    plan = plans.get(key)
+    if plan is None:
+        if len(plans) >= _MOST_PLANS:
+            plans.clear()
+        plan = make(*args)
+        plans[key] = plan
+    return plan
+
+
+_attention_plans: dict = {}
+
+
+def _plan_attention(q, k_pages, v_pages, page_table, lengths, k_new, v_new, scale, out):
+    _tensor(q, "q", 3, tuple(_KIND))
+    _pool(k_pages, v_pages)
+    batch, heads, dim = q.shape
+    pages, kv_heads, page, _ = k_pages.shape
+    _need(q.dtype in (k_pages.dtype, torch.float32), "q must have the cache's type or fp32, got %s over %s", q.dtype, k_pages.dtype)
+    _need(k_pages.shape[3] == dim and dim in HEAD_DIMS, "head size %d (cache: %d) is not one of %s", dim, k_pages.shape[3], HEAD_DIMS)
+    _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "%d heads over %d kv heads", heads, kv_heads)
+    _need(q.stride(2) == 1, "q: the last dimension must be contiguous")
+    _tensor(page_table, "page_table", 2, (torch.int32,))
+    _need(page_table.shape[0] == batch, "page_table has %d rows for %d sequences", page_table.shape[0], batch)
+    _need(page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
+    _ints(lengths, "lengths", (batch,))
+    _need((k_new is None) == (v_new is None), "k_new and v_new go together")
+    new = [0, 0, 0, 0]
+    if k_new is not None:
+        for name, x in (("k_new", k_new), ("v_new", v_new)):
+            _tensor(x, name, 3, (k_pages.dtype,))
+            _need(tuple(x.shape) == (batch, kv_heads, dim), "%s must be %s, got %s", name, (batch, kv_heads, dim), tuple(x.shape))
+            _need(x.stride(2) == 1, "%s: the last dimension must be contiguous", name)
+            _fits16(name, x)
+        new = [*_strides(k_new, 0, 1), *_strides(v_new, 0, 1)]
+    if out is not None:
+        _tensor(out, "out", 3, (q.dtype,))
+        _need(out.shape == q.shape and out.is_contiguous(), "out must be contiguous, of q's shape")
+    device = _one_device((("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("lengths", lengths),
+                          ("k_new", k_new), ("v_new", v_new), ("out", out)))
+    n = C.c_int64()
+    if batch:
+        _cabi.check(_cabi.lib().l3_paged_attention_workspace(device.index, heads, kv_heads, dim, C.byref(n)))
+    room = -(-n.value // q.element_size())
+    arg = _cabi.L3PagedAttention(
+        device.index, batch, heads, kv_heads, dim, pages, page, page_table.shape[1], _KIND[q.dtype], _KIND[k_pages.dtype],
+        _KIND[q.dtype], dim ** -0.5 if scale is None else float(scale), None, None, *_strides(q, 0, 1),
+        _cabi.L3PagePool(None, *_strides(k_pages, 0, 1, 2)), _cabi.L3PagePool(None, *_strides(v_pages, 0, 1, 2)), None,
+        *_strides(page_table, 0), None, None, None, *new, None, None, None, room * q.element_size())
+    return bytes(arg), device.index, room, q.is_contiguous(), batch
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_new=None, v_new=None, scale=None, return_lse=False, out=None):
@@ -99,60 +155,34 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_new=None, v_n
     Returns [batch, heads, head size] of q's type (written into `out` where given), and with `return_lse` also the log of the
     softmax's denominator, [batch, heads] fp32.
     """
-    _tensor(q, "q", 3, tuple(_KIND))
-    _pool(k_pages, v_pages)
-    batch, heads, dim = q.shape
-    pages, kv_heads, page, _ = k_pages.shape
-    _need(q.dtype in (k_pages.dtype, torch.float32), "q must have the cache's type or fp32, got %s over %s", q.dtype, k_pages.dtype)
-    _need(k_pages.shape[3] == dim and dim in HEAD_DIMS, "head size %d (cache: %d) is not one of %s", dim, k_pages.shape[3], HEAD_DIMS)
-    _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "%d heads over %d kv heads", heads, kv_heads)
-    _need(q.stride(2) == 1, "q: the last dimension must be contiguous")
-    _tensor(page_table, "page_table", 2, (torch.int32,))
-    _need(page_table.shape[0] == batch, "page_table has %d rows for %d sequences", page_table.shape[0], batch)
-    _need(page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
-    _ints(lengths, "lengths", (batch,))
-    _need((k_new is None) == (v_new is None), "k_new and v_new go together")
-    new = [None, None, 0, 0, 0, 0]
-    if k_new is not None:
-        for name, x in (("k_new", k_new), ("v_new", v_new)):
-            _tensor(x, name, 3, (k_pages.dtype,))
-            _need(tuple(x.shape) == (batch, kv_heads, dim), "%s must be %s, got %s", name, (batch, kv_heads, dim), tuple(x.shape))
-            _need(x.stride(2) == 1, "%s: the last dimension must be contiguous", name)
-            _fits16(name, x)
-        new = [k_new.data_ptr(), v_new.data_ptr(), *_strides(k_new, 0, 1), *_strides(v_new, 0, 1)]
-    if out is not None:
-        _tensor(out, "out", 3, (q.dtype,))
-        _need(out.shape == q.shape and out.is_contiguous() and out.data_ptr() % 16 == 0, "out must be contiguous, of q's shape")
-    device = _one_device((("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("lengths", lengths),
-                          ("k_new", k_new), ("v_new", v_new), ("out", out)))
+    args = (q, k_pages, v_pages, page_table, lengths, k_new, v_new, scale, out)
+    try:
+        key = (_form(q), _form(k_pages), _form(v_pages), _form(page_table), _form(lengths), _form(k_new), _form(v_new), scale, _form(out))
+    except (AttributeError, RuntimeError):
+        key = None                                     # not tensors, or not strided ones: refused below
+    fixed, index, room, plain, batch = _plan_attention(*args) if key is None else _planned(_attention_plans, key, _plan_attention, *args)
     if out is None:
-        out = torch.empty((batch, heads, dim), dtype=q.dtype, device=device)
-    lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
+        out = torch.empty_like(q) if plain else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
     if batch:
-        lib = _cabi.lib()
-        key = (device.index, heads, kv_heads, dim)
-        room = _workspace_bytes.get(key)
-        if room is None:
-            n = C.c_int64()
-            _cabi.check(lib.l3_paged_attention_workspace(*key, C.byref(n)))
-            room = _workspace_bytes[key] = n.value
-        ws = torch.empty(room, dtype=torch.uint8, device=device)   # of this call: a captured graph has one of its own
-        arg = _cabi.L3PagedAttention(
-            device.index, batch, heads, kv_heads, dim, pages, page, page_table.shape[1], _KIND[q.dtype], _KIND[k_pages.dtype],
-            _KIND[q.dtype], dim ** -0.5 if scale is None else float(scale), _stream(device), q.data_ptr(), *_strides(q, 0, 1),
-            _pool_arg(k_pages), _pool_arg(v_pages), page_table.data_ptr(), *_strides(page_table, 0), lengths.data_ptr(), *new,
-            out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr(), room)
-        _cabi.check(lib.l3_paged_attention(C.byref(arg)))
+        ws = q.new_empty(room)                         # of this call: a captured graph has one of its own
+        arg = _cabi.L3PagedAttention.from_buffer_copy(fixed)
+        arg.stream, arg.q, arg.table, arg.lengths = _stream(index), q.data_ptr(), page_table.data_ptr(), lengths.data_ptr()
+        arg.k.data, arg.v.data, arg.out, arg.workspace = k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ws.data_ptr()
+        if k_new is not None:
+            arg.k_new, arg.v_new = k_new.data_ptr(), v_new.data_ptr()
+        if return_lse:
+            arg.lse = lse.data_ptr()
+        rc = _cabi.lib().l3_paged_attention(C.byref(arg))
+        if rc:
+            _cabi.check(rc)
     return (out, lse) if return_lse else out
 
 
-def paged_write(k, v, k_pages, v_pages, page_table, start, count=None):
-    """Writes keys and values of a padded batch into their pages.
+_write_plans: dict = {}
 
-    k, v   [batch, tokens, kv heads, head size] of the pools' type; token t < count[b] of sequence b becomes its token start[b] + t
-    start, count   [batch] int32 (count None: every token is real)
-    Tokens that the table has no page for are dropped; what lies behind a sequence's last token stays as it was.
-    """
+
+def _plan_write(k, v, k_pages, v_pages, page_table, start, count):
     _pool(k_pages, v_pages)
     pages, kv_heads, page, dim = k_pages.shape
     for name, x in (("k", k), ("v", v)):
@@ -172,13 +202,35 @@ def paged_write(k, v, k_pages, v_pages, page_table, start, count=None):
         _ints(count, "count", (batch,))
     device = _one_device((("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("start", start),
                           ("count", count)))
-    if batch == 0 or tokens == 0:
-        return
     arg = _cabi.L3PagedWrite(
-        device.index, batch, tokens, kv_heads, dim, pages, page, page_table.shape[1], _KIND[k.dtype], _stream(device), k.data_ptr(),
-        v.data_ptr(), *_strides(k, 0, 1, 2), *_strides(v, 0, 1, 2), _pool_arg(k_pages), _pool_arg(v_pages), page_table.data_ptr(),
-        *_strides(page_table, 0), start.data_ptr(), count.data_ptr() if count is not None else None)
-    _cabi.check(_cabi.lib().l3_paged_write(C.byref(arg)))
+        device.index, batch, tokens, kv_heads, dim, pages, page, page_table.shape[1], _KIND[k.dtype], None, None, None,
+        *_strides(k, 0, 1, 2), *_strides(v, 0, 1, 2), _cabi.L3PagePool(None, *_strides(k_pages, 0, 1, 2)),
+        _cabi.L3PagePool(None, *_strides(v_pages, 0, 1, 2)), None, *_strides(page_table, 0), None, None)
+    return bytes(arg), device.index, batch * tokens
+
+
+def paged_write(k, v, k_pages, v_pages, page_table, start, count=None):
+    """Writes keys and values of a padded batch into their pages.
+
+    k, v   [batch, tokens, kv heads, head size] of the pools' type; token t < count[b] of sequence b becomes its token start[b] + t
+    start, count   [batch] int32 (count None: every token is real)
+    Tokens that the table has no page for are dropped; what lies behind a sequence's last token stays as it was.
+    """
+    args = (k, v, k_pages, v_pages, page_table, start, count)
+    try:
+        key = (_form(k), _form(v), _form(k_pages), _form(v_pages), _form(page_table), _form(start), _form(count))
+    except (AttributeError, RuntimeError):
+        key = None
+    fixed, index, some = _plan_write(*args) if key is None else _planned(_write_plans, key, _plan_write, *args)
+    if some:
+        arg = _cabi.L3PagedWrite.from_buffer_copy(fixed)
+        arg.stream, arg.k, arg.v, arg.table, arg.start = _stream(index), k.data_ptr(), v.data_ptr(), page_table.data_ptr(), start.data_ptr()
+        arg.k_pool.data, arg.v_pool.data = k_pages.data_ptr(), v_pages.data_ptr()
+        if count is not None:
+            arg.count = count.data_ptr()
+        rc = _cabi.lib().l3_paged_write(C.byref(arg))
+        if rc:
+            _cabi.check(rc)
 
 
 def _rows(tensors, what):
@@ -204,7 +256,7 @@ def _rows(tensors, what):
         span = (outer - 1) * outer_stride + run if run and outer else 0
         _need(outer <= 1 or outer_stride >= run, "%s %d overlaps itself", what, i)
         _need(x.shape[0] <= 1 or row >= span or _interleaved(x, row, run, outer, outer_stride), "%s %d: rows overlap", what, i)
-        out[i] = _cabi.L3Rows(x.data_ptr(), x.shape[0], row * size, outer, outer_stride * size, run * size)
+        out[i] = _cabi.L3Rows(None, x.shape[0], row * size, outer, outer_stride * size, run * size)
     return out
 
 
@@ -213,12 +265,10 @@ def _interleaved(x, row, run, outer, outer_stride):
     return run <= row and row * x.shape[0] <= outer_stride
 
 
-def copy_pages(pools, src, dst):
-    """Page dst[i] becomes a copy of page src[i] in every pool: pools a list of tensors [pages, ...], src and dst [n] int32.
+_copy_plans: dict = {}
 
-    Pairs with a number outside the pools are skipped.  No page may be a destination twice, nor both source and destination.
-    """
-    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+
+def _plan_copy(pools, src, dst):
     rows = _rows(pools, "pools")
     for x in pools:
         _need(x.shape[0] == pools[0].shape[0], "pools have %d and %d pages", pools[0].shape[0], x.shape[0])
@@ -226,5 +276,30 @@ def copy_pages(pools, src, dst):
     _ints(src, "src", (src.shape[0],))
     _ints(dst, "dst", (src.shape[0],))
     device = _one_device([("src", src), ("dst", dst)] + [("pools", x) for x in pools])
-    if src.shape[0]:
-        _cabi.check(_cabi.lib().l3_copy_rows(device.index, _stream(device), rows, len(pools), src.data_ptr(), dst.data_ptr(), src.shape[0]))
+    return bytes(rows), device.index
+
+
+def _filled(fixed, tensors):
+    """The L3Rows of a plan, with the tensors' addresses."""
+    rows = (_cabi.L3Rows * len(tensors)).from_buffer_copy(fixed)
+    for r, x in zip(rows, tensors):
+        r.base = x.data_ptr()
+    return rows
+
+
+def copy_pages(pools, src, dst):
+    """Page dst[i] becomes a copy of page src[i] in every pool: pools a list of tensors [pages, ...], src and dst [n] int32.
+
+    Pairs with a number outside the pools are skipped.  No page may be a destination twice, nor both source and destination.
+    """
+    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+    try:
+        key = (_form(src), _form(dst), *map(_form, pools))
+    except (AttributeError, RuntimeError):
+        key = None
+    fixed, index = _plan_copy(pools, src, dst) if key is None else _planned(_copy_plans, key, _plan_copy, pools, src, dst)
+    n = src.shape[0]
+    if n:
+        rc = _cabi.lib().l3_copy_rows(index, _stream(index), _filled(fixed, pools), len(pools), src.data_ptr(), dst.data_ptr(), n)
+        if rc:
+            _cabi.check(rc)
