@@ -2,14 +2,18 @@
 //   score(k, v) = scores[k] + logits[k, v] - log sum_u e^logits[k, u]
 // over the beams k of a sequence and the vocabulary v; equal scores go to the lowest k V + v.
 //
-// Bound by the logits, read once.  A row is cut into slices, one CTA each, whose values stay in registers: maximum and sum of
-// exponentials, and the slice's n largest logits (within a row the order of the logits is the order of the scores).  A second, dependent
-// launch, one CTA per sequence, joins the sums of a row's slices in 64 bits, turns its candidates into scores - in 64 bits too, so that
-// two that are close keep the order of the formula - and picks the n best.
-// Both find the n largest the same way: the n-th largest of the lanes' own maxima bounds the n-th largest value from below, few values
-// pass that bound, and each of those counts how many precede it.  Where more pass than there is room for (many equal values), the n
-// largest are drawn one after the other.
+// Bound by the logits.  A row is cut into segments, a warp each, which the warp streams through with the next 4 KB on their way: a lane
+// keeps a running maximum and sum of exponentials, and the three largest of its portions' maxima.  The n-th largest of the lanes' largest
+// bounds the segment's n-th logit from below, so the few portions whose maxima pass it are looked at once more, what passes is counted off
+// against the rest, and the n largest are left, in order (within a row the order of the logits is the order of the scores).  A second,
+// dependent launch, one CTA per sequence, joins the sums of a row's segments in 64 bits, turns the candidates into scores - in 64 bits too, so
+// that two that are close keep the order of the formula - and picks the n best in the same way,
+// its bound the n-th best of the segments' first candidates.
+// Where more values pass a bound than there is room for (many equal ones), the n best are drawn one after the other.
+#include <float.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -17,8 +21,9 @@
 #include "paged.h"
 
 namespace {
-constexpr int BT = 256, BW = BT / 32;
-constexpr int ROOM = 512;  // values that pass the bound
+constexpr int BT = 256, BW = BT / 32;  // of the second launch
+constexpr int ROOM = 512;               // candidates that pass its bound
+constexpr int RW = 4, HITS = 96;        // warps of a CTA of the first, values that pass a warp's bound
 
 __device__ __forceinline__ uint32_t order_key(float v) {  // larger values, larger keys; both zeros alike
   const uint32_t b = __float_as_uint(v + 0.f);
@@ -37,122 +42,263 @@ __device__ __forceinline__ uint32_t nth_of_warp(uint32_t a, uint32_t b, int n) {
   }
   return t;
 }
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
-  v = __reduce_max_sync(L3_FULL, v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < BW; ++i) m = red[i] > m ? red[i] : m;
-  return m;
+constexpr int warps_of_sm(bool f32) { return f32 ? 24 : 16; }  // two portions of a lane are 32 registers, their values 16 (32) more
+struct RowPart { float m, s; };  // of a segment: the largest logit and the sum of e^(logit - m)
+
+// 32 bits of a row: one fp32 logit or two of 16 bits
+template <typename T> struct Word {
+  static constexpr int N = sizeof(T) == 4 ? 1 : 2;
+  static constexpr uint32_t NONE = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, bf16>::value ? 0xff80u : 0xfc00u;  // -infinity
+  __device__ static __forceinline__ uint32_t bits(const T* p) {
+    if constexpr (N == 1) return __float_as_uint(__ldcs(p));
+    else return __ldcs(reinterpret_cast<const unsigned short*>(p));
+  }
+  __device__ static __forceinline__ float value(uint32_t w, int e) {
+    if constexpr (N == 1) return __uint_as_float(w);
+    else if constexpr (std::is_same<T, bf16>::value) return __uint_as_float(e ? w & 0xffff0000u : w << 16);
+    else return e ? __high2float(*reinterpret_cast<const __half2*>(&w)) : __low2float(*reinterpret_cast<const __half2*>(&w));
+  }
+};
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-struct RowPart { float m, s; };  // of a slice: the largest logit and the sum of e^(logit - m)
+// The n largest values of a warp so far, by value and then index: place r is lane r % 32 of v[r / 32].
+template <int NL> struct Best {
+  float v[NL];
+  int at[NL];
+  float least;   // the n-th, and its index (none: -infinity, -1)
+  int least_at;
+  __device__ __forceinline__ void none() {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) { v[i] = -INFINITY; at[i] = -1; }
+    least = -INFINITY;
+    least_at = -1;
+  }
+  __device__ __forceinline__ bool passes(float x, int i) const { return x > least || (x == least && x > -INFINITY && i < least_at); }
+  __device__ __forceinline__ void insert(float x, int i, int n, int lane) {
+    if constexpr (NL == 2) {
+      const int first = __popc(__ballot_sync(L3_FULL, v[0] > x || (v[0] == x && at[0] < i)));
+      const float carry = __shfl_sync(L3_FULL, v[0], 31);
+      const int carry_at = __shfl_sync(L3_FULL, at[0], 31);
+      if (first < 32) {
+        put(0, first, x, i, lane);
+        put(1, 0, carry, carry_at, lane);
+      } else put(1, __popc(__ballot_sync(L3_FULL, v[1] > x || (v[1] == x && at[1] < i))), x, i, lane);
+    } else put(0, __popc(__ballot_sync(L3_FULL, v[0] > x || (v[0] == x && at[0] < i))), x, i, lane);
+    const int last = (n - 1) & 31;
+    least = __shfl_sync(L3_FULL, NL == 2 && n > 32 ? v[NL - 1] : v[0], last);
+    least_at = __shfl_sync(L3_FULL, NL == 2 && n > 32 ? at[NL - 1] : at[0], last);
+  }
+  __device__ __forceinline__ void put(int part, int place, float x, int i, int lane) {
+    const float up = __shfl_up_sync(L3_FULL, v[part], 1);
+    const int up_at = __shfl_up_sync(L3_FULL, at[part], 1);
+    if (lane >= place) {
+      v[part] = lane == place ? x : up;
+      at[part] = lane == place ? i : up_at;
+    }
+  }
+};
 
-__device__ __forceinline__ float as_float(float v) { return v; }
-__device__ __forceinline__ float as_float(bf16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+// the row that has `nth` unfinished ones ahead of it, or -1; all lanes of a warp
+__device__ __forceinline__ int unfinished(const unsigned char* done, int rows, int nth, int lane) {
+  for (int base = 0; base < rows; base += 128) {  // four rows a lane
+    uint32_t live = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) live |= (base + 4 * lane + i < rows && !done[base + 4 * lane + i] ? 1u : 0u) << i;
+    int run = __popc(live);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(L3_FULL, run, o);
+      if (lane >= o) run += x;
+    }
+    const int all = __shfl_sync(L3_FULL, run, 31);
+    if (nth < all) {
+      const int src = __ffs(__ballot_sync(L3_FULL, run > nth)) - 1;
+      uint32_t left = __shfl_sync(L3_FULL, live, src);
+      for (int i = __shfl_sync(L3_FULL, run, src) - __popc(left); i < nth; ++i) left &= left - 1;
+      return base + 4 * src + __ffs(left) - 1;
+    }
+    nth -= all;
+  }
+  return -1;
+}
 
-// part [R, S], cand_v / cand_i [R, S, n]
-template <typename T, int EPT>
-__global__ void __launch_bounds__(BT) beam_rows_kernel(const BeamSelectArgs a, int S, RowPart* part, float* cand_v, int* cand_i) {
-  __shared__ uint32_t red[BW];
-  __shared__ float sums[BW];
-  __shared__ unsigned long long room[ROOM];
-  __shared__ int count;
+// part [R, S], cand_v / cand_i [R, S, n].  A portion is 16 words a lane; rows are cut where their addresses are multiples of 16 bytes.
+template <typename T, int NL>
+__global__ void __launch_bounds__(RW * 32, warps_of_sm(sizeof(T) == 4) / RW) beam_rows_kernel(const BeamSelectArgs a, int S, int portions, RowPart* part, float* cand_v, int* cand_i) {
+  constexpr int N = Word<T>::N, PIECE = 4 * N, PORTION = 128 * PIECE;  // logits of 16 bytes, of a portion
+  __shared__ unsigned long long hits[RW][HITS];
   pdl_launch();
   pdl_wait();
-  const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = row / a.K, k = row % a.K;
-  if (a.done && a.done[row]) return;  // a finished beam has one continuation, whatever its logits
+  const int lane = threadIdx.x & 31;
+  const long long id = (long long)blockIdx.x * RW + (threadIdx.x >> 5);
+  if (id >= (long long)a.B * a.K * S) return;
+  int row = (int)(id / S);
+  const int seg = (int)(id - (long long)row * S);
+  // A finished beam has one continuation, whatever its logits.  The warps count the others only: left where their rows are, the finished ones'
+  // would idle on some SMs more than on others.
+  if (a.done && (row = unfinished(a.done, a.B * a.K, row, lane)) < 0) return;
+  const int b = row / a.K, k = row - b * a.K;
+  const long long list = (long long)row * S + seg;
   const T* x0 = (const T*)a.logits + b * a.sb + k * a.sk;
-  const int base = slice * BT * EPT + tid;
-  if (tid == 0) count = 0;
-  float x[EPT];
+  const int skip = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));  // logit v is at place skip + v
+  const int first = seg * portions, stop = min(first + portions, (skip + a.V + PORTION - 1) / PORTION);
+  // whole portions, which are loaded 16 bytes at a time, two ahead; the first and the last of a row may be parts
+  const int lo = max(first, skip ? 1 : 0), hi = min(stop, (skip + a.V) / PORTION);
+  uint32_t wa[16], wb[16];
+  auto load_whole = [&](uint32_t (&w)[16], int p, int of) {  // of: the lane whose values
+    const T* x = x0 + (p * PORTION + of * PIECE - skip);
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    const int v = base + i * BT;
-    x[i] = v < a.V ? as_float(__ldcs(x0 + v)) : -INFINITY;
-  }
-  float ma = -INFINITY, mb = -INFINITY;
+    for (int j = 0; j < 4; ++j) {
+      const uint4 r = __ldcs(reinterpret_cast<const uint4*>(x + j * 32 * PIECE));
+      w[4 * j] = r.x; w[4 * j + 1] = r.y; w[4 * j + 2] = r.z; w[4 * j + 3] = r.w;
+    }
+  };
+  auto load = [&](uint32_t (&w)[16], int p, int of) {
+    if (p >= lo && p < hi) return load_whole(w, p, of);
+    const int base = p * PORTION + of * PIECE - skip;
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    if (i < EPT / 2) ma = fmaxf(ma, x[i]);
-    else mb = fmaxf(mb, x[i]);
-  }
-  const uint32_t ka = order_key(ma), kb = order_key(mb);
-  const float top = key_value(block_max(ka > kb ? ka : kb, red)), from = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
+    for (int i = 0; i < 16; ++i) {
+      w[i] = 0;
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x[i] - from) * 1.4426950408889634f));
-    sum += e;
-  }
-  sum = warp_sum(sum);
-  if (lane == 0) sums[warp] = sum;
-  const uint32_t nth = nth_of_warp(ka, kb, a.n);
-  __syncthreads();  // red has been read
-  uint32_t bound = block_max(nth, red);
-  bound = bound > NO_KEY ? bound : NO_KEY + 1;  // -infinity is no candidate
-  if (tid == 0) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < BW; ++i) s += sums[i];
-    part[(long long)row * S + slice] = RowPart{top, s};
-  }
-  // what passes the bound: key and, the lower the better, index
-  if (ka >= bound || kb >= bound) {
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const uint32_t key = order_key(x[i]);
-      if (key >= bound && x[i] == x[i]) {
-        const int at = atomicAdd(&count, 1);
-        if (at < ROOM) room[at] = (unsigned long long)key << 32 | (0xffffffffu - (uint32_t)(base + i * BT));
+      for (int e = 0; e < N; ++e) {
+        const int v = base + (i / 4) * 32 * PIECE + (i & 3) * N + e;
+        w[i] |= (v >= 0 && v < a.V ? Word<T>::bits(x0 + v) : Word<T>::NONE) << (16 * e);
       }
     }
+  };
+  float m = -INFINITY, s = 0.f;                             // of this lane
+  float v1 = -INFINITY, v2 = -INFINITY, v3 = -INFINITY;     // its portions' largest maxima (NaN is none), and where the first two are
+  int p1 = first, p2 = first;
+  auto take = [&](uint32_t (&w)[16], int p, bool more) {
+    float x[16 * N];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[i * N + e] = Word<T>::value(w[i], e);
+    if (more) load_whole(w, p + 2, lane);
+    float half[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 8 * N; ++i) {
+      half[0] = fmaxf(half[0], x[i]);
+      half[1] = fmaxf(half[1], x[i + 8 * N]);
+    }
+    const float top = fmaxf(half[0], half[1]), mn = fmaxf(m, top), from = mn == -INFINITY ? 0.f : mn;
+    s *= ex2((m - from) * 1.4426950408889634f);
+    m = mn;
+    float2 sum = make_float2(0.f, 0.f);
+    const float2 one = make_float2(1.f, 1.f), down = make_float2(-from, -from), log2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+#pragma unroll
+    for (int i = 0; i < 16 * N; i += 2) {
+      // the difference first and by itself: a logit's own multiple of log2 e would be off by more than the difference's
+      const float2 d = fma2(fma2(make_float2(x[i], x[i + 1]), one, down), log2e, make_float2(0.f, 0.f));
+      sum = fma2(make_float2(ex2(d.x), ex2(d.y)), one, sum);
+    }
+    s += sum.x + sum.y;
+    if (stop - first == 1) {  // one portion: its halves, which lie in the same one
+      v1 = top;
+      v2 = fminf(half[0], half[1]);
+    } else if (top > v1) {
+      v3 = v2; v2 = v1; v1 = top;
+      p2 = p1; p1 = p;
+    } else if (top > v2) {
+      v3 = v2; v2 = top;
+      p2 = p;
+    } else v3 = fmaxf(v3, top);
+  };
+  if (lo < hi) load_whole(wa, lo, lane);
+  if (lo + 1 < hi) load_whole(wb, lo + 1, lane);
+  for (int p = lo; p < hi; p += 2) {
+    take(wa, p, p + 2 < hi);
+    if (p + 1 < hi) take(wb, p + 1, p + 3 < hi);
   }
-  __syncthreads();
-  const int c = count;
-  const long long out = ((long long)row * S + slice) * a.n;
-  if (c <= ROOM) {
-    for (int i = tid; i < c; i += BT) {
-      const unsigned long long me = room[i];
+  auto take_part = [&](int p) {
+    load(wa, p, lane);
+    take(wa, p, false);
+  };
+  for (int p = first; p < min(lo, stop); ++p) take_part(p);
+  for (int p = max(lo, hi); p < stop; ++p) take_part(p);
+  const float mw = warp_max(m), from = mw == -INFINITY ? 0.f : mw;
+  s = warp_sum(s * ex2((m - from) * 1.4426950408889634f));
+  if (lane == 0) part[list] = RowPart{mw, s};
+
+  const uint32_t nth = nth_of_warp(order_key(v1), order_key(v2), a.n);
+  const float bound = nth > NO_KEY ? key_value(nth) : -FLT_MAX;
+  unsigned long long* hit = hits[threadIdx.x >> 5];
+  int count = 0;
+  auto collect = [&](const uint32_t (&w)[16], int p, int of, bool mine) {  // the values of lane `of` of portion p, if this lane has any
+    const int base = p * PORTION + of * PIECE - skip;
+#pragma unroll
+    for (int i = 0; i < 16 * N; ++i) {
+      const float x = Word<T>::value(w[i / N], i % N);
+      const bool in = mine && x >= bound;
+      const uint32_t ones = __ballot_sync(L3_FULL, in);
+      if (in) {
+        const int at = count + __popc(ones & ((1u << lane) - 1));
+        if (at < HITS) hit[at] = (unsigned long long)order_key(x) << 32 | (0xffffffffu - (uint32_t)(base + (i / PIECE) * 32 * PIECE + i % PIECE));
+      }
+      count += __popc(ones);
+    }
+  };
+  const bool one = first < stop && v1 >= bound, two = stop - first > 1 && v2 >= bound && p2 != p1;
+  if (one) load(wa, p1, lane);
+  if (two) load(wb, p2, lane);
+  collect(wa, p1, lane, one);
+  if (__any_sync(L3_FULL, two)) collect(wb, p2, lane, two);
+  // a lane with three such portions may have more: all of its values, a portion of them each lane
+  for (uint32_t many = __ballot_sync(L3_FULL, v3 >= bound); many; many &= many - 1) {
+    const int of = __ffs(many) - 1, q1 = __shfl_sync(L3_FULL, p1, of), q2 = __shfl_sync(L3_FULL, p2, of);
+    for (int p0 = first; p0 < stop; p0 += 32) {
+      const int p = p0 + lane;
+      const bool mine = p < stop && p != q1 && p != q2;
+      if (mine) load(wa, p, of);
+      collect(wa, p, of, mine);
+    }
+  }
+  __syncwarp();
+  if (count <= HITS) {
+    for (int i = lane; i < count; i += 32) {
+      const unsigned long long me = hit[i];
       int rank = 0;
-      for (int j = 0; j < c; ++j) rank += room[j] > me;
+      for (int j = 0; j < count; ++j) rank += hit[j] > me;
       if (rank < a.n) {
-        cand_v[out + rank] = key_value((uint32_t)(me >> 32));
-        cand_i[out + rank] = (int)(0xffffffffu - (uint32_t)me);
+        cand_v[list * a.n + rank] = key_value((uint32_t)(me >> 32));
+        cand_i[list * a.n + rank] = (int)(0xffffffffu - (uint32_t)me);
       }
     }
-    for (int i = c + tid; i < a.n; i += BT) cand_i[out + i] = -1;
+    for (int i = count + lane; i < a.n; i += 32) cand_i[list * a.n + i] = -1;
     return;
   }
-  unsigned long long last = ~0ull;
-  for (int it = 0; it < a.n; ++it) {
-    unsigned long long best = 0;
+  // many equal values: a list of the n largest so far, sorted
+  Best<NL> best;
+  best.none();
+  for (int p = first; p < stop; ++p) {
+    load(wa, p, lane);
+    const int base = p * PORTION + lane * PIECE - skip;
+    for (int i = 0; i < 16 * N; ++i) {
+      float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const uint32_t key = order_key(x[i]);
-      const unsigned long long me = (unsigned long long)key << 32 | (0xffffffffu - (uint32_t)(base + i * BT));
-      if (key > NO_KEY && x[i] == x[i] && me < last && me > best) best = me;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long y = __shfl_xor_sync(L3_FULL, best, o);
-      best = y > best ? y : best;
-    }
-    __syncthreads();
-    if (lane == 0) room[warp] = best;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < BW; ++i) best = room[i] > best ? room[i] : best;
-    last = best;
-    if (tid == 0) {
-      cand_v[out + it] = key_value((uint32_t)(best >> 32));
-      cand_i[out + it] = best ? (int)(0xffffffffu - (uint32_t)best) : -1;
+      for (int j = 0; j < 16 * N; ++j) x = i == j ? Word<T>::value(wa[j / N], j % N) : x;
+      const int v = base + (i / PIECE) * 32 * PIECE + i % PIECE;
+      uint32_t ones = __ballot_sync(L3_FULL, best.passes(x, v));
+      while (ones) {
+        const int src = __ffs(ones) - 1;
+        ones &= ones - 1;
+        const float nx = __shfl_sync(L3_FULL, x, src);
+        const int nv = __shfl_sync(L3_FULL, v, src);
+        if (best.passes(nx, nv)) best.insert(nx, nv, a.n, lane);
+      }
     }
   }
+#pragma unroll
+  for (int i = 0; i < NL; ++i)
+    if (i * 32 + lane < a.n) {
+      cand_v[list * a.n + i * 32 + lane] = best.v[i];
+      cand_i[list * a.n + i * 32 + lane] = best.at[i];
+    }
 }
 
 struct Scored {
@@ -165,15 +311,30 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamSelectArgs a, i
   // a beam's largest logit m and scores[k] - log sum_u e^(logit - m): apart, since logits may all be the type's lowest value
   __shared__ double add[BEAM_MAX_K];
   __shared__ float off[BEAM_MAX_K];
-  __shared__ uint32_t red[BW];
+  __shared__ uint32_t keys[2 * BT], least;
+  __shared__ int kept;
   __shared__ Scored room[ROOM];
   __shared__ Scored win[BW];
-  __shared__ int count;
+  __shared__ int open[ROOM], passed, count;
   pdl_launch();
   pdl_wait();
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = S * a.n, all = a.K * per;
-  if (tid == 0) count = 0;
+  const int per = S * a.n, lists = a.K * S;
+  if (tid == 0) {
+    count = passed = kept = 0;
+    least = NO_KEY + 1;
+  }
+  const float* cv = cand_v + (long long)b * lists * a.n;
+  const int* ci = cand_i + (long long)b * lists * a.n;
+  constexpr int HOLD = 4;  // lists whose first candidates a thread keeps; asked for ahead of the rows' sums
+  float x[HOLD];
+  int v[HOLD];
+#pragma unroll
+  for (int u = 0; u < HOLD; ++u) {
+    const int i = (tid + u * BT) * a.n;
+    x[u] = tid + u * BT < lists ? cv[i] : 0.f;
+    v[u] = tid + u * BT < lists ? ci[i] : -1;
+  }
   for (int k = warp; k < a.K; k += BW) {
     const long long row = (long long)b * a.K + k;
     const float s0 = a.scores[row];
@@ -188,7 +349,7 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamSelectArgs a, i
     double s = 0.;
     for (int i = lane; i < S; i += 32) {
       const RowPart p = part[row * S + i];
-      if (p.m > -INFINITY || p.s != p.s) s += (double)p.s * exp((double)p.m - (double)from);
+      if (p.m > -INFINITY || p.s != p.s) s += (double)p.s * (double)expf(p.m - from);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(L3_FULL, s, o);
@@ -198,32 +359,65 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamSelectArgs a, i
     }
   }
   __syncthreads();
-  // candidate i: beam i / per, its slice's list; a finished beam has the end token, at its own score
-  auto scored = [&](int i) {
-    const int k = i / per, in = i % per;
-    const long long row = (long long)b * a.K + k;
+  // candidate i: beam i / per, its segment's list; a finished beam has the end token, at its own score
+  auto scored = [&](int i, float x, int v) {
+    const int k = i / per, in = i - k * per;
     Scored c{-INFINITY, 0};
-    if (a.done && a.done[row]) {
+    if (a.done && a.done[(long long)b * a.K + k]) {
       if (in == 0) c = Scored{add[k], (unsigned)(k * a.V + a.eos)};
-    } else {
-      const int v = cand_i[row * per + in];
-      if (v >= 0) c = Scored{((double)cand_v[row * per + in] - (double)off[k]) + add[k], (unsigned)(k * a.V + v)};
-    }
+    } else if (v >= 0) c = Scored{((double)x - (double)off[k]) + add[k], (unsigned)(k * a.V + v)};
     if (!(c.s > -INFINITY) || c.s == INFINITY) c.s = -INFINITY;  // NaN, too
     return c;
   };
-  // the bound on scores rounded to fp32, which keeps their order up to ties
-  uint32_t ka = 0, kb = 0;
-  for (int i = tid; i < all; i += BT) {
-    const uint32_t key = order_key((float)scored(i).s);
+  auto read = [&](int i) { return scored(i, cv[i], ci[i]); };
+  // Every list begins with its best, so the n-th best of the lists' firsts bounds the n-th of all from below, and only lists whose first
+  // passes it hold any that do.  The bound is on scores rounded to fp32, which keeps their order up to ties.
+  auto key_of = [&](const Scored& c) { return order_key((float)c.s); };
+  uint32_t held[HOLD], ka = 0, kb = 0;
+#pragma unroll
+  for (int u = 0; u < HOLD; ++u) {
+    held[u] = tid + u * BT < lists ? key_of(scored((tid + u * BT) * a.n, x[u], v[u])) : 0;
+    if (u & 1) ka = held[u] > ka ? held[u] : ka;
+    else kb = held[u] > kb ? held[u] : kb;
+  }
+  for (int i = tid + HOLD * BT; i < lists; i += BT) {
+    const uint32_t key = key_of(read(i * a.n));
     if ((i / BT) & 1) ka = key > ka ? key : ka;
     else kb = key > kb ? key : kb;
   }
-  uint32_t bound = block_max(nth_of_warp(ka, kb, a.n), red);
-  bound = bound > NO_KEY ? bound : NO_KEY + 1;
-  for (int i = tid; i < all; i += BT) {
-    const Scored c = scored(i);
-    if (c.s > -INFINITY && order_key((float)c.s) >= bound) {
+  // ... of which each warp finds its own n-th; the largest of those leaves few that are counted off against one another
+  const uint32_t floor_key = nth_of_warp(ka, kb, a.n);
+  if (lane == 0) atomicMax(&least, floor_key);
+  __syncthreads();
+  const uint32_t rough = least;
+  for (uint32_t key : {ka, kb})
+    if (key >= rough) keys[atomicAdd(&kept, 1)] = key;
+  __syncthreads();
+  const int m = kept;
+  for (int i = tid; i < m; i += BT) {
+    const uint32_t me = keys[i];
+    int more = 0, same = 0;
+    for (int j = 0; j < m; ++j) {
+      more += keys[j] > me;
+      same += keys[j] == me;
+    }
+    if (more < a.n && more + same >= a.n) least = me;  // all that write write the same; fewer than n: what is there stays
+  }
+  __syncthreads();
+  const uint32_t bound = least;
+  auto pass = [&](int i, uint32_t key) {
+    if (key < bound) return;
+    const int at = atomicAdd(&passed, 1);
+    if (at < ROOM) open[at] = i;
+  };
+#pragma unroll
+  for (int u = 0; u < HOLD; ++u) pass(tid + u * BT, held[u]);
+  for (int i = tid + HOLD * BT; i < lists; i += BT) pass(i, key_of(read(i * a.n)));
+  __syncthreads();
+  const int some = passed;
+  for (int i = tid; i < min(some, ROOM) * a.n; i += BT) {
+    const Scored c = read(open[i / a.n] * a.n + i % a.n);
+    if (c.s > -INFINITY && key_of(c) >= bound) {
       const int at = atomicAdd(&count, 1);
       if (at < ROOM) room[at] = c;
     }
@@ -245,7 +439,7 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamSelectArgs a, i
     a.out_done[o] = 1;
   };
   const int c = count;
-  if (c <= ROOM) {
+  if (c <= ROOM && some <= ROOM) {
     for (int i = tid; i < c; i += BT) {
       const Scored me = room[i];
       int rank = 0;
@@ -258,8 +452,8 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamSelectArgs a, i
   Scored last{INFINITY, 0};
   for (int it = 0; it < a.n; ++it) {
     Scored best{-INFINITY, 0xffffffffu};
-    for (int i = tid; i < all; i += BT) {
-      const Scored x = scored(i);
+    for (int i = tid; i < lists * a.n; i += BT) {
+      const Scored x = read(i);
       if (x.s > -INFINITY && ahead(last, x) && ahead(x, best)) best = x;
     }
 #pragma unroll
@@ -281,39 +475,37 @@ __global__ void __launch_bounds__(BT) beam_pick_kernel(const BeamSelectArgs a, i
   }
 }
 
-// values of a thread: as few as still give every SM two CTAs, so that a small call ends early, and at most 32
-int values_of(int rows, int V, int n_sm) {
-  int ept = 32;
-  while (ept > 4 && (long long)rows * ((V + BT * ept - 1) / (BT * ept)) < 2 * n_sm) ept /= 2;
-  return ept;
+struct Cut { int S, portions; };
+// Segments of a row: as many as the machine has room for at once (one CTA too many and all wait for a second turn: 38 us in place of 24 for
+// 219 rows of 128256 fp32 logits), of one portion (2 KB of a row) at least.
+Cut cut_of(int rows, int V, int dtype, int n_sm) {
+  const bool f32 = dtype == L3_DTYPE_F32;
+  const int portion = f32 ? 512 : 1024, all = (V + 8 + portion - 1) / portion;  // 8: a row may begin behind a multiple of 16 bytes
+  const int want = warps_of_sm(f32) * n_sm / rows;
+  const int portions = want >= all ? 1 : want <= 1 ? all : (all + want - 1) / want;
+  return Cut{(all + portions - 1) / portions, portions};
 }
-template <typename T>
-cudaError_t rows_of(const BeamSelectArgs& a, int ept, int S, RowPart* part, float* cv, int* ci, cudaStream_t s) {
-  const dim3 g(S, a.B * a.K);
-  switch (ept) {
-    case 4: return launch_k(beam_rows_kernel<T, 4>, g, dim3(BT), 0, s, a, S, part, cv, ci);
-    case 8: return launch_k(beam_rows_kernel<T, 8>, g, dim3(BT), 0, s, a, S, part, cv, ci);
-    case 16: return launch_k(beam_rows_kernel<T, 16>, g, dim3(BT), 0, s, a, S, part, cv, ci);
-    default: return launch_k(beam_rows_kernel<T, 32>, g, dim3(BT), 0, s, a, S, part, cv, ci);
-  }
+template <typename T> cudaError_t launch_rows(const BeamSelectArgs& a, const Cut& c, RowPart* part, float* cv, int* ci, cudaStream_t s) {
+  const dim3 g((unsigned)(((long long)a.B * a.K * c.S + RW - 1) / RW));
+  if (a.n > 32) return launch_k(beam_rows_kernel<T, 2>, g, dim3(RW * 32), 0, s, a, c.S, c.portions, part, cv, ci);
+  return launch_k(beam_rows_kernel<T, 1>, g, dim3(RW * 32), 0, s, a, c.S, c.portions, part, cv, ci);
 }
 }  // namespace
 
 size_t beam_select_workspace(int B, int K, int V, int n, int n_sm) {
-  const int ept = values_of(B * K, V, n_sm);
-  const size_t lists = (size_t)B * K * ((V + BT * ept - 1) / (BT * ept));
+  const size_t lists = (size_t)B * K * cut_of(B * K, V, L3_DTYPE_F32, n_sm).S;  // 16-bit logits: no more segments
   return lists * (sizeof(RowPart) + (size_t)n * 8);
 }
 cudaError_t launch_beam_select(const BeamSelectArgs& a, int n_sm, cudaStream_t s) {
-  const int ept = values_of(a.B * a.K, a.V, n_sm), S = (a.V + BT * ept - 1) / (BT * ept);
-  const size_t lists = (size_t)a.B * a.K * S;
+  const Cut c = cut_of(a.B * a.K, a.V, a.dtype, n_sm);
+  const size_t lists = (size_t)a.B * a.K * c.S;
   RowPart* part = (RowPart*)a.ws;
   float* cv = (float*)(part + lists);
   int* ci = (int*)(cv + lists * a.n);
-  cudaError_t e = a.dtype == L3_DTYPE_F32    ? rows_of<float>(a, ept, S, part, cv, ci, s)
-                  : a.dtype == L3_DTYPE_BF16 ? rows_of<bf16>(a, ept, S, part, cv, ci, s)
-                                             : rows_of<__half>(a, ept, S, part, cv, ci, s);
+  cudaError_t e = a.dtype == L3_DTYPE_F32    ? launch_rows<float>(a, c, part, cv, ci, s)
+                  : a.dtype == L3_DTYPE_BF16 ? launch_rows<bf16>(a, c, part, cv, ci, s)
+                                             : launch_rows<__half>(a, c, part, cv, ci, s);
   if (e != cudaSuccess) return e;
   g_l3_pdl_next = true;
-  return launch_k(beam_pick_kernel, dim3(a.B), dim3(BT), 0, s, a, S, (const RowPart*)part, (const float*)cv, (const int*)ci);
+  return launch_k(beam_pick_kernel, dim3(a.B), dim3(BT), 0, s, a, c.S, (const RowPart*)part, (const float*)cv, (const int*)ci);
 }

@@ -90,6 +90,7 @@ extern "C" int l3_paged_attention(const L3PagedAttention* a) {
   p.table = a->table; p.table_stride = a->table_stride; p.max_pages = a->max_pages; p.lengths = a->lengths;
   p.B = a->batch; p.H = a->heads; p.G = a->kv_heads; p.HD = a->head_dim;
   p.scale = a->scale; p.out = a->out; p.out_dtype = a->out_dtype; p.lse = a->lse; p.ws = a->workspace;
+  REQ(paged_attn_fits(p), "a pool of %d pages spans more than 2^32 of its strides' common unit", a->pages);
   CKD(launch_paged_attention(p, n_sm, (cudaStream_t)a->stream));
   return L3_OK;
 }

@@ -3,10 +3,10 @@
 // over the tokens j < length of the sequence; token j lies in page table[j / P] at place j % P.
 //
 // Bound by the cache's bytes: every key and value is read once for all query heads of its kv head (2 HD values for 4 HD flops per
-// query head).  The keys of all (sequence, kv head) items, in tiles of 16, are one long row that the warps of the machine share
+// query head).  The keys of all (sequence, kv head) items, in tiles of 8 - 32, are one long row that the warps of the machine share
 // out evenly - lengths of any mixture leave no SM idle, and a single long sequence fills the machine.  A warp works through its
-// stretch alone, without a block barrier: a ring of tiles in shared memory filled by 16-byte asynchronous copies (a page's rows can
-// lie anywhere; the ring runs on across items), one pass with running maximum and sum.  An item that lies within one warp's stretch
+// stretch alone, without a block barrier, its next tiles on their way (16-bit caches: into two buffers of its own in shared memory, by
+// asynchronous copies; fp32: into registers), across items; one pass with running maximum and sum.  An item that lies within one warp's stretch
 // is written at once; one that several warps share leaves a partial (m, l, o) per warp, and a second, dependent launch joins those
 // in the order of the keys, so that results do not change from run to run.
 #include <math.h>
@@ -20,39 +20,22 @@
 #include "paged.h"
 
 namespace {
-constexpr int TK = 16;          // keys of a tile
-constexpr int MOST_NW = 4;      // warps of a CTA (Core::NW)
-constexpr int CTAS = 2;         // CTAs of an SM
+constexpr int MOST_WARPS = 16;  // of an SM (Core::CTAS of Core::NW warps)
 constexpr int HEADS = 8;        // most query heads of an item
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes into shared memory, zeros where !take (the address is not read then)
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
 template <typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, bf16>::value)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // two values as the nearest 16-bit ones, and what those leave (again as 16-bit values)
 template <typename T> __device__ __forceinline__ void two_parts(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -68,101 +51,236 @@ template <typename T> __device__ __forceinline__ void two_parts(float x, float y
     lo = *reinterpret_cast<const uint32_t*>(&r);
   }
 }
-__device__ __forceinline__ float2 load_q2(const PagedAttnArgs& a, long long i) {  // two neighbours of q as fp32
-  if (a.q_dtype == L3_DTYPE_F32) return make_float2(__ldg((const float*)a.q + i), __ldg((const float*)a.q + i + 1));
-  if (a.q_dtype == L3_DTYPE_BF16) {
-    const bf16* p = (const bf16*)a.q + i;
-    return make_float2(__bfloat162float(p[0]), __bfloat162float(p[1]));
-  }
-  const __half* p = (const __half*)a.q + i;
-  return make_float2(__half2float(p[0]), __half2float(p[1]));
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes into shared memory, zeros where !take (the address is not read then)
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void store_out2(const PagedAttnArgs& a, long long i, float x, float y) {  // i is even
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float load_q(const PagedAttnArgs& a, long long i) {
+  if (a.q_dtype == L3_DTYPE_F32) return __ldg((const float*)a.q + i);
+  if (a.q_dtype == L3_DTYPE_BF16) return __bfloat162float(((const bf16*)a.q)[i]);
+  return __half2float(((const __half*)a.q)[i]);
+}
+// N (2, 4 or 8) neighbouring outputs, i a multiple of N
+template <int N> __device__ __forceinline__ void store_out(const PagedAttnArgs& a, long long i, const float (&v)[N]) {
   if (a.out_dtype == L3_DTYPE_F32) {
-    if (a.out_lo) {
-      float hx, lx, hy, ly;
-      split_tf32(x, hx, lx);
-      split_tf32(y, hy, ly);
-      *reinterpret_cast<float2*>((float*)a.out + i) = make_float2(hx, hy);
-      *reinterpret_cast<float2*>(a.out_lo + i) = make_float2(lx, ly);
-    } else *reinterpret_cast<float2*>((float*)a.out + i) = make_float2(x, y);
-  } else if (a.out_dtype == L3_DTYPE_BF16) *reinterpret_cast<__nv_bfloat162*>((bf16*)a.out + i) = __floats2bfloat162_rn(x, y);
-  else *reinterpret_cast<__half2*>((__half*)a.out + i) = __floats2half2_rn(x, y);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      float2 x = make_float2(v[e], v[e + 1]);
+      if (a.out_lo) {
+        float2 lo;
+        split_tf32(v[e], x.x, lo.x);
+        split_tf32(v[e + 1], x.y, lo.y);
+        *reinterpret_cast<float2*>(a.out_lo + i + e) = lo;
+      }
+      *reinterpret_cast<float2*>((float*)a.out + i + e) = x;
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    uint32_t x, rest;
+    if (a.out_dtype == L3_DTYPE_BF16) two_parts<bf16>(v[e], v[e + 1], x, rest);
+    else two_parts<__half>(v[e], v[e + 1], x, rest);
+    *reinterpret_cast<uint32_t*>((bf16*)a.out + i + e) = x;
+  }
 }
 __device__ __forceinline__ int asked_length(const PagedAttnArgs& a, int b) { return a.lengths ? a.lengths[b] : *a.pos_ptr + 1; }
-__device__ __forceinline__ int length_of(const PagedAttnArgs& a, int b) {
-  const long long n = asked_length(a, b), cap = (long long)a.max_pages << a.log_page;
-  return (int)(n < 0 ? 0 : n > cap ? cap : n);
-}
-__device__ __forceinline__ int tiles_of(int len) { return (len + TK - 1) / TK; }
+__device__ __forceinline__ int length_of(const PagedAttnArgs& a, int b) { return min(max(asked_length(a, b), 0), a.max_pages << a.log_page); }
 
-// where a warp is in the long row of tiles: tile t of the nt tiles of item (b, gb)
+// where a warp is in the long row of tiles: tile t of the nt tiles of item (sequence b, kv head g, block of its query heads)
 struct Cursor {
-  int b, gb, t, nt, len;
+  int b, g, blk, t, nt, len;
+  __device__ __forceinline__ int head0(const PagedAttnArgs& a) const { return g * a.nrep + blk * a.heads_blk; }
+  __device__ __forceinline__ int heads(const PagedAttnArgs& a) const { return min(a.heads_blk, a.nrep - blk * a.heads_blk); }
+  __device__ __forceinline__ int item(const PagedAttnArgs& a) const { return (b * a.G + g) * a.blocks + blk; }
 };
-__device__ __forceinline__ void next_sequence(const PagedAttnArgs& a, Cursor& c) {
-  c.gb = c.t = 0;
+template <int TK> __device__ __forceinline__ int tiles_of(int len) { return (int)((unsigned)(len + TK - 1) / TK); }
+template <int TK> __device__ __forceinline__ void advance(const PagedAttnArgs& a, Cursor& c) {
+  if (++c.t < c.nt) return;
+  c.t = 0;
+  if (++c.blk < a.blocks) return;
+  c.blk = 0;
+  if (++c.g < a.G) return;
+  c.g = 0;
   do {
     ++c.b;
     c.len = c.b < a.B ? length_of(a, c.b) : 0;
-    c.nt = tiles_of(c.len);
+    c.nt = tiles_of<TK>(c.len);
   } while (c.b < a.B && c.nt == 0);
 }
-__device__ __forceinline__ void advance(const PagedAttnArgs& a, Cursor& c, int items) {
-  if (++c.t < c.nt) return;
-  c.t = 0;
-  if (++c.gb == items) next_sequence(a, c);
-}
+__device__ __forceinline__ long long weight_of(int nt) { return nt ? 2LL * nt + 1 : 0; }
+// 64-bit division that is a 32-bit one wherever that will do
+__device__ __forceinline__ long long quotient(long long x, int d) { return (unsigned long long)x >> 32 ? x / d : (long long)((uint32_t)x / (uint32_t)d); }
+
+// The rows of a tile: lane j (of TK; the others repeat them) has the places of key j's rows, in units of the pools.
+struct Rows {
+  uint32_t k, v;               // offsets in units of a.unit bytes
+  uint32_t mask;               // keys that there are
+  int fresh;                   // the key that comes from k_new / v_new, or -1
+};
+struct Fresh { const char *k, *v; };  // its rows
+__device__ __forceinline__ const char* row_at(const void* pool, uint32_t off, int unit) { return (const char*)pool + (unsigned long long)off * (uint32_t)unit; }
 
 // ------------------------------------------------------------------------------------------ 16-bit caches: tensor cores
 // The item's (up to 8) query heads are rows 0 - 7 of an m16n8k16 tile.  Rows 8 - 15, which a tile has anyway, carry what rounding to 16
 // bits leaves of the same heads: the rest of an fp32 query in S = Q K^T, the rest of the weights in O += P V, so that the weights
 // enter with 16 (bf16) or 22 (fp16) significant bits at no further instruction.  fp16 weights are scaled by 2^12 ahead of the rounding
 // (they are at most 1), which keeps weights down to 2^-36 of the largest off the subnormals.
-template <typename T, int HD> struct MmaCore {
-  static constexpr int ROW = HD * 2, NCH = ROW / 16, PITCH = ROW + 16;  // the odd number of 16-byte pieces keeps ldmatrix free of conflicts
-  static constexpr int TILE = 2 * TK * PITCH;                           // bytes of a tile's keys and values
-  static constexpr int KS = HD / 16, NT = HD / 8;
-  static constexpr int NW = 4;
+// Keys and values are copied apart, so that a tile's keys make room for those of the tile after next while its values are still in use.
+// A row's pieces of 16 bytes lie in an order that keeps the eight rows of a matrix on different banks.
+template <typename T, int HD_, bool QLO> struct MmaCore {
+  static constexpr int HD = HD_, TK = HD > 64 ? 16 : 32;
+  static constexpr int NW = 4, CTAS = HD > 96 && QLO ? 2 : HD > 32 ? 3 : 4;  // as many warps as registers and shared memory leave room for
+  static constexpr int KS = HD / 16, NT = HD / 8, NCH = HD / 8, HALF = TK * HD * 2, AHEAD = 2;
+  static constexpr int QW = (QLO ? 4 : 2) * KS;     // words of a lane's share of Q, which waits in shared memory
+  static constexpr size_t SMEM = (size_t)NW * (AHEAD * 2 * HALF + (QW + 3) / 4 * 512);
   static constexpr float BIAS = std::is_same<T, bf16>::value ? 0.f : 12.f;
-  uint32_t qa[KS][4];
+  uint32_t* q;
+  uint32_t ring;   // [AHEAD][keys | values] of the warp
   float o[NT][4];
   float m, l;  // of row lane / 4, in units of log 2; l: this lane's share
   float sc;
+  float s[TK / 8][4];
 
-  __device__ __forceinline__ void begin(const PagedAttnArgs& a, int b, int head0, int heads, int lane) {
+  __device__ static __forceinline__ int turn(int row) { return NCH % 8 == 0 ? row & 7 : NCH % 4 == 0 ? (row >> 1) & 3 : (row >> 2) & 1; }
+  __device__ static __forceinline__ uint32_t place(int row, int piece) { return (row * NCH + (piece ^ turn(row))) * 16; }
+
+  __device__ __forceinline__ void memory(uint8_t* smem, int warp) {
+    ring = smem_u32(smem) + warp * AHEAD * 2 * HALF;
+    q = reinterpret_cast<uint32_t*>(smem + NW * AHEAD * 2 * HALF) + warp * ((QW + 3) / 4 * 128);
+  }
+  // words of step ks: its two registers' high parts, then (QLO) what they leave; 16 bytes of every lane side by side
+  __device__ __forceinline__ uint32_t& q_word(int i, int lane) { return q[(i / 4 * 32 + lane) * 4 + i % 4]; }
+  // The next item's query: asked for (ask_query) ahead of the last tile of the one before, laid into shared memory (load_query) behind it.
+  uint32_t asked[QLO ? 1 : KS][2];
+  __device__ __forceinline__ void ask_query(const PagedAttnArgs& a, const Cursor& c, int lane) {
+    if (QLO || !a.q_vec) return;
     const int g = lane >> 2, t = lane & 3;
-    const long long qp = b * a.q_sb + (long long)(head0 + min(g, heads - 1)) * a.q_sh;
+    const char* p = (const char*)a.q + (c.b * a.q_sb + (long long)(c.head0(a) + min(g, c.heads(a) - 1)) * a.q_sh) * 2 + t * 4;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const float2 x = load_q2(a, qp + ks * 16 + 2 * t), y = load_q2(a, qp + ks * 16 + 8 + 2 * t);
-      two_parts<T>(x.x, x.y, qa[ks][0], qa[ks][1]);
-      two_parts<T>(y.x, y.y, qa[ks][2], qa[ks][3]);
-      if (a.q_dtype != L3_DTYPE_F32) qa[ks][1] = qa[ks][3] = 0u;  // also where an infinity would leave a NaN
+      asked[QLO ? 0 : ks][0] = __ldg(reinterpret_cast<const uint32_t*>(p + ks * 32));
+      asked[QLO ? 0 : ks][1] = __ldg(reinterpret_cast<const uint32_t*>(p + ks * 32 + 16));
     }
+  }
+  __device__ __forceinline__ void load_query(const PagedAttnArgs& a, const Cursor& c, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const long long qp = c.b * a.q_sb + (long long)(c.head0(a) + min(g, c.heads(a) - 1)) * a.q_sh;
+    if (!QLO && a.q_vec) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) *reinterpret_cast<uint2*>(&q_word(2 * ks, lane)) = make_uint2(asked[QLO ? 0 : ks][0], asked[QLO ? 0 : ks][1]);
+      return;
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long d = qp + ks * 16 + h * 8 + 2 * t;
+        uint32_t high, rest;
+        two_parts<T>(load_q(a, d), load_q(a, d + 1), high, rest);
+        q_word((QLO ? 4 : 2) * ks + h, lane) = high;
+        if (QLO) q_word(4 * ks + 2 + h, lane) = rest;
+      }
+  }
+  __device__ __forceinline__ void reset(const PagedAttnArgs& a) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     m = -INFINITY;
     l = 0.f;
     sc = a.scale * 1.4426950408889634f;
   }
-  __device__ __forceinline__ void tile(uint32_t ksm, uint32_t mask, int lane) {
-    const int t = lane & 3, mi = lane >> 3, mr = lane & 7;
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-    {
-      const uint32_t row = ksm + ((mi >> 1) * 8 + mr) * PITCH + (mi & 1) * 16;
+  // copies the tile's rows; rows that are not there become zeros (0 times whatever would lie there has to be 0)
+  __device__ __forceinline__ void copy(const void* pool, int unit, uint32_t off, uint32_t step, bool one_page, const Rows& r, const char* fresh, uint32_t dst, int lane) {
+    constexpr uint32_t ALL = TK == 32 ? 0xffffffffu : (1u << (TK & 31)) - 1;
+    constexpr bool EVEN = 32 % NCH == 0;           // every copy of a lane is of the same column of pieces
+    constexpr int RS = EVEN ? 32 / NCH : 0;        // and RS rows behind the last
+    const int row0 = lane / NCH, c0 = lane % NCH;
+    const uint32_t to = dst + row0 * NCH * 16, x = (c0 ^ turn(row0)) * 16;  // turn() of a sum of disjoint bits is the parts' exclusive or
+    if (one_page && r.mask == ALL && r.fresh < 0) {  // rows at equal distances from the first lane's
+      const uint32_t first = __shfl_sync(L3_FULL, off, 0);
+      if constexpr (EVEN) {
+        const char* base = (const char*)pool + c0 * 16;
+        const uint32_t at = first + row0 * step;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
+        for (int i = 0; i < TK * NCH / 32; ++i) cp16(to + (x ^ (turn(i * RS) * 16)) + i * 512, row_at(base, at + i * RS * step, unit), true);
+      } else {
+#pragma unroll
+        for (int i = 0; i < TK * NCH / 32; ++i) {
+          const int at = i * 32 + lane, row = at / NCH, c = at % NCH;
+          cp16(dst + place(row, c), row_at(pool, first + row * step, unit) + c * 16, true);
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < TK * NCH / 32; ++i) {
+      const int at = i * 32 + lane, row = EVEN ? i * RS + row0 : at / NCH, c = EVEN ? c0 : at % NCH;
+      const char* p = row_at(pool, __shfl_sync(L3_FULL, off, row), unit);
+      if (row == r.fresh) p = fresh;
+      cp16(EVEN ? to + (x ^ (turn(i * RS) * 16)) + i * 512 : dst + place(row, c), p + c * 16, r.mask >> row & 1);
+    }
+  }
+  // address of the pieces 2 step + second of a matrix row, ks steps on
+  __device__ static __forceinline__ uint32_t matrix_row(uint32_t half, int row, int second, int step) {
+    if constexpr (NCH % 8 == 0 || NCH == 4) return (half + row * NCH * 16 + (second ^ turn(row)) * 16) ^ (step * 32);  // halves begin on whole rows
+    else return half + place(row, step * 2 + second);
+  }
+  __device__ __forceinline__ void load_keys(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int buf, int lane) {
+    copy(a.k.p, a.unit, r.k, a.ku_token, (1 << a.log_page) >= TK, r, f.k, ring + buf * 2 * HALF, lane);
+  }
+  __device__ __forceinline__ void load_values(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int buf, int lane) {
+    copy(a.v.p, a.unit, r.v, a.vu_token, (1 << a.log_page) >= TK, r, f.v, ring + buf * 2 * HALF + HALF, lane);
+  }
+  __device__ __forceinline__ void scores(int buf, int lane) {
+    const int mi = lane >> 3, row = (mi >> 1) * 8 + (lane & 7);
+#pragma unroll
+    for (int n = 0; n < TK / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t h0, h1, l0 = 0u, l1 = 0u;
+      if constexpr (QLO) {
+        const uint4 x = *reinterpret_cast<const uint4*>(&q_word(4 * ks, lane));
+        h0 = x.x; h1 = x.y; l0 = x.z; l1 = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(&q_word(2 * ks, lane));
+        h0 = x.x; h1 = x.y;
+      }
+#pragma unroll
+      for (int u = 0; u < TK / 16; ++u) {
         uint32_t kb[4];
-        ldsm_x4(row + ks * 32, kb);
-        mma16816<T>(s0, qa[ks], kb[0], kb[1]);
-        mma16816<T>(s1, qa[ks], kb[2], kb[3]);
+        ldsm_x4(matrix_row(ring + buf * 2 * HALF, row, mi & 1, ks) + u * 16 * NCH * 16, kb);
+        mma16816<T>(s[2 * u], h0, l0, h1, l1, kb[0], kb[1]);
+        mma16816<T>(s[2 * u + 1], h0, l0, h1, l1, kb[2], kb[3]);
       }
     }
-    const uint32_t mk = mask >> (2 * t);
-    const float v00 = mk & 1 ? (s0[0] + s0[2]) * sc : -INFINITY, v01 = mk & 2 ? (s0[1] + s0[3]) * sc : -INFINITY;
-    const float v10 = mk & 256 ? (s1[0] + s1[2]) * sc : -INFINITY, v11 = mk & 512 ? (s1[1] + s1[3]) * sc : -INFINITY;
-    float mx = fmaxf(fmaxf(v00, v01), fmaxf(v10, v11));
+  }
+  // weights from the scores (first), then the tile's values (second)
+  uint32_t p[TK / 16][4];
+  __device__ __forceinline__ void weigh(uint32_t mask, int lane) {
+    constexpr uint32_t ALL = TK == 32 ? 0xffffffffu : (1u << (TK & 31)) - 1;
+    const int t = lane & 3;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < TK / 8; ++n) {
+      s[n][0] = (s[n][0] + (QLO ? s[n][2] : 0.f)) * sc;
+      s[n][1] = (s[n][1] + (QLO ? s[n][3] : 0.f)) * sc;
+      if (mask != ALL) {
+        if (!(mask >> (n * 8 + 2 * t) & 1)) s[n][0] = -INFINITY;
+        if (!(mask >> (n * 8 + 2 * t + 1) & 1)) s[n][1] = -INFINITY;
+      }
+      mx = fmaxf(mx, fmaxf(s[n][0], s[n][1]));
+    }
     mx = fmaxf(mx, __shfl_xor_sync(L3_FULL, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(L3_FULL, mx, 2));
     const float mn = fmaxf(m, mx), from = mn == -INFINITY ? 0.f : mn;  // no key so far: every weight is 0
@@ -173,21 +291,29 @@ template <typename T, int HD> struct MmaCore {
       for (int n = 0; n < NT; ++n) { o[n][0] *= alpha; o[n][1] *= alpha; o[n][2] *= alpha; o[n][3] *= alpha; }
       m = mn;
     }
-    const float p00 = ex2(v00 - from + BIAS), p01 = ex2(v01 - from + BIAS), p10 = ex2(v10 - from + BIAS), p11 = ex2(v11 - from + BIAS);
-    l += (p00 + p01) + (p10 + p11);
-    uint32_t pa[4];
-    two_parts<T>(p00, p01, pa[0], pa[1]);
-    two_parts<T>(p10, p11, pa[2], pa[3]);
-    {
-      const uint32_t row = ksm + TK * PITCH + ((mi & 1) * 8 + mr) * PITCH + (mi >> 1) * 16;
+#pragma unroll
+    for (int n = 0; n < TK / 8; ++n) {
+      s[n][0] = ex2(s[n][0] - from + BIAS);
+      s[n][1] = ex2(s[n][1] - from + BIAS);
+      l += s[n][0] + s[n][1];
+    }
+#pragma unroll
+    for (int u = 0; u < TK / 16; ++u) {
+      two_parts<T>(s[2 * u][0], s[2 * u][1], p[u][0], p[u][1]);
+      two_parts<T>(s[2 * u + 1][0], s[2 * u + 1][1], p[u][2], p[u][3]);
+    }
+  }
+  __device__ __forceinline__ void add_values(int buf, int lane) {
+    const int mi = lane >> 3, row = (mi & 1) * 8 + (lane & 7);
+#pragma unroll
+    for (int u = 0; u < TK / 16; ++u)
 #pragma unroll
       for (int np = 0; np < KS; ++np) {
         uint32_t vb[4];
-        ldsm_x4_trans(row + np * 32, vb);
-        mma16816<T>(o[2 * np], pa, vb[0], vb[1]);
-        mma16816<T>(o[2 * np + 1], pa, vb[2], vb[3]);
+        ldsm_x4_trans(matrix_row(ring + buf * 2 * HALF + HALF, row, mi >> 1, np) + u * 16 * NCH * 16, vb);
+        mma16816<T>(o[2 * np], p[u][0], p[u][1], p[u][2], p[u][3], vb[0], vb[1]);
+        mma16816<T>(o[2 * np + 1], p[u][0], p[u][1], p[u][2], p[u][3], vb[2], vb[3]);
       }
-    }
   }
   // whole: the result; else the partial of `slot`
   __device__ __forceinline__ void end(const PagedAttnArgs& a, bool whole, int b, int head0, int heads, int slot, int lane) {
@@ -199,7 +325,10 @@ template <typename T, int HD> struct MmaCore {
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       const long long oi = ((long long)b * a.H + head0 + g) * HD;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) store_out2(a, oi + n * 8 + 2 * t, (o[n][0] + o[n][2]) * inv, (o[n][1] + o[n][3]) * inv);
+      for (int n = 0; n < NT; ++n) {
+        const float x[2] = {(o[n][0] + o[n][2]) * inv, (o[n][1] + o[n][3]) * inv};
+        store_out(a, oi + n * 8 + 2 * t, x);
+      }
       if (a.lse && t == 0) a.lse[(long long)b * a.H + head0 + g] = (m - BIAS + log2f(l)) * 0.6931471805599453f;
     } else {
       float* po = a.part_o + ((long long)slot * a.heads_blk + g) * HD;
@@ -214,85 +343,116 @@ template <typename T, int HD> struct MmaCore {
 // --------------------------------------------------------------------------------------------------- fp32 caches: FFMA
 // LPK lanes share a key (DecodeCfg), KPW keys side by side; NREP query heads of an item (a.heads_blk of them real).  m, l and o are
 // kept per lane group and merged over the warp at the end of an item.
-template <int HD, int NREP> struct F32Core {
-  using C = DecodeCfg<HD, float>;
-  static constexpr int ROW = HD * 4, NCH = ROW / 16, PITCH = ROW + 16;
-  static constexpr int TILE = 2 * TK * PITCH;
-  static constexpr int NW = TILE > 14000 ? 2 : 4;                       // at least two tiles per warp in flight
-  static constexpr int EPL = C::EPL, LPK = C::LPK, KPW = C::KPW, PASSES = KPW >= TK ? 1 : TK / KPW;
-  static constexpr int U = PASSES < 16 / NREP ? PASSES : 16 / NREP < 2 ? (PASSES < 2 ? PASSES : 2) : 16 / NREP;
+template <int HD_, int NREP> struct F32Core {
+  using C = DecodeCfg<HD_, float>;
+  static constexpr int HD = HD_, NW = 4, AHEAD = 1;
+  static constexpr size_t SMEM = 0;
+  static constexpr int EPL = C::EPL, LPK = C::LPK, KPW = C::KPW;
+  // keys of a lane in a tile (U of them, TK of a warp): as many as registers hold beside the queries and sums
+  static constexpr int MOST_U = EPL >= 12 || NREP * EPL >= 64 ? 2 : EPL == 8 || NREP >= 4 ? 4 : 8, U = MOST_U * KPW > 32 ? 32 / KPW : MOST_U, TK = U * KPW;
+  static constexpr int NEED = (NREP * EPL <= 16 ? 3 : 2) * NREP * EPL + 2 * U * EPL + U * NREP + 2 * NREP + 48;
+  static constexpr int CTAS = NEED <= 124 ? 4 : NEED <= 164 ? 3 : 2;
   float q[NREP][EPL], o[NREP][EPL], m[NREP], l[NREP];
+  float k[U][EPL], v[U][EPL], s[U][NREP];
 
-  __device__ __forceinline__ void begin(const PagedAttnArgs& a, int b, int head0, int heads, int lane) {
+  __device__ __forceinline__ void memory(uint8_t*, int) {}
+  __device__ __forceinline__ void add_values(int, int) {}
+  static constexpr bool ASK = NREP * EPL <= 16;  // as MmaCore's, where the registers are there
+  float asked[ASK ? NREP : 1][EPL];
+  __device__ __forceinline__ void read_query(const PagedAttnArgs& a, const Cursor& c, int lane, float (&to)[NREP][EPL]) {
     const int sl = lane % LPK;
 #pragma unroll
     for (int r = 0; r < NREP; ++r) {
-      const long long qp = b * a.q_sb + (long long)(head0 + min(r, heads - 1)) * a.q_sh;
+      const float* p = (const float*)a.q + c.b * a.q_sb + (long long)(c.head0(a) + min(r, c.heads(a) - 1)) * a.q_sh;
+      if (a.q_vec) {
 #pragma unroll
-      for (int e = 0; e < EPL; e += 2) {
-        const float2 x = load_q2(a, qp + C::dim(sl, e));
-        q[r][e] = x.x * a.scale;
-        q[r][e + 1] = x.y * a.scale;
+        for (int e = 0; e < EPL; e += 4) {
+          const float4 x = __ldg(reinterpret_cast<const float4*>(p + C::dim(sl, e)));
+          to[r][e] = x.x; to[r][e + 1] = x.y; to[r][e + 2] = x.z; to[r][e + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) to[r][e] = __ldg(p + C::dim(sl, e));
       }
+    }
+  }
+  __device__ __forceinline__ void ask_query(const PagedAttnArgs& a, const Cursor& c, int lane) {
+    if constexpr (ASK) read_query(a, c, lane, asked);
+  }
+  __device__ __forceinline__ void load_query(const PagedAttnArgs& a, const Cursor& c, int lane) {
+    if constexpr (!ASK) read_query(a, c, lane, q);
+#pragma unroll
+    for (int r = 0; r < NREP; ++r)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) q[r][e] = (ASK ? asked[ASK ? r : 0][e] : q[r][e]) * a.scale;
+  }
+  __device__ __forceinline__ void reset(const PagedAttnArgs&) {
+#pragma unroll
+    for (int r = 0; r < NREP; ++r) {
 #pragma unroll
       for (int e = 0; e < EPL; ++e) o[r][e] = 0.f;
       m[r] = -INFINITY;
       l[r] = 0.f;
     }
   }
-  __device__ __forceinline__ void row(uint32_t addr, int sl, float (&v)[EPL]) {
-#pragma unroll
-    for (int c = 0; c < C::CPL; ++c)
-      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(v[4 * c]), "=f"(v[4 * c + 1]), "=f"(v[4 * c + 2]), "=f"(v[4 * c + 3]) : "r"(addr + (c * LPK + sl) * 16));
-  }
-  __device__ __forceinline__ void tile(uint32_t ksm, uint32_t mask, int lane) {
+  __device__ __forceinline__ void load_keys(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int, int lane) {
     const int sub = lane / LPK, sl = lane % LPK;
 #pragma unroll
-    for (int p0 = 0; p0 < PASSES; p0 += U) {
-      float s[U][NREP];
+    for (int u = 0; u < U; ++u) {
+      const char* p = row_at(a.k.p, __shfl_sync(L3_FULL, r.k, u * KPW + sub), a.unit);
+      if (u * KPW + sub == r.fresh) p = f.k;
+      load_row<HD, KV_STREAM>((const float*)p, sl, k[u]);
+    }
+  }
+  __device__ __forceinline__ void load_values(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int, int lane) {
+    const int sub = lane / LPK, sl = lane % LPK;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int key = (p0 + u) * KPW + sub;  // KPW > TK: lane groups beyond the tile have no key
-        float kk[EPL];
-        row(ksm + (key < TK ? key : 0) * PITCH, sl, kk);
-        const bool ok = key < TK && (mask >> key & 1);
+    for (int u = 0; u < U; ++u) {
+      const char* p = row_at(a.v.p, __shfl_sync(L3_FULL, r.v, u * KPW + sub), a.unit);
+      if (u * KPW + sub == r.fresh) p = f.v;
+      load_row<HD, KV_STREAM>((const float*)p, sl, v[u]);
+    }
+  }
+  __device__ __forceinline__ void scores(int, int) {
 #pragma unroll
-        for (int r = 0; r < NREP; ++r) {
-          float d = 0.f;
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) d = fmaf(q[r][e], kk[e], d);
-#pragma unroll
-          for (int off = LPK / 2; off > 0; off >>= 1) d += __shfl_xor_sync(L3_FULL, d, off);
-          s[u][r] = ok ? d : -INFINITY;
-        }
-      }
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < NREP; ++r) {
-        float mx = m[r];
+        float d = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u][r]);
-        const float from = mx == -INFINITY ? 0.f : mx;
-        const float alpha = expf(m[r] - from);
-        l[r] *= alpha;
+        for (int e = 0; e < EPL; ++e) d = fmaf(q[r][e], k[u][e], d);
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) o[r][e] *= alpha;
-        m[r] = mx;
+        for (int off = LPK / 2; off > 0; off >>= 1) d += __shfl_xor_sync(L3_FULL, d, off);
+        s[u][r] = d;
+      }
+  }
+  __device__ __forceinline__ void weigh(uint32_t mask, int lane) {
+    const int sub = lane / LPK;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          s[u][r] = expf(s[u][r] - from);
-          l[r] += s[u][r];
-        }
+    for (int u = 0; u < U; ++u)
+      if (!(mask >> (u * KPW + sub) & 1)) {
+#pragma unroll
+        for (int r = 0; r < NREP; ++r) s[u][r] = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) v[u][e] = 0.f;
       }
 #pragma unroll
+    for (int r = 0; r < NREP; ++r) {
+      float mx = m[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u][r]);
+      const float from = mx == -INFINITY ? 0.f : mx;
+      const float alpha = expf(m[r] - from);
+      l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[r][e] *= alpha;
+      m[r] = mx;
+#pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int key = (p0 + u) * KPW + sub;
-        float vv[EPL];
-        row(ksm + TK * PITCH + (key < TK ? key : 0) * PITCH, sl, vv);
+        const float p = expf(s[u][r] - from);
+        l[r] += p;
 #pragma unroll
-        for (int r = 0; r < NREP; ++r)
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) o[r][e] = key < TK ? fmaf(s[u][r], vv[e], o[r][e]) : o[r][e];
+        for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(p, v[u][e], o[r][e]);
       }
     }
   }
@@ -315,247 +475,289 @@ template <int HD, int NREP> struct F32Core {
 #pragma unroll
     for (int r = 0; r < NREP; ++r) {
       if (r >= heads) break;
-      if (whole) {
-        const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];
-        const long long oi = ((long long)b * a.H + head0 + r) * HD;
+      const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];
+      const long long oi = ((long long)b * a.H + head0 + r) * HD;
+      float* po = a.part_o + ((long long)slot * a.heads_blk + r) * HD;
 #pragma unroll
-        for (int e = 0; e < EPL; e += 2) store_out2(a, oi + C::dim(sl, e), o[r][e] * inv, o[r][e + 1] * inv);
-        if (a.lse && sl == 0) a.lse[(long long)b * a.H + head0 + r] = m[r] + logf(l[r]);
-      } else {
-        float* po = a.part_o + ((long long)slot * a.heads_blk + r) * HD;
-#pragma unroll
-        for (int e = 0; e < EPL; e += 2) *reinterpret_cast<float2*>(po + C::dim(sl, e)) = make_float2(o[r][e], o[r][e + 1]);
-        if (sl == 0) *reinterpret_cast<float2*>(a.part_ml + ((long long)slot * a.heads_blk + r) * 2) = make_float2(m[r], l[r]);
+      for (int e = 0; e < EPL; e += 4) {
+        if (whole) {
+          const float x[4] = {o[r][e] * inv, o[r][e + 1] * inv, o[r][e + 2] * inv, o[r][e + 3] * inv};
+          store_out(a, oi + C::dim(sl, e), x);
+        } else *reinterpret_cast<float4*>(po + C::dim(sl, e)) = make_float4(o[r][e], o[r][e + 1], o[r][e + 2], o[r][e + 3]);
+      }
+      if (sl == 0) {
+        if (!whole) *reinterpret_cast<float2*>(a.part_ml + ((long long)slot * a.heads_blk + r) * 2) = make_float2(m[r], l[r]);
+        else if (a.lse) a.lse[(long long)b * a.H + head0 + r] = m[r] + logf(l[r]);
       }
     }
   }
 };
 
-template <typename Core, typename T, int ST>
-__global__ void __launch_bounds__(Core::NW * 32, CTAS) paged_attn_kernel(const PagedAttnArgs a) {
-  constexpr int NW = Core::NW, HD = Core::ROW / (int)sizeof(T), NCH = Core::NCH, PITCH = Core::PITCH;
-  extern __shared__ __align__(16) uint8_t ring_raw[];
-  __shared__ uint32_t masks[NW][ST];
+template <typename Core, typename T>
+__global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+  constexpr int HD = Core::HD, TK = Core::TK, NW = Core::NW;
+  extern __shared__ __align__(256) uint8_t core_smem[];
+  __shared__ Fresh fresh[NW];
+  __shared__ long long before[NW * 32], of_warp[NW];
   pdl_launch();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int W = gridDim.x * NW, w = warp * gridDim.x + blockIdx.x;  // neighbours in the row of tiles on different SMs
   const int items = a.G * a.blocks;
 
-  // tiles of one item of every sequence, and of all
+  // The row of tiles in units of half a tile, with one more ahead of every item for its query and its result: items * weight_of of a
+  // sequence.  A thread sums a few neighbouring sequences, `before` holds the sums ahead of it.
+  const int share = (a.B + NW * 32 - 1) / (NW * 32);
   long long sum = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int b = b0 + lane;
-    sum += b < a.B ? tiles_of(length_of(a, b)) : 0;
-  }
+  for (int b = threadIdx.x * share; b < min(a.B, ((int)threadIdx.x + 1) * share); ++b) sum += weight_of(tiles_of<TK>(length_of(a, b)));
+  long long run = sum;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(L3_FULL, sum, o);
-  const long long total = sum * items, per = (total + W - 1) / W;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(L3_FULL, run, o);
+    if (lane >= o) run += x;
+  }
+  before[threadIdx.x] = run - sum;
+  if (lane == 31) of_warp[warp] = run;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) total += of_warp[i];
+  total *= items;
+  const int per = max(2, (int)quotient(total + W - 1, W));  // 2: no warp between two of an item's has none of its tiles
   // sequences without tokens
   for (int b = w; b < a.B; b += W) {
     if (length_of(a, b) > 0) continue;
-    for (int i = lane; i < a.H * (HD / 2); i += 32) store_out2(a, (long long)b * a.H * HD + 2 * i, 0.f, 0.f);
+    const float zero[2] = {0.f, 0.f};
+    for (int i = lane; i < a.H * (HD / 2); i += 32) store_out(a, (long long)b * a.H * HD + 2 * i, zero);
     if (a.lse)
       for (int h = lane; h < a.H; h += 32) a.lse[(long long)b * a.H + h] = -INFINITY;
     if (a.by_item)
       for (int i = lane; i < items; i += 32) a.info[(long long)b * items + i] = make_int4(0, 0, 0, 0);
   }
   int4 tail = make_int4(0, 0, 0, 0);  // the item that begins here and goes on in the next warps: first slot, warp, partials, item
-  const long long u0 = per * w;
+  const long long u0 = (long long)per * w;
   if (u0 < total) {
-    const int n = (int)(total - u0 < per ? total - u0 : per);
-    // the sequence that holds tile u0
+    const int stop = (int)(u0 + per < total ? per : total - u0);
+    // the first tile that begins at unit u0 or behind it
     Cursor C{};
+    int pos;  // where it begins, from u0 on
     {
-      long long before = 0;
-      for (int b0 = 0;; b0 += 32) {
-        const int b = b0 + lane, len = b < a.B ? length_of(a, b) : 0, nt = tiles_of(len);
-        long long run = nt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long x = __shfl_up_sync(L3_FULL, run, o);
-          if (lane >= o) run += x;
-        }
-        const uint32_t hit = __ballot_sync(L3_FULL, (before + run) * items > u0);
-        if (hit || b0 + 32 >= a.B) {
-          const int src = hit ? __ffs(hit) - 1 : 31;
-          C.b = b0 + src;
-          C.nt = __shfl_sync(L3_FULL, nt, src);
-          C.len = __shfl_sync(L3_FULL, len, src);
-          const long long at = u0 - (before + __shfl_sync(L3_FULL, run - nt, src)) * items;
-          C.gb = (int)(at / C.nt);
-          C.t = (int)(at - (long long)C.gb * C.nt);
-          break;
-        }
-        before += __shfl_sync(L3_FULL, run, 31);
+      long long ahead = 0;
+      int i = 0;
+      while (i < NW - 1 && (ahead + of_warp[i]) * items <= u0) ahead += of_warp[i++];
+      const uint32_t past = __ballot_sync(L3_FULL, (ahead + before[i * 32 + lane]) * items > u0);
+      const int own = i * 32 + (past ? __ffs(past) - 2 : 31);  // the thread in whose sum tile u0 lies (lane 0's own never lies past it)
+      long long at = u0 - (ahead + before[own]) * items;
+      C.b = own * share;
+      long long weight;
+      for (;;) {
+        C.len = length_of(a, C.b);
+        C.nt = tiles_of<TK>(C.len);
+        weight = weight_of(C.nt);
+        if (at < weight * items) break;
+        at -= weight * items;
+        ++C.b;
       }
+      const int gb = (int)quotient(at, (int)weight);
+      const int in = (int)(at - gb * weight);
+      C.g = gb / a.blocks;
+      C.blk = gb - C.g * a.blocks;
+      C.t = in / 2 - 1;   // tile t begins at unit 1 + 2 t of its item
+      pos = 1 + 2 * (in / 2) - in;
+      if (in / 2 == C.nt) ++pos;  // none of this item's tiles: the next one's first
+      advance<TK>(a, C);
     }
-    const uint32_t ring = smem_u32(ring_raw) + warp * ST * Core::TILE;
-    Cursor L = C;
-    int entry = 0;
-    auto look = [&] {  // the page of this lane's key of the tile that is loaded next
+    Cursor L = C;      // the tile whose rows are looked up next
+    int load_pos = pos;
+    int entry = 0;     // the page of this lane's key there
+    auto look = [&] {
       const int pos = L.t * TK + (lane & (TK - 1));
       entry = L.b < a.B && pos < L.len ? __ldg(a.table + L.b * a.table_stride + (pos >> a.log_page)) : -1;
     };
-    auto load = [&](int stage) {
-      const int pos = L.t * TK + (lane & (TK - 1)), g = L.gb / a.blocks;
+    auto rows = [&](Rows& r) {
+      const int pos = L.t * TK + (lane & (TK - 1)), g = L.g;
       const bool ok = pos < L.len && (unsigned)entry < (unsigned)a.n_pages;
-      const int in = pos & ((1 << a.log_page) - 1);
-      T* kp = (T*)a.k.p + (ok ? entry * a.k.sp + in * a.k.st + g * a.k.sh : 0);
-      T* vp = (T*)a.v.p + (ok ? entry * a.v.sp + in * a.v.st + g * a.v.sh : 0);
-      const uint32_t mask = __ballot_sync(L3_FULL, ok) & 0xffffu;
-      if (lane == 0) masks[warp][stage] = mask;
+      const uint32_t in = pos & ((1 << a.log_page) - 1);
+      r.k = ok ? (uint32_t)entry * a.ku_page + in * a.ku_token + g * a.ku_head : 0u;
+      r.v = ok ? (uint32_t)entry * a.vu_page + in * a.vu_token + g * a.vu_head : 0u;
+      r.mask = __ballot_sync(L3_FULL, ok) & (uint32_t)((1ull << TK) - 1);
+      r.fresh = -1;
       // the tile of the new token, unless that lies behind the table: its row comes from k_new / v_new, and goes to its page
       if (a.k_new && L.t == L.nt - 1 && asked_length(a, L.b) == L.len) {
         const int row = (L.len - 1) & (TK - 1);
-        T* kn = (T*)a.k_new + L.b * a.kn_sb + g * a.kn_sh;
-        T* vn = (T*)a.v_new + L.b * a.vn_sb + g * a.vn_sh;
-        if (mask >> row & 1 && L.gb % a.blocks == 0) {
-          uint4* kd = (uint4*)__shfl_sync(L3_FULL, (unsigned long long)kp, row);
-          uint4* vd = (uint4*)__shfl_sync(L3_FULL, (unsigned long long)vp, row);
+        r.fresh = row;
+        const char* kn = (const char*)((const T*)a.k_new + L.b * a.kn_sb + g * a.kn_sh);
+        const char* vn = (const char*)((const T*)a.v_new + L.b * a.vn_sb + g * a.vn_sh);
+        __syncwarp();
+        if (lane == 0) fresh[warp] = Fresh{kn, vn};
+        __syncwarp();
+        if (r.mask >> row & 1 && L.blk == 0) {
+          uint4* kd = (uint4*)row_at(a.k.p, __shfl_sync(L3_FULL, r.k, row), a.unit);
+          uint4* vd = (uint4*)row_at(a.v.p, __shfl_sync(L3_FULL, r.v, row), a.unit);
+          constexpr int NCH = HD * (int)sizeof(T) / 16;
           for (int c = lane; c < 2 * NCH; c += 32) {
             if (c < NCH) kd[c] = __ldg((const uint4*)kn + c);
             else vd[c - NCH] = __ldg((const uint4*)vn + c - NCH);
           }
         }
-        if ((lane & (TK - 1)) == row) { kp = kn; vp = vn; }
       }
-      const uint32_t dst = ring + stage * Core::TILE;
-#pragma unroll
-      for (int i = 0; i < (TK * NCH + 31) / 32; ++i) {
-        const int idx = i * 32 + lane, r = idx / NCH, c = idx % NCH;
-        const unsigned long long ks = __shfl_sync(L3_FULL, (unsigned long long)kp, r & (TK - 1));
-        const unsigned long long vs = __shfl_sync(L3_FULL, (unsigned long long)vp, r & (TK - 1));
-        if (TK * NCH % 32 == 0 || r < TK) {
-          const bool take = mask >> r & 1;
-          cp16(dst + r * PITCH + c * 16, (const uint4*)ks + c, take);
-          cp16(dst + TK * PITCH + r * PITCH + c * 16, (const uint4*)vs + c, take);
-        }
-      }
-      advance(a, L, items);
+      load_pos += L.t + 1 < L.nt ? 2 : 3;
+      advance<TK>(a, L);
       look();
     };
-    look();
+    Core core;
+    core.memory(core_smem, warp);
+    Rows r;
+    if (pos < stop) {
+      look();
+      core.ask_query(a, C, lane);
+    }
+    uint32_t masks[Core::AHEAD];
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
-      if (i < n) load(i);
+    for (int j = 0; j < Core::AHEAD; ++j) {
+      masks[j] = 0;
+      const bool some = load_pos < stop;
+      if (some) {
+        rows(r);
+        masks[j] = r.mask;
+        core.load_keys(a, r, fresh[warp], j, lane);
+      }
+      cp_commit();
+      if (some) core.load_values(a, r, fresh[warp], j, lane);
       cp_commit();
     }
-    Core core;
-    auto head0 = [&] { return (C.gb / a.blocks) * (a.H / a.G) + (C.gb % a.blocks) * a.heads_blk; };
-    auto heads = [&] { return min(a.heads_blk, a.H / a.G - (C.gb % a.blocks) * a.heads_blk); };
-    core.begin(a, C.b, head0(), heads(), lane);
+    if (pos < stop) core.load_query(a, C, lane);
+    core.reset(a);
     int t0 = C.t;          // first tile of the present item here
     bool first = true;
-    int stage = 0, fill = ST - 1;
-    for (int i = 0; i < n; ++i) {
-      if (i + ST - 1 < n) load(fill);
+    for (int buf = 0; pos < stop; buf = (buf + 1) % Core::AHEAD) {
+      const uint32_t mask = masks[0];
+      const bool more = load_pos < stop, ends = C.t == C.nt - 1;
+      pos += ends ? 3 : 2;
+      const bool goes_on = pos < stop;
+      if (more) rows(r);
+      Cursor next = C;
+      if (goes_on) advance<TK>(a, next);
+      if (ends && goes_on) core.ask_query(a, next, lane);
+#pragma unroll
+      for (int j = 0; j + 1 < Core::AHEAD; ++j) masks[j] = masks[j + 1];
+      masks[Core::AHEAD - 1] = r.mask;
+      cp_wait<2 * Core::AHEAD - 1>();
+      __syncwarp();
+      core.scores(buf, lane);
+      __syncwarp();
+      if (more) core.load_keys(a, r, fresh[warp], buf, lane);
       cp_commit();
-      fill = fill + 1 == ST ? 0 : fill + 1;
-      cp_wait<ST - 1>();
+      core.weigh(mask, lane);
+      cp_wait<2 * Core::AHEAD - 1>();
       __syncwarp();
-      core.tile(ring + stage * Core::TILE, masks[warp][stage], lane);
+      core.add_values(buf, lane);
       __syncwarp();
-      stage = stage + 1 == ST ? 0 : stage + 1;
-      if (C.t == C.nt - 1 || i == n - 1) {
-        const bool starts = t0 == 0, ends = C.t == C.nt - 1;
+      if (more) core.load_values(a, r, fresh[warp], buf, lane);
+      cp_commit();
+      if (ends || !goes_on) {
         const int slot = 2 * w + (first ? 0 : 1);
-        core.end(a, starts && ends, C.b, head0(), heads(), slot, lane);
-        if (starts) {
-          const int parts = ends ? 0 : 1 + (int)((C.nt - 1 - C.t + per - 1) / per);
-          const int4 in = make_int4(slot, w, parts, C.b * items + C.gb);
+        core.end(a, t0 == 0 && ends, C.b, C.head0(a), C.heads(a), slot, lane);
+        if (t0 == 0) {
+          // the item's last tile is 2 (nt - 1 - t) units behind this one's beginning: the warp that it begins in
+          const int parts = ends ? 0 : 1 + (int)quotient(pos - 2 + 2LL * (C.nt - 1 - C.t), per);
+          const int4 in = make_int4(slot, w, parts, C.item(a));
           if (!a.by_item) tail = in;
-          else if (lane == 0) a.info[(long long)C.b * items + C.gb] = in;
+          else if (lane == 0) a.info[C.item(a)] = in;
         }
         first = false;
-        if (i < n - 1) {
-          advance(a, C, items);
-          core.begin(a, C.b, head0(), heads(), lane);
+        if (goes_on) {
+          core.load_query(a, next, lane);
+          core.reset(a);
           t0 = 0;
         }
-      } else ++C.t;
+      }
+      C = next;
     }
   }
   if (!a.by_item && lane == 0) a.info[w] = tail;
 }
 
-// Joins the partials of one item and query head: weights e^(m_p - m) of the partials, then their sum in the order of the keys.
-constexpr int JOIN_T = 128, JOIN_MAX = 2048;
-__global__ void __launch_bounds__(JOIN_T) paged_join_kernel(const PagedAttnArgs a) {
-  __shared__ float wt[JOIN_MAX];
-  __shared__ float red[JOIN_T / 32][2];
+// Joins the partials of one item and query head.  HD / 4 threads have a partial, with running maximum and sum as in the main loop, so that
+// nothing waits for the weights of all; the groups of threads meet in shared memory.
+template <int JOIN_T>
+__global__ void __launch_bounds__(JOIN_T) paged_join_kernel(const __grid_constant__ PagedAttnArgs a) {
   __shared__ float4 acc[JOIN_T];
+  __shared__ float2 ml[JOIN_T];
   pdl_launch();
   pdl_wait();
   const int4 in = a.info[blockIdx.x];
-  const int parts = min(in.z, JOIN_MAX), r = blockIdx.y, tid = threadIdx.x;
+  const int parts = in.z, r = blockIdx.y, tid = threadIdx.x;
   if (parts == 0) return;
-  const int items = a.G * a.blocks, b = in.w / items, gb = in.w % items;
-  if (r >= min(a.heads_blk, a.H / a.G - (gb % a.blocks) * a.heads_blk)) return;
-  auto row = [&](int p) { return (long long)(p == 0 ? in.x : 2 * (in.y + p)) * a.heads_blk + r; };
-  float mx = -INFINITY;
-  for (int p = tid; p < parts; p += JOIN_T) {
-    wt[p] = a.part_ml[row(p) * 2];
-    mx = fmaxf(mx, wt[p]);
-  }
-  mx = warp_max(mx);
-  if ((tid & 31) == 0) red[tid >> 5][0] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < JOIN_T / 32; ++i) mx = fmaxf(mx, red[i][0]);
-  const float from = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f;
-  for (int p = tid; p < parts; p += JOIN_T) {
-    wt[p] = expf(wt[p] - from);
-    l = fmaf(a.part_ml[row(p) * 2 + 1], wt[p], l);
-  }
-  l = warp_sum(l);
-  if ((tid & 31) == 0) red[tid >> 5][1] = l;
-  __syncthreads();
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < JOIN_T / 32; ++i) l += red[i][1];
+  const int items = a.G * a.blocks, b = in.w / items, gb = in.w - b * items, g = gb / a.blocks, blk = gb - g * a.blocks;
+  if (r >= min(a.heads_blk, a.nrep - blk * a.heads_blk)) return;
   const int q4 = a.HD / 4, d = tid % q4, grp = tid / q4, ngrp = JOIN_T / q4;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, l = 0.f;
   if (grp < ngrp) {
-#pragma unroll 4
-    for (int p = grp; p < parts; p += ngrp) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + row(p) * a.HD + 4 * d);
-      const float w = wt[p];
-      o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+    constexpr int U = 4;
+    for (int p0 = grp; p0 < parts; p0 += U * ngrp) {
+      float4 x[U];
+      float2 y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int p = p0 + u * ngrp;
+        const long long row = (long long)(p == 0 ? in.x : 2 * (in.y + p)) * a.heads_blk + r;
+        y[u] = p < parts ? *reinterpret_cast<const float2*>(a.part_ml + row * 2) : make_float2(-INFINITY, 0.f);
+        x[u] = p < parts ? *reinterpret_cast<const float4*>(a.part_o + row * a.HD + 4 * d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float mx = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, y[u].x);
+      const float from = mx == -INFINITY ? 0.f : mx, keep = expf(m - from);
+      m = mx;
+      l *= keep;
+      o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = expf(y[u].x - from);
+        l = fmaf(w, y[u].y, l);
+        o.x = fmaf(w, x[u].x, o.x); o.y = fmaf(w, x[u].y, o.y); o.z = fmaf(w, x[u].z, o.z); o.w = fmaf(w, x[u].w, o.w);
+      }
     }
     acc[tid] = o;
+    if (d == 0) ml[grp] = make_float2(m, l);
   }
   __syncthreads();
   if (grp) return;
-  for (int i = 1; i < ngrp; ++i) {
+  const int used = min(parts, ngrp);
+  float mx = m;
+  for (int i = 1; i < used; ++i) mx = fmaxf(mx, ml[i].x);
+  const float from = mx == -INFINITY ? 0.f : mx;
+  float w = expf(m - from);
+  l *= w;
+  o.x *= w; o.y *= w; o.z *= w; o.w *= w;
+  for (int i = 1; i < used; ++i) {
     const float4 x = acc[i * q4 + d];
-    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+    w = expf(ml[i].x - from);
+    l = fmaf(w, ml[i].y, l);
+    o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const int head = (gb / a.blocks) * (a.H / a.G) + (gb % a.blocks) * a.heads_blk + r;
-  const long long oi = ((long long)b * a.H + head) * a.HD + 4 * d;
-  store_out2(a, oi, o.x * inv, o.y * inv);
-  store_out2(a, oi + 2, o.z * inv, o.w * inv);
+  const int head = g * a.nrep + blk * a.heads_blk + r;
+  const float out[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  store_out(a, ((long long)b * a.H + head) * a.HD + 4 * d, out);
   if (a.lse && d == 0) a.lse[(long long)b * a.H + head] = mx + logf(l);
 }
 
 template <typename Core, typename T>
 cudaError_t launch_core(PagedAttnArgs a, int n_sm, cudaStream_t s) {
-  // as many tiles in flight as two CTAs of an SM have room for; more than eight gain nothing
-  constexpr int NW = Core::NW, room = 110 * 1024 / (NW * Core::TILE), ST = room > 8 ? 8 : room;
-  static_assert(ST >= 2, "");
-  auto kern = paged_attn_kernel<Core, T, ST>;
-  constexpr size_t smem = (size_t)NW * ST * Core::TILE;
-  cudaError_t e = allow_smem(kern, smem);
-  if (e != cudaSuccess) return e;
-  const int W = n_sm * CTAS * NW;
+  const int W = n_sm * Core::CTAS * Core::NW;
   const long long items = (long long)a.B * a.G * a.blocks;
   a.by_item = items <= W;
   a.n_info = (int)(a.by_item ? items : W);
-  if ((e = launch_k(kern, dim3(n_sm * CTAS), dim3(NW * 32), smem, s, a)) != cudaSuccess) return e;
+  cudaError_t e = allow_smem(paged_attn_kernel<Core, T>, Core::SMEM);
+  if (e == cudaSuccess) e = launch_k(paged_attn_kernel<Core, T>, dim3(n_sm * Core::CTAS), dim3(Core::NW * 32), Core::SMEM, s, a);
+  if (e != cudaSuccess) return e;
   g_l3_pdl_next = true;  // the joining launch starts in the tail of the first
-  return launch_k(paged_join_kernel, dim3(a.n_info, a.heads_blk), dim3(JOIN_T), 0, s, a);
+  // few items have many partials each, and leave the SMs room for larger blocks
+  if (a.n_info * a.heads_blk <= 2 * n_sm) return launch_k(paged_join_kernel<512>, dim3(a.n_info, a.heads_blk), dim3(512), 0, s, a);
+  return launch_k(paged_join_kernel<128>, dim3(a.n_info, a.heads_blk), dim3(128), 0, s, a);
 }
 template <int HD> cudaError_t launch_f32(const PagedAttnArgs& a, int n_sm, cudaStream_t s) {
   if (a.heads_blk == 1) return launch_core<F32Core<HD, 1>, float>(a, n_sm, s);
@@ -564,10 +766,34 @@ template <int HD> cudaError_t launch_f32(const PagedAttnArgs& a, int n_sm, cudaS
   else if (a.heads_blk <= 4) return launch_core<F32Core<HD, 4>, float>(a, n_sm, s);
   else return launch_core<F32Core<HD, 8>, float>(a, n_sm, s);
 }
+template <typename T, int HD> cudaError_t launch_mma(const PagedAttnArgs& a, int n_sm, cudaStream_t s) {
+  if (a.q_dtype == L3_DTYPE_F32) return launch_core<MmaCore<T, HD, true>, T>(a, n_sm, s);
+  return launch_core<MmaCore<T, HD, false>, T>(a, n_sm, s);
+}
 template <int HD> cudaError_t launch_hd(const PagedAttnArgs& a, int n_sm, cudaStream_t s) {
   if (a.kv_dtype == L3_DTYPE_F32) return launch_f32<HD>(a, n_sm, s);
-  if (a.kv_dtype == L3_DTYPE_BF16) return launch_core<MmaCore<bf16, HD>, bf16>(a, n_sm, s);
-  return launch_core<MmaCore<__half, HD>, __half>(a, n_sm, s);
+  if (a.kv_dtype == L3_DTYPE_BF16) return launch_mma<bf16, HD>(a, n_sm, s);
+  return launch_mma<__half, HD>(a, n_sm, s);
+}
+// the pools' offsets in units of the largest power of two of bytes (16 at least) that divides every stride: 32 bits of them
+bool set_units(PagedAttnArgs& a) {
+  const int size = a.kv_dtype == L3_DTYPE_F32 ? 4 : 2;
+  unsigned long long bits = 0;
+  for (const PagedPool* p : {&a.k, &a.v}) bits |= (unsigned long long)p->sp | (unsigned long long)p->sh | (unsigned long long)p->st;
+  bits = bits * size | 1ull << 20;
+  int shift = 0;
+  while (!(bits >> shift & 1)) ++shift;
+  a.unit = 1 << shift;
+  uint32_t* to[2][3] = {{&a.ku_page, &a.ku_head, &a.ku_token}, {&a.vu_page, &a.vu_head, &a.vu_token}};
+  for (int i = 0; i < 2; ++i) {
+    const PagedPool& p = i ? a.v : a.k;
+    const unsigned long long last = ((unsigned long long)(a.n_pages - 1) * p.sp + (unsigned long long)(a.G - 1) * p.sh + ((1ull << a.log_page) - 1) * p.st) * size >> shift;
+    if (last >> 32) return false;
+    *to[i][0] = (uint32_t)((unsigned long long)p.sp * size >> shift);
+    *to[i][1] = (uint32_t)((unsigned long long)p.sh * size >> shift);
+    *to[i][2] = (uint32_t)((unsigned long long)p.st * size >> shift);
+  }
+  return true;
 }
 }  // namespace
 
@@ -577,15 +803,19 @@ static int heads_of_item(int H, int G, int HD, int kv_dtype) {
   return H / G < most ? H / G : most;
 }
 size_t paged_attn_workspace(int H, int G, int HD, int n_sm) {
-  const size_t W = (size_t)n_sm * CTAS * MOST_NW;
+  const size_t W = (size_t)n_sm * MOST_WARPS;
   return W * sizeof(int4) + 2 * W * (H / G < HEADS ? H / G : HEADS) * ((size_t)HD + 2) * sizeof(float);
 }
 
+bool paged_attn_fits(PagedAttnArgs a) { return set_units(a); }
 cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s) {
-  const int W = n_sm * CTAS * MOST_NW;
-  if (W > JOIN_MAX) return cudaErrorInvalidConfiguration;
+  const int W = n_sm * MOST_WARPS;
+  set_units(a);
+  const int size = a.q_dtype == L3_DTYPE_F32 ? 4 : 2;
+  a.q_vec = (((uintptr_t)a.q | (uintptr_t)(a.q_sb * size) | (uintptr_t)(a.q_sh * size)) & 15) == 0;
   a.heads_blk = heads_of_item(a.H, a.G, a.HD, a.kv_dtype);
-  a.blocks = (a.H / a.G + a.heads_blk - 1) / a.heads_blk;
+  a.nrep = a.H / a.G;
+  a.blocks = (a.nrep + a.heads_blk - 1) / a.heads_blk;
   a.info = (int4*)a.ws;
   a.part_o = (float*)(a.info + W);
   a.part_ml = a.part_o + (size_t)2 * W * a.heads_blk * a.HD;

@@ -31,13 +31,17 @@ struct PagedAttnArgs {
   float* lse;                        // [B, H] or null
   void* ws;                          // paged_attn_workspace bytes, 16-byte aligned
   // set by the launcher
-  int heads_blk, blocks;             // query heads of a work item, items per kv head
+  int unit;                          // bytes; the pools' strides below are in units of it
+  uint32_t ku_page, ku_head, ku_token, vu_page, vu_head, vu_token;
+  bool q_vec;                        // every query row begins on 16 bytes
+  int nrep, heads_blk, blocks;       // query heads of a kv head, of a work item, items per kv head
   float *part_o, *part_ml;
   int4* info;
   int n_info;
   bool by_item;
 };
 size_t paged_attn_workspace(int H, int G, int HD, int n_sm);
+bool paged_attn_fits(PagedAttnArgs a);  // the pools' offsets fit 32 bits of the largest unit that divides their strides
 cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s);
 
 struct PagedWriteArgs {
