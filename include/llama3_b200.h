@@ -127,6 +127,13 @@ int l3_generate_next(L3Model* m, int64_t* out_B);
  * pos_offset -1.  eos_id >= 0: a sequence that emitted eos_id keeps emitting it. */
 int l3_generate_ragged(L3Model* m, const int32_t* ids, const int32_t* lens, int B, int Lmax, int max_new_tokens,
                        int pos_offset, int eos_id, int64_t* out);
+/* Beam search (the reference decodes greedily only, llama3.py:310-321): the `beams` best continuations of every prompt by the sum of their log
+ * probabilities, decode steps at contiguous positions L, L + 1, ...  A beam that emitted eos_id (-1: none) keeps its score and its place among
+ * the others.  At the end a prompt's beams are sorted by score / length^length_penalty, length counting the tokens up to eos_id.
+ * out_tokens [B, beams, max_new_tokens] (behind a beam's end: eos_id), out_scores and out_lengths [B, beams].  Needs B * beams <=
+ * max_batch_size and L + max_new_tokens - 1 <= max_seq_len; beams <= 64; single-GPU Llama handles. */
+int l3_generate_beam(L3Model* m, const int32_t* ids, int B, int L, int beams, int max_new_tokens, int eos_id, float length_penalty,
+                     int64_t* out_tokens, float* out_scores, int32_t* out_lengths);
 
 
 /* -- layer-list decoders (hybrid stacks) ---------------------------------------------------------------

@@ -509,3 +509,47 @@ cudaError_t launch_beam_select(const BeamSelectArgs& a, int n_sm, cudaStream_t s
   g_l3_pdl_next = true;
   return launch_k(beam_pick_kernel, dim3(a.B), dim3(BT), 0, s, a, c.S, (const RowPart*)part, (const float*)cv, (const int*)ci);
 }
+
+// ------------------------------------------------------------------------------------------------ beam search over a model's own caches
+namespace {
+__global__ void beam_prompts_kernel(const BeamState b, int L) {
+  pdl_launch();
+  pdl_wait();
+  const int r = blockIdx.x;
+  for (int t = threadIdx.x; t < L; t += blockDim.x) b.table[(long long)r * b.M + t] = r / b.K * b.stride + t;
+  if (threadIdx.x == 0) {
+    b.scores[r] = 0.f;
+    b.done[r] = 0;
+  }
+}
+__global__ void beam_begin_kernel(const BeamState b) {
+  pdl_launch();
+  pdl_wait();
+  const int step = b.scal[1] + 1, pos = b.scal[2] + step;
+  for (int r = threadIdx.x; r < b.rows; r += blockDim.x) b.table[(long long)r * b.M + pos] = r * b.stride + pos;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    b.scal[1] = step;
+    b.scal[0] = pos;
+  }
+}
+__global__ void beam_commit_kernel(const BeamState b) {
+  pdl_launch();
+  pdl_wait();
+  const long long step = b.scal[1];
+  for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < b.rows; r += gridDim.x * blockDim.x) {
+    b.scores[r] = b.new_scores[r];
+    b.done[r] = b.new_done[r];
+    b.hist_tokens[step * b.rows + r] = b.tokens[r];
+    b.hist_parents[step * b.rows + r] = b.parents[r];
+  }
+}
+}  // namespace
+
+cudaError_t launch_beam_prompts(const BeamState& b, int L, cudaStream_t s) {
+  return launch_k(beam_prompts_kernel, dim3(b.rows), dim3(128), 0, s, b, L);
+}
+cudaError_t launch_beam_begin(const BeamState& b, cudaStream_t s) { return launch_k(beam_begin_kernel, dim3(1), dim3(256), 0, s, b); }
+cudaError_t launch_beam_commit(const BeamState& b, cudaStream_t s) {
+  return launch_k(beam_commit_kernel, dim3((b.rows + 127) / 128), dim3(128), 0, s, b);
+}

@@ -7,6 +7,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -18,6 +20,7 @@
 #include "layerlist.h"
 #include "mega.h"
 #include "model.h"
+#include "paged.h"
 #include "stack.h"
 
 static thread_local char g_err[512] = "";
@@ -171,6 +174,36 @@ extern "C" int l3_debug_fail_wait(L3Model* m) {
   return L3_OK;
 }
 
+// Beam search (l3_generate_beam): device state for every sequence slot, workspaces for the largest call so far, and one captured step.
+struct L3BeamRun {
+  BeamState s{};
+  int n_sm = 0;
+  void *attn_ws = nullptr, *select_ws = nullptr;
+  size_t select_bytes = 0;
+  int B = 0, K = 0, eos = -1;  // of the captured step
+  bool warmed = false;
+  cudaGraph_t graph = nullptr;
+  cudaGraphExec_t exec = nullptr;
+  int64_t nodes = 0;
+};
+static void beam_drop_graph(L3BeamRun* r) {
+  if (r->exec) cudaGraphExecDestroy(r->exec);
+  if (r->graph) cudaGraphDestroy(r->graph);
+  r->exec = nullptr;
+  r->graph = nullptr;
+  r->warmed = false;
+}
+static void beam_destroy(L3Model* m) {
+  L3BeamRun* r = m->beam;
+  if (!r) return;
+  beam_drop_graph(r);
+  for (void* p : {(void*)r->s.table, (void*)r->s.tokens, (void*)r->s.parents, (void*)r->s.hist_tokens, (void*)r->s.hist_parents, (void*)r->s.scores,
+                  (void*)r->s.new_scores, (void*)r->s.done, (void*)r->s.new_done, r->attn_ws, r->select_ws})
+    if (p) cudaFree(p);
+  delete r;
+  m->beam = nullptr;
+}
+
 extern "C" int l3_destroy(L3Model* m) {
   if (!m) return L3_OK;
   cudaSetDevice(m->cfg.device);
@@ -181,6 +214,7 @@ extern "C" int l3_destroy(L3Model* m) {
     if (g.graph) cudaGraphDestroy(g.graph);
   }
   m->graphs.clear();
+  beam_destroy(m);
   tp_destroy(m);
   ll_destroy(m);
   if (m->logits_loc) cudaFree(m->logits_loc);
@@ -720,12 +754,27 @@ extern "C" int l3_debug_pdl(L3Model* m, int B, int L) {
   return pdl_on(m, pdl_pays(m, B * L, L));
 }
 
+// Attention of one token per row over its ancestors' tokens (BeamState::table): the caches are pools of pages of one token.
+static cudaError_t launch_beam_attention(L3Model* m, const L3BeamRun& r, const AttnArgs& at, int rows) {
+  PagedAttnArgs a{};
+  a.q = at.q; a.q_sb = (long long)m->HN * m->HD; a.q_sh = m->HD; a.q_dtype = L3_DTYPE_F32;
+  a.k = PagedPool{(void*)at.cache_k, m->HD, (long long)m->M * m->HD, 0};
+  a.v = PagedPool{(void*)at.cache_v, m->HD, (long long)m->M * m->HD, 0};
+  a.kv_dtype = m->bf16 ? L3_DTYPE_BF16 : L3_DTYPE_F32;
+  a.n_pages = (m->maxB - 1) * r.s.stride + m->M; a.log_page = 0;
+  a.table = r.s.table; a.table_stride = m->M; a.max_pages = m->M; a.pos_ptr = at.pos_ptr;
+  a.B = rows; a.H = m->HN; a.G = m->KVHN; a.HD = m->HD; a.scale = 1.0f / sqrtf((float)m->HD);
+  a.out = at.out_bf16 ? (void*)at.out_bf16 : at.out; a.out_dtype = at.out_bf16 ? L3_DTYPE_BF16 : L3_DTYPE_F32; a.out_lo = at.out_lo;
+  a.ws = r.attn_ws;
+  return launch_paged_attention(a, r.n_sm, m->stream);
+}
+
 // Enqueue one chunk: tokens ids[b * ids_ld + ids_off + t], t < L, at start_pos = *d_pos.
 // Layer-list handles: d_rows / n_rows choose the rows whose logits are wanted (null: the last token of every sequence),
 // d_resid (may be null) receives the residual stream after every layer.
 static int enqueue_chunk(L3Model* m, const int32_t* d_ids, int ids_ld, int ids_off, int B, int L, bool want_logits,
                          bool want_argmax, OutSpec os, const Ragged* rg = nullptr, const int32_t* d_rows = nullptr,
-                         int n_rows = 0, float* d_resid = nullptr) {
+                         int n_rows = 0, float* d_resid = nullptr, const L3BeamRun* beam = nullptr) {
   const int ntok = B * L, D = m->D, HD = m->HD;
   PdlScope pdl(m, pdl_pays(m, ntok, L));
   if (m->ll) {
@@ -743,7 +792,7 @@ static int enqueue_chunk(L3Model* m, const int32_t* d_ids, int ids_ld, int ids_o
   const bool tc_rows = m->tc_ok && !linear_rows_supported(ntok, D);
   const bool tc_h = m->tc_ok && !linear_rows_supported(ntok, m->FD);
   const bool tc_ctx = m->tc_ok && !linear_rows_supported(ntok, m->HN * HD);
-  const bool in_cluster = L == 1 && !rg && B <= m->cl_maxB;
+  const bool in_cluster = L == 1 && !rg && !beam && B <= m->cl_maxB;
   int rc;
   if (in_cluster) {
     if ((rc = enqueue_cluster_layers(m, d_ids, ids_ld, ids_off, B)) != L3_OK) return rc;
@@ -772,7 +821,10 @@ static int enqueue_chunk(L3Model* m, const int32_t* d_ids, int ids_ld, int ids_o
     at.part_o = m->part_o; at.part_ml = m->part_ml; at.counters = m->attn_cnt;
     if (tc_ctx && m->bf16) at.out_bf16 = (bf16*)m->ctx16;
     else { at.out = m->ctx; at.out_lo = tc_ctx ? m->ctx_lo : nullptr; }
-    if (L == 1) {
+    if (beam) {  // one token a row, over the tokens that its table names
+      LAUNCH(m, launch_beam_attention(m, *beam, at, B));
+      m->launch_acc += 1;  // two launches
+    } else if (L == 1) {
       at.nsplit = pick_nsplit(m, B);
       LAUNCH(m, launch_attn_decode(at, m->bf16, m->stream));
     } else if (attn_tc) {
@@ -1221,6 +1273,188 @@ extern "C" int l3_generate_next(L3Model* m, int64_t* out_B) {
   CK(m, cudaStreamSynchronize(m->stream));
   for (int b = 0; b < m->gen_B; ++b) out_B[b] = m->h_next[b];
   return check_waits(m);
+}
+
+// ------------------------------------------------------------------------------ beam search
+// No counterpart in the reference (greedy only, llama3.py:310-321).  A prompt is read once, into its own slot; row r = b K + j is beam j of
+// prompt b and writes its tokens into slot r.  The caches stay where they are: what a beam descends from is a table of tokens, and a step
+// moves rows of that table in place of rows of the caches.
+static int beam_setup(L3Model* m, int B, int K) {
+  if (!m->beam) m->beam = new (std::nothrow) L3BeamRun();
+  L3BeamRun* r = m->beam;
+  if (!r) { set_err(m, "out of host memory"); return L3_ENOMEM; }
+  BeamState& s = r->s;
+  if (!r->attn_ws) {
+    CK(m, cudaDeviceGetAttribute(&r->n_sm, cudaDevAttrMultiProcessorCount, m->cfg.device));
+    const size_t n = m->maxB, all = n * m->M;
+    auto get = [](auto** p, size_t count) { return *p ? cudaSuccess : cudaMalloc((void**)p, count * sizeof(**p)); };
+    cudaError_t e;
+    if ((e = get(&s.table, all)) != cudaSuccess || (e = get(&s.hist_tokens, all)) != cudaSuccess || (e = get(&s.hist_parents, all)) != cudaSuccess ||
+        (e = get(&s.tokens, n)) != cudaSuccess || (e = get(&s.parents, n)) != cudaSuccess || (e = get(&s.scores, n)) != cudaSuccess ||
+        (e = get(&s.new_scores, n)) != cudaSuccess || (e = get(&s.done, n)) != cudaSuccess || (e = get(&s.new_done, n)) != cudaSuccess ||
+        (e = cudaMalloc(&r->attn_ws, paged_attn_workspace(m->HN, m->KVHN, m->HD, r->n_sm))) != cudaSuccess) {
+      cudaGetLastError();
+      set_err(m, "beam search: no room for its state: %s", cudaGetErrorString(e));
+      return L3_ENOMEM;
+    }
+  }
+  const size_t need = std::max(beam_select_workspace(B, 1, m->VS, K, r->n_sm), beam_select_workspace(B, K, m->VS, K, r->n_sm));
+  if (need > r->select_bytes) {
+    beam_drop_graph(r);  // holds the old one's address
+    if (r->select_ws) cudaFree(r->select_ws);
+    r->select_ws = nullptr;
+    r->select_bytes = 0;
+    if (cudaMalloc(&r->select_ws, need) != cudaSuccess) {
+      cudaGetLastError();
+      set_err(m, "beam search: no room for a workspace of %zu bytes", need);
+      return L3_ENOMEM;
+    }
+    r->select_bytes = need;
+  }
+  s.scal = m->d_scal;
+  s.rows = B * K; s.K = K; s.M = m->M; s.stride = m->KVHN * m->M;
+  return L3_OK;
+}
+
+// The K best continuations of every prompt (first) or of its beams, from m->logits into the state.
+static int beam_choose(L3Model* m, int B, bool first, int eos) {
+  L3BeamRun* r = m->beam;
+  const int beams = first ? 1 : r->s.K;
+  BeamSelectArgs a{};
+  a.logits = m->logits; a.sb = (long long)beams * m->VS; a.sk = m->VS; a.dtype = L3_DTYPE_F32;
+  a.scores = r->s.scores; a.done = !first && eos >= 0 ? r->s.done : nullptr; a.eos = eos;
+  a.B = B; a.K = beams; a.V = m->VS; a.n = r->s.K;
+  a.out_scores = r->s.new_scores; a.out_tokens = r->s.tokens; a.out_parents = r->s.parents; a.out_done = r->s.new_done; a.ws = r->select_ws;
+  LAUNCH(m, launch_beam_select(a, r->n_sm, m->stream));
+  m->launch_acc += 1;  // two launches
+  LAUNCH(m, launch_beam_commit(r->s, m->stream));
+  return L3_OK;
+}
+
+static int beam_step_nodes(L3Model* m, int B, int eos) {
+  L3BeamRun* r = m->beam;
+  int rc;
+  LAUNCH(m, launch_beam_begin(r->s, m->stream));
+  if ((rc = enqueue_chunk(m, r->s.tokens, 1, 0, r->s.rows, 1, true, false, OutSpec{m->d_fwd_arg, 1, m->d_scal + 3, m->d_fwd_next}, nullptr, nullptr, 0,
+                          nullptr, r)) != L3_OK) return rc;
+  if ((rc = beam_choose(m, B, false, eos)) != L3_OK) return rc;
+  RowsList l{};
+  l.t[0] = RowsDesc{(char*)r->s.table, (long long)m->M * 4, 0, 1, (unsigned)(m->M % 4 ? m->M : m->M / 4)};
+  LAUNCH(m, launch_reorder_rows(l, 1, r->s.parents, B, r->s.K, m->M % 4 ? 4 : 16, m->stream));
+  return L3_OK;
+}
+
+static int beam_step(L3Model* m, int B, int eos) {
+  L3BeamRun* r = m->beam;
+  if (r->B != B || r->K != r->s.K || r->eos != eos) beam_drop_graph(r);
+  r->B = B; r->K = r->s.K; r->eos = eos;
+  if (r->exec) {
+    CK(m, cudaGraphLaunch(r->exec, m->stream));
+    m->launch_acc += r->nodes;
+    return L3_OK;
+  }
+  if ((m->cfg.flags & L3_FLAG_NO_GRAPH) || !r->warmed) {  // first step runs eagerly (sets function attributes, validates the launches)
+    r->warmed = true;
+    return beam_step_nodes(m, B, eos);
+  }
+  const int64_t before = m->launch_acc;
+  CK(m, cudaStreamBeginCapture(m->stream, cudaStreamCaptureModeThreadLocal));
+  const int rc = beam_step_nodes(m, B, eos);
+  const cudaError_t e = cudaStreamEndCapture(m->stream, &r->graph);
+  r->nodes = m->launch_acc - before;
+  m->launch_acc = before;
+  if (rc != L3_OK) return rc;
+  CK(m, e);
+  CK(m, cudaGraphInstantiate(&r->exec, r->graph, 0));
+  CK(m, cudaGraphLaunch(r->exec, m->stream));
+  m->launch_acc += r->nodes;
+  return L3_OK;
+}
+
+static int generate_beam(L3Model* m, const int32_t* ids, int B, int L, int beams, int max_new_tokens, int eos_id, float length_penalty,
+                         int64_t* out_tokens, float* out_scores, int32_t* out_lengths) {
+  int rc = check_call(m, B, L, 0);
+  if (rc != L3_OK) return rc;
+  REQUIRE(m, !m->ll, "beam search is not built for layer-list handles: a recurrent state has no table to share");
+  REQUIRE(m, m->G == 1, "beam search is not built for tensor parallel handles");
+  REQUIRE(m, ids && out_tokens && out_scores && out_lengths, "a buffer is missing");
+  REQUIRE(m, beams >= 1 && beams <= BEAM_MAX_N, "beams %d: 1 to %d are supported", beams, BEAM_MAX_N);
+  REQUIRE(m, (int64_t)B * beams <= m->maxB, "%d prompts of %d beams exceed max_batch_size %d", B, beams, m->maxB);
+  REQUIRE(m, (int64_t)m->maxB * m->KVHN * m->M < ((int64_t)1 << 31), "caches of %d x %d x %d tokens are too large for beam search", m->maxB, m->KVHN, m->M);
+  REQUIRE(m, m->VS < (1 << 24) && beams <= m->VS && (int64_t)beams * m->VS < ((int64_t)1 << 31), "vocabulary of %d", m->VS);
+  REQUIRE(m, max_new_tokens >= 1 && L + max_new_tokens - 1 <= m->M, "prompt %d + %d new tokens exceed max_seq_len %d", L, max_new_tokens, m->M);
+  REQUIRE(m, eos_id < m->VS, "eos_id %d is not in the vocabulary", eos_id);
+  REQUIRE(m, length_penalty == length_penalty && length_penalty >= 0.f, "length_penalty must not be negative");
+  for (int i = 0; i < B * L; ++i)
+    REQUIRE(m, ids[i] >= 0 && ids[i] < m->cfg.vocab_size, "token id %d out of range at %d", ids[i], i);
+  CK(m, cudaSetDevice(m->cfg.device));
+  const int eos = eos_id < 0 ? -1 : eos_id, rows = B * beams;
+  if ((rc = beam_setup(m, B, beams)) != L3_OK) return rc;
+  L3BeamRun* r = m->beam;
+  m->gen_B = m->pend_B = 0;  // a generate loop under way would read what this call writes
+  CK(m, cudaMemcpyAsync(m->d_ids, ids, (size_t)B * L * 4, cudaMemcpyHostToDevice, m->stream));
+  const int h[4] = {0, 0, L - 1, 0};
+  CK(m, cudaMemcpyAsync(m->d_scal, h, sizeof h, cudaMemcpyHostToDevice, m->stream));
+  if ((rc = enqueue_prefill(m, m->d_ids, B, L, 0, true, false, OutSpec{m->d_fwd_arg, 1, m->d_scal + 3, m->d_fwd_next})) != L3_OK) return rc;
+  LAUNCH(m, launch_beam_prompts(r->s, L, m->stream));
+  if ((rc = beam_choose(m, B, true, eos)) != L3_OK) return rc;
+  std::vector<uint8_t> done(rows);
+  int steps = 1;
+  while (steps < max_new_tokens) {
+    if (eos >= 0 && steps % 8 == 0) {  // now and then: have all beams ended?
+      CK(m, cudaMemcpyAsync(done.data(), r->s.done, rows, cudaMemcpyDeviceToHost, m->stream));
+      CK(m, cudaStreamSynchronize(m->stream));
+      if (std::all_of(done.begin(), done.end(), [](uint8_t d) { return d != 0; })) break;
+    }
+    if ((rc = beam_step(m, B, eos)) != L3_OK) return rc;
+    ++steps;
+  }
+  std::vector<int32_t> tok((size_t)steps * rows), par((size_t)steps * rows);
+  std::vector<float> score(rows);
+  CK(m, cudaMemcpyAsync(tok.data(), r->s.hist_tokens, tok.size() * 4, cudaMemcpyDeviceToHost, m->stream));
+  CK(m, cudaMemcpyAsync(par.data(), r->s.hist_parents, par.size() * 4, cudaMemcpyDeviceToHost, m->stream));
+  CK(m, cudaMemcpyAsync(score.data(), r->s.scores, (size_t)rows * 4, cudaMemcpyDeviceToHost, m->stream));
+  CK(m, cudaStreamSynchronize(m->stream));
+  if ((rc = check_waits(m)) != L3_OK) return rc;
+  // every beam's tokens, from its last one back; then the prompt's beams by score / length^length_penalty
+  std::vector<int64_t> seq((size_t)rows * steps);
+  std::vector<int> len(rows), order(beams);
+  std::vector<double> value(rows);
+  for (int x = 0; x < rows; ++x) {
+    const int b = x / beams;
+    int at = x;
+    for (int s = steps - 1; s >= 0; --s) {
+      seq[(size_t)x * steps + s] = tok[(size_t)s * rows + at];
+      at = b * beams + par[(size_t)s * rows + at];
+    }
+    len[x] = steps;
+    if (eos >= 0)
+      for (int s = 0; s < steps; ++s)
+        if (seq[(size_t)x * steps + s] == eos) { len[x] = s + 1; break; }
+    value[x] = (double)score[x] / pow((double)len[x], (double)length_penalty);
+  }
+  for (int b = 0; b < B; ++b) {
+    for (int j = 0; j < beams; ++j) order[j] = b * beams + j;
+    std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return value[x] > value[y]; });
+    for (int j = 0; j < beams; ++j) {
+      const size_t o = (size_t)b * beams + j;
+      for (int s = 0; s < max_new_tokens; ++s)
+        out_tokens[o * max_new_tokens + s] = s < len[order[j]] ? seq[(size_t)order[j] * steps + s] : std::max(eos, 0);
+      out_scores[o] = (float)value[order[j]];
+      out_lengths[o] = len[order[j]];
+    }
+  }
+  return L3_OK;
+}
+
+extern "C" int l3_generate_beam(L3Model* m, const int32_t* ids, int B, int L, int beams, int max_new_tokens, int eos_id, float length_penalty,
+                                int64_t* out_tokens, float* out_scores, int32_t* out_lengths) {
+  try {
+    return generate_beam(m, ids, B, L, beams, max_new_tokens, eos_id, length_penalty, out_tokens, out_scores, out_lengths);
+  } catch (const std::bad_alloc&) {
+    set_err(m, "out of host memory");
+    return L3_ENOMEM;
+  }
 }
 
 // ------------------------------------------------------------------------------ measurement helpers

@@ -34,6 +34,8 @@ struct L3Graph {
 
 struct LayerList;  // layerlist.h: the layers, state and workspace of a layer-list decoder
 
+struct L3BeamRun;  // l3_api.cu: what l3_generate_beam keeps on the device
+
 int l3_pdl_env();  // l3_api.cu
 struct L3Model {
   L3Config cfg{};
@@ -105,6 +107,7 @@ struct L3Model {
   std::vector<float*> stack_wpack;
   float* d_stack_dbgx = nullptr;              // L3_STACK_DBG=1: [NL][maxB][D] residual stream after every layer
   unsigned long long* d_stack_dbg = nullptr;  // L3_STACK_DBG=1: [grid][64] timeline stamps of the last step
+  L3BeamRun* beam = nullptr;
   // tensor parallel (comm.cu)
   L3Comm* comm = nullptr;
   float* logits_loc = nullptr;   // [maxB, VS] local vocabulary slice (G > 1)

@@ -86,3 +86,16 @@ struct BeamSelectArgs {
 constexpr int BEAM_MAX_K = 256, BEAM_MAX_N = 64;
 size_t beam_select_workspace(int B, int K, int V, int n, int n_sm);
 cudaError_t launch_beam_select(const BeamSelectArgs& a, int n_sm, cudaStream_t s);
+
+// Beam search over a model's own caches (l3_generate_beam): rows of B prompts' K beams, tokens in pages of one.  Slot r's row of a cache holds
+// the tokens that row r wrote; table [rows, M] names, for every row and position, the token it descends from (slot * stride + position).
+struct BeamState {
+  int *table, *tokens, *parents, *hist_tokens, *hist_parents;  // [rows, M], [rows], [rows], [M, rows] twice
+  float *scores, *new_scores;                                   // [rows]
+  unsigned char *done, *new_done;
+  int* scal;                                                    // the handle's step scalars: [0] position [1] step [2] position of step 0
+  int rows, K, M, stride;                                       // stride: tokens of a slot in a pool, kv heads * M
+};
+cudaError_t launch_beam_prompts(const BeamState& b, int L, cudaStream_t s);  // every beam descends from its prompt; scores and flags start at 0
+cudaError_t launch_beam_begin(const BeamState& b, cudaStream_t s);           // the next step's position, its token the row's own
+cudaError_t launch_beam_commit(const BeamState& b, cudaStream_t s);          // the selection becomes the state, and goes into the history

@@ -9,7 +9,7 @@ namespace {
 // ------------------------------------------------------------------------------------------------ new tokens into pages
 // A token is 2 G HD values, `per` pieces of 16 bytes; a CTA takes TOK tokens of one sequence, a thread the same piece of several.
 constexpr int WT = 256, TOK = 8;
-__global__ void __launch_bounds__(WT) paged_write_kernel(const PagedWriteArgs a) {
+__global__ void __launch_bounds__(WT, 4) paged_write_kernel(const PagedWriteArgs a) {
   pdl_launch();
   pdl_wait();
   const int b = blockIdx.y, per = 2 * a.G * a.pieces;
@@ -24,22 +24,28 @@ __global__ void __launch_bounds__(WT) paged_write_kernel(const PagedWriteArgs a)
     const char* src = half ? (const char*)a.v + b * a.v_sb + g * a.v_sh : (const char*)a.k + b * a.k_sb + g * a.k_sh;
     const long long st = half ? a.v_st : a.k_st;
     const PagedPool& p = half ? a.vp : a.kp;
-    uint4 x[TOK];
-    int page[TOK];
+    src += piece * 16;
+    char* const to = (char*)p.p + g * p.sh + piece * 16;
+    const int* row = a.table + b * a.table_stride;
+    const int cap = a.max_pages << a.log_page;
 #pragma unroll
-    for (int i = 0; i < TOK; ++i) {
-      const int t = t0 + i * side;
-      const long long pos = (long long)start + t;
-      const bool ok = t < n && pos >= 0 && pos < (long long)a.max_pages << a.log_page;
-      page[i] = ok ? __ldg(a.table + b * a.table_stride + (pos >> a.log_page)) : -1;
-      if (ok) x[i] = ldg_stream16(src + t * st + piece * 16);
-    }
+    for (int i0 = 0; i0 < TOK; i0 += 4) {
+      uint4 x[4];
+      int page[4];
 #pragma unroll
-    for (int i = 0; i < TOK; ++i) {
-      if ((unsigned)page[i] >= (unsigned)a.n_pages) continue;
-      const long long pos = (long long)start + t0 + i * side;
-      char* d = (char*)p.p + page[i] * p.sp + g * p.sh + (pos & ((1 << a.log_page) - 1)) * p.st;
-      *reinterpret_cast<uint4*>(d + piece * 16) = x[i];
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + (i0 + i) * side;
+        const unsigned pos = (unsigned)start + t;  // a start near 2^31, or below 0, lies behind the table
+        const bool ok = t < n && pos < (unsigned)cap;
+        page[i] = ok ? __ldg(row + (pos >> a.log_page)) : -1;
+        if (ok) x[i] = ldg_stream16(src + t * st);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if ((unsigned)page[i] >= (unsigned)a.n_pages) continue;
+        const unsigned pos = (unsigned)start + t0 + (i0 + i) * side;
+        *reinterpret_cast<uint4*>(to + page[i] * p.sp + (pos & ((1u << a.log_page) - 1)) * p.st) = x[i];
+      }
     }
   }
 }
@@ -100,38 +106,70 @@ __global__ void __launch_bounds__(CT) copy_rows_kernel(const __grid_constant__ R
     if (to[i]) *reinterpret_cast<V*>(to[i]) = x[i];
 }
 
-// A thread has the same piece of all K rows of a group: it reads every row that another one wants into its own column of shared
+// A thread has the same pieces of all K rows of a group: it copies those of every row that another one wants into its own places in shared
 // memory and then writes the rows that change, so that any permutation works in place without a barrier and without a copy elsewhere.
+// RU pieces a turn, asynchronously, the next turn's on their way while one is written, keep enough bytes moving.
+template <typename V> __device__ __forceinline__ void fetch(V* to, const char* from) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (sizeof(V) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(from) : "memory");
+  else if constexpr (sizeof(V) >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(from), "n"((int)sizeof(V)) : "memory");
+  else *to = *reinterpret_cast<const V*>(from);
+}
 template <typename V>
-__global__ void reorder_rows_kernel(const __grid_constant__ RowsList l, const __grid_constant__ CopyDivs dv, const int* parents, int B, int K) {
-  extern __shared__ __align__(16) uint8_t cols_raw[];
-  V* col = reinterpret_cast<V*>(cols_raw) + threadIdx.x;  // [K][blockDim.x]
-  __shared__ short from[ROWS_BEAMS];      // a row's parent, itself where it stays
+__global__ void reorder_rows_kernel(const __grid_constant__ RowsList l, const __grid_constant__ CopyDivs dv, const int* parents, int B, int K, int RU, int turns) {
+  extern __shared__ __align__(16) uint8_t places_raw[];
+  V* mine = reinterpret_cast<V*>(places_raw) + threadIdx.x;  // [2][RU][K][blockDim.x] (one turn: [RU]...)
   __shared__ unsigned char wanted[ROWS_BEAMS];
+  __shared__ short need[ROWS_BEAMS], to[ROWS_BEAMS], from[ROWS_BEAMS];
+  __shared__ int needs, moves;
   pdl_launch();
   pdl_wait();
   const RowsDesc& d = l.t[blockIdx.z];
-  const unsigned per = d.outer * d.run;
-  if (blockIdx.x * blockDim.x >= per) return;
+  const unsigned per = d.outer * d.run, step = blockDim.x * RU;
+  if (blockIdx.x * step * turns >= per) return;
   const int b = blockIdx.y;
+  if (threadIdx.x == 0) needs = moves = 0;
+  for (int j = threadIdx.x; j < K; j += blockDim.x) wanted[j] = 0;
+  __syncthreads();
   for (int j = threadIdx.x; j < K; j += blockDim.x) {
     const int p = parents[(long long)b * K + j];
-    from[j] = (short)((unsigned)p < (unsigned)K ? p : j);
-    wanted[j] = 0;
+    if ((unsigned)p >= (unsigned)K || p == j) continue;  // the row stays
+    const int m = atomicAdd(&moves, 1);
+    to[m] = (short)j;
+    from[m] = (short)p;
+    wanted[p] = 1;
   }
   __syncthreads();
   for (int j = threadIdx.x; j < K; j += blockDim.x)
-    if (from[j] != j) wanted[from[j]] = 1;
+    if (wanted[j]) need[atomicAdd(&needs, 1)] = (short)j;
   __syncthreads();
-  for (unsigned at = blockIdx.x * blockDim.x + threadIdx.x; at < per; at += gridDim.x * blockDim.x) {
+  const int nn = needs, nm = moves;
+  auto piece = [&](unsigned at) {
     const unsigned o = divide(at, dv.run[blockIdx.z]), c = at - o * d.run;
-    char* p = d.base + (long long)b * K * d.row_stride + o * d.outer_stride + (long long)c * (int)sizeof(V);
+    return d.base + (long long)b * K * d.row_stride + o * d.outer_stride + (long long)c * (int)sizeof(V);
+  };
+  const unsigned base = blockIdx.x * step * turns + threadIdx.x;
+  auto get = [&](int t) {
+    if (t < turns)
+      for (int u = 0; u < RU; ++u) {
+        const unsigned at = base + t * step + u * blockDim.x;
+        if (at >= per) break;
+        const char* p = piece(at);
+        for (int i = 0; i < nn; ++i) fetch(mine + (((t & 1) * RU + u) * K + need[i]) * blockDim.x, p + need[i] * d.row_stride);
+      }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  get(0);
+  for (int t = 0; t < turns; ++t) {
+    get(t + 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    for (int u = 0; u < RU; ++u) {
+      const unsigned at = base + t * step + u * blockDim.x;
+      if (at >= per) break;
+      char* p = piece(at);
 #pragma unroll 4
-    for (int j = 0; j < K; ++j)
-      if (wanted[j]) col[j * blockDim.x] = Piece<V>::load(p + j * d.row_stride);
-#pragma unroll 4
-    for (int j = 0; j < K; ++j)
-      if (from[j] != j) *reinterpret_cast<V*>(p + j * d.row_stride) = col[from[j] * blockDim.x];
+      for (int i = 0; i < nm; ++i) *reinterpret_cast<V*>(p + to[i] * d.row_stride) = mine[(((t & 1) * RU + u) * K + from[i]) * blockDim.x];
+    }
   }
 }
 
@@ -157,17 +195,24 @@ cudaError_t copy_rows(const RowsList& l, int n_tensors, const int* src, const in
 }
 template <typename V>
 cudaError_t reorder_rows(const RowsList& l, int n_tensors, const int* parents, int B, int K, cudaStream_t s) {
-  // threads of a CTA: as many columns as 48 KB hold
-  const int fit = 48 * 1024 / (K * (int)sizeof(V));
-  const int threads = fit >= 256 ? 256 : fit >= 128 ? 128 : fit >= 64 ? 64 : 32;
-  const size_t smem = (size_t)threads * K * sizeof(V);
+  // a thread's places: K for each of its pieces, of which 32 KB of a CTA and turn hold up to four
+  const int fit = 32 * 1024 / (K * (int)sizeof(V)), threads = fit >= 256 ? 256 : fit >= 128 ? 128 : fit >= 64 ? 64 : 32;
+  long long all = 0;
   unsigned most = 0;
-  for (int i = 0; i < n_tensors; ++i) most = l.t[i].outer * l.t[i].run > most ? l.t[i].outer * l.t[i].run : most;
-  const unsigned blocks = (most + threads - 1) / threads;
+  for (int i = 0; i < n_tensors; ++i) {
+    most = l.t[i].outer * l.t[i].run > most ? l.t[i].outer * l.t[i].run : most;
+    all += (long long)l.t[i].outer * l.t[i].run * B;
+  }
+  int RU = fit / threads > 4 ? 4 : fit / threads < 1 ? 1 : fit / threads, turns = 8;
+  while (turns > 1 && all < 1024LL * threads * RU * turns) turns /= 2;  // as long as that leaves every SM some CTAs
+  while (RU > 1 && all < 1024LL * threads * RU) RU /= 2;
+  if (fit < 32) turns = 1;  // places of one turn already take up to 128 KB
+  const size_t smem = (size_t)threads * K * RU * sizeof(V) * (turns > 1 ? 2 : 1);
+  const unsigned blocks = (unsigned)(((long long)most + (long long)threads * RU * turns - 1) / ((long long)threads * RU * turns));
   if (!blocks) return cudaSuccess;
   cudaError_t e = allow_smem(reorder_rows_kernel<V>, smem);
   if (e != cudaSuccess) return e;
-  return launch_k(reorder_rows_kernel<V>, dim3(blocks, B, n_tensors), dim3(threads), smem, s, l, divs_of(l, n_tensors), parents, B, K);
+  return launch_k(reorder_rows_kernel<V>, dim3(blocks, B, n_tensors), dim3(threads), smem, s, l, divs_of(l, n_tensors), parents, B, K, RU, turns);
 }
 }  // namespace
 

@@ -236,6 +236,24 @@ class Llama:
             res.append(row.copy())
         return res
 
+    def generate_beam(self, input_ids, beams: int, max_new_tokens: int, eos_id: Optional[int] = None, length_penalty: float = 0.0):
+        """Extension (the reference decodes greedily only, llama3.py:320): beam search, on the device from the prompt to the last token.
+        `max_new_tokens` counts new tokens; decode steps run at contiguous positions L, L + 1, ... (the schedule of llama3_simple.py).
+        Returns `(tokens, scores, lengths)`: `[B, beams, max_new_tokens]` int64, best beam first, `eos_id` behind a beam's end;
+        `[B, beams]` float32, the sum of its tokens' log probabilities over `length ** length_penalty`; `[B, beams]` int32, its tokens up
+        to and with `eos_id`.  Needs `B * beams <= max_batch_size`; a prompt is read once, and beams share its cache."""
+        ids = self._ids(input_ids)
+        B, L = ids.shape
+        shape = (B, max(int(beams), 0))
+        tokens = np.empty(shape + (max(int(max_new_tokens), 0),), dtype=np.int64)
+        scores, lengths = np.empty(shape, dtype=np.float32), np.empty(shape, dtype=np.int32)
+        if eos_id is not None and int(eos_id) < 0:
+            raise ValueError(f"eos_id {eos_id} is not in the vocabulary")
+        _cabi.check(self._lib.l3_generate_beam(self._h, _cabi.i32p(ids), B, L, int(beams), int(max_new_tokens),
+                                               -1 if eos_id is None else int(eos_id), float(length_penalty), _cabi.i64p(tokens),
+                                               _cabi.f32p(scores), _cabi.i32p(lengths)), self._h)
+        return tokens, scores, lengths
+
     # ---------------------------------------------------------------- state inspection
     def read_cache(self, layer: int):
         """(cache_k, cache_v) of a layer in the reference layout `[max_batch, M, KVHN, HD]`."""
