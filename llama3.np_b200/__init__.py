@@ -37,7 +37,7 @@ def __getattr__(name):  # lazy: importing the package must not require the built
     if name in ("StackDecoder", "StackConfig", "LayerSpec"):
         from . import stack as _s
         return getattr(_s, name)
-    if name in ("paged_attention", "paged_write", "copy_pages", "PagedCache"):
+    if name in ("paged_attention", "paged_write", "copy_pages", "PagedCache", "PageTable"):
         from . import paged as _p
         return getattr(_p, name)
     if name in ("beam_select", "beam_reorder"):

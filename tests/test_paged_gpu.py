@@ -307,3 +307,53 @@ def test_copy_of_parts_of_pages():
     copy_pages(x.transpose(0, 1), one(3), one(7))
     copy_pages(x.transpose(0, 1)[:, :, 2:5], one(4), one(9))
     assert torch.equal(x, want)
+
+
+def test_a_run_of_all_operators():
+    """Two prompts, three beams each: written, forked, extended, attended, selected and forked again by parents, compacted in between;
+    two layers.  Every step's attention is that of a cache that keeps each beam's keys and values apart."""
+    from llama3_np_b200 import PagedCache, beam_reorder, beam_select
+    G, H, D, V, K = 2, 8, 64, 50, 3
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()  # noqa: E731
+    cache = PagedCache(layers=2, kv_heads=G, head_dim=D, pages=40, page_size=8)
+    waste = [cache.open() for _ in range(2)]
+    cache.extend(waste, [30, 9])                                             # so that the prompts' pages begin further up
+    prompts, count = [cache.open(), cache.open()], [21, 8]
+    view = cache.extend(prompts, count)
+    own = [[], []]                                                           # per layer: [beam] -> (keys, values) [tokens, G, D]
+    for layer in range(2):
+        k, v = rand(2, 21, G, D), rand(2, 21, G, D)
+        cache.write(layer, view, k, v)
+        own[layer] = [(k[b, :count[b]], v[b, :count[b]]) for b in range(2) for _ in range(K)]
+    for w in waste:
+        cache.free(w)
+    beams = [s if j == 0 else cache.fork(s) for s in prompts for j in range(K)]
+    history = torch.zeros(2 * K, 12, dtype=torch.int32, device="cuda")
+    scores = torch.zeros(2, K, device="cuda")
+    for step in range(12):
+        if step in (3, 7):
+            cache.compact()
+        view = cache.extend(beams)
+        for layer in range(2):
+            q, kn, vn = rand(2 * K, H, D), rand(2 * K, G, D), rand(2 * K, G, D)
+            out = cache.attend(layer, view, q, kn, vn)
+            for r in range(2 * K):
+                own[layer][r] = tuple(torch.cat([x, n[r:r + 1]]) for x, n in zip(own[layer][r], (kn, vn)))
+                kk, vv = (x.double().repeat_interleave(H // G, 1) for x in own[layer][r])
+                w = torch.softmax(torch.einsum("hd,thd->ht", q[r].double(), kk) * D ** -0.5, -1)
+                want = torch.einsum("ht,thd->hd", w, vv)
+                room = 2.0 ** -8 * want.abs() + 2.0 ** -12 * torch.einsum("ht,thd->hd", w, vv.abs())
+                assert bool(((out[r].double() - want).abs() <= room).all()), (step, layer, r)
+        logits = torch.randn(2, K, V, generator=g, device="cuda")
+        scores, tokens, parents, _ = beam_select(logits, scores)
+        beam_reorder([history], parents)
+        history[:, step] = tokens.reshape(-1)
+        p = [b * K + x for b, row in enumerate(parents.tolist()) for x in row]
+        old, beams = beams, [cache.fork(beams[x]) for x in p]
+        for s in old:
+            cache.free(s)
+        own = [[layer[x] for x in p] for layer in own]
+    for s in beams:
+        cache.free(s)
+    assert cache.free_pages == cache.pages
