@@ -10,6 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libllama3_b200.so")
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -24,11 +25,29 @@ def _digest():
     h = hashlib.sha256(" ".join(FLAGS).encode())
     for root in (CSRC, os.path.join(os.path.dirname(HERE), "include")):
         for f in sorted(os.listdir(root)):
-            if f.endswith((".cu", ".cuh", ".h")):
+            if f.endswith((".cu", ".cuh", ".h", ".cpp")):
                 h.update(f.encode())
                 with open(os.path.join(root, f), "rb") as fh:
                     h.update(fh.read())
     return h.hexdigest()
+
+
+def _torch_ops():
+    """_torch_ops.so: the operators on device buffers as calls on torch tensors (csrc/torch_ops.cpp).  The library itself does without
+    torch; where that is not installed there is nothing to build."""
+    import importlib.util
+    import sysconfig
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return
+    torch = list(spec.submodule_search_locations)[0]
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    inc = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", os.path.join(CSRC, "torch_ops.cpp"), "-o", TORCH_OPS, *("-I" + i for i in inc),
+           "-L" + os.path.join(torch, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on torch_ops.cpp:\n{r.stdout}\n{r.stderr}")
 
 
 def build(force: bool = False, verbose: bool = False, variant: str = "", defines=()) -> str:
@@ -42,7 +61,7 @@ def build(force: bool = False, verbose: bool = False, variant: str = "", defines
     os.makedirs(OBJ, exist_ok=True)
     stamp = os.path.join(OBJ, "stamp")
     dig = _digest()
-    if not force and os.path.exists(LIB) and os.path.exists(stamp) and open(stamp).read() == dig:
+    if not force and os.path.exists(LIB) and os.path.exists(TORCH_OPS) and os.path.exists(stamp) and open(stamp).read() == dig:
         return LIB
     if not os.path.exists(NVCC):
         raise RuntimeError(f"nvcc not found at {NVCC}; libllama3_b200.so cannot be built here")
@@ -60,7 +79,9 @@ def build(force: bool = False, verbose: bool = False, variant: str = "", defines
         return obj
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        ops = ex.submit(_torch_ops)
         objs = list(ex.map(compile_one, _sources()))
+        ops.result()
     cmd = [NVCC, "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a",
            "-cudart", "static", "-ldl"]
     r = subprocess.run(cmd, capture_output=True, text=True)

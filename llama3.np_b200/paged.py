@@ -15,131 +15,39 @@ from __future__ import annotations
 
 import ctypes as C
 import heapq
+import importlib.util
+import os
 
 import torch
 
 from . import _cabi
 
-_KIND = {torch.float32: _cabi.DTYPE_F32, torch.bfloat16: _cabi.DTYPE_BF16, torch.float16: _cabi.DTYPE_F16}
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 HEAD_DIMS = (16, 32, 48, 64, 96, 128)
+_module = None
+
+
+def _ops():
+    """The calls of csrc/torch_ops.cpp, bound to the library's entries."""
+    global _module
+    if _module is None:
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_torch_ops.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python llama3.np_b200/build.py` (there is no CPU fallback)")
+        spec = importlib.util.spec_from_file_location("_torch_ops", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        lib = _cabi.lib()
+        module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "l3_paged_attention_workspace", "l3_paged_attention", "l3_paged_write", "l3_copy_rows", "l3_beam_reorder",
+            "l3_beam_select_workspace", "l3_beam_select", "l3_last_error")))
+        _module = module
+    return _module
 
 
 def _need(cond, text, *args):
     if not cond:
         raise ValueError(text % args if args else text)
-
-
-def _tensor(x, name, dims, dtypes=None):
-    _need(isinstance(x, torch.Tensor), "%s must be a tensor", name)
-    _need(x.dim() == dims, "%s must have %d dimensions, got %s", name, dims, tuple(x.shape))
-    if dtypes is not None:
-        _need(x.dtype in dtypes, "%s: type %s is not one of %s", name, x.dtype, ", ".join(str(d) for d in dtypes))
-    return x
-
-
-def _ints(x, name, shape):
-    _tensor(x, name, len(shape), (torch.int32,))
-    _need(tuple(x.shape) == tuple(shape), "%s must be %s, got %s", name, tuple(shape), tuple(x.shape))
-    _need(x.is_contiguous(), "%s must be contiguous", name)
-    return x
-
-
-def _one_device(named):
-    device = None
-    for name, x in named:
-        if x is None:
-            continue
-        _need(x.is_cuda, "%s must be on a CUDA device", name)
-        device = x.device if device is None else device
-        _need(x.device == device, "%s is on %s, the others on %s", name, x.device, device)
-    return device
-
-
-def _pool(k_pages, v_pages):
-    _tensor(k_pages, "k_pages", 4, tuple(_KIND))
-    _tensor(v_pages, "v_pages", 4, (k_pages.dtype,))
-    _need(k_pages.shape == v_pages.shape, "k_pages and v_pages differ: %s and %s", tuple(k_pages.shape), tuple(v_pages.shape))
-    pages, _, page, dim = k_pages.shape
-    _need(pages >= 1 and page >= 1 and page & (page - 1) == 0 and page <= 65536, "page size %d is not a power of two up to 65536", page)
-    for name, x in (("k_pages", k_pages), ("v_pages", v_pages)):
-        _need(x.stride(3) == 1 or dim == 1, "%s: the last dimension must be contiguous", name)
-        _fits16(name, x)
-
-
-def _fits16(name, x):
-    size = x.element_size()
-    _need(x.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for n, s in zip(x.shape[:-1], x.stride()) if n > 1),
-          "%s: addresses must be multiples of 16 bytes", name)
-
-
-def _strides(x, *dims):
-    """Strides in elements; 0 where a dimension has one entry only (its stride may be anything)."""
-    return [x.stride(d) if x.shape[d] > 1 else 0 for d in dims]
-
-
-def _stream(device_index):
-    return torch._C._cuda_getCurrentRawStream(device_index)
-
-
-# A call's checks and the parts of its C struct that hang on shapes, strides, types and the device alone are made once per such
-# form: they take several times as long as the kernels of a small call.  Addresses and values are never kept.
-_MOST_PLANS = 4096
-
-
-def _form(x):
-    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
-
-
-def _planned(plans, key, make, *args):
-    plan = plans.get(key)
-    if plan is None:
-        if len(plans) >= _MOST_PLANS:
-            plans.clear()
-        plan = make(*args)
-        plans[key] = plan
-    return plan
-
-
-_attention_plans: dict = {}
-
-
-def _plan_attention(q, k_pages, v_pages, page_table, lengths, k_new, v_new, scale, out):
-    _tensor(q, "q", 3, tuple(_KIND))
-    _pool(k_pages, v_pages)
-    batch, heads, dim = q.shape
-    pages, kv_heads, page, _ = k_pages.shape
-    _need(q.dtype in (k_pages.dtype, torch.float32), "q must have the cache's type or fp32, got %s over %s", q.dtype, k_pages.dtype)
-    _need(k_pages.shape[3] == dim and dim in HEAD_DIMS, "head size %d (cache: %d) is not one of %s", dim, k_pages.shape[3], HEAD_DIMS)
-    _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "%d heads over %d kv heads", heads, kv_heads)
-    _need(q.stride(2) == 1, "q: the last dimension must be contiguous")
-    _tensor(page_table, "page_table", 2, (torch.int32,))
-    _need(page_table.shape[0] == batch, "page_table has %d rows for %d sequences", page_table.shape[0], batch)
-    _need(page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
-    _ints(lengths, "lengths", (batch,))
-    _need((k_new is None) == (v_new is None), "k_new and v_new go together")
-    new = [0, 0, 0, 0]
-    if k_new is not None:
-        for name, x in (("k_new", k_new), ("v_new", v_new)):
-            _tensor(x, name, 3, (k_pages.dtype,))
-            _need(tuple(x.shape) == (batch, kv_heads, dim), "%s must be %s, got %s", name, (batch, kv_heads, dim), tuple(x.shape))
-            _need(x.stride(2) == 1, "%s: the last dimension must be contiguous", name)
-            _fits16(name, x)
-        new = [*_strides(k_new, 0, 1), *_strides(v_new, 0, 1)]
-    if out is not None:
-        _tensor(out, "out", 3, (q.dtype,))
-        _need(out.shape == q.shape and out.is_contiguous(), "out must be contiguous, of q's shape")
-    device = _one_device((("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("lengths", lengths),
-                          ("k_new", k_new), ("v_new", v_new), ("out", out)))
-    n = C.c_int64()
-    if batch:
-        _cabi.check(_cabi.lib().l3_paged_attention_workspace(device.index, heads, kv_heads, dim, C.byref(n)))
-    room = -(-n.value // q.element_size())
-    arg = _cabi.L3PagedAttention(
-        device.index, batch, heads, kv_heads, dim, pages, page, page_table.shape[1], _KIND[q.dtype], _KIND[k_pages.dtype],
-        _KIND[q.dtype], dim ** -0.5 if scale is None else float(scale), None, None, *_strides(q, 0, 1),
-        _cabi.L3PagePool(None, *_strides(k_pages, 0, 1, 2)), _cabi.L3PagePool(None, *_strides(v_pages, 0, 1, 2)), None,
-        *_strides(page_table, 0), None, None, None, *new, None, None, None, room * q.element_size())
-    return bytes(arg), device.index, room, q.is_contiguous(), batch
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_new=None, v_new=None, scale=None, return_lse=False, out=None):
@@ -155,58 +63,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_new=None, v_n
     Returns [batch, heads, head size] of q's type (written into `out` where given), and with `return_lse` also the log of the
     softmax's denominator, [batch, heads] fp32.
     """
-    args = (q, k_pages, v_pages, page_table, lengths, k_new, v_new, scale, out)
-    try:
-        key = (_form(q), _form(k_pages), _form(v_pages), _form(page_table), _form(lengths), _form(k_new), _form(v_new), scale, _form(out))
-    except (AttributeError, RuntimeError):
-        key = None                                     # not tensors, or not strided ones: refused below
-    fixed, index, room, plain, batch = _plan_attention(*args) if key is None else _planned(_attention_plans, key, _plan_attention, *args)
-    if out is None:
-        out = torch.empty_like(q) if plain else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = q.new_empty(q.shape[:2], dtype=torch.float32) if return_lse else None
-    if batch:
-        ws = q.new_empty(room)                         # of this call: a captured graph has one of its own
-        arg = _cabi.L3PagedAttention.from_buffer_copy(fixed)
-        arg.stream, arg.q, arg.table, arg.lengths = _stream(index), q.data_ptr(), page_table.data_ptr(), lengths.data_ptr()
-        arg.k.data, arg.v.data, arg.out, arg.workspace = k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ws.data_ptr()
-        if k_new is not None:
-            arg.k_new, arg.v_new = k_new.data_ptr(), v_new.data_ptr()
-        if return_lse:
-            arg.lse = lse.data_ptr()
-        rc = _cabi.lib().l3_paged_attention(C.byref(arg))
-        if rc:
-            _cabi.check(rc)
-    return (out, lse) if return_lse else out
-
-
-_write_plans: dict = {}
-
-
-def _plan_write(k, v, k_pages, v_pages, page_table, start, count):
-    _pool(k_pages, v_pages)
-    pages, kv_heads, page, dim = k_pages.shape
-    for name, x in (("k", k), ("v", v)):
-        _tensor(x, name, 4, (k_pages.dtype,))
-        _need(x.shape == k.shape and tuple(x.shape[2:]) == (kv_heads, dim), "%s must be [batch, tokens, %d, %d], got %s", name, kv_heads,
-              dim, tuple(x.shape))
-        _need(x.stride(3) == 1 or dim == 1, "%s: the last dimension must be contiguous", name)
-        _fits16(name, x)
-    _need(dim * k.element_size() % 16 == 0, "head size %d: a head's row must be a multiple of 16 bytes", dim)
-    batch, tokens = k.shape[:2]
-    _need(batch <= 65535, "at most 65535 sequences a call")
-    _tensor(page_table, "page_table", 2, (torch.int32,))
-    _need(page_table.shape[0] == batch, "page_table has %d rows for %d sequences", page_table.shape[0], batch)
-    _need(page_table.shape[1] <= 1 or page_table.stride(1) == 1, "page_table: a row must be contiguous")
-    _ints(start, "start", (batch,))
-    if count is not None:
-        _ints(count, "count", (batch,))
-    device = _one_device((("k", k), ("v", v), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table), ("start", start),
-                          ("count", count)))
-    arg = _cabi.L3PagedWrite(
-        device.index, batch, tokens, kv_heads, dim, pages, page, page_table.shape[1], _KIND[k.dtype], None, None, None,
-        *_strides(k, 0, 1, 2), *_strides(v, 0, 1, 2), _cabi.L3PagePool(None, *_strides(k_pages, 0, 1, 2)),
-        _cabi.L3PagePool(None, *_strides(v_pages, 0, 1, 2)), None, *_strides(page_table, 0), None, None)
-    return bytes(arg), device.index, batch * tokens
+    return (_module or _ops()).paged_attention(q, k_pages, v_pages, page_table, lengths, k_new, v_new, scale, bool(return_lse), out)
 
 
 def paged_write(k, v, k_pages, v_pages, page_table, start, count=None):
@@ -216,75 +73,7 @@ def paged_write(k, v, k_pages, v_pages, page_table, start, count=None):
     start, count   [batch] int32 (count None: every token is real)
     Tokens that the table has no page for are dropped; what lies behind a sequence's last token stays as it was.
     """
-    args = (k, v, k_pages, v_pages, page_table, start, count)
-    try:
-        key = (_form(k), _form(v), _form(k_pages), _form(v_pages), _form(page_table), _form(start), _form(count))
-    except (AttributeError, RuntimeError):
-        key = None
-    fixed, index, some = _plan_write(*args) if key is None else _planned(_write_plans, key, _plan_write, *args)
-    if some:
-        arg = _cabi.L3PagedWrite.from_buffer_copy(fixed)
-        arg.stream, arg.k, arg.v, arg.table, arg.start = _stream(index), k.data_ptr(), v.data_ptr(), page_table.data_ptr(), start.data_ptr()
-        arg.k_pool.data, arg.v_pool.data = k_pages.data_ptr(), v_pages.data_ptr()
-        if count is not None:
-            arg.count = count.data_ptr()
-        rc = _cabi.lib().l3_paged_write(C.byref(arg))
-        if rc:
-            _cabi.check(rc)
-
-
-def _rows(tensors, what):
-    """L3Rows of tensors whose first dimension counts rows; a row is a contiguous run, or equal runs at equal distances."""
-    _need(len(tensors) >= 1, "no %s", what)
-    out = (_cabi.L3Rows * len(tensors))()
-    for i, x in enumerate(tensors):
-        _need(isinstance(x, torch.Tensor) and x.dim() >= 1, "%s must be tensors with rows", what)
-        size = x.element_size()
-        dims = [(n, s) for n, s in zip(x.shape[1:], x.stride()[1:]) if n != 1]
-        if any(n == 0 for n, _ in dims):
-            dims = [(0, 1)]
-        run, outer, outer_stride = 1, 1, 0
-        while dims and dims[-1][1] == run:
-            run *= dims.pop()[0]
-        if dims:                                  # the next dimensions out, as far as they are one
-            outer, outer_stride = dims.pop()
-            while dims and dims[-1][1] == outer * outer_stride:
-                outer *= dims.pop()[0]
-        _need(not dims, "%s %d: a row of shape %s and strides %s is not a run, or equal runs at equal distances", what, i,
-              tuple(x.shape[1:]), tuple(x.stride()[1:]))
-        row = x.stride(0)
-        span = (outer - 1) * outer_stride + run if run and outer else 0
-        _need(outer <= 1 or outer_stride >= run, "%s %d overlaps itself", what, i)
-        _need(x.shape[0] <= 1 or row >= span or _interleaved(x, row, run, outer, outer_stride), "%s %d: rows overlap", what, i)
-        out[i] = _cabi.L3Rows(None, x.shape[0], row * size, outer, outer_stride * size, run * size)
-    return out
-
-
-def _interleaved(x, row, run, outer, outer_stride):
-    """Rows that lie between one another's runs, as in a cache kept [heads, sequences, ...]."""
-    return run <= row and row * x.shape[0] <= outer_stride
-
-
-_copy_plans: dict = {}
-
-
-def _plan_copy(pools, src, dst):
-    rows = _rows(pools, "pools")
-    for x in pools:
-        _need(x.shape[0] == pools[0].shape[0], "pools have %d and %d pages", pools[0].shape[0], x.shape[0])
-    _tensor(src, "src", 1)
-    _ints(src, "src", (src.shape[0],))
-    _ints(dst, "dst", (src.shape[0],))
-    device = _one_device([("src", src), ("dst", dst)] + [("pools", x) for x in pools])
-    return bytes(rows), device.index
-
-
-def _filled(fixed, tensors):
-    """The L3Rows of a plan, with the tensors' addresses."""
-    rows = (_cabi.L3Rows * len(tensors)).from_buffer_copy(fixed)
-    for r, x in zip(rows, tensors):
-        r.base = x.data_ptr()
-    return rows
+    (_module or _ops()).paged_write(k, v, k_pages, v_pages, page_table, start, count)
 
 
 def copy_pages(pools, src, dst):
@@ -292,17 +81,7 @@ def copy_pages(pools, src, dst):
 
     Pairs with a number outside the pools are skipped.  No page may be a destination twice, nor both source and destination.
     """
-    pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
-    try:
-        key = (_form(src), _form(dst), *map(_form, pools))
-    except (AttributeError, RuntimeError):
-        key = None
-    fixed, index = _plan_copy(pools, src, dst) if key is None else _planned(_copy_plans, key, _plan_copy, pools, src, dst)
-    n = src.shape[0]
-    if n:
-        rc = _cabi.lib().l3_copy_rows(index, _stream(index), _filled(fixed, pools), len(pools), src.data_ptr(), dst.data_ptr(), n)
-        if rc:
-            _cabi.check(rc)
+    (_module or _ops()).copy_pages(pools, src, dst)
 
 
 class PageTable:
@@ -440,7 +219,7 @@ class PagedCache(PageTable):
         super().__init__(pages, page_size)
         _need(layers >= 1 and kv_heads >= 1, "%d layers of %d kv heads", layers, kv_heads)
         _need(head_dim in HEAD_DIMS, "head size %d is not one of %s", head_dim, HEAD_DIMS)
-        _need(dtype in _KIND, "type %s is not one of %s", dtype, ", ".join(str(d) for d in _KIND))
+        _need(dtype in _TYPES, "type %s is not one of %s", dtype, ", ".join(str(d) for d in _TYPES))
         self.device = torch.device(device)
         shape = (pages, kv_heads, page_size, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from llama3_np_b200 import _cabi, beam_reorder, beam_select, copy_pages, paged_attention, paged_write
-from llama3_np_b200.paged import _rows
+from llama3_np_b200.paged import _ops
 
 
 def _attn(**change):
@@ -85,8 +85,7 @@ def test_select_refuses():
 def test_rows_are_found():
     """A row as runs of bytes: contiguous, one dimension cut, sequences behind heads."""
     def one(x):
-        r = _rows([x], "states")[0]
-        return r.rows, r.row_stride, r.outer, r.outer_stride, r.run
+        return _ops().rows(x)
     x = torch.zeros(6, 4, 10, 8)
     assert one(x) == (6, 1280, 1, 0, 1280)
     assert one(x[:, :, 2:5]) == (6, 1280, 4, 320, 96)
