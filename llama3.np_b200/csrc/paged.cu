@@ -5,8 +5,8 @@
 // Bound by the cache's bytes: every key and value is read once for all query heads of its kv head (2 HD values for 4 HD flops per
 // query head).  The keys of all (sequence, kv head) items, in tiles of 8 - 32, are one long row that the warps of the machine share
 // out evenly - lengths of any mixture leave no SM idle, and a single long sequence fills the machine.  A warp works through its
-// stretch alone, without a block barrier, its next tiles on their way (16-bit caches: into two buffers of its own in shared memory, by
-// asynchronous copies; fp32: into registers), across items; one pass with running maximum and sum.  An item that lies within one warp's stretch
+// stretch alone, without a block barrier, its next tiles on their way into two buffers of its own in shared memory by
+// asynchronous copies, across items; one pass with running maximum and sum.  An item that lies within one warp's stretch
 // is written at once; one that several warps share leaves a partial (m, l, o) per warp, and a second, dependent launch joins those
 // in the order of the keys, so that results do not change from run to run.
 #include <math.h>
@@ -127,10 +127,58 @@ __device__ __forceinline__ long long quotient(long long x, int d) { return (unsi
 struct Rows {
   uint32_t k, v;               // offsets in units of a.unit bytes
   uint32_t mask;               // keys that there are
-  int fresh;                   // the key that comes from k_new / v_new, or -1
+  int fresh, writes;           // the key that comes from k_new / v_new, or -1; the same if this item writes it to its page
 };
 struct Fresh { const char *k, *v; };  // its rows
+struct Home { uint32_t k, v; };       // the offsets of their places in the pools
 __device__ __forceinline__ const char* row_at(const void* pool, uint32_t off, int unit) { return (const char*)pool + (unsigned long long)off * (uint32_t)unit; }
+
+// A tile's rows in shared memory: TK rows of NCH pieces of 16 bytes.  TURN: a row's pieces lie in an order that keeps the eight rows of a
+// matrix that ldmatrix reads on different banks.
+template <int TK, int NCH, bool TURN> struct Tile {
+  static_assert(NCH <= 32, "a lane writes a piece of a row");
+  static constexpr uint32_t ALL = TK == 32 ? 0xffffffffu : (1u << (TK & 31)) - 1;
+  __device__ static __forceinline__ int turn(int row) { return !TURN ? 0 : NCH % 8 == 0 ? row & 7 : NCH % 4 == 0 ? (row >> 1) & 3 : (row >> 2) & 1; }
+  __device__ static __forceinline__ uint32_t place(int row, int piece) { return (row * NCH + (piece ^ turn(row))) * 16; }
+  // writes a row that has arrived to its page
+  __device__ static __forceinline__ void write(uint32_t tile, int row, char* to, int lane) {
+    if (lane >= NCH) return;
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(tile + place(row, lane)) : "memory");
+    reinterpret_cast<uint4*>(to)[lane] = x;
+  }
+  // copies the rows, asynchronously; rows that are not there become zeros (0 times whatever would lie there has to be 0)
+  __device__ static __forceinline__ void copy(const void* pool, int unit, uint32_t off, uint32_t step, bool one_page, const Rows& r, const char* fresh,
+                                              uint32_t dst, int lane) {
+    constexpr bool EVEN = 32 % NCH == 0;           // every copy of a lane is of the same column of pieces
+    constexpr int RS = EVEN ? 32 / NCH : 0;        // and RS rows behind the last
+    const int row0 = lane / NCH, c0 = lane % NCH;
+    const uint32_t to = dst + row0 * NCH * 16, x = (c0 ^ turn(row0)) * 16;  // turn() of a sum of disjoint bits is the parts' exclusive or
+    if (one_page && r.mask == ALL && r.fresh < 0) {  // rows at equal distances from the first lane's
+      const uint32_t first = __shfl_sync(L3_FULL, off, 0);
+      if constexpr (EVEN) {
+        const char* base = (const char*)pool + c0 * 16;
+        const uint32_t at = first + row0 * step;
+#pragma unroll
+        for (int i = 0; i < TK * NCH / 32; ++i) cp16(to + (x ^ (turn(i * RS) * 16)) + i * 512, row_at(base, at + i * RS * step, unit), true);
+      } else {
+#pragma unroll
+        for (int i = 0; i < TK * NCH / 32; ++i) {
+          const int at = i * 32 + lane, row = at / NCH, c = at % NCH;
+          cp16(dst + place(row, c), row_at(pool, first + row * step, unit) + c * 16, true);
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < TK * NCH / 32; ++i) {
+      const int at = i * 32 + lane, row = EVEN ? i * RS + row0 : at / NCH, c = EVEN ? c0 : at % NCH;
+      const char* p = row_at(pool, __shfl_sync(L3_FULL, off, row), unit);
+      if (row == r.fresh) p = fresh;
+      cp16(EVEN ? to + (x ^ (turn(i * RS) * 16)) + i * 512 : dst + place(row, c), p + c * 16, r.mask >> row & 1);
+    }
+  }
+};
 
 // ------------------------------------------------------------------------------------------ 16-bit caches: tensor cores
 // The item's (up to 8) query heads are rows 0 - 7 of an m16n8k16 tile.  Rows 8 - 15, which a tile has anyway, carry what rounding to 16
@@ -138,11 +186,11 @@ __device__ __forceinline__ const char* row_at(const void* pool, uint32_t off, in
 // enter with 16 (bf16) or 22 (fp16) significant bits at no further instruction.  fp16 weights are scaled by 2^12 ahead of the rounding
 // (they are at most 1), which keeps weights down to 2^-36 of the largest off the subnormals.
 // Keys and values are copied apart, so that a tile's keys make room for those of the tile after next while its values are still in use.
-// A row's pieces of 16 bytes lie in an order that keeps the eight rows of a matrix on different banks.
 template <typename T, int HD_, bool QLO> struct MmaCore {
   static constexpr int HD = HD_, TK = HD > 64 ? 16 : 32;
   static constexpr int NW = 4, CTAS = HD > 96 && QLO ? 2 : HD > 32 ? 3 : 4;  // as many warps as registers and shared memory leave room for
   static constexpr int KS = HD / 16, NT = HD / 8, NCH = HD / 8, HALF = TK * HD * 2, AHEAD = 2;
+  using Half = Tile<TK, NCH, true>;
   static constexpr int QW = (QLO ? 4 : 2) * KS;     // words of a lane's share of Q, which waits in shared memory
   static constexpr size_t SMEM = (size_t)NW * (AHEAD * 2 * HALF + (QW + 3) / 4 * 512);
   static constexpr float BIAS = std::is_same<T, bf16>::value ? 0.f : 12.f;
@@ -152,9 +200,6 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
   float m, l;  // of row lane / 4, in units of log 2; l: this lane's share
   float sc;
   float s[TK / 8][4];
-
-  __device__ static __forceinline__ int turn(int row) { return NCH % 8 == 0 ? row & 7 : NCH % 4 == 0 ? (row >> 1) & 3 : (row >> 2) & 1; }
-  __device__ static __forceinline__ uint32_t place(int row, int piece) { return (row * NCH + (piece ^ turn(row))) * 16; }
 
   __device__ __forceinline__ void memory(uint8_t* smem, int warp) {
     ring = smem_u32(smem) + warp * AHEAD * 2 * HALF;
@@ -200,47 +245,16 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
     l = 0.f;
     sc = a.scale * 1.4426950408889634f;
   }
-  // copies the tile's rows; rows that are not there become zeros (0 times whatever would lie there has to be 0)
-  __device__ __forceinline__ void copy(const void* pool, int unit, uint32_t off, uint32_t step, bool one_page, const Rows& r, const char* fresh, uint32_t dst, int lane) {
-    constexpr uint32_t ALL = TK == 32 ? 0xffffffffu : (1u << (TK & 31)) - 1;
-    constexpr bool EVEN = 32 % NCH == 0;           // every copy of a lane is of the same column of pieces
-    constexpr int RS = EVEN ? 32 / NCH : 0;        // and RS rows behind the last
-    const int row0 = lane / NCH, c0 = lane % NCH;
-    const uint32_t to = dst + row0 * NCH * 16, x = (c0 ^ turn(row0)) * 16;  // turn() of a sum of disjoint bits is the parts' exclusive or
-    if (one_page && r.mask == ALL && r.fresh < 0) {  // rows at equal distances from the first lane's
-      const uint32_t first = __shfl_sync(L3_FULL, off, 0);
-      if constexpr (EVEN) {
-        const char* base = (const char*)pool + c0 * 16;
-        const uint32_t at = first + row0 * step;
-#pragma unroll
-        for (int i = 0; i < TK * NCH / 32; ++i) cp16(to + (x ^ (turn(i * RS) * 16)) + i * 512, row_at(base, at + i * RS * step, unit), true);
-      } else {
-#pragma unroll
-        for (int i = 0; i < TK * NCH / 32; ++i) {
-          const int at = i * 32 + lane, row = at / NCH, c = at % NCH;
-          cp16(dst + place(row, c), row_at(pool, first + row * step, unit) + c * 16, true);
-        }
-      }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < TK * NCH / 32; ++i) {
-      const int at = i * 32 + lane, row = EVEN ? i * RS + row0 : at / NCH, c = EVEN ? c0 : at % NCH;
-      const char* p = row_at(pool, __shfl_sync(L3_FULL, off, row), unit);
-      if (row == r.fresh) p = fresh;
-      cp16(EVEN ? to + (x ^ (turn(i * RS) * 16)) + i * 512 : dst + place(row, c), p + c * 16, r.mask >> row & 1);
-    }
-  }
   // address of the pieces 2 step + second of a matrix row, ks steps on
   __device__ static __forceinline__ uint32_t matrix_row(uint32_t half, int row, int second, int step) {
-    if constexpr (NCH % 8 == 0 || NCH == 4) return (half + row * NCH * 16 + (second ^ turn(row)) * 16) ^ (step * 32);  // halves begin on whole rows
-    else return half + place(row, step * 2 + second);
+    if constexpr (NCH % 8 == 0 || NCH == 4) return (half + row * NCH * 16 + (second ^ Half::turn(row)) * 16) ^ (step * 32);  // halves begin on whole rows
+    else return half + Half::place(row, step * 2 + second);
   }
   __device__ __forceinline__ void load_keys(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int buf, int lane) {
-    copy(a.k.p, a.unit, r.k, a.ku_token, (1 << a.log_page) >= TK, r, f.k, ring + buf * 2 * HALF, lane);
+    Half::copy(a.k.p, a.unit, r.k, a.ku_token, (1 << a.log_page) >= TK, r, f.k, ring + buf * 2 * HALF, lane);
   }
   __device__ __forceinline__ void load_values(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int buf, int lane) {
-    copy(a.v.p, a.unit, r.v, a.vu_token, (1 << a.log_page) >= TK, r, f.v, ring + buf * 2 * HALF + HALF, lane);
+    Half::copy(a.v.p, a.unit, r.v, a.vu_token, (1 << a.log_page) >= TK, r, f.v, ring + buf * 2 * HALF + HALF, lane);
   }
   __device__ __forceinline__ void scores(int buf, int lane) {
     const int mi = lane >> 3, row = (mi >> 1) * 8 + (lane & 7);
@@ -345,18 +359,19 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
 // kept per lane group and merged over the warp at the end of an item.
 template <int HD_, int NREP> struct F32Core {
   using C = DecodeCfg<HD_, float>;
-  static constexpr int HD = HD_, NW = 4, AHEAD = 1;
-  static constexpr size_t SMEM = 0;
+  static constexpr int HD = HD_, NW = 4, AHEAD = 2;
   static constexpr int EPL = C::EPL, LPK = C::LPK, KPW = C::KPW;
-  // keys of a lane in a tile (U of them, TK of a warp): as many as registers hold beside the queries and sums
-  static constexpr int MOST_U = EPL >= 12 || NREP * EPL >= 64 ? 2 : EPL == 8 || NREP >= 4 ? 4 : 8, U = MOST_U * KPW > 32 ? 32 / KPW : MOST_U, TK = U * KPW;
-  static constexpr int NEED = (NREP * EPL <= 16 ? 3 : 2) * NREP * EPL + 2 * U * EPL + U * NREP + 2 * NREP + 48;
-  static constexpr int CTAS = NEED <= 124 ? 4 : NEED <= 164 ? 3 : 2;
+  static constexpr int TK = HD > 64 ? 8 : HD > 32 ? 16 : 32, U = TK / KPW, NCH = HD / 4, HALF = TK * HD * 4;  // keys of a tile, of a lane
+  using Half = Tile<TK, NCH, false>;   // eight lanes read one row or two neighbouring ones: no turns
+  static constexpr size_t SMEM = (size_t)NW * AHEAD * 2 * HALF;
+  static constexpr int NEED = (NREP * EPL <= 16 ? 3 : 2) * NREP * EPL + U * NREP + 2 * EPL + 2 * NREP + 56;  // registers
+  static constexpr int BY_REGS = NEED <= 124 ? 4 : NEED <= 164 ? 3 : 2, BY_SMEM = (int)(222 * 1024 / SMEM);
+  static constexpr int CTAS = BY_REGS < BY_SMEM ? BY_REGS : BY_SMEM;
   float q[NREP][EPL], o[NREP][EPL], m[NREP], l[NREP];
-  float k[U][EPL], v[U][EPL], s[U][NREP];
+  float s[U][NREP];
+  uint32_t ring;   // as MmaCore's
+  __device__ __forceinline__ void memory(uint8_t* smem, int warp) { ring = smem_u32(smem) + warp * AHEAD * 2 * HALF; }
 
-  __device__ __forceinline__ void memory(uint8_t*, int) {}
-  __device__ __forceinline__ void add_values(int, int) {}
   static constexpr bool ASK = NREP * EPL <= 16;  // as MmaCore's, where the registers are there
   float asked[ASK ? NREP : 1][EPL];
   __device__ __forceinline__ void read_query(const PagedAttnArgs& a, const Cursor& c, int lane, float (&to)[NREP][EPL]) {
@@ -395,65 +410,75 @@ template <int HD_, int NREP> struct F32Core {
       l[r] = 0.f;
     }
   }
-  __device__ __forceinline__ void load_keys(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int, int lane) {
+  __device__ __forceinline__ void load_keys(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int buf, int lane) {
+    Half::copy(a.k.p, a.unit, r.k, a.ku_token, (1 << a.log_page) >= TK, r, f.k, ring + buf * 2 * HALF, lane);
+  }
+  __device__ __forceinline__ void load_values(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int buf, int lane) {
+    Half::copy(a.v.p, a.unit, r.v, a.vu_token, (1 << a.log_page) >= TK, r, f.v, ring + buf * 2 * HALF + HALF, lane);
+  }
+  __device__ __forceinline__ void read_row(uint32_t row, int sl, float (&x)[EPL]) {
+#pragma unroll
+    for (int c = 0; c < C::CPL; ++c)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(x[4 * c]), "=f"(x[4 * c + 1]), "=f"(x[4 * c + 2]), "=f"(x[4 * c + 3]) : "r"(row + (c * LPK + sl) * 16) : "memory");
+  }
+  __device__ __forceinline__ void scores(int buf, int lane) {
     const int sub = lane / LPK, sl = lane % LPK;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const char* p = row_at(a.k.p, __shfl_sync(L3_FULL, r.k, u * KPW + sub), a.unit);
-      if (u * KPW + sub == r.fresh) p = f.k;
-      load_row<HD, KV_STREAM>((const float*)p, sl, k[u]);
-    }
-  }
-  __device__ __forceinline__ void load_values(const PagedAttnArgs& a, const Rows& r, const Fresh& f, int, int lane) {
-    const int sub = lane / LPK, sl = lane % LPK;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const char* p = row_at(a.v.p, __shfl_sync(L3_FULL, r.v, u * KPW + sub), a.unit);
-      if (u * KPW + sub == r.fresh) p = f.v;
-      load_row<HD, KV_STREAM>((const float*)p, sl, v[u]);
-    }
-  }
-  __device__ __forceinline__ void scores(int, int) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
+      float k[EPL];
+      read_row(ring + buf * 2 * HALF + (u * KPW + sub) * HD * 4, sl, k);
 #pragma unroll
       for (int r = 0; r < NREP; ++r) {
         float d = 0.f;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) d = fmaf(q[r][e], k[u][e], d);
+        for (int e = 0; e < EPL; ++e) d = fmaf(q[r][e], k[e], d);
 #pragma unroll
         for (int off = LPK / 2; off > 0; off >>= 1) d += __shfl_xor_sync(L3_FULL, d, off);
         s[u][r] = d;
       }
+    }
   }
   __device__ __forceinline__ void weigh(uint32_t mask, int lane) {
     const int sub = lane / LPK;
+    if (mask != Half::ALL) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (!(mask >> (u * KPW + sub) & 1)) {
+      for (int u = 0; u < U; ++u)
+        if (!(mask >> (u * KPW + sub) & 1)) {
 #pragma unroll
-        for (int r = 0; r < NREP; ++r) s[u][r] = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) v[u][e] = 0.f;
-      }
+          for (int r = 0; r < NREP; ++r) s[u][r] = -INFINITY;
+        }
+    }
 #pragma unroll
     for (int r = 0; r < NREP; ++r) {
       float mx = m[r];
 #pragma unroll
       for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u][r]);
       const float from = mx == -INFINITY ? 0.f : mx;
-      const float alpha = expf(m[r] - from);
-      l[r] *= alpha;
+      if (__any_sync(L3_FULL, mx > m[r])) {
+        const float alpha = expf(m[r] - from);
+        l[r] *= alpha;
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) o[r][e] *= alpha;
-      m[r] = mx;
+        for (int e = 0; e < EPL; ++e) o[r][e] *= alpha;
+        m[r] = mx;
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float p = expf(s[u][r] - from);
-        l[r] += p;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(p, v[u][e], o[r][e]);
+        s[u][r] = expf(s[u][r] - from);
+        l[r] += s[u][r];
       }
+    }
+  }
+  __device__ __forceinline__ void add_values(int buf, int lane) {
+    const int sub = lane / LPK, sl = lane % LPK;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[EPL];
+      read_row(ring + buf * 2 * HALF + HALF + (u * KPW + sub) * HD * 4, sl, v);
+#pragma unroll
+      for (int r = 0; r < NREP; ++r)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(s[u][r], v[e], o[r][e]);
     }
   }
   __device__ __forceinline__ void end(const PagedAttnArgs& a, bool whole, int b, int head0, int heads, int slot, int lane) {
@@ -498,6 +523,7 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(c
   constexpr int HD = Core::HD, TK = Core::TK, NW = Core::NW;
   extern __shared__ __align__(256) uint8_t core_smem[];
   __shared__ Fresh fresh[NW];
+  __shared__ Home home[NW][Core::AHEAD];
   __shared__ long long before[NW * 32], of_warp[NW];
   pdl_launch();
   pdl_wait();
@@ -574,14 +600,14 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(c
       const int pos = L.t * TK + (lane & (TK - 1));
       entry = L.b < a.B && pos < L.len ? __ldg(a.table + L.b * a.table_stride + (pos >> a.log_page)) : -1;
     };
-    auto rows = [&](Rows& r) {
+    auto rows = [&](Rows& r, int buf) {
       const int pos = L.t * TK + (lane & (TK - 1)), g = L.g;
       const bool ok = pos < L.len && (unsigned)entry < (unsigned)a.n_pages;
       const uint32_t in = pos & ((1 << a.log_page) - 1);
       r.k = ok ? (uint32_t)entry * a.ku_page + in * a.ku_token + g * a.ku_head : 0u;
       r.v = ok ? (uint32_t)entry * a.vu_page + in * a.vu_token + g * a.vu_head : 0u;
       r.mask = __ballot_sync(L3_FULL, ok) & (uint32_t)((1ull << TK) - 1);
-      r.fresh = -1;
+      r.fresh = r.writes = -1;
       // the tile of the new token, unless that lies behind the table: its row comes from k_new / v_new, and goes to its page
       if (a.k_new && L.t == L.nt - 1 && asked_length(a, L.b) == L.len) {
         const int row = (L.len - 1) & (TK - 1);
@@ -591,15 +617,9 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(c
         __syncwarp();
         if (lane == 0) fresh[warp] = Fresh{kn, vn};
         __syncwarp();
-        if (r.mask >> row & 1 && L.blk == 0) {
-          uint4* kd = (uint4*)row_at(a.k.p, __shfl_sync(L3_FULL, r.k, row), a.unit);
-          uint4* vd = (uint4*)row_at(a.v.p, __shfl_sync(L3_FULL, r.v, row), a.unit);
-          constexpr int NCH = HD * (int)sizeof(T) / 16;
-          for (int c = lane; c < 2 * NCH; c += 32) {
-            if (c < NCH) kd[c] = __ldg((const uint4*)kn + c);
-            else vd[c - NCH] = __ldg((const uint4*)vn + c - NCH);
-          }
-        }
+        // its page gets them from the tile, where they have arrived by then
+        r.writes = r.mask >> row & 1 && L.blk == 0 ? row : -1;
+        if (lane == row) home[warp][buf] = Home{r.k, r.v};
       }
       load_pos += L.t + 1 < L.nt ? 2 : 3;
       advance<TK>(a, L);
@@ -613,13 +633,16 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(c
       core.ask_query(a, C, lane);
     }
     uint32_t masks[Core::AHEAD];
+    int writes[Core::AHEAD];
 #pragma unroll
     for (int j = 0; j < Core::AHEAD; ++j) {
       masks[j] = 0;
+      writes[j] = -1;
       const bool some = load_pos < stop;
       if (some) {
-        rows(r);
+        rows(r, j);
         masks[j] = r.mask;
+        writes[j] = r.writes;
         core.load_keys(a, r, fresh[warp], j, lane);
       }
       cp_commit();
@@ -632,19 +655,30 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(c
     bool first = true;
     for (int buf = 0; pos < stop; buf = (buf + 1) % Core::AHEAD) {
       const uint32_t mask = masks[0];
+      const int write = writes[0];
+      Home to{};
+      if (write >= 0) {  // ahead of rows(), which may put another tile's there
+        to = home[warp][buf];
+        __syncwarp();
+      }
       const bool more = load_pos < stop, ends = C.t == C.nt - 1;
       pos += ends ? 3 : 2;
       const bool goes_on = pos < stop;
-      if (more) rows(r);
+      if (more) rows(r, buf);
       Cursor next = C;
       if (goes_on) advance<TK>(a, next);
       if (ends && goes_on) core.ask_query(a, next, lane);
 #pragma unroll
-      for (int j = 0; j + 1 < Core::AHEAD; ++j) masks[j] = masks[j + 1];
+      for (int j = 0; j + 1 < Core::AHEAD; ++j) {
+        masks[j] = masks[j + 1];
+        writes[j] = writes[j + 1];
+      }
       masks[Core::AHEAD - 1] = r.mask;
+      writes[Core::AHEAD - 1] = more ? r.writes : -1;
       cp_wait<2 * Core::AHEAD - 1>();
       __syncwarp();
       core.scores(buf, lane);
+      if (write >= 0) Core::Half::write(core.ring + buf * 2 * Core::HALF, write, (char*)row_at(a.k.p, to.k, a.unit), lane);
       __syncwarp();
       if (more) core.load_keys(a, r, fresh[warp], buf, lane);
       cp_commit();
@@ -652,6 +686,7 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(c
       cp_wait<2 * Core::AHEAD - 1>();
       __syncwarp();
       core.add_values(buf, lane);
+      if (write >= 0) Core::Half::write(core.ring + buf * 2 * Core::HALF + Core::HALF, write, (char*)row_at(a.v.p, to.v, a.unit), lane);
       __syncwarp();
       if (more) core.load_values(a, r, fresh[warp], buf, lane);
       cp_commit();
