@@ -10,6 +10,10 @@
 // that two that are close keep the order of the formula - and picks the n best in the same way,
 // its bound the n-th best of the segments' first candidates.
 // Where more values pass a bound than there is room for (many equal ones), the n best are drawn one after the other.
+// Measured (B200, both launches): 32 sequences of 8 beams (37 of the 256 finished), 128256 fp32 logits, 8 best: 30.5 us = 3.7 TB/s, 56 % of what a
+// copy reaches (the first launch alone 27 us, 64 %: its warps end together, each with 3 us of looking again); one sequence of 4 beams, 32000
+// logits: 8 us, of which the two launches' own latency is most.  Before: a CTA per slice of 8192 logits with the n-th largest found per slice
+// 70 us; lists kept sorted while streaming 44 us; a lane's third portion looked at one portion at a time, by the lane alone, 44 us.
 #include <float.h>
 #include <math.h>
 
