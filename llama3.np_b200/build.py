@@ -32,15 +32,19 @@ def _digest():
     return h.hexdigest()
 
 
+def _torch_folder():
+    import importlib.util
+    spec = importlib.util.find_spec("torch")
+    return None if spec is None else list(spec.submodule_search_locations)[0]
+
+
 def _torch_ops():
     """_torch_ops.so: the operators on device buffers as calls on torch tensors (csrc/torch_ops.cpp).  The library itself does without
     torch; where that is not installed there is nothing to build."""
-    import importlib.util
     import sysconfig
-    spec = importlib.util.find_spec("torch")
-    if spec is None:
+    torch = _torch_folder()
+    if torch is None:
         return
-    torch = list(spec.submodule_search_locations)[0]
     cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
     inc = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", os.path.join(CSRC, "torch_ops.cpp"), "-o", TORCH_OPS, *("-I" + i for i in inc),
@@ -61,7 +65,7 @@ def build(force: bool = False, verbose: bool = False, variant: str = "", defines
     os.makedirs(OBJ, exist_ok=True)
     stamp = os.path.join(OBJ, "stamp")
     dig = _digest()
-    if not force and os.path.exists(LIB) and os.path.exists(TORCH_OPS) and os.path.exists(stamp) and open(stamp).read() == dig:
+    if not force and os.path.exists(LIB) and (os.path.exists(TORCH_OPS) or _torch_folder() is None) and os.path.exists(stamp) and open(stamp).read() == dig:
         return LIB
     if not os.path.exists(NVCC):
         raise RuntimeError(f"nvcc not found at {NVCC}; libllama3_b200.so cannot be built here")

@@ -133,7 +133,7 @@ template <typename F> static int for_portions(const L3Rows* t, int n, int64_t ro
     REQ(t[i].base || t[i].rows * t[i].outer * t[i].run == 0, "tensor %d: no data", i);
   }
   for (int i0 = 0; i0 < n;) {
-    RowsList l{};
+    RowsList l;  // the first m entries count
     int m = 0, piece = 16;
     const int i1 = n - i0 < ROWS_MAX ? n : i0 + ROWS_MAX;
     for (int i = i0; i < i1; ++i) {

@@ -75,11 +75,24 @@ template <> struct Piece<uint4> {
   }
 };
 
+// A launch's tensors with their divisors, as a kernel's parameter: of up to eight tensors 0.5 KB of it in place of 4 (a call of two pools on the
+// host 6.1 us with the long one for every call).
+template <int MAX> struct Tensors {
+  RowsDesc t[MAX];
+  Div row[MAX], run[MAX];
+};
+template <int MAX> Tensors<MAX> tensors_of(const RowsList& l, int n) {
+  Tensors<MAX> p;
+  for (int i = 0; i < n; ++i) {
+    p.t[i] = l.t[i];
+    p.row[i] = make_div(l.t[i].outer * l.t[i].run);
+    p.run[i] = make_div(l.t[i].run);
+  }
+  return p;
+}
 constexpr int CT = 256, CU = 8;  // threads, and pieces of a thread
-struct CopyDivs { Div row[ROWS_MAX], run[ROWS_MAX]; };
-template <typename V>
-__global__ void __launch_bounds__(CT) copy_rows_kernel(const __grid_constant__ RowsList l, const __grid_constant__ CopyDivs dv,
-                                                       const int* src, const int* dst, int n, int rows) {
+template <typename V, int MAX>
+__global__ void __launch_bounds__(CT) copy_rows_kernel(const __grid_constant__ Tensors<MAX> l, const int* src, const int* dst, int n, int rows) {
   pdl_launch();
   pdl_wait();
   const RowsDesc& d = l.t[blockIdx.y];
@@ -93,7 +106,7 @@ __global__ void __launch_bounds__(CT) copy_rows_kernel(const __grid_constant__ R
 #pragma unroll
   for (int i = 0; i < CU; ++i) {
     const unsigned at = off + i * CT + threadIdx.x;
-    const unsigned pr = divide(at, dv.row[blockIdx.y]), rem = at - pr * per, o = divide(rem, dv.run[blockIdx.y]), c = rem - o * d.run;
+    const unsigned pr = divide(at, l.row[blockIdx.y]), rem = at - pr * per, o = divide(rem, l.run[blockIdx.y]), c = rem - o * d.run;
     to[i] = nullptr;
     if (first + pr < (unsigned)n) {
       const int s = __ldg(src + first + pr), t = __ldg(dst + first + pr);
@@ -118,8 +131,8 @@ template <typename V> __device__ __forceinline__ void fetch(V* to, const char* f
   else if constexpr (sizeof(V) >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(from), "n"((int)sizeof(V)) : "memory");
   else *to = *reinterpret_cast<const V*>(from);
 }
-template <typename V>
-__global__ void reorder_rows_kernel(const __grid_constant__ RowsList l, const __grid_constant__ CopyDivs dv, const int* parents, int B, int K, int RU, int turns) {
+template <typename V, int MAX>
+__global__ void reorder_rows_kernel(const __grid_constant__ Tensors<MAX> l, const int* parents, int B, int K, int RU, int turns) {
   extern __shared__ __align__(16) uint8_t places_raw[];
   V* mine = reinterpret_cast<V*>(places_raw) + threadIdx.x;  // [2][RU][K][blockDim.x] (one turn: [RU]...)
   __shared__ unsigned char wanted[ROWS_BEAMS];
@@ -148,7 +161,7 @@ __global__ void reorder_rows_kernel(const __grid_constant__ RowsList l, const __
   __syncthreads();
   const int nn = needs, nm = moves;
   auto piece = [&](unsigned at) {
-    const unsigned o = divide(at, dv.run[blockIdx.z]), c = at - o * d.run;
+    const unsigned o = divide(at, l.run[blockIdx.z]), c = at - o * d.run;
     return d.base + (long long)b * K * d.row_stride + o * d.outer_stride + (long long)c * (int)sizeof(V);
   };
   const unsigned base = blockIdx.x * step * turns + threadIdx.x;
@@ -176,15 +189,7 @@ __global__ void reorder_rows_kernel(const __grid_constant__ RowsList l, const __
   }
 }
 
-CopyDivs divs_of(const RowsList& l, int n) {
-  CopyDivs v{};
-  for (int i = 0; i < n; ++i) {
-    v.row[i] = make_div(l.t[i].outer * l.t[i].run);
-    v.run[i] = make_div(l.t[i].run);
-  }
-  return v;
-}
-template <typename V>
+template <typename V, int MAX>
 cudaError_t copy_rows(const RowsList& l, int n_tensors, const int* src, const int* dst, int n, int rows, cudaStream_t s) {
   unsigned long long most = 0;
   for (int i = 0; i < n_tensors; ++i) {
@@ -194,9 +199,9 @@ cudaError_t copy_rows(const RowsList& l, int n_tensors, const int* src, const in
   const unsigned long long blocks = (most + CT * CU - 1) / (CT * CU);
   if (blocks > 0x7fffffffull) return cudaErrorInvalidConfiguration;
   if (!blocks) return cudaSuccess;
-  return launch_k(copy_rows_kernel<V>, dim3((unsigned)blocks, n_tensors), dim3(CT), 0, s, l, divs_of(l, n_tensors), src, dst, n, rows);
+  return launch_k(copy_rows_kernel<V, MAX>, dim3((unsigned)blocks, n_tensors), dim3(CT), 0, s, tensors_of<MAX>(l, n_tensors), src, dst, n, rows);
 }
-template <typename V>
+template <typename V, int MAX>
 cudaError_t reorder_rows(const RowsList& l, int n_tensors, const int* parents, int B, int K, cudaStream_t s) {
   // a thread's places: K for each of its pieces, of which 32 KB of a CTA and turn hold up to four
   const int fit = 32 * 1024 / (K * (int)sizeof(V)), threads = fit >= 256 ? 256 : fit >= 128 ? 128 : fit >= 64 ? 64 : 32;
@@ -213,9 +218,9 @@ cudaError_t reorder_rows(const RowsList& l, int n_tensors, const int* parents, i
   const size_t smem = (size_t)threads * K * RU * sizeof(V) * (turns > 1 ? 2 : 1);
   const unsigned blocks = (unsigned)(((long long)most + (long long)threads * RU * turns - 1) / ((long long)threads * RU * turns));
   if (!blocks) return cudaSuccess;
-  cudaError_t e = allow_smem(reorder_rows_kernel<V>, smem);
+  cudaError_t e = allow_smem(reorder_rows_kernel<V, MAX>, smem);
   if (e != cudaSuccess) return e;
-  return launch_k(reorder_rows_kernel<V>, dim3(blocks, B, n_tensors), dim3(threads), smem, s, l, divs_of(l, n_tensors), parents, B, K, RU, turns);
+  return launch_k(reorder_rows_kernel<V, MAX>, dim3(blocks, B, n_tensors), dim3(threads), smem, s, tensors_of<MAX>(l, n_tensors), parents, B, K, RU, turns);
 }
 }  // namespace
 
@@ -223,21 +228,24 @@ cudaError_t launch_paged_write(const PagedWriteArgs& a, cudaStream_t s) {
   const int per = 2 * a.G * a.pieces, side = per < WT ? WT / per : 1;
   return launch_k(paged_write_kernel, dim3((a.L + TOK * side - 1) / (TOK * side), a.B), dim3(WT), 0, s, a);
 }
-cudaError_t launch_copy_rows(const RowsList& l, int n_tensors, const int* src, const int* dst, int n, int rows, int piece, cudaStream_t s) {
+template <typename F> static cudaError_t with_piece(int piece, F f) {  // f(a value of the piece's type)
   switch (piece) {
-    case 16: return copy_rows<uint4>(l, n_tensors, src, dst, n, rows, s);
-    case 8: return copy_rows<uint2>(l, n_tensors, src, dst, n, rows, s);
-    case 4: return copy_rows<uint32_t>(l, n_tensors, src, dst, n, rows, s);
-    case 2: return copy_rows<uint16_t>(l, n_tensors, src, dst, n, rows, s);
-    default: return copy_rows<uint8_t>(l, n_tensors, src, dst, n, rows, s);
+    case 16: return f(uint4{});
+    case 8: return f(uint2{});
+    case 4: return f(uint32_t{});
+    case 2: return f(uint16_t{});
+    default: return f(uint8_t{});
   }
 }
+cudaError_t launch_copy_rows(const RowsList& l, int n_tensors, const int* src, const int* dst, int n, int rows, int piece, cudaStream_t s) {
+  return with_piece(piece, [&](auto v) {
+    using V = decltype(v);
+    return n_tensors <= 8 ? copy_rows<V, 8>(l, n_tensors, src, dst, n, rows, s) : copy_rows<V, ROWS_MAX>(l, n_tensors, src, dst, n, rows, s);
+  });
+}
 cudaError_t launch_reorder_rows(const RowsList& l, int n_tensors, const int* parents, int B, int K, int piece, cudaStream_t s) {
-  switch (piece) {
-    case 16: return reorder_rows<uint4>(l, n_tensors, parents, B, K, s);
-    case 8: return reorder_rows<uint2>(l, n_tensors, parents, B, K, s);
-    case 4: return reorder_rows<uint32_t>(l, n_tensors, parents, B, K, s);
-    case 2: return reorder_rows<uint16_t>(l, n_tensors, parents, B, K, s);
-    default: return reorder_rows<uint8_t>(l, n_tensors, parents, B, K, s);
-  }
+  return with_piece(piece, [&](auto v) {
+    using V = decltype(v);
+    return n_tensors <= 8 ? reorder_rows<V, 8>(l, n_tensors, parents, B, K, s) : reorder_rows<V, ROWS_MAX>(l, n_tensors, parents, B, K, s);
+  });
 }
