@@ -755,7 +755,7 @@ extern "C" int l3_debug_pdl(L3Model* m, int B, int L) {
 }
 
 // Attention of one token per row over its ancestors' tokens (BeamState::table): the caches are pools of pages of one token.
-static cudaError_t launch_beam_attention(L3Model* m, const L3BeamRun& r, const AttnArgs& at, int rows) {
+static cudaError_t launch_beam_attention(L3Model* m, const L3BeamRun& r, const AttnArgs& at, int rows, int* launches) {
   PagedAttnArgs a{};
   a.q = at.q; a.q_sb = (long long)m->HN * m->HD; a.q_sh = m->HD; a.q_dtype = L3_DTYPE_F32;
   a.k = PagedPool{(void*)at.cache_k, m->HD, (long long)m->M * m->HD, 0};
@@ -766,7 +766,7 @@ static cudaError_t launch_beam_attention(L3Model* m, const L3BeamRun& r, const A
   a.B = rows; a.H = m->HN; a.G = m->KVHN; a.HD = m->HD; a.scale = 1.0f / sqrtf((float)m->HD);
   a.out = at.out_bf16 ? (void*)at.out_bf16 : at.out; a.out_dtype = at.out_bf16 ? L3_DTYPE_BF16 : L3_DTYPE_F32; a.out_lo = at.out_lo;
   a.ws = r.attn_ws;
-  return launch_paged_attention(a, r.n_sm, m->stream);
+  return launch_paged_attention(a, r.n_sm, m->stream, launches);
 }
 
 // Enqueue one chunk: tokens ids[b * ids_ld + ids_off + t], t < L, at start_pos = *d_pos.
@@ -822,8 +822,9 @@ static int enqueue_chunk(L3Model* m, const int32_t* d_ids, int ids_ld, int ids_o
     if (tc_ctx && m->bf16) at.out_bf16 = (bf16*)m->ctx16;
     else { at.out = m->ctx; at.out_lo = tc_ctx ? m->ctx_lo : nullptr; }
     if (beam) {  // one token a row, over the tokens that its table names
-      LAUNCH(m, launch_beam_attention(m, *beam, at, B));
-      m->launch_acc += 1;  // two launches
+      int launches = 1;
+      LAUNCH(m, launch_beam_attention(m, *beam, at, B, &launches));
+      m->launch_acc += launches - 1;
     } else if (L == 1) {
       at.nsplit = pick_nsplit(m, B);
       LAUNCH(m, launch_attn_decode(at, m->bf16, m->stream));

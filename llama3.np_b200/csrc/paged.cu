@@ -8,13 +8,13 @@
 // stretch alone, without a block barrier, its next tiles on their way into two buffers of its own in shared memory by
 // asynchronous copies, across items; one pass with running maximum and sum.  An item that lies within one warp's stretch
 // is written at once; one that several warps share leaves a partial (m, l, o) per warp, and a second, dependent launch joins those
-// in the order of the keys, so that results do not change from run to run.
+// in the order of the keys, so that results do not change from run to run.  Where there are few keys and few items, an item is a block's or a
+// cluster's instead (paged_item_kernel), which joins its warps' partials itself.
 //
 // Measured (B200, both launches, replayed from a graph over inputs larger than L2): 64 sequences of 4096 tokens, 32 query heads over 8 kv heads of
 // 128 in bf16, 182 us = 5.9 TB/s, 90 % of what a copy reaches; one sequence of 131072 tokens 99 us (83 %); 48 of up to 4001 tokens, heads of 64
 // in fp16, 43 us (70 %); 256 of up to 256 tokens, 6 heads of 48 in fp32, 22 us (53 %); one of 701 tokens 8.6 us.  What the smaller ones pay is
-// fixed: the lengths, then the table, then the rows are three round trips to memory, and the join is three more behind a launch (5.3 us with one
-// tile in all).  Steps on the way, in us for the 131072 / 4001 / 256 tokens: four tiles a warp of 8 warps an SM, pointers passed between lanes
+// fixed: the lengths, then the table, then the rows are three round trips to memory, and the join is three more behind a launch.  Steps on the way, in us for the 131072 / 4001 / 256 tokens: four tiles a warp of 8 warps an SM, pointers passed between lanes
 // 105 / 70 / 37; rows straight into registers in the order that the products read them 111 / 43 / 30 (too few bytes on their way at head size
 // 128); two tiles a warp of 12 warps, offsets of 32 bits, next item's query ahead of time 98 / 45 / 29; items weighed by half a tile 98 / 44 / 26.
 #include <math.h>
@@ -337,8 +337,9 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
         mma16816<T>(o[2 * np + 1], p[u][0], p[u][1], p[u][2], p[u][3], vb[2], vb[3]);
       }
   }
-  // whole: the result; else the partial of `slot`
-  __device__ __forceinline__ void end(const PagedAttnArgs& a, bool whole, int b, int head0, int heads, int slot, int lane) {
+  // whole: the result; else the partial: o [heads][HD] and (m, l) [heads]
+  __device__ __forceinline__ void end(const PagedAttnArgs& a, bool whole, const Cursor& c, float* part_o, float2* part_ml, int lane) {
+    const int b = c.b, head0 = c.head0(a), heads = c.heads(a);
     const int g = lane >> 2, t = lane & 3;
     l += __shfl_xor_sync(L3_FULL, l, 1);
     l += __shfl_xor_sync(L3_FULL, l, 2);
@@ -353,11 +354,11 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
       }
       if (a.lse && t == 0) a.lse[(long long)b * a.H + head0 + g] = (m - BIAS + log2f(l)) * 0.6931471805599453f;
     } else {
-      float* po = a.part_o + ((long long)slot * a.heads_blk + g) * HD;
+      float* po = part_o + g * HD;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
         *reinterpret_cast<float2*>(po + n * 8 + 2 * t) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
-      if (t == 0) *reinterpret_cast<float2*>(a.part_ml + ((long long)slot * a.heads_blk + g) * 2) = make_float2((m - BIAS) * 0.6931471805599453f, l);
+      if (t == 0) part_ml[g] = make_float2((m - BIAS) * 0.6931471805599453f, l);
     }
   }
 };
@@ -489,7 +490,8 @@ template <int HD_, int NREP> struct F32Core {
         for (int e = 0; e < EPL; ++e) o[r][e] = fmaf(s[u][r], v[e], o[r][e]);
     }
   }
-  __device__ __forceinline__ void end(const PagedAttnArgs& a, bool whole, int b, int head0, int heads, int slot, int lane) {
+  __device__ __forceinline__ void end(const PagedAttnArgs& a, bool whole, const Cursor& c, float* part_o, float2* part_ml, int lane) {
+    const int b = c.b, head0 = c.head0(a), heads = c.heads(a);
     const int sub = lane / LPK, sl = lane % LPK;
 #pragma unroll
     for (int off = LPK; off < 32; off <<= 1) {
@@ -510,7 +512,7 @@ template <int HD_, int NREP> struct F32Core {
       if (r >= heads) break;
       const float inv = l[r] == 0.f ? 0.f : 1.0f / l[r];
       const long long oi = ((long long)b * a.H + head0 + r) * HD;
-      float* po = a.part_o + ((long long)slot * a.heads_blk + r) * HD;
+      float* po = part_o + r * HD;
 #pragma unroll
       for (int e = 0; e < EPL; e += 4) {
         if (whole) {
@@ -519,19 +521,142 @@ template <int HD_, int NREP> struct F32Core {
         } else *reinterpret_cast<float4*>(po + C::dim(sl, e)) = make_float4(o[r][e], o[r][e + 1], o[r][e + 2], o[r][e + 3]);
       }
       if (sl == 0) {
-        if (!whole) *reinterpret_cast<float2*>(a.part_ml + ((long long)slot * a.heads_blk + r) * 2) = make_float2(m[r], l[r]);
+        if (!whole) part_ml[r] = make_float2(m[r], l[r]);
         else if (a.lse) a.lse[(long long)b * a.H + head0 + r] = m[r] + logf(l[r]);
       }
     }
   }
 };
 
+// what a warp's lanes tell one another
+template <int AHEAD> struct Mail {
+  Fresh fresh;
+  Home home[AHEAD];
+};
+
+// A warp's stretch of the row of tiles: from tile C on, which begins at unit pos, as far as tiles begin ahead of unit `stop`.  At the end of
+// every item's part: end(core, its last tile, its first tile here, whether that is the item's end, whether it is the stretch's first, the unit
+// behind it).
+template <typename Core, typename T, typename End>
+__device__ __forceinline__ void stretch(const PagedAttnArgs& a, Cursor C, int pos, int stop, uint8_t* core_smem, Mail<Core::AHEAD>& mail, int warp, int lane,
+                                        End end) {
+  constexpr int TK = Core::TK;
+  Cursor L = C;      // the tile whose rows are looked up next
+  int load_pos = pos;
+  int entry = 0;     // the page of this lane's key there
+  auto look = [&] {
+    const int pos = L.t * TK + (lane & (TK - 1));
+    entry = L.b < a.B && pos < L.len ? __ldg(a.table + L.b * a.table_stride + (pos >> a.log_page)) : -1;
+  };
+  auto rows = [&](Rows& r, int buf) {
+    const int pos = L.t * TK + (lane & (TK - 1)), g = L.g;
+    const bool ok = pos < L.len && (unsigned)entry < (unsigned)a.n_pages;
+    const uint32_t in = pos & ((1 << a.log_page) - 1);
+    r.k = ok ? (uint32_t)entry * a.ku_page + in * a.ku_token + g * a.ku_head : 0u;
+    r.v = ok ? (uint32_t)entry * a.vu_page + in * a.vu_token + g * a.vu_head : 0u;
+    r.mask = __ballot_sync(L3_FULL, ok) & (uint32_t)((1ull << TK) - 1);
+    r.fresh = r.writes = -1;
+    // the tile of the new token, unless that lies behind the table: its row comes from k_new / v_new, and goes to its page
+    if (a.k_new && L.t == L.nt - 1 && asked_length(a, L.b) == L.len) {
+      const int row = (L.len - 1) & (TK - 1);
+      r.fresh = row;
+      const char* kn = (const char*)((const T*)a.k_new + L.b * a.kn_sb + g * a.kn_sh);
+      const char* vn = (const char*)((const T*)a.v_new + L.b * a.vn_sb + g * a.vn_sh);
+      __syncwarp();
+      if (lane == 0) mail.fresh = Fresh{kn, vn};
+      __syncwarp();
+      // its page gets them from the tile, where they have arrived by then
+      r.writes = r.mask >> row & 1 && L.blk == 0 ? row : -1;
+      if (lane == row) mail.home[buf] = Home{r.k, r.v};
+    }
+    load_pos += L.t + 1 < L.nt ? 2 : 3;
+    advance<TK>(a, L);
+    look();
+  };
+  Core core;
+  core.memory(core_smem, warp);
+  Rows r;
+  if (pos < stop) {
+    look();
+    core.ask_query(a, C, lane);
+  }
+  uint32_t masks[Core::AHEAD];
+  int writes[Core::AHEAD];
+#pragma unroll
+  for (int j = 0; j < Core::AHEAD; ++j) {
+    masks[j] = 0;
+    writes[j] = -1;
+    const bool some = load_pos < stop;
+    if (some) {
+      rows(r, j);
+      masks[j] = r.mask;
+      writes[j] = r.writes;
+      core.load_keys(a, r, mail.fresh, j, lane);
+    }
+    cp_commit();
+    if (some) core.load_values(a, r, mail.fresh, j, lane);
+    cp_commit();
+  }
+  if (pos < stop) core.load_query(a, C, lane);
+  core.reset(a);
+  __syncwarp();
+  int t0 = C.t;          // first tile of the present item here
+  bool first = true;
+  for (int buf = 0; pos < stop; buf = (buf + 1) % Core::AHEAD) {
+    const uint32_t mask = masks[0];
+    const int write = writes[0];
+    Home to{};
+    if (write >= 0) {  // ahead of rows(), which may put another tile's there
+      to = mail.home[buf];
+      __syncwarp();
+    }
+    const bool more = load_pos < stop, ends = C.t == C.nt - 1;
+    pos += ends ? 3 : 2;
+    const bool goes_on = pos < stop;
+    if (more) rows(r, buf);
+    Cursor next = C;
+    if (goes_on) advance<TK>(a, next);
+    if (ends && goes_on) core.ask_query(a, next, lane);
+#pragma unroll
+    for (int j = 0; j + 1 < Core::AHEAD; ++j) {
+      masks[j] = masks[j + 1];
+      writes[j] = writes[j + 1];
+    }
+    masks[Core::AHEAD - 1] = r.mask;
+    writes[Core::AHEAD - 1] = more ? r.writes : -1;
+    cp_wait<2 * Core::AHEAD - 1>();
+    __syncwarp();
+    core.scores(buf, lane);
+    if (write >= 0) Core::Half::write(core.ring + buf * 2 * Core::HALF, write, (char*)row_at(a.k.p, to.k, a.unit), lane);
+    __syncwarp();
+    if (more) core.load_keys(a, r, mail.fresh, buf, lane);
+    cp_commit();
+    core.weigh(mask, lane);
+    cp_wait<2 * Core::AHEAD - 1>();
+    __syncwarp();
+    core.add_values(buf, lane);
+    if (write >= 0) Core::Half::write(core.ring + buf * 2 * Core::HALF + Core::HALF, write, (char*)row_at(a.v.p, to.v, a.unit), lane);
+    __syncwarp();
+    if (more) core.load_values(a, r, mail.fresh, buf, lane);
+    cp_commit();
+    if (ends || !goes_on) {
+      end(core, C, t0, ends, first, pos);
+      first = false;
+      if (goes_on) {
+        core.load_query(a, next, lane);
+        core.reset(a);
+        t0 = 0;
+      }
+    }
+    C = next;
+  }
+}
+
 template <typename Core, typename T>
 __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
   constexpr int HD = Core::HD, TK = Core::TK, NW = Core::NW;
   extern __shared__ __align__(256) uint8_t core_smem[];
-  __shared__ Fresh fresh[NW];
-  __shared__ Home home[NW][Core::AHEAD];
+  __shared__ Mail<Core::AHEAD> mail[NW];
   __shared__ long long before[NW * 32], of_warp[NW];
   pdl_launch();
   pdl_wait();
@@ -601,123 +726,18 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_attn_kernel(c
       if (in / 2 == C.nt) ++pos;  // none of this item's tiles: the next one's first
       advance<TK>(a, C);
     }
-    Cursor L = C;      // the tile whose rows are looked up next
-    int load_pos = pos;
-    int entry = 0;     // the page of this lane's key there
-    auto look = [&] {
-      const int pos = L.t * TK + (lane & (TK - 1));
-      entry = L.b < a.B && pos < L.len ? __ldg(a.table + L.b * a.table_stride + (pos >> a.log_page)) : -1;
-    };
-    auto rows = [&](Rows& r, int buf) {
-      const int pos = L.t * TK + (lane & (TK - 1)), g = L.g;
-      const bool ok = pos < L.len && (unsigned)entry < (unsigned)a.n_pages;
-      const uint32_t in = pos & ((1 << a.log_page) - 1);
-      r.k = ok ? (uint32_t)entry * a.ku_page + in * a.ku_token + g * a.ku_head : 0u;
-      r.v = ok ? (uint32_t)entry * a.vu_page + in * a.vu_token + g * a.vu_head : 0u;
-      r.mask = __ballot_sync(L3_FULL, ok) & (uint32_t)((1ull << TK) - 1);
-      r.fresh = r.writes = -1;
-      // the tile of the new token, unless that lies behind the table: its row comes from k_new / v_new, and goes to its page
-      if (a.k_new && L.t == L.nt - 1 && asked_length(a, L.b) == L.len) {
-        const int row = (L.len - 1) & (TK - 1);
-        r.fresh = row;
-        const char* kn = (const char*)((const T*)a.k_new + L.b * a.kn_sb + g * a.kn_sh);
-        const char* vn = (const char*)((const T*)a.v_new + L.b * a.vn_sb + g * a.vn_sh);
-        __syncwarp();
-        if (lane == 0) fresh[warp] = Fresh{kn, vn};
-        __syncwarp();
-        // its page gets them from the tile, where they have arrived by then
-        r.writes = r.mask >> row & 1 && L.blk == 0 ? row : -1;
-        if (lane == row) home[warp][buf] = Home{r.k, r.v};
+    stretch<Core, T>(a, C, pos, stop, core_smem, mail[warp], warp, lane, [&](Core& core, const Cursor& c, int t0, bool ends, bool first, int behind) {
+      const int slot = 2 * w + (first ? 0 : 1);
+      core.end(a, t0 == 0 && ends, c, a.part_o + (long long)slot * a.heads_blk * HD, reinterpret_cast<float2*>(a.part_ml) + (long long)slot * a.heads_blk,
+               lane);
+      if (t0 == 0) {
+        // the item's last tile is 2 (nt - 1 - t) units behind this one's beginning: the warp that it begins in
+        const int parts = ends ? 0 : 1 + (int)quotient(behind - 2 + 2LL * (c.nt - 1 - c.t), per);
+        const int4 in = make_int4(slot, w, parts, c.item(a));
+        if (!a.by_item) tail = in;
+        else if (lane == 0) a.info[c.item(a)] = in;
       }
-      load_pos += L.t + 1 < L.nt ? 2 : 3;
-      advance<TK>(a, L);
-      look();
-    };
-    Core core;
-    core.memory(core_smem, warp);
-    Rows r;
-    if (pos < stop) {
-      look();
-      core.ask_query(a, C, lane);
-    }
-    uint32_t masks[Core::AHEAD];
-    int writes[Core::AHEAD];
-#pragma unroll
-    for (int j = 0; j < Core::AHEAD; ++j) {
-      masks[j] = 0;
-      writes[j] = -1;
-      const bool some = load_pos < stop;
-      if (some) {
-        rows(r, j);
-        masks[j] = r.mask;
-        writes[j] = r.writes;
-        core.load_keys(a, r, fresh[warp], j, lane);
-      }
-      cp_commit();
-      if (some) core.load_values(a, r, fresh[warp], j, lane);
-      cp_commit();
-    }
-    if (pos < stop) core.load_query(a, C, lane);
-    core.reset(a);
-    __syncwarp();
-    int t0 = C.t;          // first tile of the present item here
-    bool first = true;
-    for (int buf = 0; pos < stop; buf = (buf + 1) % Core::AHEAD) {
-      const uint32_t mask = masks[0];
-      const int write = writes[0];
-      Home to{};
-      if (write >= 0) {  // ahead of rows(), which may put another tile's there
-        to = home[warp][buf];
-        __syncwarp();
-      }
-      const bool more = load_pos < stop, ends = C.t == C.nt - 1;
-      pos += ends ? 3 : 2;
-      const bool goes_on = pos < stop;
-      if (more) rows(r, buf);
-      Cursor next = C;
-      if (goes_on) advance<TK>(a, next);
-      if (ends && goes_on) core.ask_query(a, next, lane);
-#pragma unroll
-      for (int j = 0; j + 1 < Core::AHEAD; ++j) {
-        masks[j] = masks[j + 1];
-        writes[j] = writes[j + 1];
-      }
-      masks[Core::AHEAD - 1] = r.mask;
-      writes[Core::AHEAD - 1] = more ? r.writes : -1;
-      cp_wait<2 * Core::AHEAD - 1>();
-      __syncwarp();
-      core.scores(buf, lane);
-      if (write >= 0) Core::Half::write(core.ring + buf * 2 * Core::HALF, write, (char*)row_at(a.k.p, to.k, a.unit), lane);
-      __syncwarp();
-      if (more) core.load_keys(a, r, fresh[warp], buf, lane);
-      cp_commit();
-      core.weigh(mask, lane);
-      cp_wait<2 * Core::AHEAD - 1>();
-      __syncwarp();
-      core.add_values(buf, lane);
-      if (write >= 0) Core::Half::write(core.ring + buf * 2 * Core::HALF + Core::HALF, write, (char*)row_at(a.v.p, to.v, a.unit), lane);
-      __syncwarp();
-      if (more) core.load_values(a, r, fresh[warp], buf, lane);
-      cp_commit();
-      if (ends || !goes_on) {
-        const int slot = 2 * w + (first ? 0 : 1);
-        core.end(a, t0 == 0 && ends, C.b, C.head0(a), C.heads(a), slot, lane);
-        if (t0 == 0) {
-          // the item's last tile is 2 (nt - 1 - t) units behind this one's beginning: the warp that it begins in
-          const int parts = ends ? 0 : 1 + (int)quotient(pos - 2 + 2LL * (C.nt - 1 - C.t), per);
-          const int4 in = make_int4(slot, w, parts, C.item(a));
-          if (!a.by_item) tail = in;
-          else if (lane == 0) a.info[C.item(a)] = in;
-        }
-        first = false;
-        if (goes_on) {
-          core.load_query(a, next, lane);
-          core.reset(a);
-          t0 = 0;
-        }
-      }
-      C = next;
-    }
+    });
   }
   if (!a.by_item && lane == 0) a.info[w] = tail;
 }
@@ -789,13 +809,110 @@ __global__ void __launch_bounds__(JOIN_T) paged_join_kernel(const __grid_constan
   if (a.lse && d == 0) a.lse[(long long)b * a.H + head] = mx + logf(l);
 }
 
+// Few keys an item: the warps of one block, or of a cluster of S blocks, share an item's tiles and join their partials through one another's
+// shared memory, in the order of the keys.  No second launch, no workspace, and no search for where a warp begins.
 template <typename Core, typename T>
-cudaError_t launch_core(PagedAttnArgs a, int n_sm, cudaStream_t s) {
+__global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_item_kernel(const __grid_constant__ PagedAttnArgs a, int S) {
+  constexpr int HD = Core::HD, NW = Core::NW, NT = NW * 32, Q4 = HD / 4;
+  static_assert(HEADS * HD * 4 <= Core::AHEAD * 2 * Core::HALF, "a warp's partial takes the place of its tiles");
+  extern __shared__ __align__(256) uint8_t core_smem[];
+  __shared__ Mail<Core::AHEAD> mail[NW];
+  __shared__ float2 ml[NW][HEADS];
+  __shared__ float4 acc[NT];
+  __shared__ float2 acc_ml[NT];
+  pdl_launch();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % S, items = a.G * a.blocks;
+  Cursor C{};
+  C.b = blockIdx.x / S / items;
+  const int gb = blockIdx.x / S - C.b * items;
+  C.g = gb / a.blocks;
+  C.blk = gb - C.g * a.blocks;
+  C.len = length_of(a, C.b);
+  C.nt = tiles_of<Core::TK>(C.len);
+  const int parts = S * NW, way = rank * NW + warp, from = (int)((long long)C.nt * way / parts), to = (int)((long long)C.nt * (way + 1) / parts);
+  const int heads = C.heads(a), head0 = C.head0(a);
+  float* part = reinterpret_cast<float*>(core_smem + warp * Core::AHEAD * 2 * Core::HALF);
+  if (lane < HEADS) ml[warp][lane] = make_float2(-INFINITY, 0.f);  // a warp without tiles
+  __syncwarp();
+  const Cursor item = C;
+  C.t = from;
+  if (from < to)
+    stretch<Core, T>(a, C, 1 + 2 * from, 1 + 2 * to, core_smem, mail[warp], warp, lane,
+                     [&](Core& core, const Cursor& c, int, bool, bool, int) { core.end(a, false, c, part, ml[warp], lane); });
+  if (S > 1) cluster_sync_all();
+  else __syncthreads();
+  // this block's outputs, groups of four of them each (head, four dimensions): rank, rank + S, ...; a few threads each, which share the partials
+  const int mine = (heads * Q4 - rank + S - 1) / S, wide = mine < NT ? mine : NT, groups = wide > 0 ? min(NT / wide, parts) : 0;
+  const uint32_t part_at = smem_u32(core_smem), ml_at = smem_u32(&ml[0][0]);
+  for (int k0 = 0; k0 < mine; k0 += wide) {
+    const int k = k0 + tid % wide, grp = tid / wide, out = rank + S * k, r = out / Q4, d = out - r * Q4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
+    const bool active = grp < groups && k < mine;
+    if (active) {
+      for (int p = grp; p < parts; p += groups) {
+        const uint32_t off_o = part_at + (p % NW) * Core::AHEAD * 2 * Core::HALF + (r * HD + 4 * d) * 4, off_ml = ml_at + ((p % NW) * HEADS + r) * 8;
+        float2 y;
+        float4 x;
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(y.x), "=f"(y.y) : "r"(cluster_at(off_ml, p / NW)) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_at(off_o, p / NW)) : "memory");
+        if (y.y == 0.f) continue;  // no key there, and nothing written
+        const float mx = fmaxf(m, y.x), base = mx == -INFINITY ? 0.f : mx, keep = expf(m - base), w = expf(y.x - base);
+        m = mx;
+        l = fmaf(w, y.y, l * keep);
+        o.x = fmaf(w, x.x, o.x * keep); o.y = fmaf(w, x.y, o.y * keep); o.z = fmaf(w, x.z, o.z * keep); o.w = fmaf(w, x.w, o.w * keep);
+      }
+      acc[tid] = o;
+      acc_ml[tid] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (active && grp == 0) {
+      float mx = m;
+      for (int i = 1; i < groups; ++i) mx = fmaxf(mx, acc_ml[i * wide + tid].x);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float w = expf(m - base);
+      l *= w;
+      o.x *= w; o.y *= w; o.z *= w; o.w *= w;
+      for (int i = 1; i < groups; ++i) {
+        const float4 x = acc[i * wide + tid];
+        const float2 y = acc_ml[i * wide + tid];
+        w = expf(y.x - base);
+        l = fmaf(w, y.y, l);
+        o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+      }
+      const float inv = l == 0.f ? 0.f : 1.0f / l, v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+      const long long row = (long long)item.b * a.H + head0 + r;
+      store_out(a, row * HD + 4 * d, v);
+      if (a.lse && d == 0) a.lse[row] = mx + logf(l);
+    }
+    __syncthreads();
+  }
+  if (S > 1) cluster_sync_all();  // the others may still read here
+}
+
+template <typename Core, typename T>
+cudaError_t launch_core(PagedAttnArgs a, int n_sm, cudaStream_t s, int& launches) {
   const int W = n_sm * Core::CTAS * Core::NW;
   const long long items = (long long)a.B * a.G * a.blocks;
   a.by_item = items <= W;
   a.n_info = (int)(a.by_item ? items : W);
-  cudaError_t e = allow_smem(paged_attn_kernel<Core, T>, Core::SMEM);
+  cudaError_t e;
+  // Items by themselves where all of them have room at once and their longest possible keys (what the table is wide) are few tiles a warp.  One
+  // launch : both, us, by items, blocks of an item and tiles a warp.  bf16, head size 128: 8 items of 8 blocks 0.25 6.9 : 8.2, 1.4 8.5 : 8.6, 3.9
+  // 11.2 : 11.3, 7.8 15.3 : 14.1; 32 of 8 1.4 9.7 : 10.1; 128 of 2 1 6.9 : 10.7, 3.9 10.6 : 13.6, 7.8 15.4 : 16.4, 15.6 24.9 : 23.6.  fp32, head
+  // size 48: 24 of 8 2 7.4 : 9.3; 192 of 1 1 5.2 : 8.3, 4 8.1 : 9.0, 8 11.5 : 10.7.  More items than have room: 696 0.25 9.6 : 8.0; 1536 1 13.0 :
+  // 7.7, 4 23.3 : 22.4.
+  int S = 1;
+  while (S < 8 && items * S <= n_sm) S *= 2;
+  if (items <= 2 * n_sm && ((long long)a.max_pages << a.log_page) <= 4LL * S * Core::NW * Core::TK) {
+    if ((e = allow_smem(paged_item_kernel<Core, T>, Core::SMEM)) != cudaSuccess) return e;
+    launches = 1;
+    return launch_kc(paged_item_kernel<Core, T>, dim3((unsigned)(items * S)), dim3(Core::NW * 32), Core::SMEM, s, S, a, S);
+  }
+  launches = 2;
+  e = allow_smem(paged_attn_kernel<Core, T>, Core::SMEM);
   if (e == cudaSuccess) e = launch_k(paged_attn_kernel<Core, T>, dim3(n_sm * Core::CTAS), dim3(Core::NW * 32), Core::SMEM, s, a);
   if (e != cudaSuccess) return e;
   g_l3_pdl_next = true;  // the joining launch starts in the tail of the first
@@ -803,21 +920,21 @@ cudaError_t launch_core(PagedAttnArgs a, int n_sm, cudaStream_t s) {
   if (a.n_info * a.heads_blk <= 2 * n_sm) return launch_k(paged_join_kernel<512>, dim3(a.n_info, a.heads_blk), dim3(512), 0, s, a);
   return launch_k(paged_join_kernel<128>, dim3(a.n_info, a.heads_blk), dim3(128), 0, s, a);
 }
-template <int HD> cudaError_t launch_f32(const PagedAttnArgs& a, int n_sm, cudaStream_t s) {
-  if (a.heads_blk == 1) return launch_core<F32Core<HD, 1>, float>(a, n_sm, s);
-  if (a.heads_blk == 2) return launch_core<F32Core<HD, 2>, float>(a, n_sm, s);
-  if constexpr (HD == 48 || HD == 96) return launch_core<F32Core<HD, 4>, float>(a, n_sm, s);
-  else if (a.heads_blk <= 4) return launch_core<F32Core<HD, 4>, float>(a, n_sm, s);
-  else return launch_core<F32Core<HD, 8>, float>(a, n_sm, s);
+template <int HD> cudaError_t launch_f32(const PagedAttnArgs& a, int n_sm, cudaStream_t s, int& launches) {
+  if (a.heads_blk == 1) return launch_core<F32Core<HD, 1>, float>(a, n_sm, s, launches);
+  if (a.heads_blk == 2) return launch_core<F32Core<HD, 2>, float>(a, n_sm, s, launches);
+  if constexpr (HD == 48 || HD == 96) return launch_core<F32Core<HD, 4>, float>(a, n_sm, s, launches);
+  else if (a.heads_blk <= 4) return launch_core<F32Core<HD, 4>, float>(a, n_sm, s, launches);
+  else return launch_core<F32Core<HD, 8>, float>(a, n_sm, s, launches);
 }
-template <typename T, int HD> cudaError_t launch_mma(const PagedAttnArgs& a, int n_sm, cudaStream_t s) {
-  if (a.q_dtype == L3_DTYPE_F32) return launch_core<MmaCore<T, HD, true>, T>(a, n_sm, s);
-  return launch_core<MmaCore<T, HD, false>, T>(a, n_sm, s);
+template <typename T, int HD> cudaError_t launch_mma(const PagedAttnArgs& a, int n_sm, cudaStream_t s, int& launches) {
+  if (a.q_dtype == L3_DTYPE_F32) return launch_core<MmaCore<T, HD, true>, T>(a, n_sm, s, launches);
+  return launch_core<MmaCore<T, HD, false>, T>(a, n_sm, s, launches);
 }
-template <int HD> cudaError_t launch_hd(const PagedAttnArgs& a, int n_sm, cudaStream_t s) {
-  if (a.kv_dtype == L3_DTYPE_F32) return launch_f32<HD>(a, n_sm, s);
-  if (a.kv_dtype == L3_DTYPE_BF16) return launch_mma<bf16, HD>(a, n_sm, s);
-  return launch_mma<__half, HD>(a, n_sm, s);
+template <int HD> cudaError_t launch_hd(const PagedAttnArgs& a, int n_sm, cudaStream_t s, int& launches) {
+  if (a.kv_dtype == L3_DTYPE_F32) return launch_f32<HD>(a, n_sm, s, launches);
+  if (a.kv_dtype == L3_DTYPE_BF16) return launch_mma<bf16, HD>(a, n_sm, s, launches);
+  return launch_mma<__half, HD>(a, n_sm, s, launches);
 }
 // the pools' offsets in units of the largest power of two of bytes (16 at least) that divides every stride: 32 bits of them
 bool set_units(PagedAttnArgs& a) {
@@ -852,7 +969,8 @@ size_t paged_attn_workspace(int H, int G, int HD, int n_sm) {
 }
 
 bool paged_attn_fits(PagedAttnArgs a) { return set_units(a); }
-cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s) {
+cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s, int* count) {
+  int none, &launches = count ? *count : none;
   const int W = n_sm * MOST_WARPS;
   set_units(a);
   const int size = a.q_dtype == L3_DTYPE_F32 ? 4 : 2;
@@ -864,12 +982,12 @@ cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s) {
   a.part_o = (float*)(a.info + W);
   a.part_ml = a.part_o + (size_t)2 * W * a.heads_blk * a.HD;
   switch (a.HD) {
-    case 16: return launch_hd<16>(a, n_sm, s);
-    case 32: return launch_hd<32>(a, n_sm, s);
-    case 48: return launch_hd<48>(a, n_sm, s);
-    case 64: return launch_hd<64>(a, n_sm, s);
-    case 96: return launch_hd<96>(a, n_sm, s);
-    case 128: return launch_hd<128>(a, n_sm, s);
+    case 16: return launch_hd<16>(a, n_sm, s, launches);
+    case 32: return launch_hd<32>(a, n_sm, s, launches);
+    case 48: return launch_hd<48>(a, n_sm, s, launches);
+    case 64: return launch_hd<64>(a, n_sm, s, launches);
+    case 96: return launch_hd<96>(a, n_sm, s, launches);
+    case 128: return launch_hd<128>(a, n_sm, s, launches);
     default: return cudaErrorInvalidValue;
   }
 }

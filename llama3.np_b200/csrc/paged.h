@@ -42,7 +42,7 @@ struct PagedAttnArgs {
 };
 size_t paged_attn_workspace(int H, int G, int HD, int n_sm);
 bool paged_attn_fits(PagedAttnArgs a);  // the pools' offsets fit 32 bits of the largest unit that divides their strides
-cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s);
+cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s, int* launches = nullptr);  // launches: how many it made, 1 or 2
 
 struct PagedWriteArgs {
   const void *k, *v;                 // [B, L, G, HD]; strides in bytes

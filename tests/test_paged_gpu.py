@@ -88,32 +88,35 @@ def check(q, k, v, table, lens, scale=None, **kw):
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("dim", [16, 32, 48, 64, 96, 128])
 @pytest.mark.parametrize("heads,kv_heads", [(6, 6), (8, 1), (6, 2), (28, 2), (20, 4)])
-def test_shapes(kind, dim, heads, kv_heads):
+@pytest.mark.parametrize("wide", [None, 4000])   # pages a row: a table of few and one of many, over which all warps share all items
+def test_shapes(kind, dim, heads, kv_heads, wide):
     lens = [37, 1, 0, 16, 150, 17, 300]
-    q, k, v, table, n = make(dim + heads, TYPES[kind], heads, kv_heads, dim, 16, lens, garbage=math.nan)
+    q, k, v, table, n = make(dim + heads, TYPES[kind], heads, kv_heads, dim, 16, lens, garbage=math.nan, max_pages=wide)
     check(q.to(TYPES[kind]), k, v, table, n)
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("page", [1, 2, 4, 8, 32, 64, 256])
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
-def test_pages_and_layouts(kind, page, layout):
+@pytest.mark.parametrize("wide", [None, 60000])
+def test_pages_and_layouts(kind, page, layout, wide):
     lens = [page, page + 1, max(page - 1, 0), 100, 15, 16, 17, 257]
-    q, k, v, table, n = make(page, TYPES[kind], 8, 2, 64, page, lens, garbage=math.inf, layout=layout)
+    q, k, v, table, n = make(page, TYPES[kind], 8, 2, 64, page, lens, garbage=math.inf, layout=layout, max_pages=wide and wide // page)
     check(q.to(TYPES[kind]), k, v, table, n)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 @pytest.mark.parametrize("dim", [48, 128])
-def test_fp32_query_over_16_bit_cache(kind, dim):
-    q, k, v, table, n = make(5, TYPES[kind], 12, 3, dim, 16, [5, 700, 64, 33])
+@pytest.mark.parametrize("wide", [None, 4000])
+def test_fp32_query_over_16_bit_cache(kind, dim, wide):
+    q, k, v, table, n = make(5, TYPES[kind], 12, 3, dim, 16, [5, 700, 64, 33], max_pages=wide)
     check(q, k, v, table, n)
     check(q, k, v, table, n, scale=-0.3)
     assert torch.equal(paged_attention(q, k, v, table, n, scale=0.0), paged_attention(q * 2, k, v, table, n, scale=0.0))
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("batch,longest", [(1, 1), (1, 9001), (2, 2500), (300, 40), (1500, 20)])
+@pytest.mark.parametrize("batch,longest", [(1, 1), (1, 500), (1, 9001), (2, 2500), (5, 900), (20, 300), (70, 60), (300, 40), (1500, 20)])
 def test_split_and_joined(kind, batch, longest):
     """From one sequence over all SMs to more items than warps."""
     lens = [1 + (longest - 1) * ((b * 37) % 101) // 100 if b else longest for b in range(batch)]
@@ -123,17 +126,19 @@ def test_split_and_joined(kind, batch, longest):
     assert torch.equal(got, paged_attention(q, k, v, table, n)), "results change from run to run"
 
 
-def test_lengths_beyond_the_table_and_below_zero():
-    q, k, v, table, n = make(3, torch.bfloat16, 4, 2, 64, 16, [64, 64, 64, 64])
+@pytest.mark.parametrize("tokens", [64, 20000])
+def test_lengths_beyond_the_table_and_below_zero(tokens):
+    q, k, v, table, n = make(3, torch.bfloat16, 4, 2, 64, 16, [tokens] * 4)
     q = q.bfloat16()
-    n.copy_(torch.tensor([1000, -5, 65, 64], dtype=torch.int32))
+    n.copy_(torch.tensor([2 * tokens, -5, tokens + 1, tokens], dtype=torch.int32))
     got = check(q, k, v, table, n)
     assert not got[1].any()
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
-def test_pages_that_are_not_there(kind):
-    q, k, v, table, n = make(4, TYPES[kind], 8, 2, 64, 8, [80, 33, 16, 8])
+@pytest.mark.parametrize("wide", [None, 8000])
+def test_pages_that_are_not_there(kind, wide):
+    q, k, v, table, n = make(4, TYPES[kind], 8, 2, 64, 8, [80, 33, 16, 8], max_pages=wide)
     table[0, 0], table[0, 4], table[1, 1], table[3, 0] = -1, k.shape[0], 1 << 30, -(1 << 31)
     table[2, :2] = -7
     got = check(q.to(TYPES[kind]), k, v, table, n)
@@ -149,10 +154,11 @@ def test_no_pages_at_all():
 
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 16), (6, 6, 48, 4), (24, 2, 64, 32)])
-def test_new_token(kind, heads, kv_heads, dim, page):
+@pytest.mark.parametrize("wide", [None, 60000])
+def test_new_token(kind, heads, kv_heads, dim, page, wide):
     """The new token's row is used and written; nothing else changes."""
     lens = [1, 16, 17, 0, 100, 33, 260]
-    q, k, v, table, n = make(dim, TYPES[kind], heads, kv_heads, dim, page, lens, garbage=math.nan)
+    q, k, v, table, n = make(dim, TYPES[kind], heads, kv_heads, dim, page, lens, garbage=math.nan, max_pages=wide and wide // page)
     q = q.to(TYPES[kind])
     new = torch.randn(2, len(lens), kv_heads, dim + 16, device="cuda").to(TYPES[kind])[..., :dim]
     want_k, want_v = k.clone(), v.clone()
@@ -218,10 +224,11 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(k[total - 4, :, 0], row[0, 0, 1]) and torch.equal(v[5, :, 63], row[1, 0, 0])
 
 
-def test_streams_and_graphs():
+@pytest.mark.parametrize("wide", [None, 4000])
+def test_streams_and_graphs(wide):
     """On a side stream, and captured: two graphs replayed at the same time have workspaces of their own."""
-    a = make(21, torch.bfloat16, 8, 2, 128, 16, [900, 300])
-    b = make(22, torch.bfloat16, 8, 2, 128, 16, [500, 1200])
+    a = make(21, torch.bfloat16, 8, 2, 128, 16, [900, 300], max_pages=wide)
+    b = make(22, torch.bfloat16, 8, 2, 128, 16, [500, 1200], max_pages=wide)
     qs = [x[0].bfloat16() for x in (a, b)]
     want = [paged_attention(q, *x[1:]) for q, x in zip(qs, (a, b))]
     side = torch.cuda.Stream()
