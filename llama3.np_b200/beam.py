@@ -2,6 +2,7 @@
 
 The reference decodes greedily only (llama3.py:320).  Both operators enqueue their kernels on the current stream of the tensors'
 device and return, and can be captured into a graph; arguments that do not fit raise ValueError before anything is enqueued.
+Neither has a backward pass: outside torch.no_grad() they refuse tensors that require a gradient.
 """
 from __future__ import annotations
 
@@ -26,7 +27,8 @@ def beam_reorder(states, parents):
     """In place, row b * beams + j of every state becomes what row b * beams + parents[b, j] was.
 
     states   a list of tensors [batch * beams, ...] of any type: recurrent states, page tables, token histories, cache rows; a row
-             is a contiguous run, or equal runs at equal distances (`cache[:, :, first:last]`)
+             is a contiguous run, or equal runs at equal distances (`cache[:, :, first:last]`);
+             no two states may share memory
     parents  [batch, beams] int32, any of a sequence's beams (up to 256), several times too; a number outside leaves its row as it is
     """
     _ops().beam_reorder(states, parents)

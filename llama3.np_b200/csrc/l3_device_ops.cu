@@ -167,6 +167,12 @@ extern "C" int l3_copy_rows(int device, void* stream, const L3Rows* tensors, int
 extern "C" int l3_beam_reorder(int device, void* stream, const L3Rows* tensors, int n_tensors, const int32_t* parents, int batch, int beams) {
   REQ(batch >= 0 && batch <= 65535 && beams >= 1 && beams <= ROWS_BEAMS, "batch %d (at most 65535) or beams %d (at most %d)", batch, beams, ROWS_BEAMS);
   REQ(batch == 0 || parents, "parents missing");
+  // in place, and all tensors at once: one that is there twice would be read while it is written
+  for (int i = 0; tensors && i < n_tensors; ++i)
+    for (int j = 0; j < i; ++j)
+      REQ(tensors[i].base != tensors[j].base || tensors[i].rows * tensors[i].outer * tensors[i].run == 0 ||
+              tensors[j].rows * tensors[j].outer * tensors[j].run == 0,
+          "tensors %d and %d are the same memory", j, i);
   OnDevice on(device);
   if (batch) CKD(on.e);
   return for_portions(tensors, n_tensors, (int64_t)batch * beams, [&](const RowsList& l, int m, int piece) {

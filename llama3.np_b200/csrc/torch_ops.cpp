@@ -3,6 +3,7 @@
 // and the filling of the C structs took 10 - 20 us a call, several times as long as a small call's kernels.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -39,7 +40,13 @@ const Tensor& tensor(PyObject* x, const char* name) {
   NEED(THPVariable_Check(x), name, " must be a tensor");
   const Tensor& t = THPVariable_Unpack(x);
   NEED(t.layout() == at::kStrided, name, " must be a strided tensor");
+  NEED(!t.is_neg(), name, " is a negated view: resolve_neg() it first");
+  NEED(!t.requires_grad() || !c10::GradMode::is_enabled(), name, " requires a gradient, and this has no backward pass: call it under torch.no_grad()");
   return t;
+}
+// what a call writes is new to autograd: a backward pass that saved the old values raises
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 const Tensor& tensor(PyObject* x, const char* name, int64_t dims) {
   const Tensor& t = tensor(x, name);
@@ -84,6 +91,9 @@ const Tensor& table_of(PyObject* x, int64_t batch) {
   NEED(t.size(0) == batch, "page_table has ", t.size(0), " rows for ", batch, " sequences");
   NEED(t.size(1) <= 1 || t.stride(1) == 1, "page_table: a row must be contiguous");
   return t;
+}
+void own_places(const Tensor& t, const char* name) {
+  for (int64_t d = 0; d < 3; ++d) NEED(t.size(d) <= 1 || t.stride(d) != 0, name, " is expanded, and would be written");
 }
 int pools_of(const Tensor& k, const Tensor& v) {
   const int type = kind(k, "k_pages");
@@ -135,6 +145,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
   NEED(given(x[5]) == given(x[6]), "k_new and v_new go together");
   OneDevice on;
   if (given(x[5])) {
+    own_places(k, "k_pages");
+    own_places(v, "v_pages");
     const Tensor *fresh[2] = {&tensor(x[5], "k_new", 3), &tensor(x[6], "v_new", 3)};
     for (int i = 0; i < 2; ++i) {
       const char* name = i ? "v_new" : "k_new";
@@ -178,7 +190,12 @@ PyObject* paged_attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
     room = at::empty({a.workspace_bytes}, q.options().dtype(at::kByte));  // of this call: a captured graph has one of its own
     a.workspace = room.data_ptr();
     done(entry.attention(&a));
+    if (given(x[5])) {
+      changed(k);
+      changed(v);
+    }
   }
+  if (given(x[9])) changed(out);
   if (!want_lse) return THPVariable_Wrap(out);
   PyObject* both = PyTuple_New(2);
   if (!both) throw python_error();
@@ -205,6 +222,8 @@ PyObject* paged_write(PyObject*, PyObject* const* x, Py_ssize_t n) {
   }
   NEED(dim * k.element_size() % 16 == 0, "head size ", dim, ": a head's row must be a multiple of 16 bytes");
   NEED(batch <= 65535, "at most 65535 sequences a call");
+  own_places(kp, "k_pages");
+  own_places(vp, "v_pages");
   const Tensor& table = table_of(x[4], batch);
   const Tensor& start = tensor(x[5], "start", 1);
   a.start = ints(start, "start", batch);
@@ -222,6 +241,8 @@ PyObject* paged_write(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.k_pool = pool(kp); a.v_pool = pool(vp);
     a.table = table.const_data_ptr<int32_t>(); a.table_stride = step_of(table, 0);
     done(entry.write(&a));
+    changed(kp);
+    changed(vp);
   }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -271,15 +292,15 @@ struct Listed {  // a tensor, or a list or tuple of them
   }
   void add(PyObject* x, const char* what) { rows.push_back(rows_of(tensor(x, what), what, (int64_t)rows.size())); }
 };
-void add_devices(PyObject* x, const char* what, OneDevice& on) {
-  if (THPVariable_Check(x)) return on.add(THPVariable_Unpack(x), what);
+template <typename F> void each(PyObject* x, F f) {
+  if (THPVariable_Check(x)) return f(THPVariable_Unpack(x));
   const Py_ssize_t n = PySequence_Size(x);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* e = PySequence_GetItem(x, i);
     if (!e) throw python_error();
     const Tensor t = THPVariable_Unpack(e);
     Py_DECREF(e);
-    on.add(t, what);
+    f(t);
   }
 }
 
@@ -294,8 +315,11 @@ PyObject* copy_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
   const int pairs = size32(src.size(0), "src");
   const int32_t *from = ints(src, "src", pairs), *to = ints(dst, "dst", pairs);
   on.add(src, "src"); on.add(dst, "dst");
-  add_devices(x[0], "pools", on);
-  if (pairs) done(entry.copy(on.index, on.stream(), pools.rows.data(), size32(pools.rows.size(), "pools"), from, to, pairs));
+  each(x[0], [&](const Tensor& t) { on.add(t, "pools"); });
+  if (pairs) {
+    done(entry.copy(on.index, on.stream(), pools.rows.data(), size32(pools.rows.size(), "pools"), from, to, pairs));
+    each(x[0], changed);
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -313,10 +337,12 @@ PyObject* beam_reorder(PyObject*, PyObject* const* x, Py_ssize_t n) {
   const Listed states(x[0], "states");
   for (const L3Rows& r : states.rows) NEED(r.rows == batch * beams, "a state has ", r.rows, " rows for ", batch, " x ", beams, " beams");
   on.add(parents, "parents");
-  add_devices(x[0], "states", on);
-  if (batch)
+  each(x[0], [&](const Tensor& t) { on.add(t, "states"); });
+  if (batch) {
     done(entry.reorder(on.index, on.stream(), states.rows.data(), size32(states.rows.size(), "states"), parents.const_data_ptr<int32_t>(), (int)batch,
                        (int)beams));
+    each(x[0], changed);
+  }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -8,6 +8,8 @@ Every operator enqueues its kernels on the current stream of the tensors' device
 Arguments that do not fit raise ValueError before anything is enqueued.  What is in device memory - lengths, tables - is not
 read by the host: a page number outside the pool names a page that holds no tokens.
 
+The operators have no backward pass: outside torch.no_grad() they refuse tensors that require a gradient.
+
 Pools have the dimensions [pages, kv heads, page size, head size] in any memory order whose last dimension is contiguous; a
 pool kept as [pages, page size, kv heads, head size] is passed as `pool.transpose(1, 2)`.
 """
@@ -71,7 +73,8 @@ def paged_write(k, v, k_pages, v_pages, page_table, start, count=None):
 
     k, v   [batch, tokens, kv heads, head size] of the pools' type; token t < count[b] of sequence b becomes its token start[b] + t
     start, count   [batch] int32 (count None: every token is real)
-    Tokens that the table has no page for are dropped; what lies behind a sequence's last token stays as it was.
+    Tokens that the table has no page for are dropped; what lies behind a sequence's last token stays as it was.  No two sequences
+    of a call may write to the same page's place.
     """
     (_module or _ops()).paged_write(k, v, k_pages, v_pages, page_table, start, count)
 
@@ -224,6 +227,7 @@ class PagedCache(PageTable):
         shape = (pages, kv_heads, page_size, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.device = self.k[0].device  # "cuda" is a device of its own now, whichever is current later
 
     def _copy(self, pairs) -> None:
         if pairs:

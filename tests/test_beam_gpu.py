@@ -168,6 +168,8 @@ def test_reorder_part_of_a_cache():
     beam_reorder([x[:, :, 5:12], y.transpose(0, 1)], parents)
     assert torch.equal(x, want) and torch.equal(y, wanty)
     beam_reorder([torch.zeros(0, 4, device="cuda")], parents[:0].contiguous())
+    with pytest.raises(ValueError, match="same memory"):
+        beam_reorder([x, y.transpose(0, 1), x], parents)
     many = [torch.full((12, 3), float(i), device="cuda") for i in range(100)]
     many[99] = torch.arange(36.0, device="cuda").reshape(12, 3)
     want = many[99][rows]

@@ -1,9 +1,13 @@
 """CPU suite: what the operators on device buffers refuse, from Python and through the C-ABI, and the index arithmetic of rows."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
+from conftest import ROOT
 from llama3_np_b200 import _cabi, beam_reorder, beam_select, copy_pages, paged_attention, paged_write
 from llama3_np_b200.paged import _ops
 
@@ -82,6 +86,46 @@ def test_select_refuses():
             beam_select(*args, **kw)
 
 
+def test_gradients_are_refused():
+    """None of the operators has a backward pass: a result without its gradient would be a silent error."""
+    def grad(*s, dtype=torch.float32):
+        return torch.zeros(*s, dtype=dtype, requires_grad=True)
+    idx, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32)
+    pool, new = torch.zeros(5, 2, 16, 64), torch.zeros(2, 2, 64)
+    calls = [lambda: paged_attention(**_attn(q=grad(2, 8, 64, dtype=torch.bfloat16))),
+             lambda: paged_attention(grad(2, 8, 64), pool, pool, table, idx, k_new=new, v_new=new),
+             lambda: paged_attention(torch.zeros(2, 8, 64), pool, pool, table, idx, k_new=new, v_new=grad(2, 2, 64)),
+             lambda: paged_write(grad(2, 4, 2, 64), torch.zeros(2, 4, 2, 64), pool, pool, table, idx),
+             lambda: copy_pages([pool, grad(5, 3)], idx, idx),
+             lambda: beam_reorder(grad(4, 3), table),
+             lambda: beam_select(grad(2, 3, 50), torch.zeros(2, 3)),
+             lambda: beam_select(torch.zeros(2, 3, 50), grad(2, 3))]
+    for call in calls:
+        with pytest.raises(ValueError, match="no backward pass"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+            call()
+
+
+def test_memory_that_would_be_written_twice_is_refused():
+    idx, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32)
+    one, new = torch.zeros(1, 2, 16, 64), torch.zeros(2, 2, 64)
+    with pytest.raises(ValueError, match="expanded"):
+        paged_attention(torch.zeros(2, 8, 64), one.expand(5, 2, 16, 64), one.expand(5, 2, 16, 64), table, idx, k_new=new, v_new=new)
+    with pytest.raises(ValueError, match="expanded"):
+        paged_write(torch.zeros(2, 4, 2, 64), torch.zeros(2, 4, 2, 64), one.expand(5, 2, 16, 64), one.expand(5, 2, 16, 64), table, idx)
+    rows = (_cabi.L3Rows * 3)(_cabi.L3Rows(0x1000, 6, 64, 1, 0, 64), _cabi.L3Rows(0x2000, 6, 64, 1, 0, 64), _cabi.L3Rows(0x1000, 6, 64, 1, 0, 64))
+    assert _cabi.lib().l3_beam_reorder(0, C.c_void_p(), rows, 3, C.c_void_p(0x1000), 2, 3) == _cabi.L3_EINVAL
+    assert b"tensors 0 and 2" in _cabi.lib().l3_last_error(None)
+
+
+def test_negated_views_are_refused():
+    q = torch.zeros(2, 8, 1, dtype=torch.complex64).conj().imag
+    assert q.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        paged_attention(**_attn(q=q))
+
+
 def test_rows_are_found():
     """A row as runs of bytes: contiguous, one dimension cut, sequences behind heads."""
     def one(x):
@@ -144,3 +188,9 @@ def test_division_by_multiplication():
         for x in [0, 1, d - 1, d, d + 1, 2 * d - 1, (1 << 31) - 1] + [rng.randrange(0, 1 << 31) for _ in range(50)]:
             if x < 1 << 31:
                 assert (x if sh == 0 else (((x * mul) >> 32) + x) >> sh) == x // d
+
+
+def test_command_line_end_token_needs_beams():
+    r = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "generate"), "--model", "nowhere", "--ids", "1", "--eos", "2"], capture_output=True, text=True,
+                       timeout=120)
+    assert r.returncode == 2 and "--beams" in r.stderr

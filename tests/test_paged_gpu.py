@@ -364,3 +364,27 @@ def test_a_run_of_all_operators():
     for s in beams:
         cache.free(s)
     assert cache.free_pages == cache.pages
+
+
+def test_autograd_sees_what_is_written():
+    """A backward pass that saved a pool's old values raises, as behind torch's own writes; and the device of a cache is a certain one."""
+    from llama3_np_b200 import PagedCache, beam_reorder
+    cache = PagedCache(layers=1, kv_heads=2, head_dim=64, pages=4, page_size=8, dtype=torch.float32)
+    assert cache.device == torch.device("cuda", torch.cuda.current_device())
+    seqs = [cache.open(), cache.open()]
+    new = torch.ones(2, 2, 64, device="cuda")
+    idx = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    state = torch.zeros(2, 3, device="cuda")
+    view = cache.extend(seqs)
+    for write in (lambda: cache.write(0, view, new[:, None], new[:, None]), lambda: cache.attend(0, view, torch.ones(2, 4, 64, device="cuda"), new, new),
+                  lambda: copy_pages(cache.k, idx[:1], idx[1:])):
+        w = torch.ones((), device="cuda", requires_grad=True)
+        loss = (w * cache.k[0]).sum()
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = state._version
+    beam_reorder(state, idx[None].flip(1).contiguous())
+    assert state._version > before
+    with torch.inference_mode():
+        beam_reorder(torch.zeros(2, 3, device="cuda"), idx[None])
