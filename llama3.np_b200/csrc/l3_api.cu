@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <string>
 #include <vector>
@@ -1364,6 +1365,7 @@ static int beam_step(L3Model* m, int B, int eos) {
   const cudaError_t e = cudaStreamEndCapture(m->stream, &r->graph);
   r->nodes = m->launch_acc - before;
   m->launch_acc = before;
+  if (rc != L3_OK || e != cudaSuccess) beam_drop_graph(r);
   if (rc != L3_OK) return rc;
   CK(m, e);
   CK(m, cudaGraphInstantiate(&r->exec, r->graph, 0));
@@ -1385,7 +1387,7 @@ static int generate_beam(L3Model* m, const int32_t* ids, int B, int L, int beams
   REQUIRE(m, m->VS < (1 << 24) && beams <= m->VS && (int64_t)beams * m->VS < ((int64_t)1 << 31), "vocabulary of %d", m->VS);
   REQUIRE(m, max_new_tokens >= 1 && L + max_new_tokens - 1 <= m->M, "prompt %d + %d new tokens exceed max_seq_len %d", L, max_new_tokens, m->M);
   REQUIRE(m, eos_id < m->VS, "eos_id %d is not in the vocabulary", eos_id);
-  REQUIRE(m, length_penalty == length_penalty && length_penalty >= 0.f, "length_penalty must not be negative");
+  REQUIRE(m, std::isfinite(length_penalty) && length_penalty >= 0.f, "length_penalty must be finite, and not negative");
   for (int i = 0; i < B * L; ++i)
     REQUIRE(m, ids[i] >= 0 && ids[i] < m->cfg.vocab_size, "token id %d out of range at %d", ids[i], i);
   CK(m, cudaSetDevice(m->cfg.device));
@@ -1432,7 +1434,7 @@ static int generate_beam(L3Model* m, const int32_t* ids, int B, int L, int beams
     if (eos >= 0)
       for (int s = 0; s < steps; ++s)
         if (seq[(size_t)x * steps + s] == eos) { len[x] = s + 1; break; }
-    value[x] = (double)score[x] / pow((double)len[x], (double)length_penalty);
+    value[x] = score[x] == -INFINITY ? -INFINITY : (double)score[x] / pow((double)len[x], (double)length_penalty);  // the power may be infinite
   }
   for (int b = 0; b < B; ++b) {
     for (int j = 0; j < beams; ++j) order[j] = b * beams + j;

@@ -133,11 +133,13 @@ def test_length_penalty_sorts():
     eos = int(free[0, 0, 2])
     t0, s0, n0 = m.generate_beam(prompt, 4, 6, eos_id=eos)
     t1, s1, n1 = m.generate_beam(prompt, 4, 6, eos_id=eos, length_penalty=1.0)
+    _, s2, n2 = m.generate_beam(prompt, 4, 6, eos_id=eos, length_penalty=1e30)   # 1^x = 1, any other length's power is infinite
     m.close()
     raw = {tuple(t[:n]): s for t, s, n in zip(t0[0].tolist(), s0[0], n0[0])}
     assert (np.diff(s0[0]) <= 0).all() and (np.diff(s1[0]) <= 0).all()
     for t, s, n in zip(t1[0].tolist(), s1[0], n1[0]):
         assert abs(s - raw[tuple(t[:n])] / n) <= 1e-6 * abs(s)
+    assert ((s2[0] == 0) == (n2[0] > 1)).all() and (np.diff(s2[0]) <= 0).all()
 
 
 @pytest.mark.parametrize("heads,kv,dim,K", [(8, 2, 512, 4), (4, 4, 256, 10), (2, 1, 256, 3)])
@@ -186,7 +188,7 @@ def test_refusals():
     ids = np.array([[1, 2, 3], [4, 5, 6]])
     for a, kw in [((ids, 4, 4), {}), ((ids, 0, 4), {}), ((ids, -1, 4), {}), ((ids, 3, 15), {}), ((ids, 3, 0), {}), ((ids, 3, -2), {}),
                   ((ids, 3, 4), dict(eos_id=30)), ((ids, 3, 4), dict(eos_id=-1)), ((ids, 3, 4), dict(length_penalty=-0.5)),
-                  ((ids, 3, 4), dict(length_penalty=float("nan"))), (([[1, 30]], 3, 4), {}), ((ids[0], 3, 4), {})]:
+                  ((ids, 3, 4), dict(length_penalty=float("nan"))), ((ids, 3, 4), dict(length_penalty=float("inf"))), (([[1, 30]], 3, 4), {}), ((ids[0], 3, 4), {})]:
         with pytest.raises(ValueError):
             m.generate_beam(*a, **kw)
     assert m.generate_beam(ids, 3, 14)[0].shape == (2, 3, 14)
