@@ -8,12 +8,12 @@
 // stretch alone, without a block barrier, its next tiles on their way into two buffers of its own in shared memory by
 // asynchronous copies, across items; one pass with running maximum and sum.  An item that lies within one warp's stretch
 // is written at once; one that several warps share leaves a partial (m, l, o) per warp, and a second, dependent launch joins those
-// in the order of the keys, so that results do not change from run to run.  Where there are few keys and few items, an item is a block's or a
-// cluster's instead (paged_item_kernel), which joins its warps' partials itself.
+// in the order of the keys, so that results do not change from run to run.  Where items have few keys, an item is one to four
+// warps' of a block (paged_whole_kernel) or, of few items, a cluster's (paged_item_kernel) instead, which join their partials themselves.
 //
 // Measured (B200, both launches, replayed from a graph over inputs larger than L2): 64 sequences of 4096 tokens, 32 query heads over 8 kv heads of
 // 128 in bf16, 182 us = 5.9 TB/s, 90 % of what a copy reaches; one sequence of 131072 tokens 99 us (83 %); 48 of up to 4001 tokens, heads of 64
-// in fp16, 43 us (70 %); 256 of up to 256 tokens, 6 heads of 48 in fp32, 22 us (53 %); one of 701 tokens 8.6 us.  What the smaller ones pay is
+// in fp16, 43 us (70 %); 256 of up to 256 tokens, 6 heads of 48 in fp32, 21 us (57 %); one of 701 tokens 8.6 us.  What the smaller ones pay is
 // fixed: the lengths, then the table, then the rows are three round trips to memory, and the join is three more behind a launch.  Steps on the way, in us for the 131072 / 4001 / 256 tokens: four tiles a warp of 8 warps an SM, pointers passed between lanes
 // 105 / 70 / 37; rows straight into registers in the order that the products read them 111 / 43 / 30 (too few bytes on their way at head size
 // 128); two tiles a warp of 12 warps, offsets of 32 bits, next item's query ahead of time 98 / 45 / 29; items weighed by half a tile 98 / 44 / 26.
@@ -809,8 +809,8 @@ __global__ void __launch_bounds__(JOIN_T) paged_join_kernel(const __grid_constan
   if (a.lse && d == 0) a.lse[(long long)b * a.H + head] = mx + logf(l);
 }
 
-// Few keys an item: the warps of one block, or of a cluster of S blocks, share an item's tiles and join their partials through one another's
-// shared memory, in the order of the keys.  No second launch, no workspace, and no search for where a warp begins.
+// Few items: the warps of a cluster of S blocks share an item's tiles and join their partials through one another's shared memory, in the order
+// of the keys.  No second launch, no workspace, and no search for where a warp begins.
 template <typename Core, typename T>
 __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_item_kernel(const __grid_constant__ PagedAttnArgs a, int S) {
   constexpr int HD = Core::HD, NW = Core::NW, NT = NW * 32, Q4 = HD / 4;
@@ -840,8 +840,7 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_item_kernel(c
   if (from < to)
     stretch<Core, T>(a, C, 1 + 2 * from, 1 + 2 * to, core_smem, mail[warp], warp, lane,
                      [&](Core& core, const Cursor& c, int, bool, bool, int) { core.end(a, false, c, part, ml[warp], lane); });
-  if (S > 1) cluster_sync_all();
-  else __syncthreads();
+  cluster_sync_all();
   // this block's outputs, groups of four of them each (head, four dimensions): rank, rank + S, ...; a few threads each, which share the partials
   const int mine = (heads * Q4 - rank + S - 1) / S, wide = mine < NT ? mine : NT, groups = wide > 0 ? min(NT / wide, parts) : 0;
   const uint32_t part_at = smem_u32(core_smem), ml_at = smem_u32(&ml[0][0]);
@@ -889,9 +888,81 @@ __global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_item_kernel(c
     }
     __syncthreads();
   }
-  if (S > 1) cluster_sync_all();  // the others may still read here
+  cluster_sync_all();  // the others may still read here
 }
 
+// Few keys an item: P warps of a block have it to themselves and join their partials through the block's shared memory.  As paged_item_kernel's, one
+// launch and no search; blocks that end make room for others, so that more items than there are places need no even shares.
+template <typename Core, typename T, int P>
+__global__ void __launch_bounds__(Core::NW * 32, Core::CTAS) paged_whole_kernel(const __grid_constant__ PagedAttnArgs a) {
+  constexpr int HD = Core::HD, NW = Core::NW, Q4 = HD / 4, RING = Core::AHEAD * 2 * Core::HALF;
+  extern __shared__ __align__(256) uint8_t core_smem[];
+  __shared__ Mail<Core::AHEAD> mail[NW];
+  __shared__ float2 ml[NW][HEADS];
+  pdl_launch();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / P, way = warp % P, items = a.G * a.blocks;
+  const int id = group * gridDim.x + blockIdx.x;  // neighbours on different SMs
+  Cursor C{};
+  C.b = id / items;
+  if (C.b >= a.B) return;
+  const int gb = id - C.b * items;
+  C.g = gb / a.blocks;
+  C.blk = gb - C.g * a.blocks;
+  C.len = length_of(a, C.b);
+  C.nt = tiles_of<Core::TK>(C.len);
+  const int heads = C.heads(a);
+  const long long row = (long long)C.b * a.H + C.head0(a);
+  if (C.nt == 0) {
+    const float zero[2] = {0.f, 0.f};
+    for (int i = way * 32 + lane; i < heads * (HD / 2); i += P * 32) store_out(a, row * HD + 2 * i, zero);
+    if (a.lse && way == 0 && lane < heads) a.lse[row + lane] = -INFINITY;
+    return;
+  }
+  const int from = C.nt * way / P, to = C.nt * (way + 1) / P;
+  if (P > 1 && lane < HEADS) ml[warp][lane] = make_float2(-INFINITY, 0.f);  // a warp without tiles
+  __syncwarp();
+  C.t = from;
+  if (from < to)
+    stretch<Core, T>(a, C, 1 + 2 * from, 1 + 2 * to, core_smem, mail[warp], warp, lane, [&](Core& core, const Cursor& c, int, bool, bool, int) {
+      core.end(a, P == 1, c, reinterpret_cast<float*>(core_smem + warp * RING), ml[warp], lane);
+    });
+  if (P == 1) return;
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(P * 32) : "memory");
+  for (int i = way * 32 + lane; i < heads * Q4; i += P * 32) {
+    const int r = i / Q4, d = i - r * Q4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) m = fmaxf(m, ml[group * P + p][r].x);
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const float2 y = ml[group * P + p][r];
+      if (y.y == 0.f) continue;  // no key there, and nothing written
+      const float4 x = *reinterpret_cast<const float4*>(core_smem + (group * P + p) * RING + (r * HD + 4 * d) * 4);
+      const float w = expf(y.x - base);
+      l = fmaf(w, y.y, l);
+      o.x = fmaf(w, x.x, o.x); o.y = fmaf(w, x.y, o.y); o.z = fmaf(w, x.z, o.z); o.w = fmaf(w, x.w, o.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l, v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    store_out(a, (row + r) * HD + 4 * d, v);
+    if (a.lse && d == 0) a.lse[row + r] = m + logf(l);
+  }
+}
+
+cudaError_t launch_join(const PagedAttnArgs& a, int n_sm, cudaStream_t s) {
+  g_l3_pdl_next = true;  // the joining launch starts in the tail of the first
+  // few items have many partials each, and leave the SMs room for larger blocks
+  if (a.n_info * a.heads_blk <= 2 * n_sm) return launch_k(paged_join_kernel<512>, dim3(a.n_info, a.heads_blk), dim3(512), 0, s, a);
+  return launch_k(paged_join_kernel<128>, dim3(a.n_info, a.heads_blk), dim3(128), 0, s, a);
+}
+template <typename Core, typename T, int P> cudaError_t launch_whole(const PagedAttnArgs& a, long long items, cudaStream_t s) {
+  const cudaError_t e = allow_smem(paged_whole_kernel<Core, T, P>, Core::SMEM);
+  if (e != cudaSuccess) return e;
+  constexpr int groups = Core::NW / P;
+  return launch_k(paged_whole_kernel<Core, T, P>, dim3((unsigned)((items + groups - 1) / groups)), dim3(Core::NW * 32), Core::SMEM, s, a);
+}
 template <typename Core, typename T>
 cudaError_t launch_core(PagedAttnArgs a, int n_sm, cudaStream_t s, int& launches) {
   const int W = n_sm * Core::CTAS * Core::NW;
@@ -899,26 +970,29 @@ cudaError_t launch_core(PagedAttnArgs a, int n_sm, cudaStream_t s, int& launches
   a.by_item = items <= W;
   a.n_info = (int)(a.by_item ? items : W);
   cudaError_t e;
-  // Items by themselves where all of them have room at once and their longest possible keys (what the table is wide) are few tiles a warp.  One
-  // launch : both, us, by items, blocks of an item and tiles a warp.  bf16, head size 128: 8 items of 8 blocks 0.25 6.9 : 8.2, 1.4 8.5 : 8.6, 3.9
-  // 11.2 : 11.3, 7.8 15.3 : 14.1; 32 of 8 1.4 9.7 : 10.1; 128 of 2 1 6.9 : 10.7, 3.9 10.6 : 13.6, 7.8 15.4 : 16.4, 15.6 24.9 : 23.6.  fp32, head
-  // size 48: 24 of 8 2 7.4 : 9.3; 192 of 1 1 5.2 : 8.3, 4 8.1 : 9.0, 8 11.5 : 10.7.  More items than have room: 696 0.25 9.6 : 8.0; 1536 1 13.0 :
-  // 7.7, 4 23.3 : 22.4.
-  int S = 1;
+  // Items by themselves where their longest possible keys (what the table is wide) are few tiles: of eight tiles a warp at most, 1 - 4 warps of a
+  // block.  One launch : both, us, by items (W warps have room) and tiles: bf16, head size 128, W 1776: 256 4 5.0 : 7.9, 16 8.8 : 10.7, 32 14.5 : 16.5; 512
+  // 4 7.6 : 11.9, 16 14.7 : 18.0, 32 22.0 : 25.8; 1600 4 10.7 : 19.6, 16 30.1 : 38.1, 32 44.0 : 57.2.  fp32, head size 48, W 2368: 768 4 6.5 : 9.7, 16 12.7 :
+  // 15.3; 1536 4 7.6 : 12.3, 16 21.1 : 22.5, 32 31.2 : 34.0; one of 16 tiles among 1535 of one 10.5 : 8.9.  More items than warps: 2000 (head size 64) 4
+  // 15.7 : 20.5, 8000 4 45 : 52, 12800 2 42 : 36, 2048 8 23.8 : 22.1.
+  const long long tiles = (((long long)a.max_pages << a.log_page) + Core::TK - 1) / Core::TK;
+  int S = 1, P = 1;
   while (S < 8 && items * S <= n_sm) S *= 2;
-  if (items <= 2 * n_sm && ((long long)a.max_pages << a.log_page) <= 4LL * S * Core::NW * Core::TK) {
+  while (P < Core::NW && (items * 2 * P <= W || tiles > 8 * P)) P *= 2;
+  launches = 1;
+  if (tiles <= (S > 1 ? 2 * Core::NW : items <= W ? 8 * P : items <= 4 * W ? 4 : 0))
+    return P == 1 ? launch_whole<Core, T, 1>(a, items, s) : P == 2 ? launch_whole<Core, T, 2>(a, items, s) : launch_whole<Core, T, Core::NW>(a, items, s);
+  // Fewer items than SMs: a cluster of S blocks an item.  Clusters : blocks as above : two launches, by items of S blocks and tiles: bf16, head size
+  // 128, 8 of 8 8 6.9 : 5.4, 16 7.0 : 8.2, 44 8.5 : - : 8.6, 125 11.2 : - : 11.3; 32 of 4 16 7.6 : 8.3; 120 of 2 16 8.3 : 8.6; 128 of 2 32 10.6 : 12.6 : 13.6.
+  if (S > 1 && tiles <= 4 * S * Core::NW) {
     if ((e = allow_smem(paged_item_kernel<Core, T>, Core::SMEM)) != cudaSuccess) return e;
-    launches = 1;
     return launch_kc(paged_item_kernel<Core, T>, dim3((unsigned)(items * S)), dim3(Core::NW * 32), Core::SMEM, s, S, a, S);
   }
   launches = 2;
   e = allow_smem(paged_attn_kernel<Core, T>, Core::SMEM);
   if (e == cudaSuccess) e = launch_k(paged_attn_kernel<Core, T>, dim3(n_sm * Core::CTAS), dim3(Core::NW * 32), Core::SMEM, s, a);
   if (e != cudaSuccess) return e;
-  g_l3_pdl_next = true;  // the joining launch starts in the tail of the first
-  // few items have many partials each, and leave the SMs room for larger blocks
-  if (a.n_info * a.heads_blk <= 2 * n_sm) return launch_k(paged_join_kernel<512>, dim3(a.n_info, a.heads_blk), dim3(512), 0, s, a);
-  return launch_k(paged_join_kernel<128>, dim3(a.n_info, a.heads_blk), dim3(128), 0, s, a);
+  return launch_join(a, n_sm, s);
 }
 template <int HD> cudaError_t launch_f32(const PagedAttnArgs& a, int n_sm, cudaStream_t s, int& launches) {
   if (a.heads_blk == 1) return launch_core<F32Core<HD, 1>, float>(a, n_sm, s, launches);

@@ -173,6 +173,27 @@ def test_new_token(kind, heads, kv_heads, dim, page, wide):
     assert torch.equal(got, check(q, want_k, want_v, table, n))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim,page", [(48, 16), (128, 4)])
+@pytest.mark.parametrize("batch,longest", [(100, 60), (300, 60), (700, 60), (1900, 30), (300, 250), (16, 300), (60, 250)])
+def test_ways_to_share_items(kind, dim, page, batch, longest):
+    """Items to a cluster, to a block, to two warps, to one and more than there are warps; new tokens, and sequences without any."""
+    lens = [(longest * ((b * 37) % 101) + 99) // 100 if b else longest for b in range(batch)]
+    q, k, v, table, n = make(batch + dim, TYPES[kind], 6, 2, dim, page, lens, garbage=math.nan)
+    q = q.to(TYPES[kind])
+    new = torch.randn(2, batch, 2, dim, device="cuda").to(TYPES[kind])
+    b = torch.arange(batch, device="cuda")[n > 0]
+    last = n.long()[b] - 1
+    p, at = table.long()[b, last // page], last % page
+    want_k, want_v = k.clone(), v.clone()
+    want_k[p, :, at], want_v[p, :, at] = new[0, b], new[1, b]
+    k[p, :, at], v[p, :, at] = math.nan, math.nan
+    got = paged_attention(q, k, v, table, n, k_new=new[0], v_new=new[1])
+    for x, y in ((k, want_k), (v, want_v)):
+        assert torch.equal(x.nan_to_num(7.5), y.nan_to_num(7.5))
+    assert torch.equal(got, check(q, want_k, want_v, table, n))
+
+
 def test_new_token_without_a_page_is_dropped():
     q, k, v, table, n = make(9, torch.bfloat16, 4, 2, 64, 16, [20, 20])
     table[0, 1] = -1
