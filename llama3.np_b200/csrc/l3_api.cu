@@ -1385,7 +1385,7 @@ static int generate_beam(L3Model* m, const int32_t* ids, int B, int L, int beams
   REQUIRE(m, (int64_t)B * beams <= m->maxB, "%d prompts of %d beams exceed max_batch_size %d", B, beams, m->maxB);
   REQUIRE(m, (int64_t)m->maxB * m->KVHN * m->M < ((int64_t)1 << 31), "caches of %d x %d x %d tokens are too large for beam search", m->maxB, m->KVHN, m->M);
   REQUIRE(m, m->VS < (1 << 24) && beams <= m->VS && (int64_t)beams * m->VS < ((int64_t)1 << 31), "vocabulary of %d", m->VS);
-  REQUIRE(m, max_new_tokens >= 1 && L + max_new_tokens - 1 <= m->M, "prompt %d + %d new tokens exceed max_seq_len %d", L, max_new_tokens, m->M);
+  REQUIRE(m, max_new_tokens >= 1 && max_new_tokens <= m->M - L + 1, "prompt %d + %d new tokens exceed max_seq_len %d", L, max_new_tokens, m->M);
   REQUIRE(m, eos_id < m->VS, "eos_id %d is not in the vocabulary", eos_id);
   REQUIRE(m, std::isfinite(length_penalty) && length_penalty >= 0.f, "length_penalty must be finite, and not negative");
   for (int i = 0; i < B * L; ++i)

@@ -244,11 +244,14 @@ class Llama:
         to and with `eos_id`.  Needs `B * beams <= max_batch_size`; a prompt is read once, and beams share its cache."""
         ids = self._ids(input_ids)
         B, L = ids.shape
-        shape = (B, max(int(beams), 0))
-        tokens = np.empty(shape + (max(int(max_new_tokens), 0),), dtype=np.int64)
+        # here, too: the results are allocated ahead of the call, and ctypes would cut larger numbers to 32 bits
+        for name, value, least, most in (("beams", beams, 1, self.args.max_batch_size), ("max_new_tokens", max_new_tokens, 1, self.args.max_seq_len),
+                                         ("eos_id", 0 if eos_id is None else eos_id, 0, self.args.vocab_size - 1)):
+            if not least <= int(value) <= most:
+                raise ValueError(f"{name} {value} is not one of {least} to {most}")
+        shape = (B, int(beams))
+        tokens = np.empty(shape + (int(max_new_tokens),), dtype=np.int64)
         scores, lengths = np.empty(shape, dtype=np.float32), np.empty(shape, dtype=np.int32)
-        if eos_id is not None and int(eos_id) < 0:
-            raise ValueError(f"eos_id {eos_id} is not in the vocabulary")
         _cabi.check(self._lib.l3_generate_beam(self._h, _cabi.i32p(ids), B, L, int(beams), int(max_new_tokens),
                                                -1 if eos_id is None else int(eos_id), float(length_penalty), _cabi.i64p(tokens),
                                                _cabi.f32p(scores), _cabi.i32p(lengths)), self._h)

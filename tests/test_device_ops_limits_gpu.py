@@ -1,0 +1,25 @@
+"""GPU suite: the operators on device buffers and beam search at the edge of what they take."""
+import numpy as np
+import pytest
+
+from llama3_np_b200 import Llama, ModelArgs, _cabi
+from llama3_np_b200.synth import make_weights
+
+pytestmark = pytest.mark.gpu
+
+
+def test_beam_search_refuses_more_tokens_than_the_cache_holds():
+    """Also where the sum with the prompt's length passes 32 bits: refused on the host, before anything is enqueued."""
+    args = ModelArgs(dim=64, n_layers=1, n_heads=2, n_kv_heads=1, vocab_size=30, max_seq_len=16, max_batch_size=6)
+    m = Llama(make_weights(args, 160, seed=1), args)
+    lib, before = _cabi.lib(), m.launch_count()
+    scores, lengths = np.zeros((1, 2), np.float32), np.zeros((1, 2), np.int32)
+    tokens = np.full((1, 2, 16), -7, np.int64)
+    for L in (1, 2, 9, 16):
+        ids = np.ones((1, L), np.int32)
+        for new in (2 ** 31 - 1, 2 ** 31 - 16, 18 - L):
+            rc = lib.l3_generate_beam(m._h, _cabi.i32p(ids), 1, L, 2, new, 3, 0.0, _cabi.i64p(tokens), _cabi.f32p(scores), _cabi.i32p(lengths))
+            assert rc == _cabi.L3_EINVAL and b"max_seq_len" in lib.l3_last_error(m._h)
+        assert m.launch_count() == before and (tokens == -7).all()
+    assert m.generate_beam(np.ones((1, 9), np.int64), 2, 8)[0].shape == (1, 2, 8)
+    m.close()
