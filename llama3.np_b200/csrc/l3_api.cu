@@ -927,7 +927,7 @@ static int check_call(L3Model* m, int B, int L, int start_pos) {
   if (!m->finalized) { set_err(m, "model not finalized"); return L3_ESTATE; }
   if (m->G > 1 && !m->comm) { set_err(m, "tensor parallel model: call l3_tp_init first"); return L3_ESTATE; }
   REQUIRE(m, B >= 1 && B <= m->maxB, "batch %d exceeds max_batch_size %d", B, m->maxB);
-  REQUIRE(m, L >= 1 && start_pos >= 0 && start_pos + L <= m->M, "start_pos %d + L %d exceeds max_seq_len %d",
+  REQUIRE(m, L >= 1 && start_pos >= 0 && L <= m->M - start_pos, "start_pos %d + L %d exceeds max_seq_len %d",
           start_pos, L, m->M);
   return L3_OK;
 }
@@ -1211,7 +1211,7 @@ extern "C" int l3_generate_ragged(L3Model* m, const int32_t* ids, const int32_t*
     for (int t = 0; t < lens[b]; ++t)
       REQUIRE(m, ids[b * Lmax + t] >= 0 && ids[b * Lmax + t] < m->cfg.vocab_size, "token id out of range in prompt %d", b);
   }
-  REQUIRE(m, lmax + pos_offset + max_new_tokens <= m->M, "longest prompt %d + %d new tokens exceed max_seq_len %d", lmax,
+  REQUIRE(m, max_new_tokens <= m->M - lmax - pos_offset, "longest prompt %d + %d new tokens exceed max_seq_len %d", lmax,
           max_new_tokens, m->M);
   REQUIRE(m, eos_id < m->cfg.vocab_size, "eos_id out of range");
   CK(m, cudaSetDevice(m->cfg.device));

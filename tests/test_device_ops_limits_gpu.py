@@ -23,3 +23,20 @@ def test_beam_search_refuses_more_tokens_than_the_cache_holds():
         assert m.launch_count() == before and (tokens == -7).all()
     assert m.generate_beam(np.ones((1, 9), np.int64), 2, 8)[0].shape == (1, 2, 8)
     m.close()
+
+
+def test_positions_near_2_31_are_refused():
+    """A position or a number of tokens whose sum with the prompt's length passes 32 bits, by the calls of a handle that take one."""
+    args = ModelArgs(dim=64, n_layers=1, n_heads=2, n_kv_heads=1, vocab_size=30, max_seq_len=16, max_batch_size=2)
+    m = Llama(make_weights(args, 160, seed=1), args)
+    lib, before = _cabi.lib(), m.launch_count()
+    logits, out, lens = np.zeros((1, 30), np.float32), np.full((1, 16), -7, np.int64), np.array([9], np.int32)
+    ids = np.ones((1, 9), np.int32)
+    for start in (2 ** 31 - 1, 2 ** 31 - 9, 8):
+        assert lib.l3_forward(m._h, _cabi.i32p(ids), 1, 9, start, _cabi.f32p(logits), None) == _cabi.L3_EINVAL
+    for new in (2 ** 31 - 1, 2 ** 31 - 8, 8):
+        assert lib.l3_generate_ragged(m._h, _cabi.i32p(ids), _cabi.i32p(lens), 1, 9, new, 0, -1, _cabi.i64p(out)) == _cabi.L3_EINVAL
+    assert m.launch_count() == before and (out == -7).all()
+    assert lib.l3_forward(m._h, _cabi.i32p(ids), 1, 9, 7, _cabi.f32p(logits), None) == _cabi.L3_OK
+    assert lib.l3_generate_ragged(m._h, _cabi.i32p(ids), _cabi.i32p(lens), 1, 9, 7, 0, -1, _cabi.i64p(out)) == _cabi.L3_OK
+    m.close()
