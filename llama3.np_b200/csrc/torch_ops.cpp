@@ -272,7 +272,8 @@ L3Rows rows_of(const Tensor& t, const char* what, int64_t i) {
   NEED(t.size(0) <= 1 || row >= span || (run <= row && row * t.size(0) <= outer_stride), what, " ", i, ": rows overlap");
   return L3Rows{t.data_ptr(), t.size(0), row * size, outer, outer_stride * size, run * size};
 }
-struct Listed {  // a tensor, or a list or tuple of them
+struct Listed {  // a tensor, or any iterable of them, which is walked once: it may be a generator that alone holds them
+  std::vector<Tensor> tensors;
   std::vector<L3Rows> rows;
   Listed(PyObject* x, const char* what) {
     if (THPVariable_Check(x)) {
@@ -287,22 +288,15 @@ struct Listed {  // a tensor, or a list or tuple of them
     } drop{seq};
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
     NEED(n >= 1, "no ", what);
+    tensors.reserve(n);
     rows.reserve(n);
     for (Py_ssize_t i = 0; i < n; ++i) add(PySequence_Fast_GET_ITEM(seq, i), what);
   }
-  void add(PyObject* x, const char* what) { rows.push_back(rows_of(tensor(x, what), what, (int64_t)rows.size())); }
-};
-template <typename F> void each(PyObject* x, F f) {
-  if (THPVariable_Check(x)) return f(THPVariable_Unpack(x));
-  const Py_ssize_t n = PySequence_Size(x);
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    PyObject* e = PySequence_GetItem(x, i);
-    if (!e) throw python_error();
-    const Tensor t = THPVariable_Unpack(e);
-    Py_DECREF(e);
-    f(t);
+  void add(PyObject* x, const char* what) {
+    tensors.push_back(tensor(x, what));
+    rows.push_back(rows_of(tensors.back(), what, (int64_t)rows.size()));
   }
-}
+};
 
 // copy_pages(pools, src, dst)
 PyObject* copy_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
@@ -314,11 +308,11 @@ PyObject* copy_pages(PyObject*, PyObject* const* x, Py_ssize_t n) {
   const Tensor &src = tensor(x[1], "src", 1), &dst = tensor(x[2], "dst", 1);
   const int pairs = size32(src.size(0), "src");
   const int32_t *from = ints(src, "src", pairs), *to = ints(dst, "dst", pairs);
+  for (const Tensor& t : pools.tensors) on.add(t, "pools");
   on.add(src, "src"); on.add(dst, "dst");
-  each(x[0], [&](const Tensor& t) { on.add(t, "pools"); });
   if (pairs) {
     done(entry.copy(on.index, on.stream(), pools.rows.data(), size32(pools.rows.size(), "pools"), from, to, pairs));
-    each(x[0], changed);
+    for (const Tensor& t : pools.tensors) changed(t);
   }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -336,12 +330,12 @@ PyObject* beam_reorder(PyObject*, PyObject* const* x, Py_ssize_t n) {
   OneDevice on;
   const Listed states(x[0], "states");
   for (const L3Rows& r : states.rows) NEED(r.rows == batch * beams, "a state has ", r.rows, " rows for ", batch, " x ", beams, " beams");
+  for (const Tensor& t : states.tensors) on.add(t, "states");
   on.add(parents, "parents");
-  each(x[0], [&](const Tensor& t) { on.add(t, "states"); });
   if (batch) {
     done(entry.reorder(on.index, on.stream(), states.rows.data(), size32(states.rows.size(), "states"), parents.const_data_ptr<int32_t>(), (int)batch,
                        (int)beams));
-    each(x[0], changed);
+    for (const Tensor& t : states.tensors) changed(t);
   }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS

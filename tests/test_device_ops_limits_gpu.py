@@ -1,8 +1,9 @@
 """GPU suite: the operators on device buffers and beam search at the edge of what they take."""
 import numpy as np
 import pytest
+import torch
 
-from llama3_np_b200 import Llama, ModelArgs, _cabi
+from llama3_np_b200 import Llama, ModelArgs, _cabi, beam_reorder, copy_pages
 from llama3_np_b200.synth import make_weights
 
 pytestmark = pytest.mark.gpu
@@ -40,3 +41,17 @@ def test_positions_near_2_31_are_refused():
     assert lib.l3_forward(m._h, _cabi.i32p(ids), 1, 9, 7, _cabi.f32p(logits), None) == _cabi.L3_OK
     assert lib.l3_generate_ragged(m._h, _cabi.i32p(ids), _cabi.i32p(lens), 1, 9, 7, 0, -1, _cabi.i64p(out)) == _cabi.L3_OK
     m.close()
+
+
+@pytest.mark.parametrize("as_what", [lambda x: (t for t in x), lambda x: dict(enumerate(x)).values(), iter, tuple])
+def test_states_from_any_iterable(as_what):
+    """Tensors that come from a generator or a dict's values are reordered and copied once, and count as modified."""
+    x = [torch.randn(6, 5, device="cuda"), torch.arange(6, device="cuda")]
+    parents = torch.tensor([[2, 0, 0], [1, 2, 2]], dtype=torch.int32, device="cuda")
+    rows = (parents.long() + torch.tensor([[0], [3]], device="cuda")).reshape(-1)
+    want, version = [t[rows] for t in x], [t._version for t in x]
+    beam_reorder(as_what(x), parents)
+    assert all(torch.equal(t, w) for t, w in zip(x, want)) and all(t._version > v for t, v in zip(x, version))
+    src, dst = (torch.tensor([i], dtype=torch.int32, device="cuda") for i in (1, 4))
+    copy_pages(as_what(x), src, dst)
+    assert all(torch.equal(t[4], w[1]) for t, w in zip(x, want))
