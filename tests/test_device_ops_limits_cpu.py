@@ -1,9 +1,11 @@
 """CPU suite: numbers and arguments at the edge of what the operators on device buffers and beam search take."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
-from llama3_np_b200 import Llama, ModelArgs, beam_reorder, copy_pages
+from llama3_np_b200 import Llama, ModelArgs, _cabi, beam_reorder, copy_pages
 
 
 class _Library:
@@ -58,3 +60,24 @@ def test_what_no_tensors_come_from_is_refused():
     for states, error in [((x for x in ()), ValueError), (7, TypeError), (["a"], ValueError)]:
         with pytest.raises(error):
             beam_reorder(states, parents)
+
+
+def _rows(*tensors):
+    return (_cabi.L3Rows * len(tensors))(*(_cabi.L3Rows(*t) for t in tensors))
+
+
+def test_every_tensor_is_checked_ahead_of_the_first_launch():
+    """A tensor that is refused behind more of them than one launch takes: nothing was enqueued, so there is no device to ask for."""
+    lib, some = _cabi.lib(), C.c_void_p(0x1000)
+    fine = [(0x100000 + 64 * i, 6, 64, 1, 0, 64) for i in range(70)]
+    for bad, text in [((0x1, 6, 1 << 31, 1, 0, 1 << 31), b"too long"), ((0x10, 6, 1 << 40, 1 << 30, 64, 64), b"too long"), ((0, 6, 64, 1, 0, 64), b"no data"),
+                      ((0x10, 5, 64, 1, 0, 64), b"5 rows"), ((0x10, 6, 64, -1, 0, 64), b"bad sizes")]:
+        rows = _rows(*fine, bad)
+        assert lib.l3_beam_reorder(0, None, rows, 71, some, 2, 3) == _cabi.L3_EINVAL and text in lib.l3_last_error(None)
+        assert lib.l3_copy_rows(0, None, rows, 71, some, some, 2) == _cabi.L3_EINVAL and text in lib.l3_last_error(None)
+
+
+def test_a_long_row_beside_odd_bytes():
+    """What a row may hold hangs on its own alignment alone."""
+    rows = _rows((0x1000, 6, 1 << 33, 1, 0, 1 << 33), (0x3, 6, 13, 1, 0, 13))
+    assert _cabi.lib().l3_copy_rows(0, None, rows, 2, None, None, 0) == _cabi.L3_OK

@@ -55,3 +55,34 @@ def test_states_from_any_iterable(as_what):
     src, dst = (torch.tensor([i], dtype=torch.int32, device="cuda") for i in (1, 4))
     copy_pages(as_what(x), src, dst)
     assert all(torch.equal(t[4], w[1]) for t, w in zip(x, want))
+
+
+@pytest.mark.parametrize("width", [3, 4096, 50000])
+def test_tensors_of_different_alignment(width):
+    """Bytes, 2-, 4-, 8- and 16-byte pieces in one call, few of them (one launch) and many (one for each size); a hundred tensors."""
+    B, K = 4, 5
+    g = torch.Generator(device="cuda").manual_seed(width)
+    ints = lambda shape, dtype: torch.randint(-100, 100, shape, generator=g, device="cuda").to(dtype)
+    x = [ints((B * K, width, 8), torch.float32), ints((B * K,), torch.bool), ints((B * K, width), torch.int8), ints((B * K, 2 * width + 1), torch.int16),
+         ints((B * K, 5), torch.int32), ints((B * K, 3), torch.int64), torch.zeros(B * K, 0, device="cuda")]
+    x += [ints((B * K, 1 + i % 7), (torch.int8, torch.int32, torch.float64)[i % 3]) for i in range(93)]
+    parents = torch.randint(0, K, (B, K), generator=g, device="cuda").int()
+    rows = (parents.long() + torch.arange(0, B * K, K, device="cuda")[:, None]).reshape(-1)
+    want = [t[rows] for t in x]
+    beam_reorder(x, parents)
+    assert all(torch.equal(t, w) for t, w in zip(x, want))
+    src, dst = torch.tensor([3, 0, -1], device="cuda").int(), torch.tensor([7, 19, 2], device="cuda").int()
+    copy_pages(x, src, dst)
+    for w in want:
+        w[7], w[19] = w[3].clone(), w[0].clone()
+    assert all(torch.equal(t, w) for t, w in zip(x, want))
+
+
+def test_a_refused_tensor_leaves_the_others_as_they_were():
+    lib = _cabi.lib()
+    x = torch.arange(70 * 6, device="cuda").reshape(70, 6).contiguous()
+    parents = torch.tensor([[1, 2, 0], [2, 1, 0]], dtype=torch.int32, device="cuda")
+    rows = (_cabi.L3Rows * 71)(*(_cabi.L3Rows(x[i].data_ptr(), 6, 8, 1, 0, 8) for i in range(70)), _cabi.L3Rows(x.data_ptr() + 1, 6, 1 << 31, 1, 0, 1 << 31))
+    assert lib.l3_beam_reorder(0, None, rows, 71, parents.data_ptr(), 2, 3) == _cabi.L3_EINVAL
+    torch.cuda.synchronize()
+    assert torch.equal(x, torch.arange(70 * 6, device="cuda").reshape(70, 6))
