@@ -10,7 +10,7 @@
 // that two that are close keep the order of the formula - and picks the n best in the same way,
 // its bound the n-th best of the segments' first candidates.
 // Where more values pass a bound than there is room for (many equal ones), the n best are drawn one after the other.
-// Measured (B200, both launches): 32 sequences of 8 beams (37 of the 256 finished), 128256 fp32 logits, 8 best: 30.5 us = 3.7 TB/s, 56 % of what a
+// Measured (B200, both launches): 32 sequences of 8 beams (37 of the 256 finished), 128256 fp32 logits, 8 best: 30.9 us = 3.6 TB/s, 55 % of what a
 // copy reaches (the first launch alone 27 us, 64 %: its warps end together, each with 3 us of looking again); one sequence of 4 beams, 32000
 // logits: 8 us, of which the two launches' own latency is most.  Before: a CTA per slice of 8192 logits with the n-th largest found per slice
 // 70 us; lists kept sorted while streaming 44 us; a lane's third portion looked at one portion at a time, by the lane alone, 44 us.
@@ -130,7 +130,46 @@ __device__ __forceinline__ int unfinished(const unsigned char* done, int rows, i
   return -1;
 }
 
-// part [R, S], cand_v / cand_i [R, S, n].  A portion is 16 words a lane; rows are cut where their addresses are multiples of 16 bytes.
+// A portion that was read from multiples of 16 bytes on, `bytes` of them ahead of its logits, becomes the portion itself: every lane's values move
+// up, and the last ones come from the next lane - lane 31's from lane 0's next four words, at the portion's end from `behind` (word i in lane i).
+__device__ __forceinline__ void move_up(uint32_t (&w)[16], uint32_t behind, int bytes, int lane) {
+  int used = 0;  // words of `behind` so far
+  auto next = [&](int j, int i) {
+    const uint32_t x = __shfl_sync(L3_FULL, lane == 0 && j < 3 ? w[4 * (j < 3 ? j + 1 : 3) + i] : w[4 * j + i], (lane + 1) & 31);
+    if (j < 3) return x;
+    const uint32_t end = __shfl_sync(L3_FULL, behind, used + i);
+    return lane == 31 ? end : x;
+  };
+  if (bytes & 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = next(j, 0), b = next(j, 1);
+      w[4 * j] = w[4 * j + 2]; w[4 * j + 1] = w[4 * j + 3]; w[4 * j + 2] = a; w[4 * j + 3] = b;
+    }
+    used = 2;
+  }
+  if (bytes & 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = next(j, 0);
+      w[4 * j] = w[4 * j + 1]; w[4 * j + 1] = w[4 * j + 2]; w[4 * j + 2] = w[4 * j + 3]; w[4 * j + 3] = a;
+    }
+    ++used;
+  }
+  if (bytes & 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = next(j, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[4 * j + i] = __funnelshift_r(w[4 * j + i], i < 3 ? w[4 * j + (i < 3 ? i + 1 : 3)] : a, 16);
+    }
+  }
+}
+
+// part [R, S], cand_v / cand_i [R, S, n].  A portion is 16 words a lane.  Which logits a lane has of which portion hangs on their index alone,
+// and not on where a row begins: beams with the same logits have the same sum to the last bit, so that equal candidates stay equal.
+// Moving up costs rows that begin between multiples of 16 bytes a tenth: 256 rows of 128257 logits 35.8 us in fp32 and 34.3 in bf16, by places of 16
+// bytes (sums that hang on the address) 33.0 and 31.5; rows of 128256 30.9 and 29.9 with either.
 template <typename T, int NL>
 __global__ void __launch_bounds__(RW * 32, warps_of_sm(sizeof(T) == 4) / RW) beam_rows_kernel(const BeamSelectArgs a, int S, int portions, RowPart* part, float* cand_v, int* cand_i) {
   constexpr int N = Word<T>::N, PIECE = 4 * N, PORTION = 128 * PIECE;  // logits of 16 bytes, of a portion
@@ -148,42 +187,45 @@ __global__ void __launch_bounds__(RW * 32, warps_of_sm(sizeof(T) == 4) / RW) bea
   const int b = row / a.K, k = row - b * a.K;
   const long long list = (long long)row * S + seg;
   const T* x0 = (const T*)a.logits + b * a.sb + k * a.sk;
-  const int skip = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));  // logit v is at place skip + v
-  const int first = seg * portions, stop = min(first + portions, (skip + a.V + PORTION - 1) / PORTION);
-  // whole portions, which are loaded 16 bytes at a time, two ahead; the first and the last of a row may be parts
-  const int lo = max(first, skip ? 1 : 0), hi = min(stop, (skip + a.V) / PORTION);
-  uint32_t wa[16], wb[16];
-  auto load_whole = [&](uint32_t (&w)[16], int p, int of) {  // of: the lane whose values
-    const T* x = x0 + (p * PORTION + of * PIECE - skip);
+  const int skip = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));  // logits from the last multiple of 16 bytes to the row's first
+  const int first = seg * portions, stop = min(first + portions, (a.V + PORTION - 1) / PORTION);
+  // whole portions, which are loaded 16 bytes at a time, two ahead; the last of a row may be a part.  Where skip is not 0, the 16 bytes ahead of a
+  // portion and behind it are touched, too, and have to lie within the row.
+  const int lo = skip ? 1 : 0, hi = min(stop, skip ? max(a.V + skip - PIECE, 0) / PORTION : a.V / PORTION);
+  uint32_t wa[16], wb[16], behind_a = 0, behind_b = 0;
+  auto load_whole = [&](uint32_t (&w)[16], uint32_t& behind, int p, int of) {  // of: the lane whose values; to be moved up by skip
+    const T* x = x0 - skip + (p * PORTION + of * PIECE);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint4 r = __ldcs(reinterpret_cast<const uint4*>(x + j * 32 * PIECE));
       w[4 * j] = r.x; w[4 * j + 1] = r.y; w[4 * j + 2] = r.z; w[4 * j + 3] = r.w;
     }
+    if (skip) behind = __ldcs(reinterpret_cast<const uint32_t*>(x0 - skip + (p + 1) * PORTION) + (lane & 3));
   };
   auto load = [&](uint32_t (&w)[16], int p, int of) {
-    if (p >= lo && p < hi) return load_whole(w, p, of);
-    const int base = p * PORTION + of * PIECE - skip;
+    if (!skip && p < hi) return load_whole(w, behind_a, p, of);
+    const int base = p * PORTION + of * PIECE;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       w[i] = 0;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const int v = base + (i / 4) * 32 * PIECE + (i & 3) * N + e;
-        w[i] |= (v >= 0 && v < a.V ? Word<T>::bits(x0 + v) : Word<T>::NONE) << (16 * e);
+        w[i] |= (v < a.V ? Word<T>::bits(x0 + v) : Word<T>::NONE) << (16 * e);
       }
     }
   };
   float m = -INFINITY, s = 0.f;                             // of this lane
   float v1 = -INFINITY, v2 = -INFINITY, v3 = -INFINITY;     // its portions' largest maxima (NaN is none), and where the first two are
   int p1 = first, p2 = first;
-  auto take = [&](uint32_t (&w)[16], int p, bool more) {
+  auto take = [&](uint32_t (&w)[16], uint32_t& behind, int p, bool whole, bool more) {
+    if (whole && skip) move_up(w, behind, skip * (int)sizeof(T), lane);
     float x[16 * N];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
 #pragma unroll
       for (int e = 0; e < N; ++e) x[i * N + e] = Word<T>::value(w[i], e);
-    if (more) load_whole(w, p + 2, lane);
+    if (more) load_whole(w, behind, p + 2, lane);
     float half[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < 8 * N; ++i) {
@@ -213,18 +255,19 @@ __global__ void __launch_bounds__(RW * 32, warps_of_sm(sizeof(T) == 4) / RW) bea
       p2 = p;
     } else v3 = fmaxf(v3, top);
   };
-  if (lo < hi) load_whole(wa, lo, lane);
-  if (lo + 1 < hi) load_whole(wb, lo + 1, lane);
-  for (int p = lo; p < hi; p += 2) {
-    take(wa, p, p + 2 < hi);
-    if (p + 1 < hi) take(wb, p + 1, p + 3 < hi);
+  if (first < hi) {
+    if (first >= lo) load_whole(wa, behind_a, first, lane);
+    else load(wa, first, lane);
   }
-  auto take_part = [&](int p) {
+  if (first + 1 < hi) load_whole(wb, behind_b, first + 1, lane);
+  for (int p = first; p < hi; p += 2) {
+    take(wa, behind_a, p, p >= lo, p + 2 < hi);
+    if (p + 1 < hi) take(wb, behind_b, p + 1, true, p + 3 < hi);
+  }
+  for (int p = max(first, hi); p < stop; ++p) {
     load(wa, p, lane);
-    take(wa, p, false);
-  };
-  for (int p = first; p < min(lo, stop); ++p) take_part(p);
-  for (int p = max(lo, hi); p < stop; ++p) take_part(p);
+    take(wa, behind_a, p, false, false);
+  }
   const float mw = warp_max(m), from = mw == -INFINITY ? 0.f : mw;
   s = warp_sum(s * ex2((m - from) * 1.4426950408889634f));
   if (lane == 0) part[list] = RowPart{mw, s};
@@ -234,7 +277,7 @@ __global__ void __launch_bounds__(RW * 32, warps_of_sm(sizeof(T) == 4) / RW) bea
   unsigned long long* hit = hits[threadIdx.x >> 5];
   int count = 0;
   auto collect = [&](const uint32_t (&w)[16], int p, int of, bool mine) {  // the values of lane `of` of portion p, if this lane has any
-    const int base = p * PORTION + of * PIECE - skip;
+    const int base = p * PORTION + of * PIECE;
 #pragma unroll
     for (int i = 0; i < 16 * N; ++i) {
       const float x = Word<T>::value(w[i / N], i % N);
@@ -281,7 +324,7 @@ __global__ void __launch_bounds__(RW * 32, warps_of_sm(sizeof(T) == 4) / RW) bea
   best.none();
   for (int p = first; p < stop; ++p) {
     load(wa, p, lane);
-    const int base = p * PORTION + lane * PIECE - skip;
+    const int base = p * PORTION + lane * PIECE;
     for (int i = 0; i < 16 * N; ++i) {
       float x = 0.f;
 #pragma unroll
@@ -484,7 +527,7 @@ struct Cut { int S, portions; };
 // 37.4), of one portion (2 KB of a row) at least.
 Cut cut_of(int rows, int V, int dtype, int n_sm) {
   const bool f32 = dtype == L3_DTYPE_F32;
-  const int portion = f32 ? 512 : 1024, all = (V + 8 + portion - 1) / portion;  // 8: a row may begin behind a multiple of 16 bytes
+  const int portion = f32 ? 512 : 1024, all = (V + portion - 1) / portion;
   const int want = warps_of_sm(f32) * n_sm / rows;
   const int portions = want >= all ? 1 : want <= 1 ? all : (all + want - 1) / want;
   return Cut{(all + portions - 1) / portions, portions};
@@ -497,7 +540,8 @@ template <typename T> cudaError_t launch_rows(const BeamSelectArgs& a, const Cut
 }  // namespace
 
 size_t beam_select_workspace(int B, int K, int V, int n, int n_sm) {
-  const size_t lists = (size_t)B * K * cut_of(B * K, V, L3_DTYPE_F32, n_sm).S;  // 16-bit logits: no more segments
+  const int wide = cut_of(B * K, V, L3_DTYPE_F32, n_sm).S, half = cut_of(B * K, V, L3_DTYPE_BF16, n_sm).S;  // any type's
+  const size_t lists = (size_t)B * K * (wide > half ? wide : half);
   return lists * (sizeof(RowPart) + (size_t)n * 8);
 }
 cudaError_t launch_beam_select(const BeamSelectArgs& a, int n_sm, cudaStream_t s) {
