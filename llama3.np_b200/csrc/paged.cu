@@ -59,6 +59,31 @@ template <typename T> __device__ __forceinline__ void two_parts(float x, float y
     lo = *reinterpret_cast<const uint32_t*>(&r);
   }
 }
+// The same where a factor that is not 0 must not become 0, since the other one may be infinite: what fp16 has no number for enters as its smallest
+// one, 2^-24, and the rest takes that back.  Weights are 0 or more, and what multiplies one of 0 is 0, too (a key that is not there).
+template <typename T> __device__ __forceinline__ void weight_parts(float x, float y, uint32_t& hi, uint32_t& lo) {
+  if constexpr (std::is_same<T, bf16>::value) two_parts<T>(x, y, hi, lo);  // fp32's exponents
+  else {
+    const __half2 h = __hmax2_nan(__floats2half2_rn(x, y), __half2_raw{0x0001, 0x0001});
+    const __half2 r = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+template <typename T> __device__ __forceinline__ void query_parts(float x, float y, uint32_t& hi, uint32_t& lo) {
+  two_parts<T>(x, y, hi, lo);
+  if constexpr (!std::is_same<T, bf16>::value) {
+    const bool low = x != 0.f && !(hi & 0x7fffu), high = y != 0.f && !(hi & 0x7fff0000u);
+    if (!low && !high) return;
+    if (low) hi |= 0x0001u;   // the sign is there already
+    if (high) hi |= 0x00010000u;
+    const __half2 h = *reinterpret_cast<const __half2*>(&hi), r = __floats2half2_rn(x - __low2float(h), y - __high2float(h));
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+// What two parts' products add up to.  Times an infinite value the rest gives an infinity of either sign, or NaN; then the first part alone has the
+// product's sign, and is NaN where the sum is.  (Scores of an fp32 query take 2 % more for it, 48 sequences of up to 4001 tokens 53.5 -> 54.5 us.)
+__device__ __forceinline__ float of_parts(float first, float rest) { return fabsf(rest) < INFINITY ? first + rest : first; }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 16 bytes into shared memory, zeros where !take (the address is not read then)
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
@@ -241,7 +266,7 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
       for (int h = 0; h < 2; ++h) {
         const long long d = qp + ks * 16 + h * 8 + 2 * t;
         uint32_t high, rest;
-        two_parts<T>(load_q(a, d), load_q(a, d + 1), high, rest);
+        query_parts<T>(load_q(a, d), load_q(a, d + 1), high, rest);
         q_word((QLO ? 4 : 2) * ks + h, lane) = high;
         if (QLO) q_word(4 * ks + 2 + h, lane) = rest;
       }
@@ -295,8 +320,8 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
     float mx = -INFINITY;
 #pragma unroll
     for (int n = 0; n < TK / 8; ++n) {
-      s[n][0] = (s[n][0] + (QLO ? s[n][2] : 0.f)) * sc;
-      s[n][1] = (s[n][1] + (QLO ? s[n][3] : 0.f)) * sc;
+      s[n][0] = (QLO ? of_parts(s[n][0], s[n][2]) : s[n][0]) * sc;
+      s[n][1] = (QLO ? of_parts(s[n][1], s[n][3]) : s[n][1]) * sc;
       if (mask != ALL) {
         if (!(mask >> (n * 8 + 2 * t) & 1)) s[n][0] = -INFINITY;
         if (!(mask >> (n * 8 + 2 * t + 1) & 1)) s[n][1] = -INFINITY;
@@ -321,8 +346,8 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
     }
 #pragma unroll
     for (int u = 0; u < TK / 16; ++u) {
-      two_parts<T>(s[2 * u][0], s[2 * u][1], p[u][0], p[u][1]);
-      two_parts<T>(s[2 * u + 1][0], s[2 * u + 1][1], p[u][2], p[u][3]);
+      weight_parts<T>(s[2 * u][0], s[2 * u][1], p[u][0], p[u][1]);
+      weight_parts<T>(s[2 * u + 1][0], s[2 * u + 1][1], p[u][2], p[u][3]);
     }
   }
   __device__ __forceinline__ void add_values(int buf, int lane) {
@@ -349,7 +374,7 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
       const long long oi = ((long long)b * a.H + head0 + g) * HD;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float x[2] = {(o[n][0] + o[n][2]) * inv, (o[n][1] + o[n][3]) * inv};
+        const float x[2] = {of_parts(o[n][0], o[n][2]) * inv, of_parts(o[n][1], o[n][3]) * inv};
         store_out(a, oi + n * 8 + 2 * t, x);
       }
       if (a.lse && t == 0) a.lse[(long long)b * a.H + head0 + g] = (m - BIAS + log2f(l)) * 0.6931471805599453f;
@@ -357,7 +382,7 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
       float* po = part_o + g * HD;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-        *reinterpret_cast<float2*>(po + n * 8 + 2 * t) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+        *reinterpret_cast<float2*>(po + n * 8 + 2 * t) = make_float2(of_parts(o[n][0], o[n][2]), of_parts(o[n][1], o[n][3]));
       if (t == 0) part_ml[g] = make_float2((m - BIAS) * 0.6931471805599453f, l);
     }
   }
