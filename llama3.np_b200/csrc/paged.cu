@@ -82,7 +82,7 @@ template <typename T> __device__ __forceinline__ void query_parts(float x, float
   }
 }
 // What two parts' products add up to.  Times an infinite value the rest gives an infinity of either sign, or NaN; then the first part alone has the
-// product's sign, and is NaN where the sum is.  (Scores of an fp32 query take 2 % more for it, 48 sequences of up to 4001 tokens 53.5 -> 54.5 us.)
+// product's sign, and is NaN where the sum is.  (Scores of an fp32 query take up to 2 % more for it.)
 __device__ __forceinline__ float of_parts(float first, float rest) { return fabsf(rest) < INFINITY ? first + rest : first; }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 16 bytes into shared memory, zeros where !take (the address is not read then)
@@ -231,7 +231,7 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
   uint32_t ring;   // [AHEAD][keys | values] of the warp
   float o[NT][4];
   float m, l;  // of row lane / 4, in units of log 2; l: this lane's share
-  float sc;
+  float sc, down;  // what turns products into scores in units of log 2; the query's share of it
   float s[TK / 8][4];
 
   __device__ __forceinline__ void memory(uint8_t* smem, int warp) {
@@ -260,13 +260,29 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
       for (int ks = 0; ks < KS; ++ks) *reinterpret_cast<uint2*>(&q_word(2 * ks, lane)) = make_uint2(asked[QLO ? 0 : ks][0], asked[QLO ? 0 : ks][1]);
       return;
     }
+    float x[2 * KS][2], up = 1.f;  // read together: fp32 queries, 48 sequences of up to 4001 tokens in fp16 46.1 us, by pairs 54.7; 64 of 4096 in bf16 180.7 : 193.5
+#pragma unroll
+    for (int i = 0; i < 2 * KS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) x[i][e] = load_q(a, qp + i * 8 + 2 * t + e);
+    if constexpr (QLO) {
+      // Times the power of two that takes the row's largest value to [2^14, 2^15), which the scores' scale takes back: two fp16 parts hold a query
+      // of any size then, and values down to 2^-17 of the largest with 22 bits (smaller ones to 2^-39 of the largest); two bf16 parts any finite one.
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) most = fmaxf(most, fmaxf(fabsf(x[i][0]), fabsf(x[i][1])));
+      most = fmaxf(most, __shfl_xor_sync(L3_FULL, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(L3_FULL, most, 2));
+      const int by = min(127 + 14 - (int)(__float_as_uint(most) >> 23), 126);  // -114 to 126
+      up = __uint_as_float((uint32_t)(127 + by) << 23);
+      down = __uint_as_float((uint32_t)(127 - by) << 23);
+    }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const long long d = qp + ks * 16 + h * 8 + 2 * t;
         uint32_t high, rest;
-        query_parts<T>(load_q(a, d), load_q(a, d + 1), high, rest);
+        query_parts<T>(x[2 * ks + h][0] * up, x[2 * ks + h][1] * up, high, rest);
         q_word((QLO ? 4 : 2) * ks + h, lane) = high;
         if (QLO) q_word(4 * ks + 2 + h, lane) = rest;
       }
@@ -276,7 +292,7 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     m = -INFINITY;
     l = 0.f;
-    sc = a.scale * 1.4426950408889634f;
+    sc = a.scale * 1.4426950408889634f * (QLO ? down : 1.f);
   }
   // address of the pieces 2 step + second of a matrix row, ks steps on
   __device__ static __forceinline__ uint32_t matrix_row(uint32_t half, int row, int second, int step) {

@@ -124,3 +124,23 @@ def test_infinite_key_under_a_small_query_value():
     q[:, :, 5] = 2.0 ** -60
     k[table[0, 1].long(), :, 7, 5] = -math.inf
     check(q, k, v, table, n)
+
+
+@pytest.mark.parametrize("kind", list(HALVES))
+@pytest.mark.parametrize("dim", [48, 64, 128])
+@pytest.mark.parametrize("lens,wide", PLANS)
+def test_fp32_queries_of_any_size(kind, dim, lens, wide):
+    """Queries 2^e times as large under a scale 2^-e times as large are the same queries, bit for bit."""
+    q, k, v, table, n = make(7, HALVES[kind], 6, 3, dim, lens, wide)
+    q[:, 1] *= 2.0 ** -12    # every head by itself
+    q[:, 2] *= 2.0 ** -12
+    q[:, 2, 0] = 1.0
+    base = check(q, k, v, table, n, scale=0.25)
+    for e in (-60, -24, -14, -3, 11, 17, 60):
+        assert torch.equal(check(q * 2.0 ** e, k, v, table, n, scale=0.25 * 2.0 ** -e), base)
+
+
+def test_largest_fp32_queries():
+    q, k, v, table, n = make(8, torch.bfloat16, 4, 2, 64, [100, 3], None)
+    q = torch.where(q > 0, 3.4e38, -3.4e38) * (torch.arange(64, device="cuda") % 5 == 0)
+    check(q, k, v, table, n, scale=1.2e-38)
