@@ -2,7 +2,7 @@
 
 The reference decodes greedily only (llama3.py:320).  Both operators enqueue their kernels on the current stream of the tensors'
 device and return, and can be captured into a graph; arguments that do not fit raise ValueError before anything is enqueued.
-Neither has a backward pass: outside torch.no_grad() they refuse tensors that require a gradient.
+Neither has a derivative: outside torch.no_grad() they refuse tensors that require a gradient, and tensors with a forward-mode gradient.
 """
 from __future__ import annotations
 

@@ -3,6 +3,7 @@
 // and the filling of the C structs took 10 - 20 us a call, several times as long as a small call's kernels.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -42,6 +43,8 @@ const Tensor& tensor(PyObject* x, const char* name) {
   NEED(t.layout() == at::kStrided, name, " must be a strided tensor");
   NEED(!t.is_neg(), name, " is a negated view: resolve_neg() it first");
   NEED(!t.requires_grad() || !c10::GradMode::is_enabled(), name, " requires a gradient, and this has no backward pass: call it under torch.no_grad()");
+  NEED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(/*level=*/0).defined(), name,
+       " has a forward-mode gradient, which this would drop: unpack the dual tensor first");
   return t;
 }
 // what a call writes is new to autograd: a backward pass that saved the old values raises

@@ -8,7 +8,8 @@ Every operator enqueues its kernels on the current stream of the tensors' device
 Arguments that do not fit raise ValueError before anything is enqueued.  What is in device memory - lengths, tables - is not
 read by the host: a page number outside the pool names a page that holds no tokens.
 
-The operators have no backward pass: outside torch.no_grad() they refuse tensors that require a gradient.
+The operators have no derivatives: outside torch.no_grad() they refuse tensors that require a gradient, and tensors with a
+forward-mode gradient.
 
 Pools have the dimensions [pages, kv heads, page size, head size] in any memory order whose last dimension is contiguous; a
 pool kept as [pages, page size, kv heads, head size] is passed as `pool.transpose(1, 2)`.

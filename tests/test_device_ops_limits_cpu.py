@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from llama3_np_b200 import Llama, ModelArgs, _cabi, beam_reorder, copy_pages
+from llama3_np_b200 import Llama, ModelArgs, _cabi, beam_reorder, beam_select, copy_pages, paged_attention, paged_write
 
 
 class _Library:
@@ -81,3 +81,25 @@ def test_a_long_row_beside_odd_bytes():
     """What a row may hold hangs on its own alignment alone."""
     rows = _rows((0x1000, 6, 1 << 33, 1, 0, 1 << 33), (0x3, 6, 13, 1, 0, 13))
     assert _cabi.lib().l3_copy_rows(0, None, rows, 2, None, None, 0) == _cabi.L3_OK
+
+
+def test_forward_mode_gradients_are_refused():
+    """A tangent that a call would drop is as wrong as a gradient without its backward pass."""
+    from torch.autograd import forward_ad
+    pool, table, idx = torch.zeros(5, 2, 16, 64), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with forward_ad.dual_level():
+        dual = lambda *shape: forward_ad.make_dual(torch.zeros(*shape), torch.ones(*shape))
+        calls = [lambda: paged_attention(dual(2, 8, 64), pool, pool, table, idx),
+                 lambda: paged_attention(torch.zeros(2, 8, 64), pool, dual(5, 2, 16, 64), table, idx),
+                 lambda: paged_attention(dual(2, 8, 128)[..., :64], pool, pool, table, idx),
+                 lambda: paged_write(dual(2, 4, 2, 64), torch.zeros(2, 4, 2, 64), pool, pool, table, idx),
+                 lambda: copy_pages([pool, dual(5, 3)], idx, idx), lambda: beam_reorder(dual(4, 3), table),
+                 lambda: beam_select(dual(2, 3, 50), torch.zeros(2, 3))]
+        for call in calls:
+            for grad in (True, False):  # no_grad() is of the other mode
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                    call()
+            with forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA device"):
+                call()
+        with pytest.raises(ValueError, match="CUDA device"):
+            beam_select(forward_ad.unpack_dual(dual(2, 3, 50)).primal, torch.zeros(2, 3))
