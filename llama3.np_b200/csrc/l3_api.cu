@@ -1368,7 +1368,12 @@ static int beam_step(L3Model* m, int B, int eos) {
   if (rc != L3_OK || e != cudaSuccess) beam_drop_graph(r);
   if (rc != L3_OK) return rc;
   CK(m, e);
-  CK(m, cudaGraphInstantiate(&r->exec, r->graph, 0));
+  const cudaError_t made = cudaGraphInstantiate(&r->exec, r->graph, 0);
+  if (made != cudaSuccess) {
+    r->exec = nullptr;
+    beam_drop_graph(r);  // the next step's capture would write over its handle
+  }
+  CK(m, made);
   CK(m, cudaGraphLaunch(r->exec, m->stream));
   m->launch_acc += r->nodes;
   return L3_OK;
