@@ -216,8 +216,9 @@ template <int TK, int NCH, bool TURN> struct Tile {
 // ------------------------------------------------------------------------------------------ 16-bit caches: tensor cores
 // The item's (up to 8) query heads are rows 0 - 7 of an m16n8k16 tile.  Rows 8 - 15, which a tile has anyway, carry what rounding to 16
 // bits leaves of the same heads: the rest of an fp32 query in S = Q K^T, the rest of the weights in O += P V, so that the weights
-// enter with 16 (bf16) or 22 (fp16) significant bits at no further instruction.  fp16 weights are scaled by 2^12 ahead of the rounding
-// (they are at most 1), which keeps weights down to 2^-36 of the largest off the subnormals.
+// enter with 16 (bf16) or 22 (fp16) significant bits at no further instruction.  fp16 weights (at most 1) are scaled by 2^12 ahead of the
+// rounding: those from 2^-15 of the largest on enter with 22 bits; below, what counts is that the rest is off by up to half of fp16's smallest
+// number, 2^-37 of the largest weight (weights down to 2^-26 of it are normal numbers themselves, down to 2^-36 more than 0).
 // Keys and values are copied apart, so that a tile's keys make room for those of the tile after next while its values are still in use.
 template <typename T, int HD_, bool QLO> struct MmaCore {
   static constexpr int HD = HD_, TK = HD > 64 ? 16 : 32;

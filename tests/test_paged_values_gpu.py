@@ -144,3 +144,17 @@ def test_largest_fp32_queries():
     q, k, v, table, n = make(8, torch.bfloat16, 4, 2, 64, [100, 3], None)
     q = torch.where(q > 0, 3.4e38, -3.4e38) * (torch.arange(64, device="cuda") % 5 == 0)
     check(q, k, v, table, n, scale=1.2e-38)
+
+
+@pytest.mark.parametrize("kind", list(HALVES))
+@pytest.mark.parametrize("two_parts", [False, True])
+@pytest.mark.parametrize("ahead", [4, 9, 13, 17, 25, 40])
+@pytest.mark.parametrize("wide", [None, 4000])
+def test_many_small_weights_beside_a_large_one(kind, two_parts, ahead, wide):
+    """One key whose score is `ahead` above some 3000 others': weights that 16 bits hold with all their bits, a few of them, and none."""
+    q, k, v, table, n = make(ahead, HALVES[kind], 4, 2, 64, [3001], wide)
+    q[:, :, 0], k[:, :, :, 0] = 8.0, 0.0
+    k[table[0, 77].long(), :, 5, 0] = float(ahead)
+    k[..., 1:] *= 0.25
+    v[table[0, 77].long(), :, 5] = 0.0   # the small ones are what is left
+    check(q if two_parts else q.to(k.dtype), k, v, table, n)
