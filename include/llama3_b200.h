@@ -451,7 +451,8 @@ int l3_copy_rows(int device, void* stream, const L3Rows* tensors, int n_tensors,
  * outside [0, beams) leaves the row as it is.  beams <= 256. */
 int l3_beam_reorder(int device, void* stream, const L3Rows* tensors, int n_tensors, const int32_t* parents, int batch, int beams);
 /* The `best` (at most 64) continuations of a sequence's beams: largest scores[b, k] + logits[b, k, v] - log sum_u exp(logits[b, k, u])
- * first, equal ones by k * vocab + v.  A finished beam (done[b, k] != 0) has one continuation, the token eos at its own score.
+ * first, equal ones by k * vocab + v (beams with the same logits have the same sum; of different ones, scores closer than 2^-19 may come in either
+ * order).  A finished beam (done[b, k] != 0) has one continuation, the token eos at its own score.
  * Candidates of score -infinity, +infinity or NaN are none; a place without candidate gets score -infinity, the token eos (0 without
  * one), parent 0 and done.  out_done: the parent was done, or the token is eos (-1: no end token). */
 typedef struct L3BeamSelect {

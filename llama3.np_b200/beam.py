@@ -19,6 +19,8 @@ def beam_select(logits, scores, best=None, *, done=None, eos_id=None):
     Returns scores [batch, best] fp32 in falling order (equal ones by beam, then token), tokens and parents (beams of the same
     sequence) [batch, best] int32, and done [batch, best] bool: the parent had ended, or the token is eos_id.  A score that is
     -inf, +inf or NaN is no continuation; a place that none is left for has score -inf, the token eos_id (or 0), parent 0, done.
+    Beams with the same logits have the same sum of exponentials; of different ones, whose sums are of fp32 terms, scores closer
+    than 2^-19 may come in either order.
     """
     return _ops().beam_select(logits, scores, best, done, eos_id)
 
