@@ -41,3 +41,28 @@ def test_equal_rows_at_any_address(kind, V, K, n):
             same = {}
             for s, t in zip(got[b].tolist(), tokens[b].tolist()):
                 assert same.setdefault(t, s) == s
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("V", [1, 3, 17, 511, 513, 1030, 4097, 30001])
+@pytest.mark.parametrize("n", [1, 33, 64])
+@pytest.mark.parametrize("values", ["random", "few", "rare"])
+def test_results_hang_on_no_address(kind, V, n, values):
+    """The same logits at every phase of 16 bytes, with steps between rows that change it and steps that do not: bit for bit the same results."""
+    g = torch.Generator(device="cuda").manual_seed(V + n)
+    B, K = 3, 3
+    x = torch.randn(B, K, V, generator=g, device="cuda") * 4
+    if values == "few":
+        x = x.round()                    # many equal ones
+    elif values == "rare":
+        x[torch.rand(x.shape, generator=g, device="cuda") < 0.97] = -torch.inf
+    x = x.to(TYPES[kind])
+    scores = torch.randn(B, K, generator=g, device="cuda")
+    wide = -(-V // 8) * 8
+    base = torch.zeros(B, K, wide, dtype=TYPES[kind], device="cuda")[:, :, :V]
+    base.copy_(x)
+    want = beam_select(base, scores, n, eos_id=0)
+    for step, first in [(wide + 8, f) for f in range(8)] + [(V + 3, f) for f in range(3)] + [(V, 0)]:
+        y = torch.full((B, K, step), 50.0, dtype=TYPES[kind], device="cuda")[:, :, first:first + V]  # what lies beside a row is larger
+        y.copy_(x)
+        assert all(torch.equal(a, b) for a, b in zip(beam_select(y, scores, n, eos_id=0), want)), (step, first)
