@@ -267,14 +267,16 @@ template <typename T, int HD_, bool QLO> struct MmaCore {
 #pragma unroll
       for (int e = 0; e < 2; ++e) x[i][e] = load_q(a, qp + i * 8 + 2 * t + e);
     if constexpr (QLO) {
-      // Times the power of two that takes the row's largest value to [2^14, 2^15), which the scores' scale takes back: two fp16 parts hold a query
-      // of any size then, and values down to 2^-17 of the largest with 22 bits (smaller ones to 2^-39 of the largest); two bf16 parts any finite one.
+      // Times a power of two, which the scores' scale takes back.  fp16: the one that takes the row's largest value to [2^14, 2^15), so that two
+      // parts hold a query of any size, values down to 2^-17 of the largest with 22 bits (smaller ones to 2^-39 of the largest).  bf16, which has
+      // fp32's exponents: one that takes a largest value of 4 or more to [2, 4), so that none rounds to infinity; never up, since keys may be as large.
       float most = 0.f;
 #pragma unroll
       for (int i = 0; i < 2 * KS; ++i) most = fmaxf(most, fmaxf(fabsf(x[i][0]), fabsf(x[i][1])));
       most = fmaxf(most, __shfl_xor_sync(L3_FULL, most, 1));
       most = fmaxf(most, __shfl_xor_sync(L3_FULL, most, 2));
-      const int by = min(127 + 14 - (int)(__float_as_uint(most) >> 23), 126);  // -114 to 126
+      constexpr bool WIDE = std::is_same<T, bf16>::value;
+      const int by = max(min(127 + (WIDE ? 1 : 14) - (int)(__float_as_uint(most) >> 23), WIDE ? 0 : 126), -126);
       up = __uint_as_float((uint32_t)(127 + by) << 23);
       down = __uint_as_float((uint32_t)(127 - by) << 23);
     }

@@ -158,3 +158,14 @@ def test_many_small_weights_beside_a_large_one(kind, two_parts, ahead, wide):
     k[..., 1:] *= 0.25
     v[table[0, 77].long(), :, 5] = 0.0   # the small ones are what is left
     check(q if two_parts else q.to(k.dtype), k, v, table, n)
+
+
+@pytest.mark.parametrize("two_parts", [False, True])
+def test_large_keys(two_parts):
+    """bf16 keys as large as fp32's under a scale that makes their scores ordinary ones: no product of theirs and a query's is infinite."""
+    q, k, v, table, n = make(9, torch.bfloat16, 4, 2, 64, [100, 3, 700], None)
+    k *= torch.where(torch.arange(64, device="cuda") % 9 == 0, 1e37, 1e30)
+    q = q.clamp(-3, 3)
+    check(q if two_parts else q.bfloat16(), k, v, table, n, scale=2e-38)
+    if two_parts:
+        check(q * 2.0 ** -70, k, v, table, n, scale=2e-38 * 2.0 ** 70)
