@@ -471,6 +471,94 @@ typedef struct L3BeamSelect {
 int l3_beam_select_workspace(int device, int batch, int beams, int vocab, int best, int64_t* bytes);
 int l3_beam_select(const L3BeamSelect* a);
 
+/* -- operators on device buffers: a packed step ---------------------------------------------------------------------
+ * The new tokens of many requests, one or thousands each, as the rows of ONE batch over a cache in pages: request b's rows are
+ * starts[b] .. starts[b + 1] - 1, its newest tokens in order.  Rows behind the last request belong to none.  Pointers, streams, workspaces and
+ * errors as above. */
+/* The step's bookkeeping on the device.  Request b has lengths[b] tokens and gets counts[b] more (negative numbers count as 0), fewer where the
+ * rows are used up: out_lengths[b] tokens then, rows out_starts[b] .. out_starts[b + 1] - 1.  New pages come from free_pages in
+ * order, request by request, and go into its row of the table behind the pages of the tokens it had; where the list is used up they are -1,
+ * and what the table has no column for is dropped.  A row's position is its token's number in its request, its slot the place
+ * page * page_size + position % page_size; both are -1 for rows of no request, the slot also where there is no page.  out_used: pages that
+ * were needed (more than n_free: too few were given). */
+typedef struct L3PagedExtend {
+  int32_t device;
+  int32_t batch, tokens, max_pages, page_size, n_free;
+  void* stream;
+  int32_t* table;                            /* [batch, max_pages], in and out */
+  int64_t table_stride;
+  const int32_t *lengths, *counts, *free_pages;  /* [batch], [batch], [n_free] */
+  int32_t *out_lengths, *out_starts, *out_positions;  /* [batch], [batch + 1], [tokens] */
+  int64_t* out_slots;                        /* [tokens] */
+  int32_t* out_used;                         /* [1] */
+} L3PagedExtend;
+int l3_paged_extend(const L3PagedExtend* a);
+/* Rotary positions: entries a and b of a pair become (a cos - b sin, b cos + a sin), each times `amplitude`, by the angle positions[row] *
+ * frequencies[pair] (taken in 64 bits); inverse != 0: by the negative angle.  The first `dims` entries of a head are turned, the others and the
+ * rows at negative positions are not.  layout 0: pairs (2 i, 2 i + 1) (llama3.py:41-76), 1: (i, i + dims / 2).  The rows are batch x tokens.
+ * With k and v (kv_heads > 0; batch 1) k is turned, too, and both go to their slots of the pools: slot page * page_size + place; a slot outside
+ * the pool is none.  No two rows share a slot. */
+typedef struct L3Rotary {
+  int32_t device;
+  int32_t batch, tokens, heads, head_dim, dims, layout, inverse, dtype;
+  int32_t kv_heads, pages, page_size;
+  float amplitude;
+  int32_t reserved;
+  void* stream;
+  const int32_t* positions;                  /* [batch * tokens] */
+  const double* frequencies;                 /* [dims / 2] */
+  const void* x;                             /* [batch, tokens, heads, head_dim], strides in elements; heads may be 0 */
+  int64_t x_batch_stride, x_token_stride, x_head_stride;
+  void* out;                                 /* may be x, with its strides */
+  int64_t out_batch_stride, out_token_stride, out_head_stride;
+  const void *k, *v;                         /* [tokens, kv_heads, head_dim] */
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const int64_t* slots;                      /* [tokens] */
+  L3PagePool k_pool, v_pool;
+} L3Rotary;
+int l3_rotary(const L3Rotary* a);
+/* Attention of the rows of a packed step over their requests' pages: row t of request b, at position p = lengths[b] - (starts[b + 1] - starts[b])
+ * + t, sees the tokens j <= p.  lengths count the rows' own tokens, whose keys and values are in their pages already.  Pages outside [0, pages) hold
+ * no tokens, lengths are cut to [0, max_pages * page_size]; a row that sees no token gets 0 and lse -infinity.  Rows of no request are left as they
+ * are, or set to 0 (lse -infinity) with clear_rest != 0.  A value that a row does not see has no part in its result, not even a NaN. */
+typedef struct L3PagedChunk {
+  int32_t device;
+  int32_t batch, tokens, heads, kv_heads, head_dim;  /* head_dim 16, 32, 48, 64, 96, 128 */
+  int32_t pages, page_size, max_pages;
+  int32_t dtype;                             /* of q, the pools and out */
+  int32_t clear_rest;
+  float scale;                               /* of q . k */
+  void* stream;
+  const void* q;                             /* [tokens, heads, head_dim] */
+  int64_t q_token_stride, q_head_stride;
+  L3PagePool k, v;
+  const int32_t* table;                      /* [batch, max_pages] */
+  int64_t table_stride;
+  const int32_t *lengths, *starts;           /* [batch], [batch + 1] */
+  void* out;                                 /* [tokens, heads, head_dim], contiguous */
+  float* lse;                                /* [tokens, heads] or null */
+  void* workspace;
+  int64_t workspace_bytes;
+} L3PagedChunk;
+/* bytes that l3_paged_chunk_attention wants as its workspace, for this type, heads, kv_heads, head_dim and number of rows and any lengths */
+int l3_paged_chunk_workspace(int device, int tokens, int heads, int kv_heads, int head_dim, int dtype, int64_t* bytes);
+int l3_paged_chunk_attention(const L3PagedChunk* a);
+/* Of every row of logits: the log probability of its token, x[token] - log sum_v e^x[v]; if asked for, the entropy - sum_v p_v log p_v
+ * and the `top` most likely tokens, largest logit first, equal ones by token.  A negative token is none: its log probability is 0; one beyond the
+ * vocabulary has NaN.  Tokens of logit -infinity have probability 0, and a place of `top` that no other token is left for gets the token -1
+ * at -infinity; a row of them alone has entropy 0 and log probabilities -infinity; +infinity or NaN in a row make its numbers NaN. */
+typedef struct L3TokenLogprobs {
+  int32_t device, rows, vocab, top, dtype, reserved;  /* top: 0 - 64 */
+  void* stream;
+  const void* logits;                        /* [rows, vocab], last dimension contiguous */
+  int64_t row_stride;
+  const int32_t* tokens;                     /* [rows] */
+  float *out_logprobs, *out_entropy;         /* [rows]; out_entropy may be null */
+  float* out_top_logprobs;                   /* [rows, top] */
+  int32_t* out_top_tokens;
+} L3TokenLogprobs;
+int l3_token_logprobs(const L3TokenLogprobs* a);
+
 /* How the model path cuts a tensor-core projection of `rows` rows in bf16 mode, or with fp32 != 0 one of up to 128 rows of the Llama
  * path's fp32 mode (epi 0: plain store, 1: added to the residual in place, 2: gated):
  * plan[0] 1 = weights as the 128-row operand (gemm_swap.cu), 0 = activations (gemm_tc.cu); [1] CTAs that share a tile as a pair or, where

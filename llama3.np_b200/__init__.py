@@ -40,6 +40,10 @@ def __getattr__(name):  # lazy: importing the package must not require the built
     if name in ("paged_attention", "paged_write", "copy_pages", "PagedCache", "PageTable"):
         from . import paged as _p
         return getattr(_p, name)
+    if name in ("PackedStep", "TokenLogprobs", "paged_chunk_attention", "paged_extend", "paged_rotary_write", "rotary", "rotary_frequencies",
+                "token_logprobs"):
+        from . import packed as _k
+        return getattr(_k, name)
     if name in ("beam_select", "beam_reorder"):
         from . import beam as _b
         return getattr(_b, name)

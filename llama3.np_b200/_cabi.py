@@ -104,6 +104,39 @@ class L3BeamSelect(C.Structure):
                 ("out_parents", C.c_void_p), ("out_done", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+class L3PagedExtend(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("device", "batch", "tokens", "max_pages", "page_size", "n_free")] + [
+                ("stream", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64)] + [
+                (n, C.c_void_p) for n in ("lengths", "counts", "free_pages", "out_lengths", "out_starts", "out_positions", "out_slots",
+                                          "out_used")]
+
+
+class L3Rotary(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("device", "batch", "tokens", "heads", "head_dim", "dims", "layout", "inverse", "dtype", "kv_heads",
+                                         "pages", "page_size")] + [
+                ("amplitude", C.c_float), ("reserved", C.c_int32), ("stream", C.c_void_p), ("positions", C.c_void_p),
+                ("frequencies", C.c_void_p), ("x", C.c_void_p), ("x_batch_stride", C.c_int64), ("x_token_stride", C.c_int64),
+                ("x_head_stride", C.c_int64), ("out", C.c_void_p), ("out_batch_stride", C.c_int64), ("out_token_stride", C.c_int64),
+                ("out_head_stride", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("k_token_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64), ("slots", C.c_void_p),
+                ("k_pool", L3PagePool), ("v_pool", L3PagePool)]
+
+
+class L3PagedChunk(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("device", "batch", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_size", "max_pages",
+                                         "dtype", "clear_rest")] + [
+                ("scale", C.c_float), ("stream", C.c_void_p), ("q", C.c_void_p), ("q_token_stride", C.c_int64),
+                ("q_head_stride", C.c_int64), ("k", L3PagePool), ("v", L3PagePool), ("table", C.c_void_p), ("table_stride", C.c_int64),
+                ("lengths", C.c_void_p), ("starts", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+class L3TokenLogprobs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("device", "rows", "vocab", "top", "dtype", "reserved")] + [
+                ("stream", C.c_void_p), ("logits", C.c_void_p), ("row_stride", C.c_int64)] + [
+                (n, C.c_void_p) for n in ("tokens", "out_logprobs", "out_entropy", "out_top_logprobs", "out_top_tokens")]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _F32P = C.POINTER(C.c_float)
@@ -159,6 +192,11 @@ SIGNATURES = {
     "l3_beam_reorder": (_I, [_I, _P, C.POINTER(L3Rows), _I, _P, _I, _I]),
     "l3_beam_select_workspace": (_I, [_I, _I, _I, _I, _I, _I64P]),
     "l3_beam_select": (_I, [C.POINTER(L3BeamSelect)]),
+    "l3_paged_extend": (_I, [C.POINTER(L3PagedExtend)]),
+    "l3_rotary": (_I, [C.POINTER(L3Rotary)]),
+    "l3_paged_chunk_workspace": (_I, [_I] * 6 + [_I64P]),
+    "l3_paged_chunk_attention": (_I, [C.POINTER(L3PagedChunk)]),
+    "l3_token_logprobs": (_I, [C.POINTER(L3TokenLogprobs)]),
     "l3_debug_tc_timeline": (_I, [_I, _I, C.POINTER(C.c_uint64)]),
     "l3_sync": (_I, [_P]),
     "l3_timer_start": (_I, [_P]),

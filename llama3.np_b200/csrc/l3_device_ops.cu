@@ -3,6 +3,7 @@
 
 #include "../../include/llama3_b200.h"
 #include "internal.h"
+#include "packed.h"
 #include "paged.h"
 
 #define CKD(call) CK(((L3Model*)nullptr), call)
@@ -228,5 +229,128 @@ extern "C" int l3_beam_select(const L3BeamSelect* a) {
   s.scores = a->scores; s.done = a->done; s.eos = a->eos; s.B = a->batch; s.K = a->beams; s.V = a->vocab; s.n = a->best;
   s.out_scores = a->out_scores; s.out_tokens = a->out_tokens; s.out_parents = a->out_parents; s.out_done = a->out_done; s.ws = a->workspace;
   CKD(launch_beam_select(s, n_sm, (cudaStream_t)a->stream));
+  return L3_OK;
+}
+
+// ------------------------------------------------------------------------------------------------------------ a packed step
+extern "C" int l3_paged_extend(const L3PagedExtend* a) {
+  REQ(a != nullptr, "no arguments");
+  REQ(a->batch >= 0 && a->tokens >= 0 && a->n_free >= 0, "bad sizes");
+  int rc;
+  if ((rc = check_pages(1, a->page_size, a->max_pages)) != L3_OK) return rc;
+  REQ(a->out_starts && a->out_used, "out_starts or out_used missing");
+  REQ(a->batch == 0 || (a->lengths && a->counts && a->out_lengths && (a->table || a->max_pages == 0)), "lengths, counts, table or out_lengths missing");
+  REQ(a->tokens == 0 || (a->out_positions && a->out_slots), "out_positions or out_slots missing");
+  REQ(a->n_free == 0 || a->free_pages, "free_pages missing");
+  OnDevice on(a->device);
+  CKD(on.e);
+  int n_sm = 0;
+  CKD(sm_count(a->device, &n_sm));
+  PagedExtendArgs p{};
+  p.table = a->table; p.table_stride = a->table_stride; p.max_pages = a->max_pages; p.log_page = log2_of(a->page_size);
+  p.B = a->batch; p.T = a->tokens; p.n_free = a->n_free;
+  p.lengths = a->lengths; p.counts = a->counts; p.free_pages = a->free_pages;
+  p.out_lengths = a->out_lengths; p.out_starts = a->out_starts; p.out_positions = a->out_positions;
+  p.out_slots = (long long*)a->out_slots; p.out_used = a->out_used;
+  CKD(launch_paged_extend(p, n_sm, (cudaStream_t)a->stream));
+  return L3_OK;
+}
+
+extern "C" int l3_rotary(const L3Rotary* a) {
+  REQ(a != nullptr, "no arguments");
+  REQ(a->batch >= 0 && a->tokens >= 0 && a->heads >= 0 && a->kv_heads >= 0, "bad sizes");
+  REQ(a->head_dim >= 1 && a->head_dim <= 1024 && a->dims >= 0 && a->dims % 2 == 0 && a->dims <= a->head_dim,
+      "dims %d of head_dim %d (at most 1024): an even number of entries is turned", a->dims, a->head_dim);
+  REQ((a->layout == 0 || a->layout == 1) && known(a->dtype), "bad layout or dtype");
+  REQ(a->kv_heads == 0 || a->batch == 1, "keys and values are rows of one batch");
+  REQ((int64_t)a->batch * a->tokens < ((int64_t)1 << 31) && ((int64_t)a->heads + 2 * (int64_t)a->kv_heads) * a->head_dim < (1 << 28),
+      "%d x %d rows of %d heads are too many", a->batch, a->tokens, a->heads);
+  const int size = size_of(a->dtype);
+  if (a->batch == 0 || a->tokens == 0 || (a->heads == 0 && a->kv_heads == 0)) return L3_OK;
+  REQ(a->positions && (a->frequencies || a->dims == 0), "positions or frequencies missing");
+  REQ(a->heads == 0 || (a->x && a->out && (uintptr_t)a->x % size == 0 && (uintptr_t)a->out % size == 0), "x or out missing, or not aligned to its type");
+  REQ(((uintptr_t)a->frequencies & 7) == 0, "frequencies must be aligned to 8 bytes");
+  RotaryArgs p{};
+  if (a->kv_heads) {
+    int rc;
+    if ((rc = check_pages(a->pages, a->page_size, 0)) != L3_OK) return rc;
+    if ((rc = check_pool(a->k_pool, size, "k_pool")) != L3_OK || (rc = check_pool(a->v_pool, size, "v_pool")) != L3_OK) return rc;
+    REQ(a->k && a->v && a->slots && (uintptr_t)a->k % size == 0 && (uintptr_t)a->v % size == 0, "k, v or slots missing, or not aligned");
+    p.log_page = log2_of(a->page_size);
+  }
+  OnDevice on(a->device);
+  CKD(on.e);
+  int n_sm = 0;
+  CKD(sm_count(a->device, &n_sm));
+  p.positions = a->positions; p.freqs = a->frequencies; p.amplitude = a->amplitude; p.inverse = a->inverse != 0;
+  p.x = a->x; p.x_sb = a->x_batch_stride; p.x_st = a->x_token_stride; p.x_sh = a->x_head_stride;
+  p.out = a->out; p.o_sb = a->out_batch_stride; p.o_st = a->out_token_stride; p.o_sh = a->out_head_stride;
+  p.k = a->k; p.v = a->v; p.k_st = a->k_token_stride; p.k_sh = a->k_head_stride; p.v_st = a->v_token_stride; p.v_sh = a->v_head_stride;
+  p.slots = (const long long*)a->slots; p.kp = pool_of(a->k_pool, 1); p.vp = pool_of(a->v_pool, 1); p.n_pages = a->pages;
+  p.B = a->batch; p.L = a->tokens; p.H = a->heads; p.G = a->kv_heads; p.D = a->head_dim; p.dims = a->dims; p.layout = a->layout; p.dtype = a->dtype;
+  CKD(launch_rotary(p, n_sm, (cudaStream_t)a->stream));
+  return L3_OK;
+}
+
+static int check_chunk(int tokens, int heads, int kv_heads, int head_dim, int dtype) {
+  REQ(tokens >= 0 && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, "heads %d not a multiple of kv_heads %d", heads, kv_heads);
+  REQ(attn_head_dim_supported(head_dim), "head_dim %d unsupported (16,32,48,64,96,128)", head_dim);
+  REQ(known(dtype), "bad dtype");
+  REQ((int64_t)tokens * (heads / kv_heads) < ((int64_t)1 << 31) - 65536, "%d rows of %d heads are too many", tokens, heads);
+  return L3_OK;
+}
+extern "C" int l3_paged_chunk_workspace(int device, int tokens, int heads, int kv_heads, int head_dim, int dtype, int64_t* bytes) {
+  REQ(bytes != nullptr, "no place for the answer");
+  int rc = check_chunk(tokens, heads, kv_heads, head_dim, dtype), n_sm = 0;
+  if (rc != L3_OK) return rc;
+  CKD(sm_count(device, &n_sm));
+  *bytes = (int64_t)paged_chunk_workspace(tokens, heads, kv_heads, head_dim, dtype, n_sm);
+  return L3_OK;
+}
+extern "C" int l3_paged_chunk_attention(const L3PagedChunk* a) {
+  REQ(a != nullptr, "no arguments");
+  int rc = check_chunk(a->tokens, a->heads, a->kv_heads, a->head_dim, a->dtype);
+  if (rc != L3_OK) return rc;
+  REQ(a->batch >= 0, "bad batch");
+  if ((rc = check_pages(a->pages, a->page_size, a->max_pages)) != L3_OK) return rc;
+  if (a->tokens == 0 || (a->batch == 0 && !a->clear_rest)) return L3_OK;
+  const int size = size_of(a->dtype);
+  if ((rc = check_pool(a->k, size, "k")) != L3_OK || (rc = check_pool(a->v, size, "v")) != L3_OK) return rc;
+  REQ(a->q && a->out && (a->batch == 0 || (a->lengths && a->starts && (a->table || a->max_pages == 0))), "q, out, lengths, starts or table missing");
+  REQ(aligned16(a->q) && strides16(size, {a->q_token_stride, a->q_head_stride}) && aligned16(a->out) && ((uintptr_t)a->lse & 3) == 0,
+      "q and out: addresses must be multiples of 16 bytes");
+  OnDevice on(a->device);
+  CKD(on.e);
+  int n_sm = 0;
+  CKD(sm_count(a->device, &n_sm));
+  const size_t need = paged_chunk_workspace(a->tokens, a->heads, a->kv_heads, a->head_dim, a->dtype, n_sm);
+  REQ(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= (int64_t)need, "the workspace must be %zu bytes, aligned to 16", need);
+  ChunkArgs p{};
+  p.q = a->q; p.q_st = a->q_token_stride; p.q_sh = a->q_head_stride;
+  p.k = pool_of(a->k, 1); p.v = pool_of(a->v, 1); p.n_pages = a->pages; p.log_page = log2_of(a->page_size);
+  p.table = a->table; p.table_stride = a->table_stride; p.max_pages = a->max_pages; p.lengths = a->lengths; p.starts = a->starts;
+  p.B = a->batch; p.T = a->tokens; p.H = a->heads; p.G = a->kv_heads; p.R = a->heads / a->kv_heads; p.HD = a->head_dim; p.dtype = a->dtype;
+  p.scale = a->scale; p.out = a->out; p.lse = a->lse; p.clear_rest = a->clear_rest != 0; p.ws = a->workspace;
+  CKD(launch_paged_chunk(p, n_sm, (cudaStream_t)a->stream));
+  return L3_OK;
+}
+
+extern "C" int l3_token_logprobs(const L3TokenLogprobs* a) {
+  REQ(a != nullptr, "no arguments");
+  REQ(a->rows >= 0 && a->vocab >= 1 && a->vocab < (1 << 24), "vocab %d or rows %d", a->vocab, a->rows);
+  REQ(a->top >= 0 && a->top <= LOGPROBS_MAX_TOP && a->top <= a->vocab, "top %d: 0 to %d, and not beyond the vocabulary", a->top, LOGPROBS_MAX_TOP);
+  REQ(known(a->dtype), "bad dtype");
+  if (a->rows == 0) return L3_OK;
+  REQ(a->logits && a->tokens && a->out_logprobs && (a->top == 0 || (a->out_top_logprobs && a->out_top_tokens)), "a buffer is missing");
+  REQ((uintptr_t)a->logits % size_of(a->dtype) == 0, "logits are not aligned to their type");
+  OnDevice on(a->device);
+  CKD(on.e);
+  int n_sm = 0;
+  CKD(sm_count(a->device, &n_sm));
+  LogprobsArgs p{};
+  p.logits = a->logits; p.stride = a->row_stride; p.dtype = a->dtype; p.R = a->rows; p.V = a->vocab; p.n = a->top;
+  p.tokens = a->tokens; p.out_logprobs = a->out_logprobs; p.out_entropy = a->out_entropy; p.out_top = a->out_top_logprobs;
+  p.out_top_tokens = a->out_top_tokens;
+  CKD(launch_token_logprobs(p, n_sm, (cudaStream_t)a->stream));
   return L3_OK;
 }

@@ -1,0 +1,331 @@
+// Attention of the rows of a packed step over a key / value cache in pages (L3PagedChunk):
+//   s_j = scale q_t . k_j,  o_t = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  lse_t = m + log sum_j e^(s_j - m),  m = max_j s_j
+// over the tokens j that row t sees, j <= its position.  paged_chunk.cuh says how the work is cut.
+//
+// This file: the products as FFMA, queries, keys, values, weights and sums in fp32; and the join of what several CTAs have of an item.
+// A CTA's 256 threads hold 64 rows and walk their keys, 64 at a time.  Keys and values come row by row through the page table, 16 bytes a
+// copy, while the tile before is worked on; rows of no token become zeros.
+//   scores   a thread has 4 rows x 4 keys, summed as even and odd entries (pairs: fma2); rows padded to an odd number of 16-byte pieces
+//   output   a thread has 4 rows x HD / 16 columns, in pairs of rows; the weights arrive through shared memory, [key][row]
+#include <algorithm>
+
+#include "paged_chunk.cuh"
+
+namespace {
+using namespace chunk;
+constexpr int TR = 64, BK = 64, NT = 256;
+constexpr int WHOLE = 4, LEAST = 4;
+template <int HD> constexpr int row_ld() { return HD + 4; }
+template <int HD> constexpr size_t smem_bytes() { return (size_t)(2 * 64 * row_ld<HD>() + 64 * HD + 64 * (TR + 4)) * 4 + 2 * 2 * BK * 8 + 2 * 8 + 16; }
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {  // zeros where !take
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const ChunkArgs a) {
+  constexpr int LD = row_ld<HD>(), PL = TR + 4;
+  constexpr int CW = HD % 64 == 0 ? 4 : HD % 32 == 0 ? 2 : 1, NC = HD / (16 * CW);  // columns side by side, and how often
+  extern __shared__ __align__(16) float sm[];
+  float* sQ = sm;                     // [64][LD]
+  float* sK = sQ + 64 * LD;           // [64][LD]
+  float* sV = sK + 64 * LD;           // [64][HD]
+  float* sP = sV + 64 * HD;           // [keys][rows]
+  long long* sOff = reinterpret_cast<long long*>(sP + 64 * PL);  // [turn][k, v][64]
+  unsigned* sThere = reinterpret_cast<unsigned*>(sOff + 2 * 2 * BK);  // [turn][2] bits of keys that there are
+  __shared__ long long room[NT / 32 + 1];
+  __shared__ Place place;
+  pdl_launch();
+  pdl_wait();
+  clear_rest<T>(a);
+  find_share<TR, BK, NT, LEAST>(a, room, &place);
+  if (threadIdx.x < 2) *info_of(a, blockIdx.x, threadIdx.x) = make_int4(-1, 0, 0, 0);
+  __syncthreads();
+  const int lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const float sc = a.scale * 1.4426950408889634f;
+  Cursor<TR, BK, WHOLE> c;
+  if (!c.start(a, place)) return;
+  do {
+    const int* table = a.table + c.b * a.table_stride;
+    const int flat0 = c.tile * TR, flats = c.r.n * a.R;
+    const int most = c.r.seen((min(flats, flat0 + TR) - 1) / a.R);   // keys that any of the rows sees
+    // the rows' queries
+    for (int i = threadIdx.x; i < TR * HD; i += NT) {
+      const int r = i / HD, d = i - r * HD, f = flat0 + r;
+      float x = 0.f;
+      if (f < flats) {
+        const int t = f / a.R;
+        x = up(((const T*)a.q)[(c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh + d]);
+      }
+      sQ[r * LD + d] = x;
+    }
+    auto offsets = [&](int j) {  // by the first 64 threads
+      if (threadIdx.x >= BK) return;
+      const int key = j * BK + threadIdx.x, turn = j & 1;
+      int page = -1;
+      if (key < most) page = table[key >> a.log_page];
+      const bool there = (unsigned)page < (unsigned)a.n_pages;
+      const long long in = key & ((1 << a.log_page) - 1);
+      sOff[turn * 2 * BK + threadIdx.x] = there ? page * a.k.sp + c.g * a.k.sh + in * a.k.st : -1;
+      sOff[turn * 2 * BK + BK + threadIdx.x] = there ? page * a.v.sp + c.g * a.v.sh + in * a.v.st : -1;
+      const unsigned bits = __ballot_sync(L3_FULL, there);
+      if (lane == 0) sThere[turn * 2 + (threadIdx.x >> 5)] = bits;
+    };
+    auto copy = [&](int j, bool value) {
+      const long long* off = sOff + (j & 1) * 2 * BK + (value ? BK : 0);
+      const T* pool = (const T*)(value ? a.v.p : a.k.p);
+      float* dst = value ? sV : sK;
+      const int ld = value ? HD : LD;
+      constexpr int E = 16 / sizeof(T), PIECES = HD / E;
+      for (int i = threadIdx.x; i < BK * PIECES; i += NT) {
+        const int r = i / PIECES, p = i - r * PIECES;
+        const long long at = off[r];
+        if constexpr (sizeof(T) == 4) {
+          cp16(smem_u32(dst + r * ld + p * 4), at >= 0 ? pool + at + p * 4 : pool, at >= 0);
+        } else {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (at >= 0) x = *reinterpret_cast<const uint4*>(pool + at + p * E);
+          const T* v = reinterpret_cast<const T*>(&x);
+#pragma unroll
+          for (int e = 0; e < E; ++e) dst[r * ld + p * E + e] = up(v[e]);
+        }
+      }
+      cp_commit();
+    };
+    int seen[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int f = flat0 + ty * 4 + i;
+      seen[i] = f < flats ? c.r.seen(f / a.R) : 0;
+    }
+    float2 o[2][NC * CW];   // pairs of rows
+    float m[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+#pragma unroll
+    for (int x = 0; x < NC * CW; ++x) o[0][x] = o[1][x] = make_float2(0.f, 0.f);
+    if (c.j0 < c.j1) {
+      offsets(c.j0);
+      __syncthreads();
+      copy(c.j0, false);
+      copy(c.j0, true);
+    }
+    for (int j = c.j0; j < c.j1; ++j) {
+      if (j + 1 < c.j1) offsets(j + 1);
+      cp_wait<1>();
+      __syncthreads();   // the keys are there, and the next ones' places
+      float2 s2[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s2[i][k] = make_float2(0.f, 0.f);
+#pragma unroll 2
+      for (int d = 0; d < HD; d += 4) {
+        float4 q[4], k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(sQ + (ty * 4 + i) * LD + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const float4*>(sK + (tx + 16 * i) * LD + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            s2[i][x] = fma2(make_float2(q[i].x, q[i].y), make_float2(k[x].x, k[x].y), s2[i][x]);
+            s2[i][x] = fma2(make_float2(q[i].z, q[i].w), make_float2(k[x].z, k[x].w), s2[i][x]);
+          }
+      }
+      const unsigned there0 = sThere[(j & 1) * 2], there1 = sThere[(j & 1) * 2 + 1];
+      __syncthreads();   // all have read the keys
+      if (j + 1 < c.j1) copy(j + 1, false);
+      else cp_commit();
+      float p[4][4], alpha[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = tx + 16 * x;
+          const bool in = j * BK + key < seen[i] && ((x < 2 ? there0 : there1) >> (key & 31) & 1);
+          p[i][x] = in ? (s2[i][x].x + s2[i][x].y) * sc : -INFINITY;
+          mx = fmaxf(mx, p[i][x]);
+        }
+#pragma unroll
+        for (int w = 8; w; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(L3_FULL, mx, w));
+        const float mn = fmaxf(m[i], mx), from = mn == -INFINITY ? 0.f : mn;
+        alpha[i] = ex2(m[i] - from);
+        m[i] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum += p[i][x] = ex2(p[i][x] - from);
+#pragma unroll
+        for (int w = 8; w; w >>= 1) sum += __shfl_xor_sync(L3_FULL, sum, w);
+        l[i] = l[i] * alpha[i] + sum;
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) *reinterpret_cast<float4*>(sP + (tx + 16 * x) * PL + ty * 4) = make_float4(p[0][x], p[1][x], p[2][x], p[3][x]);
+#pragma unroll
+      for (int x = 0; x < NC * CW; ++x) {
+        o[0][x].x *= alpha[0]; o[0][x].y *= alpha[1];
+        o[1][x].x *= alpha[2]; o[1][x].y *= alpha[3];
+      }
+      cp_wait<1>();
+      __syncthreads();   // the values are there, and the weights
+#pragma unroll 2
+      for (int k = 0; k < BK; ++k) {
+        const float4 w = *reinterpret_cast<const float4*>(sP + k * PL + ty * 4);
+        const float2 w01 = make_float2(w.x, w.y), w23 = make_float2(w.z, w.w);
+        float v[NC * CW];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          const float* at = sV + k * HD + n * 16 * CW + tx * CW;
+          if constexpr (CW == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(at);
+            v[n * 4] = x.x; v[n * 4 + 1] = x.y; v[n * 4 + 2] = x.z; v[n * 4 + 3] = x.w;
+          } else if constexpr (CW == 2) {
+            const float2 x = *reinterpret_cast<const float2*>(at);
+            v[n * 2] = x.x; v[n * 2 + 1] = x.y;
+          } else v[n] = *at;
+        }
+#pragma unroll
+        for (int x = 0; x < NC * CW; ++x) {
+          o[0][x] = fma2(w01, make_float2(v[x], v[x]), o[0][x]);
+          o[1][x] = fma2(w23, make_float2(v[x], v[x]), o[1][x]);
+        }
+      }
+      __syncthreads();   // all have read the values and the weights
+      if (j + 1 < c.j1) copy(j + 1, true);
+      else cp_commit();
+    }
+    cp_wait<0>();
+    // the result, or this CTA's part of it
+    const bool whole = c.whole();
+    float* part_o = whole ? nullptr : a.part_o + (size_t)(2 * blockIdx.x + c.slot()) * TR * HD;
+    float2* part_ml = whole ? nullptr : a.part_ml + (size_t)(2 * blockIdx.x + c.slot()) * TR;
+    if (!whole && threadIdx.x == 0) *info_of(a, blockIdx.x, c.slot()) = make_int4(c.b, c.tile, c.g, c.j1 == c.nb);
+    unsigned odd = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int f = flat0 + ty * 4 + i;
+      float y[NC * CW];
+      bool finite = l[i] < INFINITY;
+#pragma unroll
+      for (int x = 0; x < NC * CW; ++x) {
+        y[x] = i & 1 ? o[i / 2][x].y : o[i / 2][x].x;
+        finite = finite && fabsf(y[x]) < INFINITY;
+      }
+      if (f < flats) {
+        if (!finite) odd |= 1u << i;
+        const int t = f / a.R;
+        const long long at = (long long)(c.r.s0 + t) * a.H + c.g * a.R + f - t * a.R;
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int e = 0; e < CW; ++e) {
+            const int d = n * 16 * CW + tx * CW + e;
+            if (whole) ((T*)a.out)[at * HD + d] = down<T>(y[n * CW + e] * inv);
+            else part_o[(ty * 4 + i) * HD + d] = y[n * CW + e];
+          }
+        if (tx == 0) {
+          if (!whole) part_ml[ty * 4 + i] = make_float2(m[i], l[i]);
+          else if (a.lse) a.lse[at] = (m[i] + log2f(l[i])) * 0.6931471805599453f;
+        }
+      }
+    }
+    // rows whose sums are not finite: a warp has 8 rows, 16 lanes each 4
+    unsigned rows = __reduce_or_sync(L3_FULL, odd << (lane >> 4) * 4);
+    __syncwarp();
+    for (; rows; rows &= rows - 1) {
+      const int in_tile = (threadIdx.x >> 5) * 8 + __ffs(rows) - 1;
+      end_by_formula<T, HD>(a, c, BK, in_tile, flat0 + in_tile, part_o, part_ml);
+    }
+    __syncthreads();
+  } while (c.next(a));
+}
+
+// ---------------------------------------------------------------------------------------------------------------- the join
+// Block (c, y) joins 16 rows of the item that CTA c began and others ended: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+constexpr int JROWS = 16, JT = 256;
+template <typename T, int HD, int ROWS>
+__global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
+  pdl_launch();
+  pdl_wait();
+  const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int4 first = *info_of(a, c0, 1);
+  if (first.x < 0) return;
+  const Request r = request(a, first.x);
+  for (int i = warp; i < JROWS; i += JT / 32) {
+    const int in_tile = blockIdx.y * JROWS + i, f = first.y * ROWS + in_tile;
+    if (f >= r.n * a.R) return;
+    const int t = f / a.R;
+    const long long at = (long long)(r.s0 + t) * a.H + first.z * a.R + f - t * a.R;
+    constexpr int N = (HD + 31) / 32;
+    float o[N], m, l;
+    const size_t own = (size_t)(2 * c0 + 1) * ROWS + in_tile;
+    m = a.part_ml[own].x;
+    l = a.part_ml[own].y;
+#pragma unroll
+    for (int x = 0; x < N; ++x) o[x] = lane + 32 * x < HD ? a.part_o[own * HD + lane + 32 * x] : 0.f;
+    bool ends = false;
+    for (int c = c0 + 1; c < a.n_cta && !ends; ++c) {
+      const int4 more = *info_of(a, c, 0);
+      if (more.x < 0) continue;
+      ends = more.w;
+      const size_t p = (size_t)(2 * c) * ROWS + in_tile;
+      const float2 ml = a.part_ml[p];
+      const float mn = fmaxf(m, ml.x), from = mn == -INFINITY ? 0.f : mn;
+      const float fa = exp2f(m - from), fb = exp2f(ml.x - from);
+      l = l * fa + ml.y * fb;
+      m = mn;
+#pragma unroll
+      for (int x = 0; x < N; ++x)
+        if (lane + 32 * x < HD) {
+          const float y = a.part_o[p * HD + lane + 32 * x];
+          // an infinite sum stays one, however small its part
+          o[x] = (fabsf(o[x]) < INFINITY || fa > 0.f ? o[x] * fa : o[x]) + (fabsf(y) < INFINITY || fb > 0.f ? y * fb : y);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+      if (lane + 32 * x < HD) ((T*)a.out)[at * HD + lane + 32 * x] = down<T>(o[x] * inv);
+    if (a.lse && lane == 0) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
+  }
+}
+
+size_t partials(int n_cta, int rows, int HD) { return (size_t)n_cta * 2 * (rows * ((size_t)HD * 4 + 8) + 16); }
+template <typename T, int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
+  constexpr size_t smem = smem_bytes<HD>();
+  a.n_cta = (HD > 64 ? 1 : 2) * n_sm;
+  a.part_o = (float*)a.ws;
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * TR * HD);
+  a.info = reinterpret_cast<int4*>(a.part_ml + (size_t)a.n_cta * 2 * TR);
+  cudaError_t e = allow_smem(chunk_fma_kernel<T, HD>, smem);
+  if (e != cudaSuccess) return e;
+  if ((e = launch_k(chunk_fma_kernel<T, HD>, dim3(a.n_cta), dim3(NT), smem, s, a)) != cudaSuccess) return e;
+  g_l3_pdl_next = true;
+  return launch_k(chunk_join_kernel<T, HD, TR>, dim3(a.n_cta, TR / JROWS), dim3(JT), 0, s, a);
+}
+template <typename T> cudaError_t launch_t(const ChunkArgs& a, int n_sm, cudaStream_t s) {
+  switch (a.HD) {
+    case 16: return launch_hd<T, 16>(a, n_sm, s);
+    case 32: return launch_hd<T, 32>(a, n_sm, s);
+    case 48: return launch_hd<T, 48>(a, n_sm, s);
+    case 64: return launch_hd<T, 64>(a, n_sm, s);
+    case 96: return launch_hd<T, 96>(a, n_sm, s);
+    case 128: return launch_hd<T, 128>(a, n_sm, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+}  // namespace
+
+size_t paged_chunk_workspace(int T, int H, int G, int HD, int dtype, int n_sm) { return partials(2 * n_sm, TR, HD); }
+
+cudaError_t launch_paged_chunk(ChunkArgs a, int n_sm, cudaStream_t s) {
+  if (a.dtype == L3_DTYPE_F32) return launch_t<float>(a, n_sm, s);
+  if (a.dtype == L3_DTYPE_BF16) return launch_t<bf16>(a, n_sm, s);
+  return launch_t<__half>(a, n_sm, s);
+}

@@ -1,0 +1,243 @@
+// What the kernels of attention of a packed step share (paged_chunk.cu, paged_chunk_tc.cu): how the work is cut, and the slow path of rows
+// that a value without a number has reached.
+//
+// The R query heads of a kv head and the n rows of a request are n R flat rows that see (nearly) the same keys; row f is token f / R, head f % R of
+// the group.  An item is TR of them (a tile) against the blocks of BK keys that its last row sees.  The items of all requests, tiles and kv heads, in
+// that order, are one long line, weighed by their blocks, that the CTAs share out evenly: prompts, portions and single tokens of any mixture leave no
+// SM idle.  An item of few blocks goes to the CTA that has its middle; longer ones are cut where the shares end, leave partials (m, l, o) that a
+// second, dependent launch joins in the order of the keys, so that results do not change from run to run.
+#pragma once
+#include <math.h>
+
+#include <cuda_fp16.h>
+
+#include "../../include/llama3_b200.h"
+#include "packed.h"
+
+namespace chunk {
+template <typename T> __device__ __forceinline__ float up(T x) { return to_f32(x); }
+template <> __device__ __forceinline__ float up<__half>(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T down(float x) { return from_f32<T>(x); }
+template <> __device__ __forceinline__ __half down<__half>(float x) { return __float2half_rn(x); }
+
+struct Request {
+  int s0, n;      // its rows
+  int len;        // its tokens, those of the rows among them
+  int keys;       // tokens that the table has columns for
+  __device__ __forceinline__ int seen(int t) const { return min(max(len - n + t + 1, 0), keys); }  // by its row t: [0, seen)
+};
+__device__ __forceinline__ Request request(const ChunkArgs& a, int b) {
+  Request r;
+  r.s0 = min(max(a.starts[b], 0), a.T);
+  r.n = min(max(a.starts[b + 1], r.s0), a.T) - r.s0;
+  r.len = max(a.lengths[b], 0);
+  r.keys = a.max_pages << a.log_page;
+  return r;
+}
+template <int TR> __device__ __forceinline__ int tiles(const ChunkArgs& a, int n) { return (int)((unsigned)(n * a.R + TR - 1) / TR); }
+template <int TR, int BK> __device__ __forceinline__ int blocks(const ChunkArgs& a, const Request& r, int tile) {
+  const int last = min(r.n * a.R, (tile + 1) * TR) - 1;
+  return (int)((unsigned)(r.seen(last / a.R) + BK - 1) / BK);
+}
+// An item's weight: two a block, and what begins and ends it like half a block.
+__device__ __forceinline__ int weight(int nb) { return 2 * nb + 1; }
+// The blocks of an item of nb that lie ahead of weight x.  Whole: items of so few blocks are not cut.
+template <int WHOLE> __device__ __forceinline__ int ahead(long long x, int nb) {
+  const int w = weight(nb);
+  if (x <= 0) return 0;
+  if (x >= w) return nb;
+  if (nb <= WHOLE) return 2 * x >= w ? nb : 0;
+  return (int)x / 2;
+}
+
+struct Place { int b, tile, g; long long off, rest; };  // an item, the weight of it that others have, and what this CTA has from there on
+
+// This CTA's share, by all NT threads (`room`: NT / 32 + 1 words of shared memory).  LEAST: the least weight of a share.
+template <int TR, int BK, int NT, int LEAST>
+__device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, Place* place) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // a thread takes `each` requests, or one of `parts` parts of a request's tiles
+  const int parts = max(NT / max(a.B, 1), 1), each = (a.B + NT - 1) / NT;
+  auto walk = [&](auto f) {
+    const int b0 = parts > 1 ? threadIdx.x / parts : threadIdx.x * each, b1 = min(parts > 1 ? b0 + 1 : b0 + each, a.B);
+    for (int b = b0; b < b1; ++b) {
+      const Request r = request(a, b);
+      const int nt = tiles<TR>(a, r.n), part = parts > 1 ? threadIdx.x % parts : 0;
+      const int t0 = (int)((long long)nt * part / parts), t1 = (int)((long long)nt * (part + 1) / parts);
+      for (int t = t0; t < t1; ++t)
+        if (f(b, t, weight(blocks<TR, BK>(a, r, t)))) return;
+    }
+  };
+  long long sum = 0;
+  walk([&](int, int, int w) {
+    sum += (long long)w * a.G;
+    return false;
+  });
+  long long run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(L3_FULL, run, o);
+    if (lane >= o) run += y;
+  }
+  if (lane == 31) room[warp] = run;
+  if (threadIdx.x == 0) *place = Place{-1, 0, 0, 0, 0};
+  __syncthreads();
+  long long before = run - sum, all = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    if (w < warp) before += room[w];
+    all += room[w];
+  }
+  const long long ctas = min((long long)a.n_cta, max(all / LEAST, 1LL));
+  if (blockIdx.x < ctas) {
+    const long long w0 = all * blockIdx.x / ctas, w1 = all * (blockIdx.x + 1) / ctas;
+    if (before <= w0 && w0 < before + sum) {
+      long long at = before;
+      walk([&](int b, int t, int w) {
+        const long long whole = (long long)w * a.G;
+        if (w0 >= at + whole) {
+          at += whole;
+          return false;
+        }
+        const int g = (int)((w0 - at) / w);
+        *place = Place{b, t, g, w0 - at - (long long)g * w, w1 - w0};
+        return true;
+      });
+    }
+  }
+  __syncthreads();
+}
+
+// One stretch of blocks after the other.
+template <int TR, int BK, int WHOLE> struct Cursor {
+  int b, tile, g, nt, nb;
+  Request r;
+  long long off, rest;
+  int j0, j1;               // blocks of this stretch
+  __device__ __forceinline__ void at_tile(const ChunkArgs& a) { nb = blocks<TR, BK>(a, r, tile); }
+  __device__ __forceinline__ bool start(const ChunkArgs& a, const Place& p) {
+    b = p.b; tile = p.tile; g = p.g; off = p.off; rest = p.rest;
+    if (b < 0) return false;
+    r = request(a, b);
+    nt = tiles<TR>(a, r.n);
+    at_tile(a);
+    return settle(a) ? true : next(a);
+  }
+  // the stretch of this item, if there is one
+  __device__ __forceinline__ bool settle(const ChunkArgs&) {
+    if (rest <= 0) return false;
+    j0 = ahead<WHOLE>(off, nb);
+    j1 = ahead<WHOLE>(off + rest, nb);
+    return j1 > j0 || (nb == 0 && off == 0);
+  }
+  __device__ __forceinline__ bool next(const ChunkArgs& a) {
+    for (;;) {
+      rest -= weight(nb) - off;
+      off = 0;
+      if (rest <= 0) return false;
+      if (++g == a.G) {
+        g = 0;
+        if (++tile == nt) {
+          tile = 0;
+          do {
+            if (++b >= a.B) return false;
+            r = request(a, b);
+            nt = tiles<TR>(a, r.n);
+          } while (nt == 0);
+        }
+        at_tile(a);
+      }
+      if (settle(a)) return true;
+    }
+  }
+  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nb; }
+  __device__ __forceinline__ int slot() const { return j0 > 0 ? 0 : 1; }  // of a partial: of the item that this CTA goes on with, or begins
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The values of a key that a row sees may be infinite or NaN, those of keys that it does not see have to be kept out even so, and tiles
+// multiply them by a weight of 0.  A row whose sums are not finite is therefore taken once more, by the formula alone: the keys k0 <= j < k1 one at a
+// time, by a warp; only what the row sees enters.  A weight is 0 for a score of -infinity only, however small, as its value may be infinite.
+// m is in units of log 2, l and o as the tiles' are.
+template <typename T, int HD>
+__device__ __noinline__ void by_formula(const ChunkArgs& a, int b, int g, int row, int head, int k0, int k1, float (&o)[(HD + 31) / 32], float& m, float& l) {
+  constexpr int N = (HD + 31) / 32;
+  const int lane = threadIdx.x & 31;
+  const int* table = a.table + b * a.table_stride;
+  const T* q = (const T*)a.q + row * a.q_st + head * a.q_sh;
+  const float sc = a.scale * 1.4426950408889634f;
+  auto row_of = [&](const PagedPool& p, int j, bool& there) {
+    const int page = table[j >> a.log_page];
+    there = (unsigned)page < (unsigned)a.n_pages;
+    return (const T*)p.p + page * p.sp + g * p.sh + (j & ((1 << a.log_page) - 1)) * p.st;
+  };
+  auto score = [&](int j, bool& there) {
+    const T* k = row_of(a.k, j, there);
+    if (!there) return -INFINITY;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane + 32 * i < HD) s += up(q[lane + 32 * i]) * up(k[lane + 32 * i]);
+    return warp_sum(s) * sc;
+  };
+  m = -INFINITY;
+  l = 0.f;
+  bool there;
+  for (int j = k0; j < k1; ++j) m = fmaxf(m, score(j, there));
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
+  const float from = m == -INFINITY ? 0.f : m;
+  for (int j = k0; j < k1; ++j) {
+    const float s = score(j, there);
+    if (!there) continue;
+    const float x = s - from;
+    const float w = x < -149.f && s > -INFINITY ? 1.4e-45f : exp2f(x);
+    l += w;
+    const T* v = row_of(a.v, j, there);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane + 32 * i < HD) o[i] += w * up(v[lane + 32 * i]);
+  }
+}
+// the same, with its result where the tile would have put it
+template <typename T, int HD, typename Cur>
+__device__ __forceinline__ void end_by_formula(const ChunkArgs& a, const Cur& c, int BK, int in_tile, int flat, float* part_o, float2* part_ml) {
+  float o[(HD + 31) / 32], m, l;
+  const int lane = threadIdx.x & 31, t = flat / a.R, head = c.g * a.R + flat - t * a.R, row = c.r.s0 + t;
+  by_formula<T, HD>(a, c.b, c.g, row, head, c.j0 * BK, min(c.j1 * BK, c.r.seen(t)), o, m, l);
+  const long long at = (long long)row * a.H + head;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < (HD + 31) / 32; ++i) {
+    const int d = lane + 32 * i;
+    if (d < HD) {
+      if (part_o) part_o[(long long)in_tile * HD + d] = o[i];
+      else ((T*)a.out)[at * HD + d] = down<T>(o[i] * inv);
+    }
+  }
+  if (lane == 0) {
+    if (part_o) part_ml[in_tile] = make_float2(m, l);
+    else if (a.lse) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
+  }
+}
+
+// rows of no request: as they are, or 0
+template <typename T> __device__ __forceinline__ void clear_rest(const ChunkArgs& a) {
+  if (!a.clear_rest) return;
+  const int from = a.B ? min(max(a.starts[a.B], 0), a.T) : 0;
+  const long long n = (long long)(a.T - from) * a.H, at = (long long)from * a.H;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n * a.HD; i += (long long)gridDim.x * blockDim.x) {
+    ((T*)a.out)[at * a.HD + i] = down<T>(0.f);
+    if (a.lse && i < n) a.lse[at + i] = -INFINITY;
+  }
+}
+
+// what a CTA leaves for the join about its two partials: (request, tile, kv head, 1 if the item ends with it), request -1: none
+__device__ __forceinline__ int4* info_of(const ChunkArgs& a, int cta, int slot) { return a.info + 2 * cta + slot; }
+}  // namespace chunk
+

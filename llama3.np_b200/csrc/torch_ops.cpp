@@ -26,6 +26,11 @@ struct Entries {
   decltype(&l3_beam_select_workspace) select_workspace;
   decltype(&l3_beam_select) select;
   decltype(&l3_last_error) last_error;
+  decltype(&l3_paged_extend) extend;
+  decltype(&l3_rotary) rotary;
+  decltype(&l3_paged_chunk_workspace) chunk_workspace;
+  decltype(&l3_paged_chunk_attention) chunk;
+  decltype(&l3_token_logprobs) logprobs;
 } entry{};
 
 using at::Tensor;
@@ -393,6 +398,280 @@ PyObject* beam_select(PyObject*, PyObject* const* x, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A tuple of what a call returns; an undefined tensor is None.
+PyObject* tuple_of(std::initializer_list<Tensor> list) {
+  PyObject* all = PyTuple_New((Py_ssize_t)list.size());
+  if (!all) throw python_error();
+  Py_ssize_t i = 0;
+  for (const Tensor& t : list) {
+    PyObject* x = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
+    PyTuple_SET_ITEM(all, i++, x);
+  }
+  return all;
+}
+int page_of(int64_t page) {
+  NEED(page >= 1 && page <= 65536 && (page & (page - 1)) == 0, "page size ", page, " is not a power of two up to 65536");
+  return (int)page;
+}
+
+// paged_extend(page_table, lengths, counts, free_pages, page_size, tokens)
+PyObject* paged_extend(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  args(n, 6);
+  const Tensor& lengths = tensor(x[1], "lengths", 1);
+  const int64_t batch = lengths.size(0);
+  const Tensor& table = table_of(x[0], batch);
+  const Tensor &counts = tensor(x[2], "counts", 1), &pages = tensor(x[3], "free_pages", 1);
+  L3PagedExtend a{};
+  a.batch = size32(batch, "batch");
+  a.lengths = ints(lengths, "lengths", batch);
+  a.counts = ints(counts, "counts", batch);
+  a.n_free = size32(pages.size(0), "free_pages");
+  a.free_pages = ints(pages, "free_pages", a.n_free);
+  a.page_size = page_of(integer(x[4]));
+  const int64_t tokens = integer(x[5]);
+  NEED(tokens >= 0, "tokens ", tokens);
+  a.tokens = size32(tokens, "tokens");
+  a.max_pages = size32(table.size(1), "page_table");
+  NEED(batch <= 1 || table.size(1) == 0 || table.stride(0) >= table.size(1), "page_table is expanded, and would be written");
+  OneDevice on;
+  on.add(table, "page_table"); on.add(lengths, "lengths"); on.add(counts, "counts"); on.add(pages, "free_pages");
+  const auto like = lengths.options();
+  const Tensor len = at::empty({batch}, like), starts = at::empty({batch + 1}, like), positions = at::empty({tokens}, like),
+               slots = at::empty({tokens}, like.dtype(at::kLong)), used = at::empty({1}, like);
+  a.device = on.index;
+  a.stream = on.stream();
+  a.table = table.data_ptr<int32_t>(); a.table_stride = step_of(table, 0);
+  a.out_lengths = len.data_ptr<int32_t>(); a.out_starts = starts.data_ptr<int32_t>(); a.out_positions = positions.data_ptr<int32_t>();
+  a.out_slots = slots.data_ptr<int64_t>(); a.out_used = used.data_ptr<int32_t>();
+  done(entry.extend(&a));
+  if (batch && tokens) changed(table);
+  return tuple_of({len, starts, positions, slots, used});
+  END_HANDLE_TH_ERRORS
+}
+
+// what every rotary call has: positions of `rows`, frequencies, layout, amplitude, inverse
+void turn_of(L3Rotary& a, const Tensor& positions, PyObject* frequencies, PyObject* layout, PyObject* amplitude, PyObject* inverse) {
+  typed(positions, "positions", at::kInt);
+  NEED(positions.is_contiguous(), "positions must be contiguous");
+  const Tensor& f = tensor(frequencies, "frequencies", 1);
+  typed(f, "frequencies", at::kDouble);
+  NEED(f.is_contiguous(), "frequencies must be contiguous");
+  NEED(a.head_dim <= 1024, "head size ", a.head_dim, ": up to 1024 are supported");
+  NEED(2 * f.size(0) <= a.head_dim, f.size(0), " frequencies for heads of ", a.head_dim);
+  a.dims = 2 * (int)f.size(0);
+  const char* name = PyUnicode_Check(layout) ? PyUnicode_AsUTF8(layout) : nullptr;
+  NEED(name && (std::string(name) == "pairs" || std::string(name) == "halves"), "layout must be \"pairs\" or \"halves\"");
+  a.layout = std::string(name) == "halves";
+  a.amplitude = (float)real(amplitude);
+  a.inverse = inverse == Py_True;
+  a.positions = positions.const_data_ptr<int32_t>();
+  a.frequencies = f.const_data_ptr<double>();
+}
+void no_overlap(const Tensor& t, const char* name) {
+  for (int64_t d = 0; d < t.dim(); ++d) NEED(t.size(d) <= 1 || t.stride(d) != 0, name, " is expanded, and would be written");
+}
+// whether the stretches of memory from the first entry to the last meet
+bool meets(const Tensor& a, const Tensor& b) {
+  auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (uintptr_t)t.const_data_ptr() + (last + 1) * t.element_size();
+  };
+  return a.numel() && b.numel() && (uintptr_t)a.const_data_ptr() < end(b) && (uintptr_t)b.const_data_ptr() < end(a);
+}
+bool same_place(const Tensor& a, const Tensor& b) { return a.const_data_ptr() == b.const_data_ptr() && a.strides() == b.strides(); }
+
+// rotary(x, positions, frequencies, layout, amplitude, inverse, out)
+PyObject* rotary(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  args(n, 7);
+  const Tensor& t = tensor(x[0], "x");
+  NEED(t.dim() == 3 || t.dim() == 4, "x must be [tokens, heads, size] or [batch, tokens, heads, size], got ", t.sizes());
+  const int64_t d = t.dim() - 3;
+  L3Rotary a{};
+  a.dtype = kind(t, "x");
+  last_is_dense(t, "x");
+  const Tensor& positions = tensor(x[1], "positions");
+  NEED(positions.sizes() == t.sizes().slice(0, d + 1), "positions must be ", t.sizes().slice(0, d + 1), ", got ", positions.sizes());
+  a.batch = d ? size32(t.size(0), "batch") : 1;
+  a.tokens = size32(t.size(d), "tokens"); a.heads = size32(t.size(d + 1), "heads"); a.head_dim = size32(t.size(d + 2), "head size");
+  turn_of(a, positions, x[2], x[3], x[4], x[5]);
+  if (given(x[6])) {
+    const Tensor& o = tensor(x[6], "out");
+    typed(o, "out", t.scalar_type());
+    NEED(o.sizes() == t.sizes(), "out must be ", t.sizes(), ", got ", o.sizes());
+    last_is_dense(o, "out");
+    no_overlap(o, "out");
+    NEED(!meets(o, t) || same_place(o, t), "out shares memory with x and is not x itself");
+  }
+  OneDevice on;
+  on.add(t, "x"); on.add(positions, "positions"); on.add(THPVariable_Unpack(x[2]), "frequencies");
+  if (given(x[6])) on.add(THPVariable_Unpack(x[6]), "out");
+  const Tensor out = given(x[6]) ? THPVariable_Unpack(x[6]) : at::empty(t.sizes(), t.options());
+  a.device = on.index;
+  a.stream = on.stream();
+  a.x = t.const_data_ptr();
+  a.x_batch_stride = d ? step_of(t, 0) : 0; a.x_token_stride = step_of(t, d); a.x_head_stride = step_of(t, d + 1);
+  a.out = out.data_ptr();
+  a.out_batch_stride = d ? step_of(out, 0) : 0; a.out_token_stride = step_of(out, d); a.out_head_stride = step_of(out, d + 1);
+  if (t.numel()) {
+    done(entry.rotary(&a));
+    if (given(x[6])) changed(out);
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_rotary_write(q, k, v, positions, slots, k_pages, v_pages, frequencies, layout, amplitude, out)
+PyObject* paged_rotary_write(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  args(n, 11);
+  const Tensor &q = tensor(x[0], "q", 3), &k = tensor(x[1], "k", 3), &v = tensor(x[2], "v", 3), &kp = tensor(x[5], "k_pages", 4),
+               &vp = tensor(x[6], "v_pages", 4);
+  L3Rotary a{};
+  a.dtype = pools_of(kp, vp);
+  const int64_t tokens = q.size(0), G = kp.size(1), dim = kp.size(3);
+  typed(q, "q", kp.scalar_type());
+  NEED(q.size(2) == dim, "q must be [", tokens, ", heads, ", dim, "], got ", q.sizes());
+  last_is_dense(q, "q");
+  for (const Tensor* t : {&k, &v}) {
+    const char* name = t == &k ? "k" : "v";
+    typed(*t, name, kp.scalar_type());
+    NEED(t->size(0) == tokens && t->size(1) == G && t->size(2) == dim, name, " must be [", tokens, ", ", G, ", ", dim, "], got ", t->sizes());
+    last_is_dense(*t, name);
+  }
+  own_places(kp, "k_pages");
+  own_places(vp, "v_pages");
+  const Tensor &positions = tensor(x[3], "positions", 1), &slots = tensor(x[4], "slots", 1);
+  NEED(positions.size(0) == tokens, "positions must be [", tokens, "], got ", positions.sizes());
+  typed(slots, "slots", at::kLong);
+  NEED(slots.size(0) == tokens && slots.is_contiguous(), "slots must be contiguous, [", tokens, "], got ", slots.sizes());
+  a.batch = 1;
+  a.tokens = size32(tokens, "tokens"); a.heads = size32(q.size(1), "heads"); a.head_dim = size32(dim, "head size"); a.kv_heads = size32(G, "kv heads");
+  a.pages = size32(kp.size(0), "pages"); a.page_size = (int)kp.size(2);
+  turn_of(a, positions, x[7], x[8], x[9], Py_False);
+  if (given(x[10])) {
+    const Tensor& o = tensor(x[10], "out", 3);
+    typed(o, "out", q.scalar_type());
+    NEED(o.sizes() == q.sizes(), "out must be ", q.sizes(), ", got ", o.sizes());
+    last_is_dense(o, "out");
+    no_overlap(o, "out");
+    NEED(!meets(o, q) || same_place(o, q), "out shares memory with q and is not q itself");
+  }
+  OneDevice on;
+  on.add(q, "q"); on.add(k, "k"); on.add(v, "v"); on.add(positions, "positions"); on.add(slots, "slots"); on.add(kp, "k_pages"); on.add(vp, "v_pages");
+  on.add(THPVariable_Unpack(x[7]), "frequencies");
+  if (given(x[10])) on.add(THPVariable_Unpack(x[10]), "out");
+  const Tensor out = given(x[10]) ? THPVariable_Unpack(x[10]) : at::empty(q.sizes(), q.options());
+  if (tokens) {
+    a.device = on.index;
+    a.stream = on.stream();
+    a.x = q.const_data_ptr(); a.x_token_stride = step_of(q, 0); a.x_head_stride = step_of(q, 1);
+    a.out = out.data_ptr(); a.out_token_stride = step_of(out, 0); a.out_head_stride = step_of(out, 1);
+    a.k = k.const_data_ptr(); a.k_token_stride = step_of(k, 0); a.k_head_stride = step_of(k, 1);
+    a.v = v.const_data_ptr(); a.v_token_stride = step_of(v, 0); a.v_head_stride = step_of(v, 1);
+    a.slots = slots.const_data_ptr<int64_t>();
+    a.k_pool = pool(kp); a.v_pool = pool(vp);
+    done(entry.rotary(&a));
+    changed(kp);
+    changed(vp);
+    if (given(x[10])) changed(out);
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_chunk_attention(q, k_pages, v_pages, page_table, lengths, starts, scale, return_lse, out)
+PyObject* paged_chunk_attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  args(n, 9);
+  const Tensor &q = tensor(x[0], "q", 3), &k = tensor(x[1], "k_pages", 4), &v = tensor(x[2], "v_pages", 4), &lengths = tensor(x[4], "lengths", 1),
+               &starts = tensor(x[5], "starts", 1);
+  L3PagedChunk a{};
+  a.dtype = pools_of(k, v);
+  const int64_t batch = lengths.size(0), tokens = q.size(0), heads = q.size(1), dim = q.size(2), G = k.size(1);
+  typed(q, "q", k.scalar_type());
+  NEED(k.size(3) == dim && (dim == 16 || dim == 32 || dim == 48 || dim == 64 || dim == 96 || dim == 128), "head size ", dim, " (cache: ", k.size(3),
+       ") is not one of 16, 32, 48, 64, 96, 128");
+  NEED(G >= 1 && heads >= 1 && heads % G == 0, heads, " heads over ", G, " kv heads");
+  last_is_dense(q, "q");
+  fits16(q, "q");
+  const Tensor& table = table_of(x[3], batch);
+  a.lengths = ints(lengths, "lengths", batch);
+  a.starts = ints(starts, "starts", batch + 1);
+  if (given(x[8])) {
+    const Tensor& out = tensor(x[8], "out", 3);
+    typed(out, "out", q.scalar_type());
+    NEED(out.sizes() == q.sizes() && out.is_contiguous() && (reinterpret_cast<uintptr_t>(out.const_data_ptr()) & 15) == 0,
+         "out must be contiguous, of q's shape");
+    NEED(!meets(out, q), "out shares memory with q");
+  }
+  OneDevice on;
+  on.add(q, "q"); on.add(k, "k_pages"); on.add(v, "v_pages"); on.add(table, "page_table"); on.add(lengths, "lengths"); on.add(starts, "starts");
+  if (given(x[8])) on.add(THPVariable_Unpack(x[8]), "out");
+  const bool want_lse = x[7] == Py_True;
+  const Tensor out = given(x[8]) ? THPVariable_Unpack(x[8]) : at::empty({tokens, heads, dim}, q.options());
+  Tensor lse, room;
+  if (want_lse) lse = at::empty({tokens, heads}, q.options().dtype(at::kFloat));
+  if (tokens) {
+    a.device = on.index; a.batch = size32(batch, "batch"); a.tokens = size32(tokens, "tokens"); a.heads = size32(heads, "heads"); a.kv_heads = size32(G, "kv heads");
+    a.head_dim = (int)dim; a.pages = size32(k.size(0), "pages"); a.page_size = (int)k.size(2); a.max_pages = size32(table.size(1), "page_table");
+    a.clear_rest = !given(x[8]);
+    a.scale = given(x[6]) ? (float)real(x[6]) : (float)(1.0 / std::sqrt((double)dim));
+    a.stream = on.stream();
+    a.q = q.const_data_ptr(); a.q_token_stride = step_of(q, 0); a.q_head_stride = step_of(q, 1);
+    a.k = pool(k); a.v = pool(v);
+    a.table = table.const_data_ptr<int32_t>(); a.table_stride = step_of(table, 0);
+    a.out = out.data_ptr();
+    a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+    done(entry.chunk_workspace(on.index, a.tokens, a.heads, a.kv_heads, a.head_dim, a.dtype, &a.workspace_bytes));
+    room = at::empty({a.workspace_bytes}, q.options().dtype(at::kByte));  // of this call: a captured graph has one of its own
+    a.workspace = room.data_ptr();
+    done(entry.chunk(&a));
+  }
+  if (given(x[8])) changed(out);
+  if (!want_lse) return THPVariable_Wrap(out);
+  return tuple_of({out, lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs(logits, tokens, top, entropy)
+PyObject* token_logprobs(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  args(n, 4);
+  const Tensor &logits = tensor(x[0], "logits", 2), &tokens = tensor(x[1], "tokens", 1);
+  L3TokenLogprobs a{};
+  a.dtype = kind(logits, "logits");
+  const int64_t rows = logits.size(0), vocab = logits.size(1), top = integer(x[2]);
+  NEED(vocab >= 1 && vocab < (1 << 24), "logits of shape ", logits.sizes(), ": 1 to 2^24 - 1 tokens are supported");
+  NEED(top >= 0 && top <= 64 && top <= vocab, "top ", top, ": 0 to 64, and no more than the vocabulary's ", vocab, " are supported");
+  last_is_dense(logits, "logits");
+  a.tokens = ints(tokens, "tokens", rows);
+  OneDevice on;
+  on.add(logits, "logits"); on.add(tokens, "tokens");
+  const auto like = logits.options().dtype(at::kFloat);
+  const Tensor lp = at::empty({rows}, like);
+  Tensor entropy, best, best_tokens;
+  if (x[3] == Py_True) entropy = at::empty({rows}, like);
+  if (top) {
+    best = at::empty({rows, top}, like);
+    best_tokens = at::empty({rows, top}, like.dtype(at::kInt));
+  }
+  if (rows) {
+    a.device = on.index; a.rows = size32(rows, "rows"); a.vocab = (int)vocab; a.top = (int)top;
+    a.stream = on.stream();
+    a.logits = logits.const_data_ptr(); a.row_stride = step_of(logits, 0);
+    a.out_logprobs = lp.data_ptr<float>();
+    a.out_entropy = entropy.defined() ? entropy.data_ptr<float>() : nullptr;
+    a.out_top_logprobs = top ? best.data_ptr<float>() : nullptr;
+    a.out_top_tokens = top ? best_tokens.data_ptr<int32_t>() : nullptr;
+    done(entry.logprobs(&a));
+  }
+  return tuple_of({lp, entropy, best, best_tokens});
+  END_HANDLE_TH_ERRORS
+}
+
 // rows(tensor): how copy_pages and beam_reorder take a tensor (rows, row stride, runs of a row, their distance, their bytes)
 PyObject* rows(PyObject*, PyObject* const* x, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -405,11 +684,12 @@ PyObject* rows(PyObject*, PyObject* const* x, Py_ssize_t n) {
 // bind(addresses of the C-ABI's entries, in Entries' order)
 PyObject* bind(PyObject*, PyObject* const* x, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  args(n, 8);
-  void* p[8];
-  for (int i = 0; i < 8; ++i) p[i] = reinterpret_cast<void*>(integer(x[i]));
+  constexpr int N = sizeof(Entries) / sizeof(void*);
+  args(n, N);
+  void* p[N];
+  for (int i = 0; i < N; ++i) p[i] = reinterpret_cast<void*>(integer(x[i]));
   static_assert(sizeof(entry) == sizeof p, "");
-  std::copy(p, p + 8, reinterpret_cast<void**>(&entry));
+  std::copy(p, p + N, reinterpret_cast<void**>(&entry));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -419,6 +699,11 @@ PyMethodDef methods[] = {{"paged_attention", (PyCFunction)(void (*)())paged_atte
                          {"copy_pages", (PyCFunction)(void (*)())copy_pages, METH_FASTCALL, nullptr},
                          {"beam_reorder", (PyCFunction)(void (*)())beam_reorder, METH_FASTCALL, nullptr},
                          {"beam_select", (PyCFunction)(void (*)())beam_select, METH_FASTCALL, nullptr},
+                         {"paged_extend", (PyCFunction)(void (*)())paged_extend, METH_FASTCALL, nullptr},
+                         {"rotary", (PyCFunction)(void (*)())rotary, METH_FASTCALL, nullptr},
+                         {"paged_rotary_write", (PyCFunction)(void (*)())paged_rotary_write, METH_FASTCALL, nullptr},
+                         {"paged_chunk_attention", (PyCFunction)(void (*)())paged_chunk_attention, METH_FASTCALL, nullptr},
+                         {"token_logprobs", (PyCFunction)(void (*)())token_logprobs, METH_FASTCALL, nullptr},
                          {"rows", (PyCFunction)(void (*)())rows, METH_FASTCALL, nullptr},
                          {"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

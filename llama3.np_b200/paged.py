@@ -43,7 +43,8 @@ def _ops():
         lib = _cabi.lib()
         module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
             "l3_paged_attention_workspace", "l3_paged_attention", "l3_paged_write", "l3_copy_rows", "l3_beam_reorder",
-            "l3_beam_select_workspace", "l3_beam_select", "l3_last_error")))
+            "l3_beam_select_workspace", "l3_beam_select", "l3_last_error", "l3_paged_extend", "l3_rotary", "l3_paged_chunk_workspace",
+            "l3_paged_chunk_attention", "l3_token_logprobs")))
         _module = module
     return _module
 
@@ -208,16 +209,31 @@ class PagedCache(PageTable):
         view = cache.extend(beams)                            # one more token each; a shared, partly filled page is copied first
         out = cache.attend(layer, view, q, k_new, v_new)      # [4, heads, 128], for every layer
         cache.free(seq)
+        view = cache.extend([a, b, c], [512, 1, 1])           # a portion of a prompt beside single tokens, as 514 rows
+        q = cache.write_packed(layer, view, q, k, v, frequencies)   # turned to their positions
+        out = cache.attend_packed(layer, view, q)             # [514, heads, 128]
 
     Everything runs on the current stream of the cache's device: a page that is freed and taken again is written behind what read
     it before.  A view is good until the next call that changes one of its sequences, or compacts."""
 
     class View:
         """Sequences of a cache as its operators take them: `table` [n, pages], `lengths` and `start` [n], int32 on the device; the
-        tokens from start on are the newest."""
+        tokens from start on are the newest.  As rows of a packed step those of sequence i are the rows starts[i] .. starts[i + 1] - 1, with
+        `positions` and `slots`: made by `paged_extend` when first asked for."""
 
-        def __init__(self, seqs, table, lengths, start):
+        def __init__(self, seqs, table, lengths, start, packed=None):
             self.seqs, self.table, self.lengths, self.start = seqs, table, lengths, start
+            self._packed, self._step = packed, None
+
+        def _rows(self):
+            if self._step is None:
+                _need(self._packed is not None, "this view was not made by a cache")
+                self._step = self._packed()
+            return self._step
+
+        starts = property(lambda self: self._rows().starts)
+        positions = property(lambda self: self._rows().positions)
+        slots = property(lambda self: self._rows().slots)
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page_size: int = 16, dtype=torch.bfloat16, device="cuda"):
         super().__init__(pages, page_size)
@@ -239,8 +255,17 @@ class PagedCache(PageTable):
         rows, lengths = [self.pages_of(s) for s in seqs], [self.length(s) for s in seqs]
         wide = max((len(r) for r in rows), default=0)
         flat = torch.tensor([r + [-1] * (wide - len(r)) for r in rows], dtype=torch.int32).reshape(len(rows), wide)
-        ends = torch.tensor([lengths, lengths if start is None else start], dtype=torch.int32).to(self.device)
-        return PagedCache.View(list(seqs), flat.to(self.device), ends[0], ends[1])
+        start = lengths if start is None else list(start)
+        ends = torch.tensor([lengths, start], dtype=torch.int32).to(self.device)
+        table = flat.to(self.device)
+
+        def packed():
+            from .packed import paged_extend
+            new = [p for r, n in zip(rows, start) for p in r[-(-n // self.page_size):]]  # go where they are already
+            return paged_extend(table, ends[1], ends[0] - ends[1], torch.tensor(new, dtype=torch.int32).to(self.device), page_size=self.page_size,
+                                tokens=sum(lengths) - sum(start))
+
+        return PagedCache.View(list(seqs), table, ends[0], ends[1], packed)
 
     def extend(self, seqs, tokens=1) -> "PagedCache.View":
         """`grow`, with the copies that it takes, and the sequences' view: their new tokens are still to be written (`write`, `attend`)."""
@@ -261,3 +286,13 @@ class PagedCache(PageTable):
     def attend(self, layer: int, view, q, k_new=None, v_new=None, **options):
         """`paged_attention` of the view's sequences over a layer; with k_new and v_new, the newest token of each is written, too."""
         return paged_attention(q, self.k[layer], self.v[layer], view.table, view.lengths, k_new=k_new, v_new=v_new, **options)
+
+    def write_packed(self, layer: int, view, q, k, v, frequencies, **options):
+        """`paged_rotary_write` of the view's newest tokens, [rows, heads, head size]; the turned queries."""
+        from .packed import paged_rotary_write
+        return paged_rotary_write(q, k, v, view.positions, view.slots, self.k[layer], self.v[layer], frequencies, **options)
+
+    def attend_packed(self, layer: int, view, q, **options):
+        """`paged_chunk_attention` of the view's newest tokens over a layer, once they are written."""
+        from .packed import paged_chunk_attention
+        return paged_chunk_attention(q, self.k[layer], self.v[layer], view.table, view.lengths, view.starts, **options)
