@@ -51,9 +51,9 @@ struct ChunkArgs {
   int n_cta;
   float* part_o;                     // [n_cta][2][rows of a tile][HD]
   float2* part_ml;                   // [n_cta][2][rows of a tile]
-  int4* info;                        // [n_cta][2]
+  void* left;                        // [n_cta] chunk::Left
 };
-size_t paged_chunk_workspace(int T, int H, int G, int HD, int dtype, int n_sm);
+size_t paged_chunk_workspace(int HD, int dtype, int n_sm);
 cudaError_t launch_paged_chunk(ChunkArgs a, int n_sm, cudaStream_t s);
 
 struct LogprobsArgs {

@@ -2,7 +2,7 @@
 //   s_j = scale q_t . k_j,  o_t = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  lse_t = m + log sum_j e^(s_j - m),  m = max_j s_j
 // over the tokens j that row t sees, j <= its position.  paged_chunk.cuh says how the work is cut.
 //
-// This file: the products as FFMA, queries, keys, values, weights and sums in fp32; and the join of what several CTAs have of an item.
+// This file: fp32 caches, the products as FFMA; and the join of what several CTAs have of an item.
 // A CTA's 256 threads hold 64 rows and walk their keys, 64 at a time.  Keys and values come row by row through the page table, 16 bytes a
 // copy, while the tile before is worked on; rows of no token become zeros.
 //   scores   a thread has 4 rows x 4 keys, summed as even and odd entries (pairs: fma2); rows padded to an odd number of 16-byte pieces
@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "paged_chunk.cuh"
+#include "paged_chunk_tc.h"
 
 namespace {
 using namespace chunk;
@@ -25,8 +26,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, int HD>
+template <int HD>
 __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const ChunkArgs a) {
+  using T = float;
   constexpr int LD = row_ld<HD>(), PL = TR + 4;
   constexpr int CW = HD % 64 == 0 ? 4 : HD % 32 == 0 ? 2 : 1, NC = HD / (16 * CW);  // columns side by side, and how often
   extern __shared__ __align__(16) float sm[];
@@ -42,7 +44,7 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
   pdl_wait();
   clear_rest<T>(a);
   find_share<TR, BK, NT, LEAST>(a, room, &place);
-  if (threadIdx.x < 2) *info_of(a, blockIdx.x, threadIdx.x) = make_int4(-1, 0, 0, 0);
+  if (threadIdx.x == 0) leave_nothing(a, place);
   __syncthreads();
   const int lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float sc = a.scale * 1.4426950408889634f;
@@ -79,19 +81,11 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
       const T* pool = (const T*)(value ? a.v.p : a.k.p);
       float* dst = value ? sV : sK;
       const int ld = value ? HD : LD;
-      constexpr int E = 16 / sizeof(T), PIECES = HD / E;
+      constexpr int PIECES = HD / 4;
       for (int i = threadIdx.x; i < BK * PIECES; i += NT) {
         const int r = i / PIECES, p = i - r * PIECES;
         const long long at = off[r];
-        if constexpr (sizeof(T) == 4) {
-          cp16(smem_u32(dst + r * ld + p * 4), at >= 0 ? pool + at + p * 4 : pool, at >= 0);
-        } else {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (at >= 0) x = *reinterpret_cast<const uint4*>(pool + at + p * E);
-          const T* v = reinterpret_cast<const T*>(&x);
-#pragma unroll
-          for (int e = 0; e < E; ++e) dst[r * ld + p * E + e] = up(v[e]);
-        }
+        cp16(smem_u32(dst + r * ld + p * 4), at >= 0 ? pool + at + p * 4 : pool, at >= 0);
       }
       cp_commit();
     };
@@ -204,8 +198,7 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
     const bool whole = c.whole();
     float* part_o = whole ? nullptr : a.part_o + (size_t)(2 * blockIdx.x + c.slot()) * TR * HD;
     float2* part_ml = whole ? nullptr : a.part_ml + (size_t)(2 * blockIdx.x + c.slot()) * TR;
-    if (!whole && threadIdx.x == 0) *info_of(a, blockIdx.x, c.slot()) = make_int4(c.b, c.tile, c.g, c.j1 == c.nb);
-    unsigned odd = 0;
+    if (!whole && threadIdx.x == 0) left_of(a, blockIdx.x).part[c.slot()] = make_int4(c.b, c.tile, c.g, c.j1 == c.nb);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int f = flat0 + ty * 4 + i;
@@ -217,7 +210,7 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
         finite = finite && fabsf(y[x]) < INFINITY;
       }
       if (f < flats) {
-        if (!finite) odd |= 1u << i;
+        if (!finite && whole) left_of(a, blockIdx.x).odd = 1;
         const int t = f / a.R;
         const long long at = (long long)(c.r.s0 + t) * a.H + c.g * a.R + f - t * a.R;
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
@@ -235,97 +228,121 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
         }
       }
     }
-    // rows whose sums are not finite: a warp has 8 rows, 16 lanes each 4
-    unsigned rows = __reduce_or_sync(L3_FULL, odd << (lane >> 4) * 4);
-    __syncwarp();
-    for (; rows; rows &= rows - 1) {
-      const int in_tile = (threadIdx.x >> 5) * 8 + __ffs(rows) - 1;
-      end_by_formula<T, HD>(a, c, BK, in_tile, flat0 + in_tile, part_o, part_ml);
-    }
     __syncthreads();
   } while (c.next(a));
 }
 
 // ---------------------------------------------------------------------------------------------------------------- the join
-// Block (c, y) joins 16 rows of the item that CTA c began and others ended: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+// Block (c, y) joins 16 rows of the item that CTA c began and others ended, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, and looks after
+// the rows of all its items that are not finite.
 constexpr int JROWS = 16, JT = 256;
-template <typename T, int HD, int ROWS>
+template <typename T, int HD, int TR, int BK, int WHOLE>
 __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
   pdl_launch();
   pdl_wait();
+  constexpr int N = (HD + 31) / 32;
   const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int4 first = *info_of(a, c0, 1);
-  if (first.x < 0) return;
-  const Request r = request(a, first.x);
-  for (int i = warp; i < JROWS; i += JT / 32) {
-    const int in_tile = blockIdx.y * JROWS + i, f = first.y * ROWS + in_tile;
-    if (f >= r.n * a.R) return;
-    const int t = f / a.R;
-    const long long at = (long long)(r.s0 + t) * a.H + first.z * a.R + f - t * a.R;
-    constexpr int N = (HD + 31) / 32;
-    float o[N], m, l;
-    const size_t own = (size_t)(2 * c0 + 1) * ROWS + in_tile;
-    m = a.part_ml[own].x;
-    l = a.part_ml[own].y;
+  const Left& own = left_of(a, c0);
+  const int4 first = own.part[1];
+  if (first.x >= 0) {
+    const Request r = request(a, first.x);
+    for (int i = warp; i < JROWS; i += JT / 32) {
+      const int in_tile = blockIdx.y * JROWS + i, f = first.y * TR + in_tile;
+      if (f >= r.n * a.R) break;
+      const int t = f / a.R, head = first.z * a.R + f - t * a.R;
+      const long long at = (long long)(r.s0 + t) * a.H + head;
+      float o[N], m, l;
+      const size_t p0 = (size_t)(2 * c0 + 1) * TR + in_tile;
+      m = a.part_ml[p0].x;
+      l = a.part_ml[p0].y;
 #pragma unroll
-    for (int x = 0; x < N; ++x) o[x] = lane + 32 * x < HD ? a.part_o[own * HD + lane + 32 * x] : 0.f;
-    bool ends = false;
-    for (int c = c0 + 1; c < a.n_cta && !ends; ++c) {
-      const int4 more = *info_of(a, c, 0);
-      if (more.x < 0) continue;
-      ends = more.w;
-      const size_t p = (size_t)(2 * c) * ROWS + in_tile;
-      const float2 ml = a.part_ml[p];
-      const float mn = fmaxf(m, ml.x), from = mn == -INFINITY ? 0.f : mn;
-      const float fa = exp2f(m - from), fb = exp2f(ml.x - from);
-      l = l * fa + ml.y * fb;
-      m = mn;
+      for (int x = 0; x < N; ++x) o[x] = lane + 32 * x < HD ? a.part_o[p0 * HD + lane + 32 * x] : 0.f;
+      bool ends = false;
+      for (int c = c0 + 1; c < a.n_cta && !ends; ++c) {
+        const int4 more = left_of(a, c).part[0];
+        if (more.x < 0) continue;
+        ends = more.w;
+        const size_t p = (size_t)(2 * c) * TR + in_tile;
+        const float2 ml = a.part_ml[p];
+        const float mn = fmaxf(m, ml.x), from = mn == -INFINITY ? 0.f : mn;
+        const float fa = exp2f(m - from), fb = exp2f(ml.x - from);
+        l = l * fa + ml.y * fb;
+        m = mn;
 #pragma unroll
-      for (int x = 0; x < N; ++x)
-        if (lane + 32 * x < HD) {
-          const float y = a.part_o[p * HD + lane + 32 * x];
-          // an infinite sum stays one, however small its part
-          o[x] = (fabsf(o[x]) < INFINITY || fa > 0.f ? o[x] * fa : o[x]) + (fabsf(y) < INFINITY || fb > 0.f ? y * fb : y);
-        }
+        for (int x = 0; x < N; ++x)
+          if (lane + 32 * x < HD) o[x] = o[x] * fa + a.part_o[p * HD + lane + 32 * x] * fb;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      bool odd = !(l < INFINITY);
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        odd = odd || !(fabsf(o[x]) < INFINITY);
+        if (lane + 32 * x < HD) ((T*)a.out)[at * HD + lane + 32 * x] = down<T>(o[x] * inv);
+      }
+      if (a.lse && lane == 0) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
+      if (__any_sync(L3_FULL, odd)) by_formula<T, HD>(a, first.x, first.z, r.s0 + t, head, r.seen(t));
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int x = 0; x < N; ++x)
-      if (lane + 32 * x < HD) ((T*)a.out)[at * HD + lane + 32 * x] = down<T>(o[x] * inv);
-    if (a.lse && lane == 0) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
   }
+  if (!own.odd) return;
+  Cursor<TR, BK, WHOLE> c;
+  if (c.start(a, own.place)) do {
+    if (!c.whole()) continue;
+    for (int i = warp; i < JROWS; i += JT / 32) {
+      const int f = c.tile * TR + blockIdx.y * JROWS + i;
+      if (f >= c.r.n * a.R) break;
+      const int t = f / a.R, head = c.g * a.R + f - t * a.R;
+      const T* out = (const T*)a.out + ((long long)(c.r.s0 + t) * a.H + head) * HD;
+      bool odd = false;
+#pragma unroll
+      for (int x = 0; x < N; ++x) odd = odd || (lane + 32 * x < HD && !(fabsf(up(out[lane + 32 * x])) < INFINITY));
+      if (__any_sync(L3_FULL, odd)) by_formula<T, HD>(a, c.b, c.g, c.r.s0 + t, head, c.r.seen(t));
+    }
+  } while (c.next(a));
 }
 
-size_t partials(int n_cta, int rows, int HD) { return (size_t)n_cta * 2 * (rows * ((size_t)HD * 4 + 8) + 16); }
-template <typename T, int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
+size_t partials(int n_cta, int rows, int HD) { return (size_t)n_cta * (2 * rows * ((size_t)HD * 4 + 8) + sizeof(Left)); }
+template <typename T, int TR, int BK, int WHOLE> cudaError_t join_t(const ChunkArgs& a, cudaStream_t s) {
+  const dim3 grid(a.n_cta, TR / JROWS), block(JT);
+  g_l3_pdl_next = true;
+  switch (a.HD) {
+    case 16: return launch_k(chunk_join_kernel<T, 16, TR, BK, WHOLE>, grid, block, 0, s, a);
+    case 32: return launch_k(chunk_join_kernel<T, 32, TR, BK, WHOLE>, grid, block, 0, s, a);
+    case 48: return launch_k(chunk_join_kernel<T, 48, TR, BK, WHOLE>, grid, block, 0, s, a);
+    case 64: return launch_k(chunk_join_kernel<T, 64, TR, BK, WHOLE>, grid, block, 0, s, a);
+    case 96: return launch_k(chunk_join_kernel<T, 96, TR, BK, WHOLE>, grid, block, 0, s, a);
+    default: return launch_k(chunk_join_kernel<T, 128, TR, BK, WHOLE>, grid, block, 0, s, a);
+  }
+}
+template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
   constexpr size_t smem = smem_bytes<HD>();
   a.n_cta = (HD > 64 ? 1 : 2) * n_sm;
   a.part_o = (float*)a.ws;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * TR * HD);
-  a.info = reinterpret_cast<int4*>(a.part_ml + (size_t)a.n_cta * 2 * TR);
-  cudaError_t e = allow_smem(chunk_fma_kernel<T, HD>, smem);
+  a.left = a.part_ml + (size_t)a.n_cta * 2 * TR;
+  cudaError_t e = allow_smem(chunk_fma_kernel<HD>, smem);
   if (e != cudaSuccess) return e;
-  if ((e = launch_k(chunk_fma_kernel<T, HD>, dim3(a.n_cta), dim3(NT), smem, s, a)) != cudaSuccess) return e;
-  g_l3_pdl_next = true;
-  return launch_k(chunk_join_kernel<T, HD, TR>, dim3(a.n_cta, TR / JROWS), dim3(JT), 0, s, a);
-}
-template <typename T> cudaError_t launch_t(const ChunkArgs& a, int n_sm, cudaStream_t s) {
-  switch (a.HD) {
-    case 16: return launch_hd<T, 16>(a, n_sm, s);
-    case 32: return launch_hd<T, 32>(a, n_sm, s);
-    case 48: return launch_hd<T, 48>(a, n_sm, s);
-    case 64: return launch_hd<T, 64>(a, n_sm, s);
-    case 96: return launch_hd<T, 96>(a, n_sm, s);
-    case 128: return launch_hd<T, 128>(a, n_sm, s);
-    default: return cudaErrorInvalidValue;
-  }
+  if ((e = launch_k(chunk_fma_kernel<HD>, dim3(a.n_cta), dim3(NT), smem, s, a)) != cudaSuccess) return e;
+  return join_t<float, TR, BK, WHOLE>(a, s);
 }
 }  // namespace
 
-size_t paged_chunk_workspace(int T, int H, int G, int HD, int dtype, int n_sm) { return partials(2 * n_sm, TR, HD); }
+cudaError_t launch_chunk_join_tc(const ChunkArgs& a, int rows, cudaStream_t s) {
+  if (a.dtype == L3_DTYPE_BF16) return rows == 256 ? join_t<bf16, 256, TC_BK, TC_WHOLE>(a, s) : join_t<bf16, 128, TC_BK, TC_WHOLE>(a, s);
+  return rows == 256 ? join_t<__half, 256, TC_BK, TC_WHOLE>(a, s) : join_t<__half, 128, TC_BK, TC_WHOLE>(a, s);
+}
+
+// the larger of either number of rows
+size_t paged_chunk_workspace(int HD, int dtype, int n_sm) { return dtype == L3_DTYPE_F32 ? partials(2 * n_sm, TR, HD) : partials(n_sm, 256, HD); }
 
 cudaError_t launch_paged_chunk(ChunkArgs a, int n_sm, cudaStream_t s) {
-  if (a.dtype == L3_DTYPE_F32) return launch_t<float>(a, n_sm, s);
-  if (a.dtype == L3_DTYPE_BF16) return launch_t<bf16>(a, n_sm, s);
-  return launch_t<__half>(a, n_sm, s);
+  if (a.dtype != L3_DTYPE_F32) return launch_paged_chunk_tc(a, n_sm, s);
+  switch (a.HD) {
+    case 16: return launch_hd<16>(a, n_sm, s);
+    case 32: return launch_hd<32>(a, n_sm, s);
+    case 48: return launch_hd<48>(a, n_sm, s);
+    case 64: return launch_hd<64>(a, n_sm, s);
+    case 96: return launch_hd<96>(a, n_sm, s);
+    case 128: return launch_hd<128>(a, n_sm, s);
+    default: return cudaErrorInvalidValue;
+  }
 }

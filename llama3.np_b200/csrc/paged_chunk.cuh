@@ -1,4 +1,4 @@
-// What the kernels of attention of a packed step share (paged_chunk.cu, paged_chunk_tc.cu): how the work is cut, and the slow path of rows
+// What the kernels of attention of a packed step share (paged_chunk.cu: fp32 caches, paged_chunk_tc.cu: 16-bit ones): how the work is cut, and the slow path of rows
 // that a value without a number has reached.
 //
 // The R query heads of a kv head and the n rows of a request are n R flat rows that see (nearly) the same keys; row f is token f / R, head f % R of
@@ -50,7 +50,7 @@ template <int WHOLE> __device__ __forceinline__ int ahead(long long x, int nb) {
   return (int)x / 2;
 }
 
-struct Place { int b, tile, g; long long off, rest; };  // an item, the weight of it that others have, and what this CTA has from there on
+struct Place { int b, tile, g, pad; long long off, rest; };  // an item, the weight of it that others have, and what this CTA has from there on
 
 // This CTA's share, by all NT threads (`room`: NT / 32 + 1 words of shared memory).  LEAST: the least weight of a share.
 template <int TR, int BK, int NT, int LEAST>
@@ -80,7 +80,7 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, 
     if (lane >= o) run += y;
   }
   if (lane == 31) room[warp] = run;
-  if (threadIdx.x == 0) *place = Place{-1, 0, 0, 0, 0};
+  if (threadIdx.x == 0) *place = Place{-1, 0, 0, 0, 0, 0};
   __syncthreads();
   long long before = run - sum, all = 0;
 #pragma unroll
@@ -100,7 +100,7 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, 
           return false;
         }
         const int g = (int)((w0 - at) / w);
-        *place = Place{b, t, g, w0 - at - (long long)g * w, w1 - w0};
+        *place = Place{b, t, g, 0, w0 - at - (long long)g * w, w1 - w0};
         return true;
       });
     }
@@ -161,11 +161,9 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // The values of a key that a row sees may be infinite or NaN, those of keys that it does not see have to be kept out even so, and tiles
-// multiply them by a weight of 0.  A row whose sums are not finite is therefore taken once more, by the formula alone: the keys k0 <= j < k1 one at a
-// time, by a warp; only what the row sees enters.  A weight is 0 for a score of -infinity only, however small, as its value may be infinite.
-// m is in units of log 2, l and o as the tiles' are.
-template <typename T, int HD>
-__device__ __noinline__ void by_formula(const ChunkArgs& a, int b, int g, int row, int head, int k0, int k1, float (&o)[(HD + 31) / 32], float& m, float& l) {
+// multiply them by a weight of 0.  A row whose result is not finite is therefore taken once more, behind the join, by the formula alone: its keys one
+// at a time, by a warp; only what the row sees enters.  A weight is 0 for a score of -infinity only, however small, as its value may be infinite.
+template <typename T, int HD> __device__ __forceinline__ void by_formula(const ChunkArgs& a, int b, int g, int row, int head, int seen) {
   constexpr int N = (HD + 31) / 32;
   const int lane = threadIdx.x & 31;
   const int* table = a.table + b * a.table_stride;
@@ -185,14 +183,13 @@ __device__ __noinline__ void by_formula(const ChunkArgs& a, int b, int g, int ro
       if (lane + 32 * i < HD) s += up(q[lane + 32 * i]) * up(k[lane + 32 * i]);
     return warp_sum(s) * sc;
   };
-  m = -INFINITY;
-  l = 0.f;
+  float o[N], m = -INFINITY, l = 0.f;
   bool there;
-  for (int j = k0; j < k1; ++j) m = fmaxf(m, score(j, there));
+  for (int j = 0; j < seen; ++j) m = fmaxf(m, score(j, there));
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   const float from = m == -INFINITY ? 0.f : m;
-  for (int j = k0; j < k1; ++j) {
+  for (int j = 0; j < seen; ++j) {
     const float s = score(j, there);
     if (!there) continue;
     const float x = s - from;
@@ -203,27 +200,12 @@ __device__ __noinline__ void by_formula(const ChunkArgs& a, int b, int g, int ro
     for (int i = 0; i < N; ++i)
       if (lane + 32 * i < HD) o[i] += w * up(v[lane + 32 * i]);
   }
-}
-// the same, with its result where the tile would have put it
-template <typename T, int HD, typename Cur>
-__device__ __forceinline__ void end_by_formula(const ChunkArgs& a, const Cur& c, int BK, int in_tile, int flat, float* part_o, float2* part_ml) {
-  float o[(HD + 31) / 32], m, l;
-  const int lane = threadIdx.x & 31, t = flat / a.R, head = c.g * a.R + flat - t * a.R, row = c.r.s0 + t;
-  by_formula<T, HD>(a, c.b, c.g, row, head, c.j0 * BK, min(c.j1 * BK, c.r.seen(t)), o, m, l);
   const long long at = (long long)row * a.H + head;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int i = 0; i < (HD + 31) / 32; ++i) {
-    const int d = lane + 32 * i;
-    if (d < HD) {
-      if (part_o) part_o[(long long)in_tile * HD + d] = o[i];
-      else ((T*)a.out)[at * HD + d] = down<T>(o[i] * inv);
-    }
-  }
-  if (lane == 0) {
-    if (part_o) part_ml[in_tile] = make_float2(m, l);
-    else if (a.lse) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
-  }
+  for (int i = 0; i < N; ++i)
+    if (lane + 32 * i < HD) ((T*)a.out)[at * HD + lane + 32 * i] = down<T>(o[i] * inv);
+  if (lane == 0 && a.lse) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // rows of no request: as they are, or 0
@@ -237,7 +219,19 @@ template <typename T> __device__ __forceinline__ void clear_rest(const ChunkArgs
   }
 }
 
-// what a CTA leaves for the join about its two partials: (request, tile, kv head, 1 if the item ends with it), request -1: none
-__device__ __forceinline__ int4* info_of(const ChunkArgs& a, int cta, int slot) { return a.info + 2 * cta + slot; }
+// What a CTA leaves for the join: its share, whether a result of an item that it has whole is not finite, and of its two partials - of the
+// item that it goes on with, and of the one that it begins - (request, tile, kv head, 1 if the item ends with it), request -1: none.
+struct Left {
+  Place place;
+  int4 part[2];
+  int odd, pad[3];
+};
+static_assert(sizeof(Left) % 16 == 0, "");
+__device__ __forceinline__ Left& left_of(const ChunkArgs& a, int cta) { return reinterpret_cast<Left*>(a.left)[cta]; }
+__device__ __forceinline__ void leave_nothing(const ChunkArgs& a, const Place& place) {  // by one thread, ahead of all others' words
+  Left& left = left_of(a, blockIdx.x);
+  left.place = place;
+  left.part[0] = left.part[1] = make_int4(-1, 0, 0, 0);
+  left.odd = 0;
+}
 }  // namespace chunk
-

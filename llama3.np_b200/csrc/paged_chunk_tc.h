@@ -1,0 +1,8 @@
+// Interface between paged_chunk.cu and paged_chunk_tc.cu (caches of 16 bits).
+#pragma once
+#include "packed.h"
+
+int paged_chunk_tc_rows(int T, int H, int G, int B, long long keys, int n_sm);  // of an item: 128 or 256
+cudaError_t launch_paged_chunk_tc(const ChunkArgs& a, int n_sm, cudaStream_t s);
+constexpr int TC_BK = 128, TC_WHOLE = 4;                                             // keys of a block; items of so few blocks are not cut
+cudaError_t launch_chunk_join_tc(const ChunkArgs& a, int rows, cudaStream_t s);  // paged_chunk.cu; rows: of an item
