@@ -49,6 +49,10 @@ int tc_debug_timeline(int enable, unsigned long long* out64);
 // (ld: row stride in elements, 0 = cols; multiples of 16 bytes)
 const CUtensorMap* tc_get_map(const void* ptr, bool is_bf16, int rows, int cols, int box_rows, int ld = 0);
 
+// a map of up to five dimensions of 16-bit values for tiles with rows of 128 bytes, 128-byte swizzle, zeros outside; strides in bytes, from the
+// second dimension on (false: no driver entry point, or sizes that it refuses)
+bool tc_make_map(CUtensorMap* tm, const void* ptr, bool is_bf16, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
+
 // fp32 projections at fp32 precision on the tensor cores (gemm_f32.cu): fp32 A, W fp32 or bf16; EPI_STORE, EPI_RESID, EPI_SWIGLU
 struct GemmF32Args {
   const float* A;       // [rows, K], row stride lda (0: K)

@@ -48,7 +48,7 @@ struct ChunkArgs {
   bool clear_rest;
   void* ws;                          // paged_chunk_workspace bytes, 16-byte aligned
   // set by the launcher
-  int n_cta;
+  int n_cta, tile_rows;              // CTAs, flat rows of an item
   float* part_o;                     // [n_cta][2][rows of a tile][HD]
   float2* part_ml;                   // [n_cta][2][rows of a tile]
   void* left;                        // [n_cta] chunk::Left

@@ -43,12 +43,12 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
   pdl_launch();
   pdl_wait();
   clear_rest<T>(a);
-  find_share<TR, BK, NT, LEAST>(a, room, &place);
+  find_share<BK, NT, LEAST>(a, room, &place);
   if (threadIdx.x == 0) leave_nothing(a, place);
   __syncthreads();
   const int lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float sc = a.scale * 1.4426950408889634f;
-  Cursor<TR, BK, WHOLE> c;
+  Cursor<BK, WHOLE> c;
   if (!c.start(a, place)) return;
   do {
     const int* table = a.table + c.b * a.table_stride;
@@ -236,11 +236,12 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
 // Block (c, y) joins 16 rows of the item that CTA c began and others ended, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, and looks after
 // the rows of all its items that are not finite.
 constexpr int JROWS = 16, JT = 256;
-template <typename T, int HD, int TR, int BK, int WHOLE>
+template <typename T, int HD, int BK, int WHOLE>
 __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
   pdl_launch();
   pdl_wait();
   constexpr int N = (HD + 31) / 32;
+  const int TR = a.tile_rows;
   const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Left& own = left_of(a, c0);
   const int4 first = own.part[1];
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
     }
   }
   if (!own.odd) return;
-  Cursor<TR, BK, WHOLE> c;
+  Cursor<BK, WHOLE> c;
   if (c.start(a, own.place)) do {
     if (!c.whole()) continue;
     for (int i = warp; i < JROWS; i += JT / 32) {
@@ -301,34 +302,34 @@ __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
 }
 
 size_t partials(int n_cta, int rows, int HD) { return (size_t)n_cta * (2 * rows * ((size_t)HD * 4 + 8) + sizeof(Left)); }
-template <typename T, int TR, int BK, int WHOLE> cudaError_t join_t(const ChunkArgs& a, cudaStream_t s) {
-  const dim3 grid(a.n_cta, TR / JROWS), block(JT);
+template <typename T, int BK, int WHOLE> cudaError_t join_t(const ChunkArgs& a, cudaStream_t s) {
+  const dim3 grid(a.n_cta, a.tile_rows / JROWS), block(JT);
   g_l3_pdl_next = true;
   switch (a.HD) {
-    case 16: return launch_k(chunk_join_kernel<T, 16, TR, BK, WHOLE>, grid, block, 0, s, a);
-    case 32: return launch_k(chunk_join_kernel<T, 32, TR, BK, WHOLE>, grid, block, 0, s, a);
-    case 48: return launch_k(chunk_join_kernel<T, 48, TR, BK, WHOLE>, grid, block, 0, s, a);
-    case 64: return launch_k(chunk_join_kernel<T, 64, TR, BK, WHOLE>, grid, block, 0, s, a);
-    case 96: return launch_k(chunk_join_kernel<T, 96, TR, BK, WHOLE>, grid, block, 0, s, a);
-    default: return launch_k(chunk_join_kernel<T, 128, TR, BK, WHOLE>, grid, block, 0, s, a);
+    case 16: return launch_k(chunk_join_kernel<T, 16, BK, WHOLE>, grid, block, 0, s, a);
+    case 32: return launch_k(chunk_join_kernel<T, 32, BK, WHOLE>, grid, block, 0, s, a);
+    case 48: return launch_k(chunk_join_kernel<T, 48, BK, WHOLE>, grid, block, 0, s, a);
+    case 64: return launch_k(chunk_join_kernel<T, 64, BK, WHOLE>, grid, block, 0, s, a);
+    case 96: return launch_k(chunk_join_kernel<T, 96, BK, WHOLE>, grid, block, 0, s, a);
+    default: return launch_k(chunk_join_kernel<T, 128, BK, WHOLE>, grid, block, 0, s, a);
   }
 }
 template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
   constexpr size_t smem = smem_bytes<HD>();
   a.n_cta = (HD > 64 ? 1 : 2) * n_sm;
+  a.tile_rows = TR;
   a.part_o = (float*)a.ws;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * TR * HD);
   a.left = a.part_ml + (size_t)a.n_cta * 2 * TR;
   cudaError_t e = allow_smem(chunk_fma_kernel<HD>, smem);
   if (e != cudaSuccess) return e;
   if ((e = launch_k(chunk_fma_kernel<HD>, dim3(a.n_cta), dim3(NT), smem, s, a)) != cudaSuccess) return e;
-  return join_t<float, TR, BK, WHOLE>(a, s);
+  return join_t<float, BK, WHOLE>(a, s);
 }
 }  // namespace
 
-cudaError_t launch_chunk_join_tc(const ChunkArgs& a, int rows, cudaStream_t s) {
-  if (a.dtype == L3_DTYPE_BF16) return rows == 256 ? join_t<bf16, 256, TC_BK, TC_WHOLE>(a, s) : join_t<bf16, 128, TC_BK, TC_WHOLE>(a, s);
-  return rows == 256 ? join_t<__half, 256, TC_BK, TC_WHOLE>(a, s) : join_t<__half, 128, TC_BK, TC_WHOLE>(a, s);
+cudaError_t launch_chunk_join_tc(const ChunkArgs& a, cudaStream_t s) {
+  return a.dtype == L3_DTYPE_BF16 ? join_t<bf16, TC_BK, TC_WHOLE>(a, s) : join_t<__half, TC_BK, TC_WHOLE>(a, s);
 }
 
 // the larger of either number of rows

@@ -2,7 +2,7 @@
 // that a value without a number has reached.
 //
 // The R query heads of a kv head and the n rows of a request are n R flat rows that see (nearly) the same keys; row f is token f / R, head f % R of
-// the group.  An item is TR of them (a tile) against the blocks of BK keys that its last row sees.  The items of all requests, tiles and kv heads, in
+// the group.  An item is tile_rows of them (a tile) against the blocks of BK keys that its last row sees.  The items of all requests, tiles and kv heads, in
 // that order, are one long line, weighed by their blocks, that the CTAs share out evenly: prompts, portions and single tokens of any mixture leave no
 // SM idle.  An item of few blocks goes to the CTA that has its middle; longer ones are cut where the shares end, leave partials (m, l, o) that a
 // second, dependent launch joins in the order of the keys, so that results do not change from run to run.
@@ -34,9 +34,9 @@ __device__ __forceinline__ Request request(const ChunkArgs& a, int b) {
   r.keys = a.max_pages << a.log_page;
   return r;
 }
-template <int TR> __device__ __forceinline__ int tiles(const ChunkArgs& a, int n) { return (int)((unsigned)(n * a.R + TR - 1) / TR); }
-template <int TR, int BK> __device__ __forceinline__ int blocks(const ChunkArgs& a, const Request& r, int tile) {
-  const int last = min(r.n * a.R, (tile + 1) * TR) - 1;
+__device__ __forceinline__ int tiles(const ChunkArgs& a, int n) { return (int)((unsigned)(n * a.R + a.tile_rows - 1) / (unsigned)a.tile_rows); }
+template <int BK> __device__ __forceinline__ int blocks(const ChunkArgs& a, const Request& r, int tile) {
+  const int last = min(r.n * a.R, (tile + 1) * a.tile_rows) - 1;
   return (int)((unsigned)(r.seen(last / a.R) + BK - 1) / BK);
 }
 // An item's weight: two a block, and what begins and ends it like half a block.
@@ -53,7 +53,7 @@ template <int WHOLE> __device__ __forceinline__ int ahead(long long x, int nb) {
 struct Place { int b, tile, g, pad; long long off, rest; };  // an item, the weight of it that others have, and what this CTA has from there on
 
 // This CTA's share, by all NT threads (`room`: NT / 32 + 1 words of shared memory).  LEAST: the least weight of a share.
-template <int TR, int BK, int NT, int LEAST>
+template <int BK, int NT, int LEAST>
 __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, Place* place) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // a thread takes `each` requests, or one of `parts` parts of a request's tiles
@@ -62,10 +62,10 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, 
     const int b0 = parts > 1 ? threadIdx.x / parts : threadIdx.x * each, b1 = min(parts > 1 ? b0 + 1 : b0 + each, a.B);
     for (int b = b0; b < b1; ++b) {
       const Request r = request(a, b);
-      const int nt = tiles<TR>(a, r.n), part = parts > 1 ? threadIdx.x % parts : 0;
+      const int nt = tiles(a, r.n), part = parts > 1 ? threadIdx.x % parts : 0;
       const int t0 = (int)((long long)nt * part / parts), t1 = (int)((long long)nt * (part + 1) / parts);
       for (int t = t0; t < t1; ++t)
-        if (f(b, t, weight(blocks<TR, BK>(a, r, t)))) return;
+        if (f(b, t, weight(blocks<BK>(a, r, t)))) return;
     }
   };
   long long sum = 0;
@@ -109,17 +109,17 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, 
 }
 
 // One stretch of blocks after the other.
-template <int TR, int BK, int WHOLE> struct Cursor {
+template <int BK, int WHOLE> struct Cursor {
   int b, tile, g, nt, nb;
   Request r;
   long long off, rest;
   int j0, j1;               // blocks of this stretch
-  __device__ __forceinline__ void at_tile(const ChunkArgs& a) { nb = blocks<TR, BK>(a, r, tile); }
+  __device__ __forceinline__ void at_tile(const ChunkArgs& a) { nb = blocks<BK>(a, r, tile); }
   __device__ __forceinline__ bool start(const ChunkArgs& a, const Place& p) {
     b = p.b; tile = p.tile; g = p.g; off = p.off; rest = p.rest;
     if (b < 0) return false;
     r = request(a, b);
-    nt = tiles<TR>(a, r.n);
+    nt = tiles(a, r.n);
     at_tile(a);
     return settle(a) ? true : next(a);
   }
@@ -142,7 +142,7 @@ template <int TR, int BK, int WHOLE> struct Cursor {
           do {
             if (++b >= a.B) return false;
             r = request(a, b);
-            nt = tiles<TR>(a, r.n);
+            nt = tiles(a, r.n);
           } while (nt == 0);
         }
         at_tile(a);

@@ -1,9 +1,9 @@
 // Attention of the rows of a packed step over a 16-bit cache in pages (paged_chunk.cu has the formula, paged_chunk.cuh how the work is cut), on
 // tcgen05: a CTA an SM, blocks of 128 keys, score tiles of 128 rows x 128 keys.
 //
-//   warps 10, 11  loaders: the item's queries, then keys and values of its blocks, row by row through the page table, 16 bytes a copy
-//                 (cp.async; any page size and strides), into a ring of operand tiles (K-major rows of 128 bytes, swizzled); rows of no
-//                 token become zeros, and their bits go to the softmax warps
+//   warps 10, 11  loaders: the item's queries, then keys and values of its blocks, a page a TMA copy, into a ring of operand tiles (K-major rows of
+//                 128 bytes, swizzled); rows of no token become zeros, and their bits go to the softmax warps.  Pages of fewer than 8 tokens,
+//                 expanded strides, and queries whose heads do not fill 128 rows evenly go row by row, 16 bytes a copy (cp.async)
 //   warp 8        products: S = Q K^T into TMEM, O += P V with P from TMEM and V as it lies, an MN-major operand
 //   warps 0 - 7   softmax, a thread a row, four warps a score tile: its 128 scores in registers, exponentials against a maximum that follows
 //                 the running one lazily (O is rescaled in TMEM only when that has grown by 2^GROW), weights as 16-bit values over the scores
@@ -27,15 +27,15 @@ namespace {
 using namespace chunk;
 constexpr int BK = TC_BK, NT = 384, SOFT = 256, LOADERS = 2, SETS = 4 / LOADERS;  // SETS: of 32 rows of a tile, a loader's
 constexpr int WHOLE = TC_WHOLE, LEAST = 4;
+constexpr int POLY = 1;    // of four neighbouring pairs of exponentials, how many are taken by a polynomial
 constexpr int THERE = 16;  // blocks whose keys' bits are kept: more than the ring holds
 
-template <typename T, int HD, bool TWO> struct Cfg {
-  static constexpr int TR = TWO ? 256 : 128;
+template <typename T, int HD> struct Cfg {
   static constexpr int QS = (HD + 63) / 64;             // slices of 64 entries, rows of 128 bytes
   static constexpr int TILE = QS * 128 * 128;           // bytes of 128 rows
-  static constexpr int NS = HD > 64 ? 5 : 8;            // tiles of the ring
-  static constexpr int AHEAD = TWO ? 1 : 2;             // blocks of keys that are multiplied ahead of the first one's values
-  static constexpr int SMEM = (TWO ? 2 : 1) * TILE + NS * TILE + THERE * 16 + (TWO ? 0 : 2 * 128 * 8) + 256 + 1024;
+  static constexpr int NS = HD > 64 ? 4 : 8;            // tiles of the ring
+  static constexpr int STAGE = 4096;                    // bytes of a softmax warp's results on their way out, 32 rows of 128
+  static constexpr int SMEM = 2 * TILE + NS * TILE + 8 * STAGE + THERE * 16 + 256 + 1024;
   static constexpr uint32_t FMT = std::is_same<T, bf16>::value ? 1u : 0u;
   static constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(BK >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr uint32_t IDESC_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);
@@ -123,41 +123,76 @@ template <typename T> __device__ __forceinline__ uint32_t pack(float x, float y)
   }
 }
 
-// Barriers of a CTA, 8 bytes each.
-struct Bars {
-  uint32_t q_full, q_empty, s_full, p_full, o_full, full, empty;  // s_full, p_full, o_full: of both score tiles
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {  // NaN if one of them is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d) : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
+  return *reinterpret_cast<const float2*>(&d);
+}
+// 2^x without the unit for it, for x <= 20: x = n + f, |f| <= 1/2, by adding and taking off a number whose last bit is 1, and a polynomial of degree 4
+// (minimax of the relative error on [-1/2, 1/2] by Remez's exchange: at most 2.6e-6 off, 4e-8 on average).  Below 2^-125 the result is about that.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
+  x.x = fmaxf(x.x, -125.f);
+  x.y = fmaxf(x.y, -125.f);
+  const float2 t = add2(x, magic), f = fma2(add2(t, back), minus, x);
+  float2 y = make_float2(0.009570102207362652f, 0.009570102207362652f);
+  y = fma2(y, f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+  y = fma2(y, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
+}
+// Maps of the queries (entries, heads, rows) and the pools (entries, tokens, heads, pages), where tiles are copied by them.
+struct Maps {
+  CUtensorMap q, k, v;
 };
 
-template <typename T, int HD, bool TWO>
-__global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
-  using C = Cfg<T, HD, TWO>;
-  constexpr int TR = C::TR, NS = C::NS, TILE = C::TILE, AHEAD = C::AHEAD;
-  using Cur = Cursor<TR, BK, WHOLE>;
+// Barriers of a CTA, 8 bytes each.
+struct Bars {
+  uint32_t q_full, q_empty, landed, s_full, half_p, p_full, o_full, full, empty;  // s_full .. o_full: of both score tiles
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ Maps maps, const bool tma_q, const bool tma_kv) {
+  using C = Cfg<T, HD>;
+  constexpr int NS = C::NS, TILE = C::TILE;
+  using Cur = Cursor<BK, WHOLE>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long room[NT / 32 + 1];
   __shared__ Place place;
   __shared__ int failed;
   volatile int* const fail = &failed;
-  const uint32_t raw = smem_u32(smem_raw), sQ = (raw + 1023u) & ~1023u, ring = sQ + (TWO ? 2 : 1) * TILE;
-  uint8_t* const rest = smem_raw + (ring + NS * TILE - raw);
-  uint32_t* const there = reinterpret_cast<uint32_t*>(rest);                  // [THERE][4]
-  float2* const xch = reinterpret_cast<float2*>(rest + THERE * 16);           // [2][128], one tile of rows
-  const uint32_t bars = ring + NS * TILE + THERE * 16 + (TWO ? 0 : 2 * 128 * 8);
-  const Bars B{bars, bars + 8, bars + 16, bars + 32, bars + 48, bars + 64, bars + 64 + 8 * NS};
+  const uint32_t raw = smem_u32(smem_raw), sQ = (raw + 1023u) & ~1023u, ring = sQ + 2 * TILE;
+  uint8_t* const stages = smem_raw + (ring + NS * TILE - raw);
+  uint32_t* const there = reinterpret_cast<uint32_t*>(stages + 8 * C::STAGE);  // [THERE][4]
+  const uint32_t bars = ring + NS * TILE + 8 * C::STAGE + THERE * 16;
+  const Bars B{bars, bars + 8, bars + 16, bars + 24, bars + 40, bars + 56, bars + 72, bars + 88, bars + 88 + 8 * NS};
   const uint32_t tmem_slot = B.empty + 8 * NS;
   uint32_t* const tmem_slot_ptr = reinterpret_cast<uint32_t*>(smem_raw + (tmem_slot - raw));
   const int warp = __shfl_sync(L3_FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   pdl_launch();
-  pdl_wait();
-  clear_rest<T>(a);
-  find_share<TR, BK, NT, LEAST>(a, room, &place);
-  if (threadIdx.x == 0) leave_nothing(a, place);
-  if (place.b < 0) return;
   if (threadIdx.x == 0) {
-    mbar_init(B.q_full, LOADERS);
+    mbar_init(B.q_full, tma_q ? 1 : LOADERS);
     mbar_init(B.q_empty, 1);
-    for (int w = 0; w < 2; ++w) { mbar_init(B.s_full + 8 * w, 1); mbar_init(B.p_full + 8 * w, 4); mbar_init(B.o_full + 8 * w, 1); }
-    for (int s = 0; s < NS; ++s) { mbar_init(B.full + 8 * s, LOADERS); mbar_init(B.empty + 8 * s, 1); }
+    mbar_init(B.landed, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(B.s_full + 8 * w, 1); mbar_init(B.half_p + 8 * w, 4); mbar_init(B.p_full + 8 * w, 4); mbar_init(B.o_full + 8 * w, 1);
+    }
+    for (int s = 0; s < NS; ++s) { mbar_init(B.full + 8 * s, tma_kv ? 1 : LOADERS); mbar_init(B.empty + 8 * s, 1); }
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -165,11 +200,16 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "n"(T_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  pdl_wait();
+  clear_rest<T>(a);
   tc_fence_before();
-  __syncthreads();
+  find_share<BK, NT, LEAST>(a, room, &place);
   tc_fence_after();
+  if (threadIdx.x == 0) leave_nothing(a, place);
   const uint32_t tmem = *tmem_slot_ptr;
-  Cur c;
+  Cur c{};
+  // an item of up to 128 rows has one tile of rows, whose blocks the two score tiles share out; else there are two over the same blocks
+  auto two_tiles = [&]() { return min(c.r.n * a.R - c.tile * a.tile_rows, a.tile_rows) > 128; };
   // 168 registers a thread at launch: twice 216 and 72 of the warps that share a scheduler
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -179,12 +219,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
     uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0};
     auto arrived = [&]() {  // the ring's next tile
       mbar_wait(B.full + 8 * slot, phase, fail);
+      tc_fence_after();
       const int s = slot;
       if (++slot == NS) { slot = 0; phase ^= 1; }
       return s;
     };
-    auto scores = [&](int w, int s) {
-      const uint32_t q = sQ + (TWO ? w * TILE : 0), k = ring + s * TILE;
+    auto scores = [&](int w, int q_tile, int s) {
+      const uint32_t q = sQ + q_tile * TILE, k = ring + s * TILE;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
@@ -195,17 +236,20 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
       }
       __syncwarp();
     };
-    auto weighted = [&](int w, int s, bool first) {
-      mbar_wait(B.p_full + 8 * w, p_phase[w], fail);
-      p_phase[w] ^= 1;
-      tc_fence_after();
+    auto weighted = [&](int w, int s, bool first) {  // a half of the keys as soon as their weights are there
       const uint32_t v = ring + s * TILE;
-      if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk)
-          mma_ts(tmem + T_O + w * 128, tmem + w * BK + kk * 8, desc_mn(v + kk * 2048, 16384), C::IDESC_PV, !first || kk > 0);
+      for (int h = 0; h < 2; ++h) {
+        mbar_wait((h ? B.p_full : B.half_p) + 8 * w, p_phase[w], fail);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+            mma_ts(tmem + T_O + w * 128, tmem + w * BK + kk * 8, desc_mn(v + kk * 2048, 16384), C::IDESC_PV, !first || kk > 0);
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      p_phase[w] ^= 1;
     };
     auto commit = [&](uint32_t bar) {
       if (elect_one()) tc_commit(bar);
@@ -217,11 +261,10 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
       mbar_wait(B.q_full, q_phase, fail);
       q_phase ^= 1;
       tc_fence_after();
-      if constexpr (TWO) {
+      if (two_tiles()) {
         int k = arrived();
-        tc_fence_after();
-        scores(0, k);
-        scores(1, k);
+        scores(0, 0, k);
+        scores(1, 1, k);
         commit(B.empty + 8 * k);
         if (n == 1) commit(B.q_empty);
         for (int j = 0; j < n; ++j) {
@@ -231,7 +274,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             weighted(w, v, j == 0);
-            if (more) scores(w, k);
+            if (more) scores(w, w, k);
             else commit(B.o_full + 8 * w);
           }
           commit(B.empty + 8 * v);
@@ -241,8 +284,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
       } else {
         for (int i = 0; i < min(n, 2); ++i) {
           const int k = arrived();
-          tc_fence_after();
-          scores(i, k);
+          scores(i, 0, k);
           commit(B.empty + 8 * k);
         }
         if (n <= 2) commit(B.q_empty);
@@ -250,17 +292,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
         for (int i = 0; i < n; ++i) {
           const int w = i & 1, v = arrived();
           weighted(w, v, i < 2);
+          commit(B.empty + 8 * v);
           if (i + 2 < n) {
-            commit(B.empty + 8 * v);
             const int k = arrived();
-            tc_fence_after();
-            scores(w, k);
+            scores(w, 0, k);
             commit(B.empty + 8 * k);
             if (i + 3 == n) commit(B.q_empty);
-          } else {
-            commit(B.o_full + 8 * w);
-            commit(B.empty + 8 * v);
-          }
+          } else commit(B.o_full + 8 * w);
         }
       }
     } while (c.next(a));
@@ -268,7 +306,8 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
     constexpr int PIECES = HD / 8;
     const int row0 = (warp - 10) * 32 * SETS;
     int slot = 0, blocks_so_far = 0, waiting = 0;
-    uint32_t phase = 1, q_phase = 1, w0 = 0, w1 = 0;  // waiting: fills that have not been told of, at w0 (the older) and w1
+    const bool first_loader = warp == 10;
+    uint32_t phase = 1, q_phase = 1, landed_phase = 0, w0 = 0, w1 = 0;  // waiting: fills that have not been told of, at w0 (the older) and w1
     auto tell = [&](uint32_t bar) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // what the copies wrote -> the tensor core
       __syncwarp();
@@ -300,7 +339,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
     };
     // 32 rows, lane r's at src (null: zeros), into rows row0 .. of the tile
     auto rows = [&](const T* src, uint32_t tile, int row0) {
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < PIECES; ++i) {
         const int at = i * 32 + lane, r = at / PIECES, p = at % PIECES, row = row0 + r;
         const T* from = reinterpret_cast<const T*>(__shfl_sync(L3_FULL, reinterpret_cast<unsigned long long>(src), r));
@@ -311,17 +350,101 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
     if (c.start(a, place)) do {
       const int n = c.j1 - c.j0;
       if (n == 0) continue;
-      const int flat0 = c.tile * TR, flats = c.r.n * a.R;
-      const int most = c.r.seen((min(flats, flat0 + TR) - 1) / a.R);
+      const int flat0 = c.tile * a.tile_rows, flats = c.r.n * a.R;
+      const int most = c.r.seen((min(flats, flat0 + a.tile_rows) - 1) / a.R);
       const int* table = a.table + c.b * a.table_stride;
-      free_to_fill(B.q_empty, q_phase);
-      q_phase ^= 1;
+      const bool two = two_tiles();
+      const int ahead = two ? 1 : 2;  // blocks of keys that are multiplied ahead of the first one's values
+      if (tma_q) {
+        if (first_loader) {
+          free_to_fill(B.q_empty, q_phase);
+          if (elect_one()) {
+            mbar_expect_tx(B.q_full, (two ? 2 : 1) * TILE);
 #pragma unroll 1
-      for (int h = 0; h < TR / 128 * SETS; ++h) {
-        const int in = row0 + h % SETS * 32, f = flat0 + h / SETS * 128 + in + lane, t = f / a.R;
-        rows(f < flats ? (const T*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh : nullptr, sQ + h / SETS * TILE, in);
+            for (int h = 0; h < (two ? 2 : 1); ++h)
+#pragma unroll
+              for (int x = 0; x < C::QS; ++x)
+                tma_3d(sQ + h * TILE + x * 16384, &maps.q, x * 64, c.g * a.R, c.r.s0 + (flat0 + h * 128) / a.R, B.q_full);
+          }
+          __syncwarp();
+        }
+      } else {
+        free_to_fill(B.q_empty, q_phase);
+#pragma unroll 1
+        for (int h = 0; h < (two ? 2 : 1) * SETS; ++h) {
+          const int in = row0 + h % SETS * 32, f = flat0 + h / SETS * 128 + in + lane, t = f / a.R;
+          rows(f < flats ? (const T*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh : nullptr, sQ + h / SETS * TILE, in);
+        }
+        filled(B.q_full);
+        if (tma_kv) told();  // nothing else would
       }
-      filled(B.q_full);
+      q_phase ^= 1;
+      if (tma_kv) {
+        if (!first_loader) continue;
+        // one lane a page of the block, or the first one for a part of a page
+        const int page_size = 1 << a.log_page, box = min(page_size, BK), pages = BK / box;
+        auto page_of = [&](int j) {
+          const int key = j * BK + lane * box;
+          int page = -1;
+          if (lane < pages && key < most) page = __ldg(table + (key >> a.log_page));
+          return (unsigned)page < (unsigned)a.n_pages ? page : a.n_pages;  // outside: the copy's rows are zeros
+        };
+        auto fill = [&](const CUtensorMap* map, int page, int j, bool keys) {
+          const uint32_t bar = B.full + 8 * slot, tile = ring + slot * TILE;
+          mbar_wait(B.empty + 8 * slot, phase, fail);
+          if (keys) {
+            const uint32_t ok = __ballot_sync(L3_FULL, page < a.n_pages);
+            if (lane < 4) {  // the bits of 32 keys
+              uint32_t bits = 0;
+              if (box >= 32) bits = ok >> (lane * 32 / box) & 1 ? L3_FULL : 0u;
+              else
+                for (int x = 0; x < 32 / box; ++x) bits |= ok >> (lane * (32 / box) + x) & 1 ? ((1u << box) - 1) << (x * box) : 0u;
+              there[(blocks_so_far & (THERE - 1)) * 4 + lane] = bits;
+            }
+            ++blocks_so_far;
+          }
+          // values behind the last token that is seen lie in the last page, and may be no numbers: they become 0
+          const int left = most - j * BK, stop = min((left + box - 1) & -box, BK);
+          const bool clean = !keys && left < BK && left < stop;
+          const uint32_t to = clean ? B.landed : bar;
+          if (lane == 0) mbar_expect_tx(to, TILE);
+          __syncwarp();
+          if (lane < pages) {
+#pragma unroll
+            for (int x = 0; x < C::QS; ++x)
+              tma_4d(tile + x * 16384 + lane * box * 128, map, x * 64, (j * BK) & (page_size - 1) & -box, c.g, page, to);
+          }
+          __syncwarp();
+          if (clean) {
+            mbar_wait(B.landed, landed_phase, fail);
+            landed_phase ^= 1;
+            for (int i = left * 8 + lane; i < stop * 8; i += 32)
+#pragma unroll
+              for (int x = 0; x < C::QS; ++x)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + x * 16384 + i * 16), "r"(0) : "memory");
+            tell(bar);
+          }
+          if (++slot == NS) { slot = 0; phase ^= 1; }
+        };
+        int next = page_of(c.j0), had = next, had1 = next;  // had, had1: of the blocks whose values come next
+        for (int x = 0; x < min(ahead, n); ++x) {
+          (x ? had1 : had) = next;
+          const int page = next;
+          next = page_of(c.j0 + x + 1);
+          fill(&maps.k, page, c.j0 + x, true);
+        }
+        for (int i = 0; i < n; ++i) {
+          fill(&maps.v, had, c.j0 + i, false);
+          had = had1;
+          if (i + ahead < n) {
+            (two ? had : had1) = next;
+            const int page = next;
+            next = page_of(c.j0 + i + ahead + 1);
+            fill(&maps.k, page, c.j0 + i + ahead, true);
+          }
+        }
+        continue;
+      }
       auto pages_of = [&](int j) {  // of this lane's keys of block j
         Pages p;
 #pragma unroll
@@ -347,22 +470,21 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
         filled(B.full + 8 * slot);
         if (++slot == NS) { slot = 0; phase ^= 1; }
       };
-      Pages next = pages_of(c.j0), had[AHEAD];
-#pragma unroll
-      for (int x = 0; x < AHEAD; ++x)
-        if (x < n) {
-          had[x] = next;
-          next = pages_of(c.j0 + x + 1);
-          fill(a.k, had[x], c.j0 + x, true);
-        }
+      Pages next = pages_of(c.j0), had = next, had1 = next;
+      for (int x = 0; x < min(ahead, n); ++x) {
+        (x ? had1 : had) = next;
+        const Pages page = next;
+        next = pages_of(c.j0 + x + 1);
+        fill(a.k, page, c.j0 + x, true);
+      }
       for (int i = 0; i < n; ++i) {
-        fill(a.v, had[0], c.j0 + i, false);
-#pragma unroll
-        for (int x = 0; x + 1 < AHEAD; ++x) had[x] = had[x + 1];
-        if (i + AHEAD < n) {
-          had[AHEAD - 1] = next;
-          next = pages_of(c.j0 + i + AHEAD + 1);
-          fill(a.k, had[AHEAD - 1], c.j0 + i + AHEAD, true);
+        fill(a.v, had, c.j0 + i, false);
+        had = had1;
+        if (i + ahead < n) {
+          (two ? had : had1) = next;
+          const Pages page = next;
+          next = pages_of(c.j0 + i + ahead + 1);
+          fill(a.k, page, c.j0 + i + ahead, true);
         }
       }
     } while (c.next(a));
@@ -371,17 +493,18 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
     const int quarter = warp & 3, w = warp >> 2, r = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + w * BK + lanes, tO = tmem + T_O + lanes;
     // log2(e) |scale|: a weight is 2^(s sc - m sc); of 0 the smallest number, so that a score of -infinity keeps its weight of 0
-    const float sc = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
+    const float sc = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f), growth = fminf(C::GROW / sc, 3e38f);
     const bool negative = a.scale < 0.f;
     int blocks_so_far = 0;
     uint32_t s_phase = 0, o_phase = 0;
     if (c.start(a, place)) do {
       const int n = c.j1 - c.j0;
-      const int in_tile = (TWO ? w * 128 : 0) + r, f = c.tile * TR + in_tile, flats = c.r.n * a.R, t = f / a.R;
+      const bool two = two_tiles();
+      const int in_tile = (two ? w * 128 : 0) + r, f = c.tile * a.tile_rows + in_tile, flats = c.r.n * a.R, t = f / a.R;
       const int seen = f < flats ? c.r.seen(t) : 0;
       float m = -INFINITY, l = 0.f;  // m: of s, what the exponentials are taken against
       bool begun = false;
-      for (int j = TWO ? 0 : w; j < n; j += TWO ? 1 : 2) {
+      for (int j = two ? 0 : w; j < n; j += two ? 1 : 2) {
         mbar_wait(B.s_full + 8 * w, s_phase, fail);
         s_phase ^= 1;
         tc_fence_after();
@@ -406,16 +529,20 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
               if (!(in >> i & 1)) v[32 * k + i] = -INFINITY;
           }
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // NaN where one of the scores is
+        float top[4] = {max3(v[0], v[4], v[8]), max3(v[1], v[5], v[9]), max3(v[2], v[6], v[10]), max3(v[3], v[7], v[11])};
 #pragma unroll
-        for (int i = 0; i < BK; i += 4)
+        for (int i = 12; i + 8 <= BK; i += 8)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) top[x] = fmaxf(top[x], v[i + x]);
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          for (int x = 0; x < 4; ++x) top[x] = max3(top[x], v[i + x], v[i + 4 + x]);
+        top[0] = max3(top[0], v[BK - 4], v[BK - 3]);
+        top[1] = max3(top[1], v[BK - 2], v[BK - 1]);
+        float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+        if (mx == INFINITY) mx = NAN;  // as the definition has it: infinity less infinity
         if (!begun) m = mx;
         else {
           // the scores of block j are there: the products of every block before have ended, and the output rests
-          const bool grow = (mx - m) * sc > C::GROW;
+          const bool grow = !(mx <= m + growth);
           if (__any_sync(L3_FULL, grow)) {
             const float alpha = grow ? ex2((m - mx) * sc) : 1.f;
             if (grow) { m = mx; l *= alpha; }
@@ -432,95 +559,131 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
         }
         begun = true;
         const float down = C::BIAS - (m == -INFINITY ? 0.f : m * sc);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 sc2 = make_float2(sc, sc), down2 = make_float2(down, down);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t p[32];
 #pragma unroll
           for (int i = 0; i < 64; i += 2) {
-            const float x = ex2(fmaf(v[64 * h + i], sc, down)), y = ex2(fmaf(v[64 * h + i + 1], sc, down));
-            sum[i & 2] += x;
-            sum[(i & 2) + 1] += y;
-            p[i / 2] = pack<T>(x, y);
+            const float2 x = fma2(make_float2(v[64 * h + i], v[64 * h + i + 1]), sc2, down2);
+            const float2 e = i % 8 < 2 * POLY ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum[i / 2 & 1] = add2(sum[i / 2 & 1], e);
+            p[i / 2] = pack<T>(e.x, e.y);
           }
           tmem_st32(tS + 32 * h, p);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive((h ? B.p_full : B.half_p) + 8 * w);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(B.p_full + 8 * w);
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
       }
       blocks_so_far += n;
+      if (m == -INFINITY) l = 0.f;  // nothing seen
       // ---- the result, or this CTA's part of it
       const bool whole = c.whole();
-      float* const part_o = whole ? nullptr : a.part_o + (size_t)(2 * blockIdx.x + c.slot()) * TR * HD;
-      float2* const part_ml = whole ? nullptr : a.part_ml + (size_t)(2 * blockIdx.x + c.slot()) * TR;
+      float* const part_o = whole ? nullptr : a.part_o + (size_t)(2 * blockIdx.x + c.slot()) * a.tile_rows * HD;
+      float2* const part_ml = whole ? nullptr : a.part_ml + (size_t)(2 * blockIdx.x + c.slot()) * a.tile_rows;
       if (!whole && threadIdx.x == 0) left_of(a, blockIdx.x).part[c.slot()] = make_int4(c.b, c.tile, c.g, c.j1 == c.nb);
       float m2 = m == -INFINITY ? m : m * sc - C::BIAS;  // in units of log 2
       float share = 1.f, share1 = 0.f;                    // of the outputs: this tile's, or the first's and the second's
       if (n) {
         mbar_wait(B.o_full + 8 * w, o_phase, fail);
-        if constexpr (!TWO) {
+        if (!two) {
           mbar_wait(B.o_full + 8 * (w ^ 1), o_phase, fail);
-          xch[w * 128 + r] = make_float2(m2, l);
+          float2* const mine = reinterpret_cast<float2*>(stages + warp * C::STAGE);
+          const float2* const others = reinterpret_cast<const float2*>(stages + (warp ^ 4) * C::STAGE);
+          mine[lane] = make_float2(m2, l);
           asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");
-          const float2 other = xch[(w ^ 1) * 128 + r];
+          const float2 other = others[lane];
+          asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");
           const float both = fmaxf(m2, other.x), from = both == -INFINITY ? 0.f : both;
-          const float mine = ex2(m2 - from), its = ex2(other.x - from);
-          l = l * mine + other.y * its;
+          const float mf = ex2(m2 - from), of = ex2(other.x - from);
+          l = l * mf + other.y * of;
           m2 = both;
-          share = w ? its : mine;
-          share1 = w ? mine : its;
+          share = w ? of : mf;
+          share1 = w ? mf : of;
         }
         o_phase ^= 1;
         tc_fence_after();
       }
-      constexpr int D0 = TWO ? HD : HD / 2, STEP = D0 % 16 ? 8 : 16;  // columns of this thread
-      const int first = TWO ? 0 : w * D0;
+      const int D0 = two ? HD : HD / 2, first = two ? 0 : w * D0;  // columns of this thread
       const long long at = (long long)(c.r.s0 + t) * a.H + c.g * a.R + f - t * a.R;
       const float inv = *fail ? NAN : l == 0.f ? 0.f : 1.f / l;
       bool finite = l < INFINITY;
+      // 32 rows of up to 128 bytes at a time by way of shared memory, so that a store covers whole rows and not 16 bytes of 32 of them
+      auto out = [&](auto as_result, auto of_two) {
+        constexpr bool RESULT = decltype(as_result)::value, TWO = decltype(of_two)::value;
+        constexpr int UNITS = RESULT && TWO ? 8 : 4, PER = RESULT ? 1 : 2, CH = UNITS * PER;  // units of 8 columns, their 16-byte pieces, of a row
+        constexpr int D0 = TWO ? HD : HD / 2;
+        uint8_t* const stage = stages + warp * C::STAGE;
 #pragma unroll 1
-      for (int d = first; d < first + D0; d += STEP) {
-        float o[STEP];
-        if (n) {
-          if constexpr (STEP == 16) tmem_ld16(tO + (TWO ? w * 128 : 0) + d, o);
-          else tmem_ld8(tO + d, o);
-          if constexpr (!TWO) {
-            float o1[STEP];
-            if constexpr (STEP == 16) tmem_ld16(tO + 128 + d, o1);
-            else tmem_ld8(tO + 128 + d, o1);
+        for (int u0 = 0; u0 < D0 / 8; u0 += UNITS) {
+          float o[UNITS * 8];
+          [[maybe_unused]] float o1[TWO ? 1 : UNITS * 8];
+          if (n) {
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+              if (u0 + u < D0 / 8) {
+                tmem_ld8(tO + (TWO ? w * 128 : 0) + first + (u0 + u) * 8, o + u * 8);
+                if constexpr (!TWO) tmem_ld8(tO + 128 + first + (u0 + u) * 8, o1 + u * 8);
+              }
             tmem_ld_wait();
+            if constexpr (!TWO) {
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) o[i] = n > 1 ? o[i] * share + o1[i] * share1 : o[i] * share;
-          } else tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < STEP; ++i) o[i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < STEP; ++i) finite = finite && fabsf(o[i]) < INFINITY;
-        if (f < flats) {
-          if (whole) {
-            uint32_t x[STEP / 2];
-#pragma unroll
-            for (int i = 0; i < STEP; i += 2) x[i / 2] = pack<T>(o[i] * inv, o[i + 1] * inv);
-#pragma unroll
-            for (int i = 0; i < STEP / 2; i += 4) *reinterpret_cast<uint4*>((T*)a.out + at * HD + d + 2 * i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+              for (int i = 0; i < UNITS * 8; ++i) o[i] = n > 1 ? o[i] * share + o1[i] * share1 : o[i] * share;
+            }
           } else {
 #pragma unroll
-            for (int i = 0; i < STEP; i += 4) *reinterpret_cast<float4*>(part_o + (size_t)in_tile * HD + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < UNITS * 8; ++i) o[i] = 0.f;
           }
+#pragma unroll
+          for (int u = 0; u < UNITS; ++u)
+            if (u0 + u < D0 / 8) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) finite = finite && fabsf(o[u * 8 + i]) < INFINITY;
+              if constexpr (RESULT) {
+                uint32_t x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = pack<T>(o[u * 8 + 2 * i] * inv, o[u * 8 + 2 * i + 1] * inv);
+                *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                  *reinterpret_cast<float4*>(stage + lane * 128 + (((2 * u + i) ^ (lane & 7)) << 4)) =
+                      make_float4(o[u * 8 + 4 * i], o[u * 8 + 4 * i + 1], o[u * 8 + 4 * i + 2], o[u * 8 + 4 * i + 3]);
+              }
+            }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < CH; ++i) {
+            const int row = i * (32 / CH) + lane / CH, ch = lane % CH, d = first + u0 * 8 + ch * (8 / PER);
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + row * 128 + ((ch ^ (row & 7)) << 4));
+            const long long to = __shfl_sync(L3_FULL, at, row);
+            if (f - lane + row < flats && u0 + ch / PER < D0 / 8) {
+              if constexpr (RESULT) *reinterpret_cast<uint4*>((T*)a.out + to * HD + d) = x;
+              else *reinterpret_cast<uint4*>(part_o + (size_t)(in_tile - lane + row) * HD + d) = x;
+            }
+          }
+          __syncwarp();
         }
+      };
+      if (two) {
+        if (whole) out(std::true_type{}, std::true_type{});
+        else out(std::false_type{}, std::true_type{});
+      } else {
+        if (whole) out(std::true_type{}, std::false_type{});
+        else out(std::false_type{}, std::false_type{});
       }
-      if (f < flats && (TWO || w == 0)) {
+      if (f < flats && (two || w == 0)) {
         if (!whole) part_ml[in_tile] = make_float2(*fail ? NAN : m2, l);
         else if (a.lse) a.lse[at] = (m2 + log2f(l)) * 0.6931471805599453f;
       }
       tc_fence_before();
       if (whole && f < flats && !finite) left_of(a, blockIdx.x).odd = 1;
-      if constexpr (!TWO) asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");  // both have read the outputs, and the other's maximum
+      if (!two) asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");  // both have read the outputs
     } while (c.next(a));
   }
   tc_fence_before();
@@ -529,21 +692,40 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a) {
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(T_COLS));
 }
 
-template <typename T, int HD, bool TWO> cudaError_t launch_one(ChunkArgs a, int n_sm, cudaStream_t s) {
-  using C = Cfg<T, HD, TWO>;
-  a.n_cta = n_sm;
-  a.part_o = (float*)a.ws;
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * C::TR * HD);
-  a.left = a.part_ml + (size_t)a.n_cta * 2 * C::TR;
-  cudaError_t e = allow_smem(chunk_tc_kernel<T, HD, TWO>, C::SMEM);
-  if (e != cudaSuccess) return e;
-  if ((e = launch_k(chunk_tc_kernel<T, HD, TWO>, dim3(a.n_cta), dim3(NT), (size_t)C::SMEM, s, a)) != cudaSuccess) return e;
-  return launch_chunk_join_tc(a, C::TR, s);
+// Rows of an item, 128 or 256: 256 where that makes items enough for all SMs, or a request has many rows and may have many keys.
+int rows_of_item(const ChunkArgs& a, int n_sm) {
+  const long long rows = (long long)a.T * a.R, tiles = (rows + 255) / 256 * a.G, keys = (long long)a.max_pages << a.log_page;
+  return tiles >= n_sm || (rows >= 256LL * a.B && tiles * keys >= (long long)n_sm * 2048) ? 256 : 128;
 }
-// Two tiles of rows where there are enough of them for all SMs, or a request has many rows and may have many keys.
-template <typename T, int HD> cudaError_t launch_hd(const ChunkArgs& a, int n_sm, cudaStream_t s) {
-  if (paged_chunk_tc_rows(a.T, a.H, a.G, a.B, a.max_pages << a.log_page, n_sm) == 256) return launch_one<T, HD, true>(a, n_sm, s);
-  return launch_one<T, HD, false>(a, n_sm, s);
+// Whether, and how, tiles are copied by TMA: a box is 64 entries of as many rows as lie side by side.  Distances of 0 between different rows are not for it.
+bool usable(long long stride, long long n) { return n <= 1 || (stride > 0 && stride < (1LL << 38)); }
+bool map_pool(const ChunkArgs& a, const PagedPool& p, CUtensorMap* map) {
+  if (a.log_page < 3 || !usable(p.sp, a.n_pages) || !usable(p.sh, a.G) || !usable(p.st, 2)) return false;
+  const uint64_t dims[4] = {(uint64_t)a.HD, 1ull << a.log_page, (uint64_t)a.G, (uint64_t)a.n_pages};
+  const uint64_t strides[3] = {(uint64_t)p.st * 2, (uint64_t)std::max(p.sh, 8LL) * 2, (uint64_t)std::max(p.sp, 8LL) * 2};
+  const uint32_t box[4] = {64, (uint32_t)std::min(1 << a.log_page, BK), 1, 1};
+  return tc_make_map(map, p.p, a.dtype == L3_DTYPE_BF16, 4, dims, strides, box);
+}
+bool map_q(const ChunkArgs& a, CUtensorMap* map) {
+  if (128 % a.R || !usable(a.q_sh, a.H) || !usable(a.q_st, a.T)) return false;
+  const uint64_t dims[3] = {(uint64_t)a.HD, (uint64_t)a.H, (uint64_t)a.T};
+  const uint64_t strides[2] = {(uint64_t)std::max(a.q_sh, 8LL) * 2, (uint64_t)std::max(a.q_st, 8LL) * 2};
+  const uint32_t box[3] = {64, (uint32_t)a.R, (uint32_t)(128 / a.R)};
+  return tc_make_map(map, a.q, a.dtype == L3_DTYPE_BF16, 3, dims, strides, box);
+}
+template <typename T, int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
+  using C = Cfg<T, HD>;
+  a.n_cta = n_sm;
+  a.tile_rows = rows_of_item(a, n_sm);
+  a.part_o = (float*)a.ws;
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * a.tile_rows * HD);
+  a.left = a.part_ml + (size_t)a.n_cta * 2 * a.tile_rows;
+  cudaError_t e = allow_smem(chunk_tc_kernel<T, HD>, C::SMEM);
+  if (e != cudaSuccess) return e;
+  Maps maps{};
+  const bool tma_q = map_q(a, &maps.q), tma_kv = map_pool(a, a.k, &maps.k) && map_pool(a, a.v, &maps.v);
+  if ((e = launch_k(chunk_tc_kernel<T, HD>, dim3(a.n_cta), dim3(NT), (size_t)C::SMEM, s, a, maps, tma_q, tma_kv)) != cudaSuccess) return e;
+  return launch_chunk_join_tc(a, s);
 }
 template <typename T> cudaError_t launch_t(const ChunkArgs& a, int n_sm, cudaStream_t s) {
   switch (a.HD) {
@@ -558,10 +740,6 @@ template <typename T> cudaError_t launch_t(const ChunkArgs& a, int n_sm, cudaStr
 }
 }  // namespace
 
-int paged_chunk_tc_rows(int T, int H, int G, int B, long long keys, int n_sm) {
-  const long long rows = (long long)T * (H / G), tiles = (rows + 255) / 256 * G;  // about
-  return tiles >= n_sm || (rows >= 256LL * B && tiles * keys >= (long long)n_sm * 2048) ? 256 : 128;
-}
 cudaError_t launch_paged_chunk_tc(const ChunkArgs& a, int n_sm, cudaStream_t s) {
   return a.dtype == L3_DTYPE_BF16 ? launch_t<bf16>(a, n_sm, s) : launch_t<__half>(a, n_sm, s);
 }

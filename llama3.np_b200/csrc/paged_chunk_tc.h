@@ -2,7 +2,6 @@
 #pragma once
 #include "packed.h"
 
-int paged_chunk_tc_rows(int T, int H, int G, int B, long long keys, int n_sm);  // of an item: 128 or 256
 cudaError_t launch_paged_chunk_tc(const ChunkArgs& a, int n_sm, cudaStream_t s);
 constexpr int TC_BK = 128, TC_WHOLE = 4;                                             // keys of a block; items of so few blocks are not cut
-cudaError_t launch_chunk_join_tc(const ChunkArgs& a, int rows, cudaStream_t s);  // paged_chunk.cu; rows: of an item
+cudaError_t launch_chunk_join_tc(const ChunkArgs& a, cudaStream_t s);   // paged_chunk.cu
