@@ -15,7 +15,7 @@
 namespace {
 using namespace chunk;
 constexpr int TR = 64, BK = 64, NT = 256;
-constexpr int WHOLE = 4, LEAST = 4;
+__host__ __device__ constexpr Split fma_split() { return Split{BK, 4, 8, TR}; }
 template <int HD> constexpr int row_ld() { return HD + 4; }
 template <int HD> constexpr size_t smem_bytes() { return (size_t)(2 * 64 * row_ld<HD>() + 64 * HD + 64 * (TR + 4)) * 4 + 2 * 2 * BK * 8 + 2 * 8 + 16; }
 
@@ -29,6 +29,7 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 template <int HD>
 __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const ChunkArgs a) {
   using T = float;
+  constexpr Split SPLIT = fma_split();
   constexpr int LD = row_ld<HD>(), PL = TR + 4;
   constexpr int CW = HD % 64 == 0 ? 4 : HD % 32 == 0 ? 2 : 1, NC = HD / (16 * CW);  // columns side by side, and how often
   extern __shared__ __align__(16) float sm[];
@@ -43,13 +44,13 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
   pdl_launch();
   pdl_wait();
   clear_rest<T>(a);
-  find_share<BK, NT, LEAST>(a, room, &place);
+  find_share<BK, NT>(a, SPLIT, room, &place);
   if (threadIdx.x == 0) leave_nothing(a, place);
   __syncthreads();
   const int lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float sc = a.scale * 1.4426950408889634f;
-  Cursor<BK, WHOLE> c;
-  if (!c.start(a, place)) return;
+  Cursor<BK> c;
+  if (!c.start(a, SPLIT, place)) return;
   do {
     const int* table = a.table + c.b * a.table_stride;
     const int flat0 = c.tile * TR, flats = c.r.n * a.R;
@@ -229,15 +230,15 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
       }
     }
     __syncthreads();
-  } while (c.next(a));
+  } while (c.next(a, SPLIT));
 }
 
 // ---------------------------------------------------------------------------------------------------------------- the join
 // Block (c, y) joins 16 rows of the item that CTA c began and others ended, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, and looks after
 // the rows of all its items that are not finite.
 constexpr int JROWS = 16, JT = 256;
-template <typename T, int HD, int BK, int WHOLE>
-__global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
+template <typename T, int HD, int BK>
+__global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a, const Split sp) {
   pdl_launch();
   pdl_wait();
   constexpr int N = (HD + 31) / 32;
@@ -258,20 +259,37 @@ __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
       l = a.part_ml[p0].y;
 #pragma unroll
       for (int x = 0; x < N; ++x) o[x] = lane + 32 * x < HD ? a.part_o[p0 * HD + lane + 32 * x] : 0.f;
-      bool ends = false;
-      for (int c = c0 + 1; c < a.n_cta && !ends; ++c) {
-        const int4 more = left_of(a, c).part[0];
-        if (more.x < 0) continue;
-        ends = more.w;
-        const size_t p = (size_t)(2 * c) * TR + in_tile;
-        const float2 ml = a.part_ml[p];
-        const float mn = fmaxf(m, ml.x), from = mn == -INFINITY ? 0.f : mn;
-        const float fa = exp2f(m - from), fb = exp2f(ml.x - from);
-        l = l * fa + ml.y * fb;
+      // the CTAs behind, 32 at a time, a lane each; those that ended nothing and went on with nothing have no part
+      for (int c = c0 + 1;; c += 32) {
+        const int4 its = c + lane < a.n_cta ? left_of(a, c + lane).part[0] : make_int4(-1, 0, 0, 0);
+        const unsigned ends = __ballot_sync(L3_FULL, its.x >= 0 && its.w);
+        const bool part = its.x >= 0 && (!ends || lane < __ffs(ends));
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (part) ml = a.part_ml[(size_t)(2 * (c + lane)) * TR + in_tile];
+        const float mn = fmaxf(m, warp_max(ml.x)), from = mn == -INFINITY ? 0.f : mn;
+        const float f0 = exp2f(m - from), fp = exp2f(ml.x - from);
+        l = l * f0 + warp_sum(ml.y * fp);
         m = mn;
 #pragma unroll
-        for (int x = 0; x < N; ++x)
-          if (lane + 32 * x < HD) o[x] = o[x] * fa + a.part_o[p * HD + lane + 32 * x] * fb;
+        for (int x = 0; x < N; ++x) o[x] *= f0;
+        unsigned list = __ballot_sync(L3_FULL, part);
+        while (list) {
+          float f[4], y[4][N];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // four partials' rows on their way together
+            const int of = list ? __ffs(list) - 1 : -1;
+            list &= list - 1;
+            f[k] = __shfl_sync(L3_FULL, fp, max(of, 0));
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+              y[k][x] = of >= 0 && lane + 32 * x < HD ? a.part_o[((size_t)(2 * (c + of)) * TR + in_tile) * HD + lane + 32 * x] : 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int x = 0; x < N; ++x) o[x] += y[k][x] * f[k];
+        }
+        if (ends || c + 32 >= a.n_cta) break;
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       bool odd = !(l < INFINITY);
@@ -285,8 +303,8 @@ __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
     }
   }
   if (!own.odd) return;
-  Cursor<BK, WHOLE> c;
-  if (c.start(a, own.place)) do {
+  Cursor<BK> c;
+  if (c.start(a, sp, own.place)) do {
     if (!c.whole()) continue;
     for (int i = warp; i < JROWS; i += JT / 32) {
       const int f = c.tile * TR + blockIdx.y * JROWS + i;
@@ -298,20 +316,20 @@ __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a) {
       for (int x = 0; x < N; ++x) odd = odd || (lane + 32 * x < HD && !(fabsf(up(out[lane + 32 * x])) < INFINITY));
       if (__any_sync(L3_FULL, odd)) by_formula<T, HD>(a, c.b, c.g, c.r.s0 + t, head, c.r.seen(t));
     }
-  } while (c.next(a));
+  } while (c.next(a, sp));
 }
 
 size_t partials(int n_cta, int rows, int HD) { return (size_t)n_cta * (2 * rows * ((size_t)HD * 4 + 8) + sizeof(Left)); }
-template <typename T, int BK, int WHOLE> cudaError_t join_t(const ChunkArgs& a, cudaStream_t s) {
+template <typename T, int BK> cudaError_t join_t(const ChunkArgs& a, const Split& sp, cudaStream_t s) {
   const dim3 grid(a.n_cta, a.tile_rows / JROWS), block(JT);
   g_l3_pdl_next = true;
   switch (a.HD) {
-    case 16: return launch_k(chunk_join_kernel<T, 16, BK, WHOLE>, grid, block, 0, s, a);
-    case 32: return launch_k(chunk_join_kernel<T, 32, BK, WHOLE>, grid, block, 0, s, a);
-    case 48: return launch_k(chunk_join_kernel<T, 48, BK, WHOLE>, grid, block, 0, s, a);
-    case 64: return launch_k(chunk_join_kernel<T, 64, BK, WHOLE>, grid, block, 0, s, a);
-    case 96: return launch_k(chunk_join_kernel<T, 96, BK, WHOLE>, grid, block, 0, s, a);
-    default: return launch_k(chunk_join_kernel<T, 128, BK, WHOLE>, grid, block, 0, s, a);
+    case 16: return launch_k(chunk_join_kernel<T, 16, BK>, grid, block, 0, s, a, sp);
+    case 32: return launch_k(chunk_join_kernel<T, 32, BK>, grid, block, 0, s, a, sp);
+    case 48: return launch_k(chunk_join_kernel<T, 48, BK>, grid, block, 0, s, a, sp);
+    case 64: return launch_k(chunk_join_kernel<T, 64, BK>, grid, block, 0, s, a, sp);
+    case 96: return launch_k(chunk_join_kernel<T, 96, BK>, grid, block, 0, s, a, sp);
+    default: return launch_k(chunk_join_kernel<T, 128, BK>, grid, block, 0, s, a, sp);
   }
 }
 template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
@@ -324,12 +342,12 @@ template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
   cudaError_t e = allow_smem(chunk_fma_kernel<HD>, smem);
   if (e != cudaSuccess) return e;
   if ((e = launch_k(chunk_fma_kernel<HD>, dim3(a.n_cta), dim3(NT), smem, s, a)) != cudaSuccess) return e;
-  return join_t<float, BK, WHOLE>(a, s);
+  return join_t<float, BK>(a, fma_split(), s);
 }
 }  // namespace
 
 cudaError_t launch_chunk_join_tc(const ChunkArgs& a, cudaStream_t s) {
-  return a.dtype == L3_DTYPE_BF16 ? join_t<bf16, TC_BK, TC_WHOLE>(a, s) : join_t<__half, TC_BK, TC_WHOLE>(a, s);
+  return a.dtype == L3_DTYPE_BF16 ? join_t<bf16, TC_BK>(a, tc_split(a.HD), s) : join_t<__half, TC_BK>(a, tc_split(a.HD), s);
 }
 
 // the larger of either number of rows

@@ -13,6 +13,7 @@
 
 #include "../../include/llama3_b200.h"
 #include "packed.h"
+#include "paged_chunk_tc.h"
 
 namespace chunk {
 template <typename T> __device__ __forceinline__ float up(T x) { return to_f32(x); }
@@ -39,22 +40,28 @@ template <int BK> __device__ __forceinline__ int blocks(const ChunkArgs& a, cons
   const int last = min(r.n * a.R, (tile + 1) * a.tile_rows) - 1;
   return (int)((unsigned)(r.seen(last / a.R) + BK - 1) / BK);
 }
-// An item's weight: two a block, and what begins and ends it like half a block.
-__device__ __forceinline__ int weight(int nb) { return 2 * nb + 1; }
-// The blocks of an item of nb that lie ahead of weight x.  Whole: items of so few blocks are not cut.
-template <int WHOLE> __device__ __forceinline__ int ahead(long long x, int nb) {
-  const int w = weight(nb);
+// An item's weight: `per` a block - 2, or 4 of a tile that takes a block's time twice as long (Split) - and 2 for what begins and ends it.
+struct Split { int block, whole, least, rows_of_half; };  // keys of a block; items of so few blocks are not cut; least weight of a share; rows that a block costs half for
+// paged_chunk_tc.cu: one tile of rows has two blocks at a time, which takes half the time as long as the tiles' copies keep up.  us, half : three quarters :
+// all of a block's weight: heads of 64, 48 requests of up to 3001 tokens 125 : 131 : 141; of 128, six prompts of up to 4096 tokens 666 : 600 : 575
+__host__ __device__ constexpr Split tc_split(int HD) { return Split{TC_BK, 4, 4, HD <= 64 ? 128 : 0}; }
+__device__ __forceinline__ int per_block(const ChunkArgs& a, const Split& sp, const Request& r, int tile) {
+  return min(r.n * a.R - tile * a.tile_rows, a.tile_rows) > sp.rows_of_half ? 4 : 2;
+}
+// The blocks of an item of nb that lie ahead of weight x.
+__device__ __forceinline__ int ahead(long long x, int nb, int per, int whole) {
+  const int w = per * nb + 2;
   if (x <= 0) return 0;
   if (x >= w) return nb;
-  if (nb <= WHOLE) return 2 * x >= w ? nb : 0;
-  return (int)x / 2;
+  if (nb <= whole) return 2 * x >= w ? nb : 0;
+  return min((int)x / per, nb);
 }
 
 struct Place { int b, tile, g, pad; long long off, rest; };  // an item, the weight of it that others have, and what this CTA has from there on
 
-// This CTA's share, by all NT threads (`room`: NT / 32 + 1 words of shared memory).  LEAST: the least weight of a share.
-template <int BK, int NT, int LEAST>
-__device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, Place* place) {
+// This CTA's share, by all NT threads (`room`: NT / 32 + 1 words of shared memory).
+template <int BK, int NT>
+__device__ __forceinline__ void find_share(const ChunkArgs& a, const Split& sp, long long* room, Place* place) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // a thread takes `each` requests, or one of `parts` parts of a request's tiles
   const int parts = max(NT / max(a.B, 1), 1), each = (a.B + NT - 1) / NT;
@@ -65,7 +72,7 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, 
       const int nt = tiles(a, r.n), part = parts > 1 ? threadIdx.x % parts : 0;
       const int t0 = (int)((long long)nt * part / parts), t1 = (int)((long long)nt * (part + 1) / parts);
       for (int t = t0; t < t1; ++t)
-        if (f(b, t, weight(blocks<BK>(a, r, t)))) return;
+        if (f(b, t, per_block(a, sp, r, t) * blocks<BK>(a, r, t) + 2)) return;
     }
   };
   long long sum = 0;
@@ -88,7 +95,7 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, 
     if (w < warp) before += room[w];
     all += room[w];
   }
-  const long long ctas = min((long long)a.n_cta, max(all / LEAST, 1LL));
+  const long long ctas = min((long long)a.n_cta, max(all / sp.least, 1LL));
   if (blockIdx.x < ctas) {
     const long long w0 = all * blockIdx.x / ctas, w1 = all * (blockIdx.x + 1) / ctas;
     if (before <= w0 && w0 < before + sum) {
@@ -109,30 +116,33 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, long long* room, 
 }
 
 // One stretch of blocks after the other.
-template <int BK, int WHOLE> struct Cursor {
-  int b, tile, g, nt, nb;
+template <int BK> struct Cursor {
+  int b, tile, g, nt, nb, per;
   Request r;
   long long off, rest;
   int j0, j1;               // blocks of this stretch
-  __device__ __forceinline__ void at_tile(const ChunkArgs& a) { nb = blocks<BK>(a, r, tile); }
-  __device__ __forceinline__ bool start(const ChunkArgs& a, const Place& p) {
+  __device__ __forceinline__ void at_tile(const ChunkArgs& a, const Split& sp) {
+    nb = blocks<BK>(a, r, tile);
+    per = per_block(a, sp, r, tile);
+  }
+  __device__ __forceinline__ bool start(const ChunkArgs& a, const Split& sp, const Place& p) {
     b = p.b; tile = p.tile; g = p.g; off = p.off; rest = p.rest;
     if (b < 0) return false;
     r = request(a, b);
     nt = tiles(a, r.n);
-    at_tile(a);
-    return settle(a) ? true : next(a);
+    at_tile(a, sp);
+    return settle(sp) ? true : next(a, sp);
   }
   // the stretch of this item, if there is one
-  __device__ __forceinline__ bool settle(const ChunkArgs&) {
+  __device__ __forceinline__ bool settle(const Split& sp) {
     if (rest <= 0) return false;
-    j0 = ahead<WHOLE>(off, nb);
-    j1 = ahead<WHOLE>(off + rest, nb);
+    j0 = ahead(off, nb, per, sp.whole);
+    j1 = ahead(off + rest, nb, per, sp.whole);
     return j1 > j0 || (nb == 0 && off == 0);
   }
-  __device__ __forceinline__ bool next(const ChunkArgs& a) {
+  __device__ __forceinline__ bool next(const ChunkArgs& a, const Split& sp) {
     for (;;) {
-      rest -= weight(nb) - off;
+      rest -= per * nb + 2 - off;
       off = 0;
       if (rest <= 0) return false;
       if (++g == a.G) {
@@ -145,9 +155,9 @@ template <int BK, int WHOLE> struct Cursor {
             nt = tiles(a, r.n);
           } while (nt == 0);
         }
-        at_tile(a);
+        at_tile(a, sp);
       }
-      if (settle(a)) return true;
+      if (settle(sp)) return true;
     }
   }
   __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == nb; }

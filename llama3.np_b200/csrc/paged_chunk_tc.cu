@@ -6,7 +6,8 @@
 //                 expanded strides, and queries whose heads do not fill 128 rows evenly go row by row, 16 bytes a copy (cp.async)
 //   warp 8        products: S = Q K^T into TMEM, O += P V with P from TMEM and V as it lies, an MN-major operand
 //   warps 0 - 7   softmax, a thread a row, four warps a score tile: its 128 scores in registers, exponentials against a maximum that follows
-//                 the running one lazily (O is rescaled in TMEM only when that has grown by 2^GROW), weights as 16-bit values over the scores
+//                 the running one lazily (O is rescaled in TMEM only when that has grown by 2^GROW), weights as 16-bit values, over the
+//                 scores where TMEM has no room beside them
 // The two score tiles take turns: one's softmax runs while the tensor core works on the other's products.  With many rows they are two tiles of
 // rows over the same keys, so that every key and value that arrives is used for 256 rows; with few rows they are one tile of rows over every other
 // block of keys, and meet at the end.
@@ -14,35 +15,35 @@
 // A weight enters the product rounded to the cache's type (half a step: bf16 2^-9 of it, as much as the result's own rounding; sums are of the unrounded
 // ones, in fp32).  fp16 weights are scaled by 2^BIAS ahead of the rounding: the largest lies in [2^12, 2^15], what fp16 has no number for is below
 // 2^-37 of it.
+#include <limits.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 #include <type_traits>
 
 #include "gemm_tc_dev.cuh"
-#include "paged_chunk_tc.h"
 #include "paged_chunk.cuh"
 
 namespace {
 using namespace chunk;
 constexpr int BK = TC_BK, NT = 384, SOFT = 256, LOADERS = 2, SETS = 4 / LOADERS;  // SETS: of 32 rows of a tile, a loader's
-constexpr int WHOLE = TC_WHOLE, LEAST = 4;
 constexpr int POLY = 1;    // of four neighbouring pairs of exponentials, how many are taken by a polynomial
 constexpr int THERE = 16;  // blocks whose keys' bits are kept: more than the ring holds
 
 template <typename T, int HD> struct Cfg {
   static constexpr int QS = (HD + 63) / 64;             // slices of 64 entries, rows of 128 bytes
   static constexpr int TILE = QS * 128 * 128;           // bytes of 128 rows
-  static constexpr int NS = HD > 64 ? 4 : 8;            // tiles of the ring
-  static constexpr int STAGE = 4096;                    // bytes of a softmax warp's results on their way out, 32 rows of 128
-  static constexpr int SMEM = 2 * TILE + NS * TILE + 8 * STAGE + THERE * 16 + 256 + 1024;
+  static constexpr int NS = HD > 64 ? 5 : 8;            // tiles of the ring
+  static constexpr int SMEM = 2 * TILE + NS * TILE + THERE * 16 + 256 + 1024;
+  static constexpr bool BESIDE = HD <= 64;              // the weights have TMEM of their own: a block's scores are multiplied while the last one's are weighed
+  static constexpr int T_O = 256, O_COLS = BESIDE ? 64 : 128, T_P = BESIDE ? 384 : 0, P_COLS = BESIDE ? 64 : 128;
   static constexpr uint32_t FMT = std::is_same<T, bf16>::value ? 1u : 0u;
   static constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(BK >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr uint32_t IDESC_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr float BIAS = FMT ? 0.f : 12.f, GROW = FMT ? 8.f : 3.f;
 };
-// TMEM columns: two score tiles (the weights lie over their first halves), two outputs
-constexpr int T_O = 256, T_COLS = 512;
+constexpr int T_COLS = 512;  // of TMEM: two score tiles, two outputs (and weights)
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {  // zeros where !take
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -58,16 +59,22 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
-// MN-major operand, 128-byte swizzle: rows are the keys (the product's K), 8 of them a 1024-byte atom; atoms of 64 columns are lbo bytes apart
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Operand descriptors, their lower halves (start address and leading offset): the upper half is the same for all - 8-row groups 1024 bytes apart, 128-byte
+// swizzle.  K-major: rows of 128 bytes.  MN-major: rows are the keys (the product's K), atoms of 64 columns are 16384 bytes apart.
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29), DESC_K = 1u << 16, DESC_MN = (16384u >> 4) << 16;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) { return (addr & 0x3FFFF) >> 4 | lead; }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.b32 p, %4, 0;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accum), "r"(DESC_HI) : "memory");
 }
 // A from TMEM: a lane a row, two neighbouring entries a column
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accum) : "memory");
+      "{\n.reg .pred p;\n.reg .b64 y;\nsetp.ne.b32 p, %4, 0;\nmov.b64 y, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accum), "r"(DESC_HI) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t at, float* v) {  // without the wait
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -123,17 +130,21 @@ template <typename T> __device__ __forceinline__ uint32_t pack(float x, float y)
   }
 }
 
+__device__ __forceinline__ void store32(void* to, const uint32_t* x) {  // to a multiple of 32 bytes
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-               ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap* tm, int c0, int c1, int c2, int c3, int c4, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+               ::"r"(dst), "l"(tm), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar) : "memory");
 }
-__device__ __forceinline__ float max3(float x, float y, float z) {  // NaN if one of them is
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one of them is
   float m;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
   return m;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -156,31 +167,33 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   y = fma2(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
   return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(t.y) << 23)));
 }
-// Maps of the queries (entries, heads, rows) and the pools (entries, tokens, heads, pages), where tiles are copied by them.
+// Maps of the queries (entries, heads, rows) and the pools (entries, tokens, heads, pages, keys or values), where tiles are copied by them.  To make one
+// takes the host 2 us: both pools are one, the distance between them a stride.
 struct Maps {
-  CUtensorMap q, k, v;
+  CUtensorMap q, kv;
 };
 
 // Barriers of a CTA, 8 bytes each.
 struct Bars {
-  uint32_t q_full, q_empty, landed, s_full, half_p, p_full, o_full, full, empty;  // s_full .. o_full: of both score tiles
+  uint32_t q_full, q_empty, landed, s_full, s_read, half_p, p_full, p_read, o_full, full, empty;  // s_full .. o_full: of both score tiles
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ Maps maps, const bool tma_q, const bool tma_kv) {
+__global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, const __grid_constant__ Maps maps, const bool tma_q, const bool tma_kv, const bool keys_first) {
   using C = Cfg<T, HD>;
   constexpr int NS = C::NS, TILE = C::TILE;
-  using Cur = Cursor<BK, WHOLE>;
+  using Cur = Cursor<BK>;
+  constexpr Split SPLIT = tc_split(HD);
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long room[NT / 32 + 1];
   __shared__ Place place;
   __shared__ int failed;
+  __shared__ float xch[8][32];  // from score tile to score tile
   volatile int* const fail = &failed;
   const uint32_t raw = smem_u32(smem_raw), sQ = (raw + 1023u) & ~1023u, ring = sQ + 2 * TILE;
-  uint8_t* const stages = smem_raw + (ring + NS * TILE - raw);
-  uint32_t* const there = reinterpret_cast<uint32_t*>(stages + 8 * C::STAGE);  // [THERE][4]
-  const uint32_t bars = ring + NS * TILE + 8 * C::STAGE + THERE * 16;
-  const Bars B{bars, bars + 8, bars + 16, bars + 24, bars + 40, bars + 56, bars + 72, bars + 88, bars + 88 + 8 * NS};
+  uint32_t* const there = reinterpret_cast<uint32_t*>(smem_raw + (ring + NS * TILE - raw));  // [THERE][4]
+  const uint32_t bars = ring + NS * TILE + THERE * 16;
+  const Bars B{bars, bars + 8, bars + 16, bars + 24, bars + 40, bars + 56, bars + 72, bars + 88, bars + 104, bars + 120, bars + 120 + 8 * NS};
   const uint32_t tmem_slot = B.empty + 8 * NS;
   uint32_t* const tmem_slot_ptr = reinterpret_cast<uint32_t*>(smem_raw + (tmem_slot - raw));
   const int warp = __shfl_sync(L3_FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -190,7 +203,8 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
     mbar_init(B.q_empty, 1);
     mbar_init(B.landed, 1);
     for (int w = 0; w < 2; ++w) {
-      mbar_init(B.s_full + 8 * w, 1); mbar_init(B.half_p + 8 * w, 4); mbar_init(B.p_full + 8 * w, 4); mbar_init(B.o_full + 8 * w, 1);
+      mbar_init(B.s_full + 8 * w, 1); mbar_init(B.s_read + 8 * w, 4); mbar_init(B.half_p + 8 * w, 4); mbar_init(B.p_full + 8 * w, 4);
+      mbar_init(B.p_read + 8 * w, 1); mbar_init(B.o_full + 8 * w, 1);
     }
     for (int s = 0; s < NS; ++s) { mbar_init(B.full + 8 * s, tma_kv ? 1 : LOADERS); mbar_init(B.empty + 8 * s, 1); }
     failed = 0;
@@ -203,7 +217,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
   pdl_wait();
   clear_rest<T>(a);
   tc_fence_before();
-  find_share<BK, NT, LEAST>(a, room, &place);
+  find_share<BK, NT>(a, SPLIT, room, &place);
   tc_fence_after();
   if (threadIdx.x == 0) leave_nothing(a, place);
   const uint32_t tmem = *tmem_slot_ptr;
@@ -216,7 +230,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
 
   if (warp == 8) {  // ------------------------------------------------------------------------------------------- products
     int slot = 0;
-    uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0};
+    uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0}, s_phase[2] = {1, 1};
     auto arrived = [&]() {  // the ring's next tile
       mbar_wait(B.full + 8 * slot, phase, fail);
       tc_fence_after();
@@ -225,19 +239,24 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       return s;
     };
     auto scores = [&](int w, int q_tile, int s) {
-      const uint32_t q = sQ + q_tile * TILE, k = ring + s * TILE;
+      const uint32_t q = desc_lo(sQ + q_tile * TILE, DESC_K), k = desc_lo(ring + s * TILE, DESC_K);
+      if constexpr (C::BESIDE) {  // else that the weights are there says so
+        mbar_wait(B.s_read + 8 * w, s_phase[w], fail);
+        s_phase[w] ^= 1;
+        tc_fence_after();
+      }
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint64_t step = (uint64_t)((kk & 3) * 2);
-          tc_mma<TC_BF16>(tmem + w * BK, umma_desc_sw128(q + (kk >> 2) * 16384) + step, umma_desc_sw128(k + (kk >> 2) * 16384) + step, C::IDESC_S, kk > 0);
+        for (int kk = 0; kk < HD / 16; ++kk) {  // 32 bytes of a row, 16384 from slice to slice
+          const uint32_t step = (kk >> 2) * 1024 + (kk & 3) * 2;
+          mma_ss(tmem + w * BK, q + step, k + step, C::IDESC_S, kk > 0);
         }
         tc_commit(B.s_full + 8 * w);
       }
       __syncwarp();
     };
     auto weighted = [&](int w, int s, bool first) {  // a half of the keys as soon as their weights are there
-      const uint32_t v = ring + s * TILE;
+      const uint32_t v = desc_lo(ring + s * TILE, DESC_MN);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         mbar_wait((h ? B.p_full : B.half_p) + 8 * w, p_phase[w], fail);
@@ -245,7 +264,8 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         if (elect_one()) {
 #pragma unroll
           for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-            mma_ts(tmem + T_O + w * 128, tmem + w * BK + kk * 8, desc_mn(v + kk * 2048, 16384), C::IDESC_PV, !first || kk > 0);
+            mma_ts(tmem + C::T_O + w * C::O_COLS, tmem + C::T_P + w * C::P_COLS + kk * 8, v + kk * 128, C::IDESC_PV, !first || kk > 0);
+          if (C::BESIDE && h) tc_commit(B.p_read + 8 * w);
         }
         __syncwarp();
       }
@@ -255,7 +275,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       if (elect_one()) tc_commit(bar);
       __syncwarp();
     };
-    if (c.start(a, place)) do {
+    if (c.start(a, SPLIT, place)) do {
       const int n = c.j1 - c.j0;
       if (n == 0) continue;
       mbar_wait(B.q_full, q_phase, fail);
@@ -269,16 +289,33 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         if (n == 1) commit(B.q_empty);
         for (int j = 0; j < n; ++j) {
           const bool more = j + 1 < n;
-          const int v = arrived();
-          k = more ? arrived() : 0;
+          if constexpr (C::BESIDE) {
+            if (more) {
+              k = arrived();
+              scores(0, 0, k);
+              scores(1, 1, k);
+              commit(B.empty + 8 * k);
+            }
+            const int v = arrived();
+            weighted(0, v, j == 0);
+            weighted(1, v, j == 0);
+            commit(B.empty + 8 * v);
+            if (!more) {
+              commit(B.o_full);
+              commit(B.o_full + 8);
+            }
+          } else {
+            const int v = arrived();
+            k = more ? arrived() : 0;
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            weighted(w, v, j == 0);
-            if (more) scores(w, w, k);
-            else commit(B.o_full + 8 * w);
+            for (int w = 0; w < 2; ++w) {
+              weighted(w, v, j == 0);
+              if (more) scores(w, w, k);
+              else commit(B.o_full + 8 * w);
+            }
+            commit(B.empty + 8 * v);
+            if (more) commit(B.empty + 8 * k);
           }
-          commit(B.empty + 8 * v);
-          if (more) commit(B.empty + 8 * k);
           if (j + 2 == n) commit(B.q_empty);
         }
       } else {
@@ -288,20 +325,24 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           commit(B.empty + 8 * k);
         }
         if (n <= 2) commit(B.q_empty);
-        if (n == 1) commit(B.o_full + 8);  // it has no block
         for (int i = 0; i < n; ++i) {
-          const int w = i & 1, v = arrived();
-          weighted(w, v, i < 2);
-          commit(B.empty + 8 * v);
-          if (i + 2 < n) {
+          const int w = i & 1;
+          auto more = [&]() {
+            if (i + 2 >= n) return;
             const int k = arrived();
             scores(w, 0, k);
             commit(B.empty + 8 * k);
             if (i + 3 == n) commit(B.q_empty);
-          } else commit(B.o_full + 8 * w);
+          };
+          if constexpr (C::BESIDE) more();
+          const int v = arrived();
+          weighted(w, v, i < 2);
+          commit(B.empty + 8 * v);
+          if constexpr (!C::BESIDE) more();
+          if (i + 2 >= n) commit(B.o_full + 8 * w);
         }
       }
-    } while (c.next(a));
+    } while (c.next(a, SPLIT));
   } else if (warp >= 10) {  // ------------------------------------------------------------------------------------- loaders
     constexpr int PIECES = HD / 8;
     const int row0 = (warp - 10) * 32 * SETS;
@@ -333,7 +374,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       }
     };
     auto free_to_fill = [&](uint32_t bar, uint32_t parity) {
-      if (mbar_test(bar, parity)) return;
+      if (__all_sync(L3_FULL, mbar_test(bar, parity))) return;
       told();
       mbar_wait(bar, parity, fail);
     };
@@ -347,14 +388,14 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       }
     };
     struct Pages { int of[SETS]; };
-    if (c.start(a, place)) do {
+    if (c.start(a, SPLIT, place)) do {
       const int n = c.j1 - c.j0;
       if (n == 0) continue;
       const int flat0 = c.tile * a.tile_rows, flats = c.r.n * a.R;
       const int most = c.r.seen((min(flats, flat0 + a.tile_rows) - 1) / a.R);
       const int* table = a.table + c.b * a.table_stride;
       const bool two = two_tiles();
-      const int ahead = two ? 1 : 2;  // blocks of keys that are multiplied ahead of the first one's values
+      const int ahead = (two ? 1 : 2) + (C::BESIDE ? 1 : 0);  // blocks of keys that are multiplied ahead of the first one's values
       if (tma_q) {
         if (first_loader) {
           free_to_fill(B.q_empty, q_phase);
@@ -389,7 +430,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           if (lane < pages && key < most) page = __ldg(table + (key >> a.log_page));
           return (unsigned)page < (unsigned)a.n_pages ? page : a.n_pages;  // outside: the copy's rows are zeros
         };
-        auto fill = [&](const CUtensorMap* map, int page, int j, bool keys) {
+        auto fill = [&](int page, int j, bool keys) {
           const uint32_t bar = B.full + 8 * slot, tile = ring + slot * TILE;
           mbar_wait(B.empty + 8 * slot, phase, fail);
           if (keys) {
@@ -407,12 +448,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           const int left = most - j * BK, stop = min((left + box - 1) & -box, BK);
           const bool clean = !keys && left < BK && left < stop;
           const uint32_t to = clean ? B.landed : bar;
+          __syncwarp();  // the bits of all four lanes, ahead of the arrival
           if (lane == 0) mbar_expect_tx(to, TILE);
           __syncwarp();
           if (lane < pages) {
 #pragma unroll
             for (int x = 0; x < C::QS; ++x)
-              tma_4d(tile + x * 16384 + lane * box * 128, map, x * 64, (j * BK) & (page_size - 1) & -box, c.g, page, to);
+              tma_5d(tile + x * 16384 + lane * box * 128, &maps.kv, x * 64, (j * BK) & (page_size - 1) & -box, c.g, page, keys != keys_first, to);
           }
           __syncwarp();
           if (clean) {
@@ -426,21 +468,22 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           }
           if (++slot == NS) { slot = 0; phase ^= 1; }
         };
-        int next = page_of(c.j0), had = next, had1 = next;  // had, had1: of the blocks whose values come next
+        int next = page_of(c.j0), had = next, had1 = next, had2 = next;  // had ..: of the blocks whose values come next
         for (int x = 0; x < min(ahead, n); ++x) {
-          (x ? had1 : had) = next;
+          (x == 0 ? had : x == 1 ? had1 : had2) = next;
           const int page = next;
           next = page_of(c.j0 + x + 1);
-          fill(&maps.k, page, c.j0 + x, true);
+          fill(page, c.j0 + x, true);
         }
         for (int i = 0; i < n; ++i) {
-          fill(&maps.v, had, c.j0 + i, false);
+          fill(had, c.j0 + i, false);
           had = had1;
+          had1 = had2;
           if (i + ahead < n) {
-            (two ? had : had1) = next;
+            (ahead == 1 ? had : ahead == 2 ? had1 : had2) = next;
             const int page = next;
             next = page_of(c.j0 + i + ahead + 1);
-            fill(&maps.k, page, c.j0 + i + ahead, true);
+            fill(page, c.j0 + i + ahead, true);
           }
         }
         continue;
@@ -470,9 +513,9 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         filled(B.full + 8 * slot);
         if (++slot == NS) { slot = 0; phase ^= 1; }
       };
-      Pages next = pages_of(c.j0), had = next, had1 = next;
+      Pages next = pages_of(c.j0), had = next, had1 = next, had2 = next;
       for (int x = 0; x < min(ahead, n); ++x) {
-        (x ? had1 : had) = next;
+        (x == 0 ? had : x == 1 ? had1 : had2) = next;
         const Pages page = next;
         next = pages_of(c.j0 + x + 1);
         fill(a.k, page, c.j0 + x, true);
@@ -480,38 +523,59 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       for (int i = 0; i < n; ++i) {
         fill(a.v, had, c.j0 + i, false);
         had = had1;
+        had1 = had2;
         if (i + ahead < n) {
-          (two ? had : had1) = next;
+          (ahead == 1 ? had : ahead == 2 ? had1 : had2) = next;
           const Pages page = next;
           next = pages_of(c.j0 + i + ahead + 1);
           fill(a.k, page, c.j0 + i + ahead, true);
         }
       }
-    } while (c.next(a));
+    } while (c.next(a, SPLIT));
     told();
   } else if (warp < 8) {  // ---------------------------------------------------------------------------------------- softmax
     const int quarter = warp & 3, w = warp >> 2, r = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + w * BK + lanes, tO = tmem + T_O + lanes;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + w * BK + lanes, tO = tmem + C::T_O + lanes, tP = tmem + C::T_P + w * C::P_COLS + lanes;
     // log2(e) |scale|: a weight is 2^(s sc - m sc); of 0 the smallest number, so that a score of -infinity keeps its weight of 0
     const float sc = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f), growth = fminf(C::GROW / sc, 3e38f);
     const bool negative = a.scale < 0.f;
     int blocks_so_far = 0;
-    uint32_t s_phase = 0, o_phase = 0;
-    if (c.start(a, place)) do {
+    uint32_t s_phase = 0, o_phase[2] = {0, 0}, p_phase = 1;
+    if (c.start(a, SPLIT, place)) do {
       const int n = c.j1 - c.j0;
       const bool two = two_tiles();
       const int in_tile = (two ? w * 128 : 0) + r, f = c.tile * a.tile_rows + in_tile, flats = c.r.n * a.R, t = f / a.R;
-      const int seen = f < flats ? c.r.seen(t) : 0;
+      const int seen = f < flats ? c.r.seen(t) : INT_MAX;  // a row behind the last: whatever it has goes nowhere, and masks cost time
+      const bool idle = f - lane >= flats;                 // none of the warp's rows is one: it only keeps step
       float m = -INFINITY, l = 0.f;  // m: of s, what the exponentials are taken against
       bool begun = false;
       for (int j = two ? 0 : w; j < n; j += two ? 1 : 2) {
         mbar_wait(B.s_full + 8 * w, s_phase, fail);
         s_phase ^= 1;
         tc_fence_after();
+        if (idle) {
+          if constexpr (C::BESIDE) {
+            mbar_wait(B.p_read + 8 * w, p_phase, fail);
+            p_phase ^= 1;
+          }
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (C::BESIDE) mbar_arrive(B.s_read + 8 * w);
+            mbar_arrive(B.half_p + 8 * w);
+            mbar_arrive(B.p_full + 8 * w);
+          }
+          __syncwarp();
+          continue;
+        }
         float v[BK];
 #pragma unroll
         for (int i = 0; i < BK; i += 32) tmem_ld32(tS + i, v + i);
         tmem_ld_wait();
+        if constexpr (C::BESIDE) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(B.s_read + 8 * w);
+        }
         const int visible = seen - (c.j0 + j) * BK;
         const uint4 bits = *reinterpret_cast<const uint4*>(there + ((blocks_so_far + j) & (THERE - 1)) * 4);
         if (negative) {
@@ -530,30 +594,34 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           }
         }
         // NaN where one of the scores is
-        float top[4] = {max3(v[0], v[4], v[8]), max3(v[1], v[5], v[9]), max3(v[2], v[6], v[10]), max3(v[3], v[7], v[11])};
+        float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int i = 12; i + 8 <= BK; i += 8)
+        for (int i = 4; i < BK; i += 4)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) top[x] = max3(top[x], v[i + x], v[i + 4 + x]);
-        top[0] = max3(top[0], v[BK - 4], v[BK - 3]);
-        top[1] = max3(top[1], v[BK - 2], v[BK - 1]);
-        float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+          for (int x = 0; x < 4; ++x) top[x] = max_nan(top[x], v[i + x]);
+        float mx = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
         if (mx == INFINITY) mx = NAN;  // as the definition has it: infinity less infinity
+        bool p_free = !C::BESIDE;
         if (!begun) m = mx;
         else {
-          // the scores of block j are there: the products of every block before have ended, and the output rests
           const bool grow = !(mx <= m + growth);
           if (__any_sync(L3_FULL, grow)) {
+            // the output rests once the products of the block before have ended (which they have where its weights lay over these scores)
+            if constexpr (C::BESIDE) {
+              mbar_wait(B.p_read + 8 * w, p_phase, fail);
+              tc_fence_after();
+              p_free = true;
+            }
             const float alpha = grow ? ex2((m - mx) * sc) : 1.f;
             if (grow) { m = mx; l *= alpha; }
 #pragma unroll 1
             for (int d = 0; d < HD; d += 16) {
               float o[16];
-              tmem_ld16(tO + w * 128 + d, o);
+              tmem_ld16(tO + w * C::O_COLS + d, o);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] *= alpha;
-              tmem_st16(tO + w * 128 + d, o);
+              tmem_st16(tO + w * C::O_COLS + d, o);
             }
           }
         }
@@ -571,12 +639,19 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
             sum[i / 2 & 1] = add2(sum[i / 2 & 1], e);
             p[i / 2] = pack<T>(e.x, e.y);
           }
-          tmem_st32(tS + 32 * h, p);
+          if constexpr (C::BESIDE) {
+            if (!h && !p_free) {
+              mbar_wait(B.p_read + 8 * w, p_phase, fail);
+              tc_fence_after();
+            }
+          }
+          tmem_st32(tP + 32 * h, p);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive((h ? B.p_full : B.half_p) + 8 * w);
         }
+        p_phase ^= 1;
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
@@ -590,15 +665,23 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       float m2 = m == -INFINITY ? m : m * sc - C::BIAS;  // in units of log 2
       float share = 1.f, share1 = 0.f;                    // of the outputs: this tile's, or the first's and the second's
       if (n) {
-        mbar_wait(B.o_full + 8 * w, o_phase, fail);
+        // an output's end is told of only where it has blocks: else the next item's could come before a warp has seen this one's
+        const bool second = two || n > 1;
+        if (!two || w == 0) mbar_wait(B.o_full, o_phase[0], fail);
+        if (second && (!two || w == 1)) mbar_wait(B.o_full + 8, o_phase[1], fail);
+        o_phase[0] ^= 1;
+        o_phase[1] ^= second;
+        __syncwarp();
         if (!two) {
-          mbar_wait(B.o_full + 8 * (w ^ 1), o_phase, fail);
-          float2* const mine = reinterpret_cast<float2*>(stages + warp * C::STAGE);
-          const float2* const others = reinterpret_cast<const float2*>(stages + (warp ^ 4) * C::STAGE);
-          mine[lane] = make_float2(m2, l);
+          // one float a row, twice: there is no more room beside the tiles
+          xch[warp][lane] = m2;
           asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");
-          const float2 other = others[lane];
+          float2 other;
+          other.x = xch[warp ^ 4][lane];
           asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");
+          xch[warp][lane] = l;
+          asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");
+          other.y = xch[warp ^ 4][lane];
           const float both = fmaxf(m2, other.x), from = both == -INFINITY ? 0.f : both;
           const float mf = ex2(m2 - from), of = ex2(other.x - from);
           l = l * mf + other.y * of;
@@ -606,85 +689,78 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           share = w ? of : mf;
           share1 = w ? mf : of;
         }
-        o_phase ^= 1;
         tc_fence_after();
       }
-      const int D0 = two ? HD : HD / 2, first = two ? 0 : w * D0;  // columns of this thread
       const long long at = (long long)(c.r.s0 + t) * a.H + c.g * a.R + f - t * a.R;
-      const float inv = *fail ? NAN : l == 0.f ? 0.f : 1.f / l;
+      if (*fail) l = NAN;  // a wait ran out
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       bool finite = l < INFINITY;
-      // 32 rows of up to 128 bytes at a time by way of shared memory, so that a store covers whole rows and not 16 bytes of 32 of them
-      auto out = [&](auto as_result, auto of_two) {
-        constexpr bool RESULT = decltype(as_result)::value, TWO = decltype(of_two)::value;
-        constexpr int UNITS = RESULT && TWO ? 8 : 4, PER = RESULT ? 1 : 2, CH = UNITS * PER;  // units of 8 columns, their 16-byte pieces, of a row
-        constexpr int D0 = TWO ? HD : HD / 2;
-        uint8_t* const stage = stages + warp * C::STAGE;
+      if (two) {  // a row's columns, 16 at a time: 32 bytes of the result, 64 of a partial
+        const bool wide = ((uintptr_t)a.out & 31) == 0;
 #pragma unroll 1
-        for (int u0 = 0; u0 < D0 / 8; u0 += UNITS) {
-          float o[UNITS * 8];
-          [[maybe_unused]] float o1[TWO ? 1 : UNITS * 8];
+        for (int d = 0; d < HD; d += 16) {
+          float o[16];
           if (n) {
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u)
-              if (u0 + u < D0 / 8) {
-                tmem_ld8(tO + (TWO ? w * 128 : 0) + first + (u0 + u) * 8, o + u * 8);
-                if constexpr (!TWO) tmem_ld8(tO + 128 + first + (u0 + u) * 8, o1 + u * 8);
-              }
+            tmem_ld16(tO + w * C::O_COLS + d, o);
             tmem_ld_wait();
-            if constexpr (!TWO) {
-#pragma unroll
-              for (int i = 0; i < UNITS * 8; ++i) o[i] = n > 1 ? o[i] * share + o1[i] * share1 : o[i] * share;
-            }
           } else {
 #pragma unroll
-            for (int i = 0; i < UNITS * 8; ++i) o[i] = 0.f;
+            for (int i = 0; i < 16; ++i) o[i] = 0.f;
           }
 #pragma unroll
-          for (int u = 0; u < UNITS; ++u)
-            if (u0 + u < D0 / 8) {
+          for (int i = 0; i < 16; ++i) finite = finite && fabsf(o[i]) < INFINITY;
+          if (f < flats) {
+            if (whole) {
+              uint32_t x[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) finite = finite && fabsf(o[u * 8 + i]) < INFINITY;
-              if constexpr (RESULT) {
-                uint32_t x[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = pack<T>(o[u * 8 + 2 * i] * inv, o[u * 8 + 2 * i + 1] * inv);
-                *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                  *reinterpret_cast<float4*>(stage + lane * 128 + (((2 * u + i) ^ (lane & 7)) << 4)) =
-                      make_float4(o[u * 8 + 4 * i], o[u * 8 + 4 * i + 1], o[u * 8 + 4 * i + 2], o[u * 8 + 4 * i + 3]);
+              for (int i = 0; i < 8; ++i) x[i] = pack<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
+              T* const to = (T*)a.out + at * HD + d;
+              if (wide) store32(to, x);
+              else {
+                *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint4*>(to + 8) = make_uint4(x[4], x[5], x[6], x[7]);
               }
-            }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < CH; ++i) {
-            const int row = i * (32 / CH) + lane / CH, ch = lane % CH, d = first + u0 * 8 + ch * (8 / PER);
-            const uint4 x = *reinterpret_cast<const uint4*>(stage + row * 128 + ((ch ^ (row & 7)) << 4));
-            const long long to = __shfl_sync(L3_FULL, at, row);
-            if (f - lane + row < flats && u0 + ch / PER < D0 / 8) {
-              if constexpr (RESULT) *reinterpret_cast<uint4*>((T*)a.out + to * HD + d) = x;
-              else *reinterpret_cast<uint4*>(part_o + (size_t)(in_tile - lane + row) * HD + d) = x;
+            } else {
+              float* const to = part_o + (size_t)in_tile * HD + d;
+              store32(to, reinterpret_cast<const uint32_t*>(o));
+              store32(to + 8, reinterpret_cast<const uint32_t*>(o) + 8);
             }
           }
           __syncwarp();
         }
-      };
-      if (two) {
-        if (whole) out(std::true_type{}, std::true_type{});
-        else out(std::false_type{}, std::true_type{});
-      } else {
-        if (whole) out(std::true_type{}, std::false_type{});
-        else out(std::false_type{}, std::false_type{});
+      } else {  // half of a row's columns, 8 at a time, of both outputs
+#pragma unroll 1
+        for (int d = w * (HD / 2); d < (w + 1) * (HD / 2); d += 8) {
+          float o[8], o1[8];
+          if (n) {
+            tmem_ld8(tO + d, o);
+            tmem_ld8(tO + C::O_COLS + d, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = n > 1 ? o[i] * share + o1[i] * share1 : o[i] * share;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) finite = finite && fabsf(o[i]) < INFINITY;
+          if (f < flats) {
+            if (whole) {
+              *reinterpret_cast<uint4*>((T*)a.out + at * HD + d) =
+                  make_uint4(pack<T>(o[0] * inv, o[1] * inv), pack<T>(o[2] * inv, o[3] * inv), pack<T>(o[4] * inv, o[5] * inv), pack<T>(o[6] * inv, o[7] * inv));
+            } else store32(part_o + (size_t)in_tile * HD + d, reinterpret_cast<const uint32_t*>(o));
+          }
+          __syncwarp();
+        }
       }
       if (f < flats && (two || w == 0)) {
-        if (!whole) part_ml[in_tile] = make_float2(*fail ? NAN : m2, l);
+        if (!whole) part_ml[in_tile] = make_float2(m2, l);
         else if (a.lse) a.lse[at] = (m2 + log2f(l)) * 0.6931471805599453f;
       }
       tc_fence_before();
       if (whole && f < flats && !finite) left_of(a, blockIdx.x).odd = 1;
       if (!two) asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory");  // both have read the outputs
-    } while (c.next(a));
+    } while (c.next(a, SPLIT));
   }
   tc_fence_before();
   __syncthreads();
@@ -699,15 +775,21 @@ int rows_of_item(const ChunkArgs& a, int n_sm) {
 }
 // Whether, and how, tiles are copied by TMA: a box is 64 entries of as many rows as lie side by side.  Distances of 0 between different rows are not for it.
 bool usable(long long stride, long long n) { return n <= 1 || (stride > 0 && stride < (1LL << 38)); }
-bool map_pool(const ChunkArgs& a, const PagedPool& p, CUtensorMap* map) {
-  if (a.log_page < 3 || !usable(p.sp, a.n_pages) || !usable(p.sh, a.G) || !usable(p.st, 2)) return false;
-  const uint64_t dims[4] = {(uint64_t)a.HD, 1ull << a.log_page, (uint64_t)a.G, (uint64_t)a.n_pages};
-  const uint64_t strides[3] = {(uint64_t)p.st * 2, (uint64_t)std::max(p.sh, 8LL) * 2, (uint64_t)std::max(p.sp, 8LL) * 2};
-  const uint32_t box[4] = {64, (uint32_t)std::min(1 << a.log_page, BK), 1, 1};
-  return tc_make_map(map, p.p, a.dtype == L3_DTYPE_BF16, 4, dims, strides, box);
+bool map_pools(const ChunkArgs& a, CUtensorMap* map, bool* keys_first) {
+  const PagedPool &p = a.k, &v = a.v;
+  const long long apart = (const char*)v.p - (const char*)p.p;
+  *keys_first = apart > 0;
+  if (a.log_page < 3 || p.sp != v.sp || p.sh != v.sh || p.st != v.st || apart == 0 || !usable(p.sp, a.n_pages) || !usable(p.sh, a.G) || !usable(p.st, 2) ||
+      !usable(std::abs(apart) / 2, 2))
+    return false;
+  const uint64_t dims[5] = {(uint64_t)a.HD, 1ull << a.log_page, (uint64_t)a.G, (uint64_t)a.n_pages, 2};
+  const uint64_t strides[4] = {(uint64_t)p.st * 2, (uint64_t)std::max(p.sh, 8LL) * 2, (uint64_t)std::max(p.sp, 8LL) * 2, (uint64_t)std::abs(apart)};
+  const uint32_t box[5] = {64, (uint32_t)std::min(1 << a.log_page, BK), 1, 1, 1};
+  return tc_make_map(map, apart > 0 ? p.p : v.p, a.dtype == L3_DTYPE_BF16, 5, dims, strides, box);
 }
 bool map_q(const ChunkArgs& a, CUtensorMap* map) {
-  if (128 % a.R || !usable(a.q_sh, a.H) || !usable(a.q_st, a.T)) return false;
+  // (few rows: copied sooner than the map is made)
+  if (a.T * a.R < 1024 || 128 % a.R || !usable(a.q_sh, a.H) || !usable(a.q_st, a.T)) return false;
   const uint64_t dims[3] = {(uint64_t)a.HD, (uint64_t)a.H, (uint64_t)a.T};
   const uint64_t strides[2] = {(uint64_t)std::max(a.q_sh, 8LL) * 2, (uint64_t)std::max(a.q_st, 8LL) * 2};
   const uint32_t box[3] = {64, (uint32_t)a.R, (uint32_t)(128 / a.R)};
@@ -723,8 +805,9 @@ template <typename T, int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaS
   cudaError_t e = allow_smem(chunk_tc_kernel<T, HD>, C::SMEM);
   if (e != cudaSuccess) return e;
   Maps maps{};
-  const bool tma_q = map_q(a, &maps.q), tma_kv = map_pool(a, a.k, &maps.k) && map_pool(a, a.v, &maps.v);
-  if ((e = launch_k(chunk_tc_kernel<T, HD>, dim3(a.n_cta), dim3(NT), (size_t)C::SMEM, s, a, maps, tma_q, tma_kv)) != cudaSuccess) return e;
+  bool keys_first;
+  const bool tma_q = map_q(a, &maps.q), tma_kv = map_pools(a, &maps.kv, &keys_first);
+  if ((e = launch_k(chunk_tc_kernel<T, HD>, dim3(a.n_cta), dim3(NT), (size_t)C::SMEM, s, a, maps, tma_q, tma_kv, keys_first)) != cudaSuccess) return e;
   return launch_chunk_join_tc(a, s);
 }
 template <typename T> cudaError_t launch_t(const ChunkArgs& a, int n_sm, cudaStream_t s) {

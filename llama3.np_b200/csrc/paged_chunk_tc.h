@@ -3,5 +3,5 @@
 #include "packed.h"
 
 cudaError_t launch_paged_chunk_tc(const ChunkArgs& a, int n_sm, cudaStream_t s);
-constexpr int TC_BK = 128, TC_WHOLE = 4;                                             // keys of a block; items of so few blocks are not cut
+constexpr int TC_BK = 128;  // keys of a block
 cudaError_t launch_chunk_join_tc(const ChunkArgs& a, cudaStream_t s);   // paged_chunk.cu
