@@ -545,28 +545,13 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       const int n = c.j1 - c.j0;
       const bool two = two_tiles();
       const int in_tile = (two ? w * 128 : 0) + r, f = c.tile * a.tile_rows + in_tile, flats = c.r.n * a.R, t = f / a.R;
-      const int seen = f < flats ? c.r.seen(t) : INT_MAX;  // a row behind the last: whatever it has goes nowhere, and masks cost time
-      const bool idle = f - lane >= flats;                 // none of the warp's rows is one: it only keeps step
+      const int seen = f < flats ? c.r.seen(t) : INT_MAX;  // a row behind the last: what it has goes nowhere, and masks cost time
       float m = -INFINITY, l = 0.f;  // m: of s, what the exponentials are taken against
       bool begun = false;
       for (int j = two ? 0 : w; j < n; j += two ? 1 : 2) {
         mbar_wait(B.s_full + 8 * w, s_phase, fail);
         s_phase ^= 1;
         tc_fence_after();
-        if (idle) {
-          if constexpr (C::BESIDE) {
-            mbar_wait(B.p_read + 8 * w, p_phase, fail);
-            p_phase ^= 1;
-          }
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (C::BESIDE) mbar_arrive(B.s_read + 8 * w);
-            mbar_arrive(B.half_p + 8 * w);
-            mbar_arrive(B.p_full + 8 * w);
-          }
-          __syncwarp();
-          continue;
-        }
         float v[BK];
 #pragma unroll
         for (int i = 0; i < BK; i += 32) tmem_ld32(tS + i, v + i);
