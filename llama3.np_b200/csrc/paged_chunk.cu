@@ -15,7 +15,7 @@
 namespace {
 using namespace chunk;
 constexpr int TR = 64, BK = 64, NT = 256;
-__host__ __device__ constexpr Split fma_split() { return Split{BK, 4, 8, TR}; }
+__host__ __device__ constexpr Split fma_split() { return Split{BK, 4, 8, TR, 2}; }
 template <int HD> constexpr int row_ld() { return HD + 4; }
 template <int HD> constexpr size_t smem_bytes() { return (size_t)(2 * 64 * row_ld<HD>() + 64 * HD + 64 * (TR + 4)) * 4 + 2 * 2 * BK * 8 + 2 * 8 + 16; }
 
@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
   __shared__ Place place;
   pdl_launch();
   pdl_wait();
-  clear_rest<T>(a);
+  clear_rest<T>(a, threadIdx.x, NT);
   find_share<BK, NT>(a, SPLIT, room, &place);
   if (threadIdx.x == 0) leave_nothing(a, place);
   __syncthreads();

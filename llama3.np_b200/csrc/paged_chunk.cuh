@@ -40,25 +40,30 @@ template <int BK> __device__ __forceinline__ int blocks(const ChunkArgs& a, cons
   const int last = min(r.n * a.R, (tile + 1) * a.tile_rows) - 1;
   return (int)((unsigned)(r.seen(last / a.R) + BK - 1) / BK);
 }
-// An item's weight: `per` a block - 2, or 4 of a tile that takes a block's time twice as long (Split) - and 2 for what begins and ends it.
-struct Split { int block, whole, least, rows_of_half; };  // keys of a block; items of so few blocks are not cut; least weight of a share; rows that a block costs half for
+// An item's weight: `per` a block - 2, or 4 of a tile of more than rows_of_half rows - and `ends` for what begins and ends it.  Items of `whole` blocks or
+// fewer are not cut; `least`: the least weight of a share.
+struct Split { int block, whole, least, rows_of_half, ends; };
 // paged_chunk_tc.cu: one tile of rows has two blocks at a time, which takes half the time as long as the tiles' copies keep up.  us, half : three quarters :
 // all of a block's weight: heads of 64, 48 requests of up to 3001 tokens 125 : 131 : 141; of 128, six prompts of up to 4096 tokens 666 : 600 : 575
-__host__ __device__ constexpr Split tc_split(int HD) { return Split{TC_BK, 4, 4, HD <= 64 ? 128 : 0}; }
+__host__ __device__ constexpr Split tc_split(int HD) { return Split{TC_BK, 4, 4, HD <= 64 ? 128 : 0, 6}; }
 __device__ __forceinline__ int per_block(const ChunkArgs& a, const Split& sp, const Request& r, int tile) {
   return min(r.n * a.R - tile * a.tile_rows, a.tile_rows) > sp.rows_of_half ? 4 : 2;
 }
 // The blocks of an item of nb that lie ahead of weight x.
-__device__ __forceinline__ int ahead(long long x, int nb, int per, int whole) {
-  const int w = per * nb + 2;
+__device__ __forceinline__ int ahead(long long x, int nb, int per, const Split& sp) {
+  const int w = per * nb + sp.ends;
   if (x <= 0) return 0;
   if (x >= w) return nb;
-  if (nb <= whole) return 2 * x >= w ? nb : 0;
+  if (nb <= sp.whole) return 2 * x >= w ? nb : 0;
   return min((int)x / per, nb);
 }
 
 struct Place { int b, tile, g, pad; long long off, rest; };  // an item, the weight of it that others have, and what this CTA has from there on
 
+// all * i / n, in 32 bits where that will do
+__device__ __forceinline__ long long share_of(long long all, int i, int n) {
+  return all < (1 << 21) && i < (1 << 11) ? (long long)((uint32_t)all * (uint32_t)i / (uint32_t)n) : all * i / n;
+}
 // This CTA's share, by all NT threads (`room`: NT / 32 + 1 words of shared memory).
 template <int BK, int NT>
 __device__ __forceinline__ void find_share(const ChunkArgs& a, const Split& sp, long long* room, Place* place) {
@@ -70,9 +75,9 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, const Split& sp, 
     for (int b = b0; b < b1; ++b) {
       const Request r = request(a, b);
       const int nt = tiles(a, r.n), part = parts > 1 ? threadIdx.x % parts : 0;
-      const int t0 = (int)((long long)nt * part / parts), t1 = (int)((long long)nt * (part + 1) / parts);
+      const int t0 = share_of(nt, part, parts), t1 = share_of(nt, part + 1, parts);
       for (int t = t0; t < t1; ++t)
-        if (f(b, t, per_block(a, sp, r, t) * blocks<BK>(a, r, t) + 2)) return;
+        if (f(b, t, per_block(a, sp, r, t) * blocks<BK>(a, r, t) + sp.ends)) return;
     }
   };
   long long sum = 0;
@@ -95,9 +100,9 @@ __device__ __forceinline__ void find_share(const ChunkArgs& a, const Split& sp, 
     if (w < warp) before += room[w];
     all += room[w];
   }
-  const long long ctas = min((long long)a.n_cta, max(all / sp.least, 1LL));
+  const int ctas = (int)min((long long)a.n_cta, max(all / sp.least, 1LL));
   if (blockIdx.x < ctas) {
-    const long long w0 = all * blockIdx.x / ctas, w1 = all * (blockIdx.x + 1) / ctas;
+    const long long w0 = share_of(all, blockIdx.x, ctas), w1 = share_of(all, blockIdx.x + 1, ctas);
     if (before <= w0 && w0 < before + sum) {
       long long at = before;
       walk([&](int b, int t, int w) {
@@ -136,13 +141,13 @@ template <int BK> struct Cursor {
   // the stretch of this item, if there is one
   __device__ __forceinline__ bool settle(const Split& sp) {
     if (rest <= 0) return false;
-    j0 = ahead(off, nb, per, sp.whole);
-    j1 = ahead(off + rest, nb, per, sp.whole);
+    j0 = ahead(off, nb, per, sp);
+    j1 = ahead(off + rest, nb, per, sp);
     return j1 > j0 || (nb == 0 && off == 0);
   }
   __device__ __forceinline__ bool next(const ChunkArgs& a, const Split& sp) {
     for (;;) {
-      rest -= per * nb + 2 - off;
+      rest -= per * nb + sp.ends - off;
       off = 0;
       if (rest <= 0) return false;
       if (++g == a.G) {
@@ -219,11 +224,11 @@ template <typename T, int HD> __device__ __forceinline__ void by_formula(const C
 }
 
 // rows of no request: as they are, or 0
-template <typename T> __device__ __forceinline__ void clear_rest(const ChunkArgs& a) {
+template <typename T> __device__ __forceinline__ void clear_rest(const ChunkArgs& a, int thread, int threads) {  // by some of a CTA's threads
   if (!a.clear_rest) return;
   const int from = a.B ? min(max(a.starts[a.B], 0), a.T) : 0;
   const long long n = (long long)(a.T - from) * a.H, at = (long long)from * a.H;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n * a.HD; i += (long long)gridDim.x * blockDim.x) {
+  for (long long i = (long long)blockIdx.x * threads + thread; i < n * a.HD; i += (long long)gridDim.x * threads) {
     ((T*)a.out)[at * a.HD + i] = down<T>(0.f);
     if (a.lse && i < n) a.lse[at + i] = -INFINITY;
   }

@@ -215,7 +215,6 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   pdl_wait();
-  clear_rest<T>(a);
   tc_fence_before();
   find_share<BK, NT>(a, SPLIT, room, &place);
   tc_fence_after();
@@ -396,41 +395,47 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       const int* table = a.table + c.b * a.table_stride;
       const bool two = two_tiles();
       const int ahead = (two ? 1 : 2) + (C::BESIDE ? 1 : 0);  // blocks of keys that are multiplied ahead of the first one's values
-      if (tma_q) {
-        if (first_loader) {
-          free_to_fill(B.q_empty, q_phase);
-          if (elect_one()) {
-            mbar_expect_tx(B.q_full, (two ? 2 : 1) * TILE);
+      auto queries = [&]() {  // behind the first keys: they need not wait for the products of the item before
+        if (tma_q) {
+          if (first_loader) {
+            free_to_fill(B.q_empty, q_phase);
+            if (elect_one()) {
+              mbar_expect_tx(B.q_full, (two ? 2 : 1) * TILE);
 #pragma unroll 1
-            for (int h = 0; h < (two ? 2 : 1); ++h)
+              for (int h = 0; h < (two ? 2 : 1); ++h)
 #pragma unroll
-              for (int x = 0; x < C::QS; ++x)
-                tma_3d(sQ + h * TILE + x * 16384, &maps.q, x * 64, c.g * a.R, c.r.s0 + (flat0 + h * 128) / a.R, B.q_full);
+                for (int x = 0; x < C::QS; ++x)
+                  tma_3d(sQ + h * TILE + x * 16384, &maps.q, x * 64, c.g * a.R, c.r.s0 + (flat0 + h * 128) / a.R, B.q_full);
+            }
+            __syncwarp();
           }
-          __syncwarp();
-        }
-      } else {
-        free_to_fill(B.q_empty, q_phase);
+        } else {
+          free_to_fill(B.q_empty, q_phase);
 #pragma unroll 1
-        for (int h = 0; h < (two ? 2 : 1) * SETS; ++h) {
-          const int in = row0 + h % SETS * 32, f = flat0 + h / SETS * 128 + in + lane, t = f / a.R;
-          rows(f < flats ? (const T*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh : nullptr, sQ + h / SETS * TILE, in);
+          for (int h = 0; h < (two ? 2 : 1) * SETS; ++h) {
+            const int in = row0 + h % SETS * 32, f = flat0 + h / SETS * 128 + in + lane, t = f / a.R;
+            rows(f < flats ? (const T*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh : nullptr, sQ + h / SETS * TILE, in);
+          }
+          filled(B.q_full);
+          if (tma_kv) told();  // nothing else would
         }
-        filled(B.q_full);
-        if (tma_kv) told();  // nothing else would
-      }
-      q_phase ^= 1;
+        q_phase ^= 1;
+      };
       if (tma_kv) {
-        if (!first_loader) continue;
+        if (!first_loader) {
+          queries();
+          continue;
+        }
         // one lane a page of the block, or the first one for a part of a page
         const int page_size = 1 << a.log_page, box = min(page_size, BK), pages = BK / box;
         auto page_of = [&](int j) {
           const int key = j * BK + lane * box;
           int page = -1;
           if (lane < pages && key < most) page = __ldg(table + (key >> a.log_page));
-          return (unsigned)page < (unsigned)a.n_pages ? page : a.n_pages;  // outside: the copy's rows are zeros
+          return page;
         };
-        auto fill = [&](int page, int j, bool keys) {
+        auto fill = [&](int named, int j, bool keys) {
+          const int page = (unsigned)named < (unsigned)a.n_pages ? named : a.n_pages;  // outside: the copy's rows are zeros
           const uint32_t bar = B.full + 8 * slot, tile = ring + slot * TILE;
           mbar_wait(B.empty + 8 * slot, phase, fail);
           if (keys) {
@@ -475,6 +480,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           next = page_of(c.j0 + x + 1);
           fill(page, c.j0 + x, true);
         }
+        queries();
         for (int i = 0; i < n; ++i) {
           fill(had, c.j0 + i, false);
           had = had1;
@@ -520,6 +526,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         next = pages_of(c.j0 + x + 1);
         fill(a.k, page, c.j0 + x, true);
       }
+      queries();
       for (int i = 0; i < n; ++i) {
         fill(a.v, had, c.j0 + i, false);
         had = had1;
@@ -533,6 +540,8 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       }
     } while (c.next(a, SPLIT));
     told();
+  } else if (warp == 9) {
+    clear_rest<T>(a, lane, 32);
   } else if (warp < 8) {  // ---------------------------------------------------------------------------------------- softmax
     const int quarter = warp & 3, w = warp >> 2, r = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + w * BK + lanes, tO = tmem + C::T_O + lanes, tP = tmem + C::T_P + w * C::P_COLS + lanes;
