@@ -13,6 +13,11 @@ from .utils import load_parameters  # noqa: F401
 
 
 def __getattr__(name):  # lazy: importing the package must not require the built library
+    value = globals()[name] = _lazy(name)  # found once: the search takes a microsecond of every call
+    return value
+
+
+def _lazy(name):
     if name in ("Llama", "compute_cos_sin_cache"):
         from . import llama3 as _l
         return getattr(_l, name)

@@ -304,7 +304,7 @@ extern "C" int l3_paged_chunk_workspace(int device, int tokens, int heads, int k
   int rc = check_chunk(tokens, heads, kv_heads, head_dim, dtype), n_sm = 0;
   if (rc != L3_OK) return rc;
   CKD(sm_count(device, &n_sm));
-  *bytes = (int64_t)paged_chunk_workspace(head_dim, dtype, n_sm);
+  *bytes = (int64_t)paged_chunk_workspace(heads, kv_heads, head_dim, dtype, n_sm);
   return L3_OK;
 }
 extern "C" int l3_paged_chunk_attention(const L3PagedChunk* a) {
@@ -323,7 +323,7 @@ extern "C" int l3_paged_chunk_attention(const L3PagedChunk* a) {
   CKD(on.e);
   int n_sm = 0;
   CKD(sm_count(a->device, &n_sm));
-  const size_t need = paged_chunk_workspace(a->head_dim, a->dtype, n_sm);
+  const size_t need = paged_chunk_workspace(a->heads, a->kv_heads, a->head_dim, a->dtype, n_sm);
   REQ(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= (int64_t)need, "the workspace must be %zu bytes, aligned to 16", need);
   ChunkArgs p{};
   p.q = a->q; p.q_st = a->q_token_stride; p.q_sh = a->q_head_stride;

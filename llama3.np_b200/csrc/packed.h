@@ -53,7 +53,7 @@ struct ChunkArgs {
   float2* part_ml;                   // [n_cta][2][rows of a tile]
   void* left;                        // [n_cta] chunk::Left
 };
-size_t paged_chunk_workspace(int HD, int dtype, int n_sm);
+size_t paged_chunk_workspace(int H, int G, int HD, int dtype, int n_sm);
 cudaError_t launch_paged_chunk(ChunkArgs a, int n_sm, cudaStream_t s);
 
 struct LogprobsArgs {

@@ -128,7 +128,24 @@ template <int N> __device__ __forceinline__ void store_out(const PagedAttnArgs& 
     *reinterpret_cast<uint32_t*>((bf16*)a.out + i + e) = x;
   }
 }
-__device__ __forceinline__ int asked_length(const PagedAttnArgs& a, int b) { return a.lengths ? a.lengths[b] : *a.pos_ptr + 1; }
+// the sequence that row b belongs to (a packed step's rows), or -1
+__device__ __forceinline__ int sequence_of(const PagedAttnArgs& a, int b) {
+  int lo = -1, hi = a.requests;  // starts[lo] <= b < starts[hi], as far as they rise
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.starts[mid] <= b) lo = mid;
+    else hi = mid;
+  }
+  return lo >= 0 && b < a.starts[lo + 1] ? lo : -1;
+}
+__device__ __forceinline__ int asked_length(const PagedAttnArgs& a, int b) {
+  if (a.starts) {
+    const int r = sequence_of(a, b);
+    return r < 0 ? 0 : max(a.lengths[r], 0) - min(a.starts[r + 1], a.B) + b + 1;
+  }
+  return a.lengths ? a.lengths[b] : *a.pos_ptr + 1;
+}
+__device__ __forceinline__ const int* table_of(const PagedAttnArgs& a, int b) { return a.table + (a.starts ? sequence_of(a, b) : b) * a.table_stride; }
 __device__ __forceinline__ int length_of(const PagedAttnArgs& a, int b) { return min(max(asked_length(a, b), 0), a.max_pages << a.log_page); }
 
 // where a warp is in the long row of tiles: tile t of the nt tiles of item (sequence b, kv head g, block of its query heads)
@@ -590,7 +607,7 @@ __device__ __forceinline__ void stretch(const PagedAttnArgs& a, Cursor C, int po
   int entry = 0;     // the page of this lane's key there
   auto look = [&] {
     const int pos = L.t * TK + (lane & (TK - 1));
-    entry = L.b < a.B && pos < L.len ? __ldg(a.table + L.b * a.table_stride + (pos >> a.log_page)) : -1;
+    entry = L.b < a.B && pos < L.len ? __ldg(table_of(a, L.b) + (pos >> a.log_page)) : -1;
   };
   auto rows = [&](Rows& r, int buf) {
     const int pos = L.t * TK + (lane & (TK - 1)), g = L.g;

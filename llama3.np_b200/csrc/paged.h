@@ -23,6 +23,8 @@ struct PagedAttnArgs {
   int max_pages;
   const int* lengths;                // [B], or null: *pos_ptr + 1 tokens for every sequence
   const int* pos_ptr;
+  const int* starts;                 // null, or [requests + 1]: B rows of `requests` sequences; lengths and table are theirs, row b's tokens end with its own
+  int requests;
   int B, H, G, HD;
   float scale;
   void* out;                         // [B, H, HD]

@@ -15,7 +15,8 @@
 namespace {
 using namespace chunk;
 constexpr int TR = 64, BK = 64, NT = 256;
-__host__ __device__ constexpr Split fma_split() { return Split{BK, 4, 8, TR, 2}; }
+__host__ __device__ constexpr Split fma_split() { return Split{BK, 4, 8, TR, 3}; }
+constexpr int ctas_of_sm(int HD) { return HD > 64 ? 1 : HD > 48 ? 2 : 3; }  // as shared memory has room for
 template <int HD> constexpr int row_ld() { return HD + 4; }
 template <int HD> constexpr size_t smem_bytes() { return (size_t)(2 * 64 * row_ld<HD>() + 64 * HD + 64 * (TR + 4)) * 4 + 2 * 2 * BK * 8 + 2 * 8 + 16; }
 
@@ -27,7 +28,7 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <int HD>
-__global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_fma_kernel(const ChunkArgs a) {
   using T = float;
   constexpr Split SPLIT = fma_split();
   constexpr int LD = row_ld<HD>(), PL = TR + 4;
@@ -49,21 +50,17 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
   __syncthreads();
   const int lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float sc = a.scale * 1.4426950408889634f;
+  auto token_of = [&](int f) { return a.R == 1 ? f : f / a.R; };
   Cursor<BK> c;
   if (!c.start(a, SPLIT, place)) return;
   do {
     const int* table = a.table + c.b * a.table_stride;
     const int flat0 = c.tile * TR, flats = c.r.n * a.R;
-    const int most = c.r.seen((min(flats, flat0 + TR) - 1) / a.R);   // keys that any of the rows sees
-    // the rows' queries
-    for (int i = threadIdx.x; i < TR * HD; i += NT) {
-      const int r = i / HD, d = i - r * HD, f = flat0 + r;
-      float x = 0.f;
-      if (f < flats) {
-        const int t = f / a.R;
-        x = up(((const T*)a.q)[(c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh + d]);
-      }
-      sQ[r * LD + d] = x;
+    const int most = c.r.seen(token_of(min(flats, flat0 + TR) - 1));   // keys that any of the rows sees
+    for (int i = threadIdx.x; i < TR * (HD / 4); i += NT) {  // the rows' queries
+      const int r = i / (HD / 4), p = i - r * (HD / 4), f = flat0 + r, t = token_of(f);
+      const bool in = f < flats;
+      cp16(smem_u32(sQ + r * LD + p * 4), in ? (const T*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh + p * 4 : (const T*)a.q, in);
     }
     auto offsets = [&](int j) {  // by the first 64 threads
       if (threadIdx.x >= BK) return;
@@ -94,7 +91,7 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int f = flat0 + ty * 4 + i;
-      seen[i] = f < flats ? c.r.seen(f / a.R) : 0;
+      seen[i] = f < flats ? c.r.seen(token_of(f)) : 0;
     }
     float2 o[2][NC * CW];   // pairs of rows
     float m[4], l[4];
@@ -212,7 +209,7 @@ __global__ void __launch_bounds__(NT, HD > 64 ? 1 : 2) chunk_fma_kernel(const Ch
       }
       if (f < flats) {
         if (!finite && whole) left_of(a, blockIdx.x).odd = 1;
-        const int t = f / a.R;
+        const int t = token_of(f);
         const long long at = (long long)(c.r.s0 + t) * a.H + c.g * a.R + f - t * a.R;
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
 #pragma unroll
@@ -334,7 +331,7 @@ template <typename T, int BK> cudaError_t join_t(const ChunkArgs& a, const Split
 }
 template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
   constexpr size_t smem = smem_bytes<HD>();
-  a.n_cta = (HD > 64 ? 1 : 2) * n_sm;
+  a.n_cta = ctas_of_sm(HD) * n_sm;
   a.tile_rows = TR;
   a.part_o = (float*)a.ws;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * TR * HD);
@@ -350,10 +347,34 @@ cudaError_t launch_chunk_join_tc(const ChunkArgs& a, cudaStream_t s) {
   return a.dtype == L3_DTYPE_BF16 ? join_t<bf16, TC_BK>(a, tc_split(a.HD), s) : join_t<__half, TC_BK>(a, tc_split(a.HD), s);
 }
 
-// the larger of either number of rows
-size_t paged_chunk_workspace(int HD, int dtype, int n_sm) { return dtype == L3_DTYPE_F32 ? partials(2 * n_sm, TR, HD) : partials(n_sm, 256, HD); }
+namespace {
+// Few rows over few keys as single tokens (paged.cu), which read their request's keys anew each.  us, so : as tiles, 32 heads over 8 kv heads of 128, one
+// request, by rows x keys and what is read: bf16 5 x 1505 29 MB 14.2 : 23.0, 16 x 1516 95 MB 23.0 : 23.4, 8 x 6008 188 MB 34.4 : 29.2, 2 x 60002 469 MB 88 : 63;
+// fp32 5 x 6005 235 MB 50 : 75, 8 x 6008 376 MB 72 : 78, 16 x 6016 752 MB 130 : 82.  (That path writes every row.)
+bool as_single_tokens(const ChunkArgs& a) {
+  const long long size = a.dtype == L3_DTYPE_F32 ? 4 : 2, keys = (long long)a.max_pages << a.log_page;
+  return a.clear_rest && a.B > 0 && a.T <= 16 && a.T * keys * a.G * a.HD * 2 * size <= (size == 4 ? 384LL : 128LL) << 20;
+}
+PagedAttnArgs single_tokens(const ChunkArgs& a) {
+  PagedAttnArgs p{};
+  p.q = a.q; p.q_sb = a.q_st; p.q_sh = a.q_sh; p.q_dtype = p.kv_dtype = p.out_dtype = a.dtype;
+  p.k = a.k; p.v = a.v; p.n_pages = a.n_pages; p.log_page = a.log_page;
+  p.table = a.table; p.table_stride = a.table_stride; p.max_pages = a.max_pages; p.lengths = a.lengths; p.starts = a.starts; p.requests = a.B;
+  p.B = a.T; p.H = a.H; p.G = a.G; p.HD = a.HD; p.scale = a.scale; p.out = a.out; p.lse = a.lse; p.ws = a.ws;
+  return p;
+}
+}  // namespace
+
+// of whichever kernels a call takes, and either number of rows
+size_t paged_chunk_workspace(int H, int G, int HD, int dtype, int n_sm) {
+  return std::max(dtype == L3_DTYPE_F32 ? partials(ctas_of_sm(HD) * n_sm, TR, HD) : partials(n_sm, 256, HD), paged_attn_workspace(H, G, HD, n_sm));
+}
 
 cudaError_t launch_paged_chunk(ChunkArgs a, int n_sm, cudaStream_t s) {
+  if (as_single_tokens(a)) {
+    const PagedAttnArgs p = single_tokens(a);
+    if (paged_attn_fits(p)) return launch_paged_attention(p, n_sm, s);
+  }
   if (a.dtype != L3_DTYPE_F32) return launch_paged_chunk_tc(a, n_sm, s);
   switch (a.HD) {
     case 16: return launch_hd<16>(a, n_sm, s);

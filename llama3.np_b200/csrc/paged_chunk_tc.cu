@@ -6,8 +6,7 @@
 //                 expanded strides, and queries whose heads do not fill 128 rows evenly go row by row, 16 bytes a copy (cp.async)
 //   warp 8        products: S = Q K^T into TMEM, O += P V with P from TMEM and V as it lies, an MN-major operand
 //   warps 0 - 7   softmax, a thread a row, four warps a score tile: its 128 scores in registers, exponentials against a maximum that follows
-//                 the running one lazily (O is rescaled in TMEM only when that has grown by 2^GROW), weights as 16-bit values, over the
-//                 scores where TMEM has no room beside them
+//                 the running one lazily (O is rescaled in TMEM only when that has grown by 2^GROW), weights as 16-bit values over the scores
 // The two score tiles take turns: one's softmax runs while the tensor core works on the other's products.  With many rows they are two tiles of
 // rows over the same keys, so that every key and value that arrives is used for 256 rows; with few rows they are one tile of rows over every other
 // block of keys, and meet at the end.
@@ -36,14 +35,12 @@ template <typename T, int HD> struct Cfg {
   static constexpr int TILE = QS * 128 * 128;           // bytes of 128 rows
   static constexpr int NS = HD > 64 ? 5 : 8;            // tiles of the ring
   static constexpr int SMEM = 2 * TILE + NS * TILE + THERE * 16 + 256 + 1024;
-  static constexpr bool BESIDE = HD <= 64;              // the weights have TMEM of their own: a block's scores are multiplied while the last one's are weighed
-  static constexpr int T_O = 256, O_COLS = BESIDE ? 64 : 128, T_P = BESIDE ? 384 : 0, P_COLS = BESIDE ? 64 : 128;
   static constexpr uint32_t FMT = std::is_same<T, bf16>::value ? 1u : 0u;
   static constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(BK >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr uint32_t IDESC_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr float BIAS = FMT ? 0.f : 12.f, GROW = FMT ? 8.f : 3.f;
 };
-constexpr int T_COLS = 512;  // of TMEM: two score tiles, two outputs (and weights)
+constexpr int T_O = 256, T_COLS = 512;  // TMEM: two score tiles (the weights lie over their first halves), two outputs
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {  // zeros where !take
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -175,7 +172,7 @@ struct Maps {
 
 // Barriers of a CTA, 8 bytes each.
 struct Bars {
-  uint32_t q_full, q_empty, landed, s_full, s_read, half_p, p_full, p_read, o_full, full, empty;  // s_full .. o_full: of both score tiles
+  uint32_t q_full, q_empty, landed, s_full, half_p, p_full, o_full, full, empty;  // s_full .. o_full: of both score tiles
 };
 
 template <typename T, int HD>
@@ -193,7 +190,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
   const uint32_t raw = smem_u32(smem_raw), sQ = (raw + 1023u) & ~1023u, ring = sQ + 2 * TILE;
   uint32_t* const there = reinterpret_cast<uint32_t*>(smem_raw + (ring + NS * TILE - raw));  // [THERE][4]
   const uint32_t bars = ring + NS * TILE + THERE * 16;
-  const Bars B{bars, bars + 8, bars + 16, bars + 24, bars + 40, bars + 56, bars + 72, bars + 88, bars + 104, bars + 120, bars + 120 + 8 * NS};
+  const Bars B{bars, bars + 8, bars + 16, bars + 24, bars + 40, bars + 56, bars + 72, bars + 88, bars + 88 + 8 * NS};
   const uint32_t tmem_slot = B.empty + 8 * NS;
   uint32_t* const tmem_slot_ptr = reinterpret_cast<uint32_t*>(smem_raw + (tmem_slot - raw));
   const int warp = __shfl_sync(L3_FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -203,8 +200,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
     mbar_init(B.q_empty, 1);
     mbar_init(B.landed, 1);
     for (int w = 0; w < 2; ++w) {
-      mbar_init(B.s_full + 8 * w, 1); mbar_init(B.s_read + 8 * w, 4); mbar_init(B.half_p + 8 * w, 4); mbar_init(B.p_full + 8 * w, 4);
-      mbar_init(B.p_read + 8 * w, 1); mbar_init(B.o_full + 8 * w, 1);
+      mbar_init(B.s_full + 8 * w, 1); mbar_init(B.half_p + 8 * w, 4); mbar_init(B.p_full + 8 * w, 4); mbar_init(B.o_full + 8 * w, 1);
     }
     for (int s = 0; s < NS; ++s) { mbar_init(B.full + 8 * s, tma_kv ? 1 : LOADERS); mbar_init(B.empty + 8 * s, 1); }
     failed = 0;
@@ -229,7 +225,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
 
   if (warp == 8) {  // ------------------------------------------------------------------------------------------- products
     int slot = 0;
-    uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0}, s_phase[2] = {1, 1};
+    uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0};
     auto arrived = [&]() {  // the ring's next tile
       mbar_wait(B.full + 8 * slot, phase, fail);
       tc_fence_after();
@@ -239,11 +235,6 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
     };
     auto scores = [&](int w, int q_tile, int s) {
       const uint32_t q = desc_lo(sQ + q_tile * TILE, DESC_K), k = desc_lo(ring + s * TILE, DESC_K);
-      if constexpr (C::BESIDE) {  // else that the weights are there says so
-        mbar_wait(B.s_read + 8 * w, s_phase[w], fail);
-        s_phase[w] ^= 1;
-        tc_fence_after();
-      }
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {  // 32 bytes of a row, 16384 from slice to slice
@@ -263,8 +254,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         if (elect_one()) {
 #pragma unroll
           for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-            mma_ts(tmem + C::T_O + w * C::O_COLS, tmem + C::T_P + w * C::P_COLS + kk * 8, v + kk * 128, C::IDESC_PV, !first || kk > 0);
-          if (C::BESIDE && h) tc_commit(B.p_read + 8 * w);
+            mma_ts(tmem + T_O + w * 128, tmem + w * BK + kk * 8, v + kk * 128, C::IDESC_PV, !first || kk > 0);
         }
         __syncwarp();
       }
@@ -288,33 +278,16 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         if (n == 1) commit(B.q_empty);
         for (int j = 0; j < n; ++j) {
           const bool more = j + 1 < n;
-          if constexpr (C::BESIDE) {
-            if (more) {
-              k = arrived();
-              scores(0, 0, k);
-              scores(1, 1, k);
-              commit(B.empty + 8 * k);
-            }
-            const int v = arrived();
-            weighted(0, v, j == 0);
-            weighted(1, v, j == 0);
-            commit(B.empty + 8 * v);
-            if (!more) {
-              commit(B.o_full);
-              commit(B.o_full + 8);
-            }
-          } else {
-            const int v = arrived();
-            k = more ? arrived() : 0;
+          const int v = arrived();
+          k = more ? arrived() : 0;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              weighted(w, v, j == 0);
-              if (more) scores(w, w, k);
-              else commit(B.o_full + 8 * w);
-            }
-            commit(B.empty + 8 * v);
-            if (more) commit(B.empty + 8 * k);
+          for (int w = 0; w < 2; ++w) {
+            weighted(w, v, j == 0);
+            if (more) scores(w, w, k);
+            else commit(B.o_full + 8 * w);
           }
+          commit(B.empty + 8 * v);
+          if (more) commit(B.empty + 8 * k);
           if (j + 2 == n) commit(B.q_empty);
         }
       } else {
@@ -325,20 +298,15 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         }
         if (n <= 2) commit(B.q_empty);
         for (int i = 0; i < n; ++i) {
-          const int w = i & 1;
-          auto more = [&]() {
-            if (i + 2 >= n) return;
+          const int w = i & 1, v = arrived();
+          weighted(w, v, i < 2);
+          commit(B.empty + 8 * v);
+          if (i + 2 < n) {
             const int k = arrived();
             scores(w, 0, k);
             commit(B.empty + 8 * k);
             if (i + 3 == n) commit(B.q_empty);
-          };
-          if constexpr (C::BESIDE) more();
-          const int v = arrived();
-          weighted(w, v, i < 2);
-          commit(B.empty + 8 * v);
-          if constexpr (!C::BESIDE) more();
-          if (i + 2 >= n) commit(B.o_full + 8 * w);
+          } else commit(B.o_full + 8 * w);
         }
       }
     } while (c.next(a, SPLIT));
@@ -394,7 +362,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       const int most = c.r.seen((min(flats, flat0 + a.tile_rows) - 1) / a.R);
       const int* table = a.table + c.b * a.table_stride;
       const bool two = two_tiles();
-      const int ahead = (two ? 1 : 2) + (C::BESIDE ? 1 : 0);  // blocks of keys that are multiplied ahead of the first one's values
+      const int ahead = two ? 1 : 2;  // blocks of keys that are multiplied ahead of the first one's values
       auto queries = [&]() {  // behind the first keys: they need not wait for the products of the item before
         if (tma_q) {
           if (first_loader) {
@@ -473,9 +441,9 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           }
           if (++slot == NS) { slot = 0; phase ^= 1; }
         };
-        int next = page_of(c.j0), had = next, had1 = next, had2 = next;  // had ..: of the blocks whose values come next
+        int next = page_of(c.j0), had = next, had1 = next;  // had ..: of the blocks whose values come next
         for (int x = 0; x < min(ahead, n); ++x) {
-          (x == 0 ? had : x == 1 ? had1 : had2) = next;
+          (x ? had1 : had) = next;
           const int page = next;
           next = page_of(c.j0 + x + 1);
           fill(page, c.j0 + x, true);
@@ -484,9 +452,8 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         for (int i = 0; i < n; ++i) {
           fill(had, c.j0 + i, false);
           had = had1;
-          had1 = had2;
           if (i + ahead < n) {
-            (ahead == 1 ? had : ahead == 2 ? had1 : had2) = next;
+            (two ? had : had1) = next;
             const int page = next;
             next = page_of(c.j0 + i + ahead + 1);
             fill(page, c.j0 + i + ahead, true);
@@ -519,9 +486,9 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         filled(B.full + 8 * slot);
         if (++slot == NS) { slot = 0; phase ^= 1; }
       };
-      Pages next = pages_of(c.j0), had = next, had1 = next, had2 = next;
+      Pages next = pages_of(c.j0), had = next, had1 = next;
       for (int x = 0; x < min(ahead, n); ++x) {
-        (x == 0 ? had : x == 1 ? had1 : had2) = next;
+        (x ? had1 : had) = next;
         const Pages page = next;
         next = pages_of(c.j0 + x + 1);
         fill(a.k, page, c.j0 + x, true);
@@ -530,9 +497,8 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
       for (int i = 0; i < n; ++i) {
         fill(a.v, had, c.j0 + i, false);
         had = had1;
-        had1 = had2;
         if (i + ahead < n) {
-          (ahead == 1 ? had : ahead == 2 ? had1 : had2) = next;
+          (two ? had : had1) = next;
           const Pages page = next;
           next = pages_of(c.j0 + i + ahead + 1);
           fill(a.k, page, c.j0 + i + ahead, true);
@@ -544,12 +510,12 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
     clear_rest<T>(a, lane, 32);
   } else if (warp < 8) {  // ---------------------------------------------------------------------------------------- softmax
     const int quarter = warp & 3, w = warp >> 2, r = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + w * BK + lanes, tO = tmem + C::T_O + lanes, tP = tmem + C::T_P + w * C::P_COLS + lanes;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + w * BK + lanes, tO = tmem + T_O + lanes;
     // log2(e) |scale|: a weight is 2^(s sc - m sc); of 0 the smallest number, so that a score of -infinity keeps its weight of 0
     const float sc = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f), growth = fminf(C::GROW / sc, 3e38f);
     const bool negative = a.scale < 0.f;
     int blocks_so_far = 0;
-    uint32_t s_phase = 0, o_phase[2] = {0, 0}, p_phase = 1;
+    uint32_t s_phase = 0, o_phase[2] = {0, 0};
     if (c.start(a, SPLIT, place)) do {
       const int n = c.j1 - c.j0;
       const bool two = two_tiles();
@@ -565,11 +531,6 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
 #pragma unroll
         for (int i = 0; i < BK; i += 32) tmem_ld32(tS + i, v + i);
         tmem_ld_wait();
-        if constexpr (C::BESIDE) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(B.s_read + 8 * w);
-        }
         const int visible = seen - (c.j0 + j) * BK;
         const uint4 bits = *reinterpret_cast<const uint4*>(there + ((blocks_so_far + j) & (THERE - 1)) * 4);
         if (negative) {
@@ -595,27 +556,21 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           for (int x = 0; x < 4; ++x) top[x] = max_nan(top[x], v[i + x]);
         float mx = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
         if (mx == INFINITY) mx = NAN;  // as the definition has it: infinity less infinity
-        bool p_free = !C::BESIDE;
         if (!begun) m = mx;
         else {
           const bool grow = !(mx <= m + growth);
           if (__any_sync(L3_FULL, grow)) {
-            // the output rests once the products of the block before have ended (which they have where its weights lay over these scores)
-            if constexpr (C::BESIDE) {
-              mbar_wait(B.p_read + 8 * w, p_phase, fail);
-              tc_fence_after();
-              p_free = true;
-            }
+            // the scores of this block are there: the products of every block before have ended, and the output rests
             const float alpha = grow ? ex2((m - mx) * sc) : 1.f;
             if (grow) { m = mx; l *= alpha; }
 #pragma unroll 1
             for (int d = 0; d < HD; d += 16) {
               float o[16];
-              tmem_ld16(tO + w * C::O_COLS + d, o);
+              tmem_ld16(tO + w * 128 + d, o);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] *= alpha;
-              tmem_st16(tO + w * C::O_COLS + d, o);
+              tmem_st16(tO + w * 128 + d, o);
             }
           }
         }
@@ -633,19 +588,12 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
             sum[i / 2 & 1] = add2(sum[i / 2 & 1], e);
             p[i / 2] = pack<T>(e.x, e.y);
           }
-          if constexpr (C::BESIDE) {
-            if (!h && !p_free) {
-              mbar_wait(B.p_read + 8 * w, p_phase, fail);
-              tc_fence_after();
-            }
-          }
-          tmem_st32(tP + 32 * h, p);
+          tmem_st32(tS + 32 * h, p);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive((h ? B.p_full : B.half_p) + 8 * w);
         }
-        p_phase ^= 1;
         sum[0] = add2(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
@@ -695,7 +643,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
         for (int d = 0; d < HD; d += 16) {
           float o[16];
           if (n) {
-            tmem_ld16(tO + w * C::O_COLS + d, o);
+            tmem_ld16(tO + w * 128 + d, o);
             tmem_ld_wait();
           } else {
 #pragma unroll
@@ -728,7 +676,7 @@ __global__ void __launch_bounds__(NT, 1) chunk_tc_kernel(const ChunkArgs a, cons
           float o[8], o1[8];
           if (n) {
             tmem_ld8(tO + d, o);
-            tmem_ld8(tO + C::O_COLS + d, o1);
+            tmem_ld8(tO + 128 + d, o1);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = n > 1 ? o[i] * share + o1[i] * share1 : o[i] * share;

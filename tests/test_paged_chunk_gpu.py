@@ -140,6 +140,22 @@ def test_split_and_joined(kind, dim, requests):
     args = make(len(requests), TYPES[kind], 4, 2, dim, 16, requests)
     got = check(*args)
     assert torch.equal(got, paged_chunk_attention(*args)), "results change from run to run"
+    out = check(*args, out=torch.empty_like(got))     # few rows go another way where the result is made by the call
+    assert torch.equal(out, paged_chunk_attention(*args, out=torch.empty_like(got)))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim,heads,kv_heads", [(16, 4, 4), (48, 6, 2), (128, 32, 8)])
+@pytest.mark.parametrize("requests", [[(1500, 5)], [(0, 1)], [(0, 0), (7, 2), (0, 0), (300, 1), (0, 3), (40, 0)], [(3, 1)] * 16, [(100, 0)] * 50 + [(90, 9)] + [(1, 0)] * 50])
+@pytest.mark.parametrize("rest", [0, 4])
+def test_few_rows(kind, dim, heads, kv_heads, requests, rest):
+    args = make(len(requests), TYPES[kind], heads, kv_heads, dim, 16, requests, garbage=math.nan, rest=rest)
+    got, n = check(*args), int(args[-1][-1])
+    assert not got[n:].any()
+    out = torch.full_like(got, 7.0)
+    paged_chunk_attention(*args, out=out)
+    assert bool((out[n:] == 7).all())
+    near(out[:n], paged_chunk_attention(*args, return_lse=True)[1][:n], [x[:n] for x in formula(*args)])
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
