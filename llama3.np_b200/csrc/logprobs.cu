@@ -3,10 +3,10 @@
 // (both terms of H are 0 or more: no difference of near equals where one token has nearly all).
 //
 // Bound by the logits, read once.  A row is a CTA's, or of few rows a cluster's, whose CTAs meet over shared memory.  A thread streams
-// 16-byte pieces with a running maximum and sums of its own.  The n most likely: the n-th largest of the threads' maxima - found bit by bit, a
-// count over the CTA a time - bounds the n-th largest logit from below, so only the few threads whose maximum passes it look at their logits
+// 16-byte pieces with a running maximum and sums of its own.  The n most likely: the threads' maxima
+// bound the n-th largest logit from below, so only the few threads whose maximum passes the bound look at their logits
 // again (a warp together at one thread's, 32 pieces at a time), and what passes is ranked by counting.  Where more values pass than there is room
-// for (many equal ones), the n are drawn one after the other.
+// for, a better bound is found; where that does not help (many equal ones), the n are drawn one after the other.
 #include <float.h>
 #include <math.h>
 
@@ -42,6 +42,16 @@ template <typename T> struct Piece {  // 16 bytes of a row
   uint4 w;
   __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ void again(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ float most() const {  // 16-bit values two at a time; NaN is none
+    if constexpr (N == 4) return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    else {
+      using T2 = typename std::conditional<std::is_same<T, bf16>::value, __nv_bfloat162, __half2>::type;
+      const T2 *a = reinterpret_cast<const T2*>(&w.x), *b = reinterpret_cast<const T2*>(&w.y), *c = reinterpret_cast<const T2*>(&w.z),
+               *d = reinterpret_cast<const T2*>(&w.w);
+      const T2 m = __hmax2(__hmax2(*a, *b), __hmax2(*c, *d));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
   __device__ __forceinline__ void values(float (&x)[N]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -58,46 +68,85 @@ template <typename T> struct Piece {  // 16 bytes of a row
     }
   }
 };
-struct Sums { float m, s, t; };  // largest logit, sum e^(x - m), sum (x - m) e^(x - m)
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-  const float m = fmaxf(a.m, b.m), from = m == -INFINITY ? 0.f : m;
-  const float da = a.m == -INFINITY ? 0.f : a.m - from, db = b.m == -INFINITY ? 0.f : b.m - from;
-  const float fa = ex2(da * 1.4426950408889634f), fb = ex2(db * 1.4426950408889634f);
+struct Sums { float m, s, t; };  // a logit, sum e^(x - m), sum (x - m) e^(x - m)
+// sums against another logit, none of the row's beyond it by much
+__device__ __forceinline__ Sums moved(const Sums& a, float m) {
+  const float from = m == -INFINITY ? 0.f : m, d = a.m == -INFINITY ? 0.f : a.m - from, f = ex2(d * 1.4426950408889634f);
   // a side at -infinity has sums 0, or NaN of a NaN; one too far down for its factor may have s d = -infinity
-  return Sums{m, a.s * fa + b.s * fb, (fa > 0.f ? (a.t + a.s * da) * fa : 0.f) + (fb > 0.f ? (b.t + b.s * db) * fb : 0.f)};
+  return Sums{m, a.s * f, f > 0.f ? (a.t + a.s * d) * f : 0.f};
 }
-template <bool ENTROPY, int N> __device__ __forceinline__ void take(Sums& a, const float (&x)[N]) {
-  float top = x[0];
+// of the N neighbouring lanes (the least of them the whole one's)
+template <int N> __device__ __forceinline__ Sums joined(Sums a) {
+  const uint32_t key = __reduce_max_sync(L3_FULL, order_key(a.m));
+  a = moved(a, key > NO_KEY ? key_value(key) : -INFINITY);
 #pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-  if (top > a.m) {
+  for (int o = N / 2; o; o >>= 1) {
+    a.s += __shfl_xor_sync(L3_FULL, a.s, o);
+    a.t += __shfl_xor_sync(L3_FULL, a.t, o);
+  }
+  return a;
+}
+// how many of the n entries at `list` (shared memory, 16-byte aligned, one of 0 behind an odd number) are larger
+__device__ __forceinline__ int larger(const unsigned long long* list, int n, unsigned long long me) {
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; j += 2) {
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list + j);
+    rank += (x.x > me) + (x.y > me);
+  }
+  return rank;
+}
+__device__ __forceinline__ float2 pair(float x, float y) { return make_float2(x, y); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d) : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
+  return *reinterpret_cast<const float2*>(&d);
+}
+// More values, the largest of them `top`.  m follows the largest lazily, when that is e^8 times beyond it: some lane of a warp has a new largest
+// value in nearly every piece, and would move its sums each time.
+template <bool ENTROPY, int N> __device__ __forceinline__ void take(Sums& a, const float (&x)[N], float top) {
+  if (top > a.m + 8.f) {
     const float d = a.m == -INFINITY ? 0.f : a.m - top, f = ex2(d * 1.4426950408889634f);
     if (ENTROPY) a.t = f > 0.f ? (a.t + a.s * d) * f : 0.f;
     a.s *= f;
     a.m = top;
   }
   const float from = a.m == -INFINITY ? 0.f : a.m;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    // the difference first and by itself: a logit's own multiple of log2 e would be off by more than the difference's
-    const float d = x[i] - from, e = ex2(d * 1.4426950408889634f);
+  // the difference first and by itself: a logit's own multiple of log2 e would be off by more than the difference's
+  if constexpr (N == 1) {
+    const float d = x[0] - from, e = ex2(d * 1.4426950408889634f);
     a.s += e;
     if (ENTROPY) a.t += e * fmaxf(d, -FLT_MAX);  // 0 for a logit of -infinity
+  } else {
+    const float2 one = pair(1.f, 1.f), down = pair(-from, -from), log2e = pair(1.4426950408889634f, 1.4426950408889634f);
+    float2 s = pair(0.f, 0.f), t = pair(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 d = fma2(pair(x[i], x[i + 1]), one, down), y = mul2(d, log2e), e = pair(ex2(y.x), ex2(y.y));
+      s = fma2(e, one, s);
+      if (ENTROPY) t = fma2(e, pair(fmaxf(d.x, -FLT_MAX), fmaxf(d.y, -FLT_MAX)), t);
+    }
+    a.s += s.x + s.y;
+    if (ENTROPY) a.t += t.x + t.y;
   }
 }
 
 // A cluster of S CTAs (gridDim.x = S) has a row; its CTA c the pieces c, c + S, ... of LT threads' pieces each.
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(LT, TOP ? 2 : 3) logprobs_kernel(const LogprobsArgs a) {
+__global__ void __launch_bounds__(LT, 2) logprobs_kernel(const LogprobsArgs a) {
   constexpr int N = Piece<T>::N;
   __shared__ Sums parts[LW];
-  __shared__ Sums cta_sums;
-  __shared__ unsigned long long hits[TOP ? ROOM : 1], best[TOP ? LOGPROBS_MAX_TOP : 1];
+  __shared__ Sums gathered[8];  // of the cluster's CTAs, in the first one's; its own ones in the others'
+  __shared__ __align__(16) unsigned long long hits[TOP ? ROOM : 1], best[TOP ? 8 * LOGPROBS_MAX_TOP : 1], chosen[TOP ? LOGPROBS_MAX_TOP : 1];  // best: likewise
   __shared__ int count;
   __shared__ unsigned long long draw[LW];
+  __shared__ uint32_t kths[LW];
+  const int S = gridDim.x;
+  if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // has begun
   pdl_launch();
   pdl_wait();
-  const int S = gridDim.x, c = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int  c = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* x0 = (const T*)a.logits + row * a.stride;
   const int token = a.tokens[row];
   // logits ahead of the first whole piece, pieces, logits behind the last; those at the ends are the first threads' of CTA 0
@@ -106,52 +155,66 @@ __global__ void __launch_bounds__(LT, TOP ? 2 : 3) logprobs_kernel(const Logprob
   const int ends = c == 0 && (int)threadIdx.x < ahead + behind ? (int)threadIdx.x + ((int)threadIdx.x < ahead ? 0 : pieces * N) : -1;
   Sums my{-INFINITY, 0.f, 0.f};
   const int first = c * LT + threadIdx.x, step = S * LT;
+  float most = -INFINITY;  // of this thread
   {
     constexpr int AHEAD = 4;
+    const int mine = first < pieces ? (pieces - first + step - 1) / step : 0;  // pieces of this thread
+    const T* at = xp + (size_t)first * N;
+    const size_t apart = (size_t)step * N;
     Piece<T> p[AHEAD];
+    auto use = [&](Piece<T>& q, const T* next) {  // and ask for another
+      float x[N];
+      q.values(x);
+      const float top = q.most();
+      if (next) q.load(next);
+      if (TOP) most = fmaxf(most, top);
+      take<ENTROPY>(my, x, top);
+    };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
-      if (first + i * step < pieces) p[i].load(xp + (size_t)(first + i * step) * N);
-    for (int at = first; at < pieces; at += AHEAD * step) {
+      if (i < mine) p[i].load(at + i * apart);
+    int k = 0;
+    for (; k + 2 * AHEAD <= mine; k += AHEAD) {
+      at += AHEAD * apart;
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        if (at + i * step < pieces) {
-          float x[N];
-          p[i].values(x);
-          if (at + (i + AHEAD) * step < pieces) p[i].load(xp + (size_t)(at + (i + AHEAD) * step) * N);
-          take<ENTROPY>(my, x);
-        }
-      }
+      for (int i = 0; i < AHEAD; ++i) use(p[i], at + i * apart);
     }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (k + i < mine) use(p[i], k + AHEAD + i < mine ? at + (AHEAD + i) * apart : nullptr);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (k + AHEAD + i < mine) use(p[i], nullptr);
     if (ends >= 0) {
       const float x[1] = {value(x0 + ends)};
-      take<ENTROPY>(my, x);
+      most = fmaxf(most, x[0]);
+      take<ENTROPY>(my, x, fmaxf(x[0], -INFINITY));
     }
   }
-  const float most = my.m;  // of this thread
-#pragma unroll
-  for (int o = 16; o; o >>= 1)
-    my = joined(my, Sums{__shfl_xor_sync(L3_FULL, my.m, o), __shfl_xor_sync(L3_FULL, my.s, o), __shfl_xor_sync(L3_FULL, my.t, o)});
+  my = joined<32>(my);
   if (lane == 0) parts[warp] = my;
   if (threadIdx.x == 0) count = 0;
   __syncthreads();
   if (warp == 0) {
-    my = parts[lane & (LW - 1)];
-#pragma unroll
-    for (int o = LW / 2; o; o >>= 1)
-      my = joined(my, Sums{__shfl_xor_sync(L3_FULL, my.m, o), __shfl_xor_sync(L3_FULL, my.s, o), __shfl_xor_sync(L3_FULL, my.t, o)});
-    if (lane == 0) cta_sums = my;
+    my = joined<LW>(parts[lane & (LW - 1)]);
+    if (lane == 0) gathered[0] = my;
   }
   if constexpr (TOP) {
     const int n = a.n;
-    // the largest key that at least n threads' maxima reach (of the first 20 bits: it is a bound only); none: every finite logit passes
     const uint32_t mine = order_key(most);
-    uint32_t bound = 0;
-    for (int bit = 31; bit >= 12; --bit) {
-      const uint32_t with = bound | 1u << bit;
-      if (__syncthreads_count(most > -INFINITY && mine >= with) >= n) bound = with;
+    // n values reach the least of the warps' k-th largest maxima, k = n over the warps
+    uint32_t bound = most > -INFINITY ? mine : 0;
+    {
+      uint32_t left = bound, kth = 0;
+      for (int k = 0; k < (n + LW - 1) / LW; ++k) {
+        kth = __reduce_max_sync(L3_FULL, left);
+        if (__ffs(__ballot_sync(L3_FULL, left == kth)) - 1 == lane) left = 0;
+      }
+      if (lane == 0) kths[warp] = kth;
     }
-    bound = max(bound, NO_KEY + 1);
+    __syncthreads();
+    bound = kths[lane & (LW - 1)];
+    bound = max(__reduce_min_sync(L3_FULL, bound), NO_KEY + 1);  // where a warp has too few, every finite logit passes
     auto offer = [&](float x, int v) {
       const uint32_t key = order_key(x);
       if (x > -INFINITY && key >= bound) {  // NaN is none
@@ -159,27 +222,60 @@ __global__ void __launch_bounds__(LT, TOP ? 2 : 3) logprobs_kernel(const Logprob
         if (at < ROOM) hits[at] = entry(key, v);
       }
     };
-    for (uint32_t who = __ballot_sync(L3_FULL, most > -INFINITY && mine >= bound); who; who &= who - 1) {
-      const int of = __ffs(who) - 1, its_first = c * LT + warp * 32 + of, its_ends = __shfl_sync(L3_FULL, ends, of);
-      for (int at = its_first + lane * step; at < pieces; at += 32 * step) {
-        Piece<T> p;
-        p.again(xp + (size_t)at * N);
-        float x[N];
-        p.values(x);
+    const int most_pieces = (pieces + step - 1) / step;  // of a thread
+    auto collect = [&]() {
+      uint32_t who = __ballot_sync(L3_FULL, most > -INFINITY && mine >= bound);
+      while (who) {
+        constexpr int TOGETHER = 4;  // threads whose pieces are on their way at once
+        int of[TOGETHER];
 #pragma unroll
-        for (int e = 0; e < N; ++e) offer(x[e], ahead + at * N + e);
+        for (int i = 0; i < TOGETHER; ++i) {
+          of[i] = who ? __ffs(who) - 1 : -1;
+          who &= who - 1;
+        }
+        for (int at = lane; at < most_pieces; at += 32) {
+          Piece<T> p[TOGETHER];
+#pragma unroll
+          for (int i = 0; i < TOGETHER; ++i) {
+            const int piece = c * LT + warp * 32 + of[i] + at * step;
+            if (of[i] >= 0 && piece < pieces) p[i].again(xp + (size_t)piece * N);
+          }
+#pragma unroll
+          for (int i = 0; i < TOGETHER; ++i) {
+            const int piece = c * LT + warp * 32 + of[i] + at * step;
+            if (of[i] < 0 || piece >= pieces) continue;
+            float x[N];
+            p[i].values(x);
+            if (order_key(p[i].most()) < bound) continue;
+#pragma unroll
+            for (int e = 0; e < N; ++e) offer(x[e], ahead + piece * N + e);
+          }
+        }
       }
-      if (lane == 0 && its_ends >= 0) offer(value(x0 + its_ends), its_ends);
+      if (ends >= 0) offer(value(x0 + ends), ends);
+    };
+    collect();
+    __syncthreads();
+    if (count > ROOM) {  // the best bound that the threads' maxima give: the largest key that n of them reach (its first 20 bits)
+      __syncthreads();
+      if (threadIdx.x == 0) count = 0;
+      bound = 0;
+      for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t with = bound | 1u << bit;
+        if (__syncthreads_count(most > -INFINITY && mine >= with) >= n) bound = with;
+      }
+      bound = max(bound, NO_KEY + 1);
+      collect();
     }
     __syncthreads();
     const int found = count;
     if (found <= ROOM) {
       for (int i = threadIdx.x; i < n; i += LT) best[i] = 0;
+      if (threadIdx.x == 0 && found < ROOM) hits[found] = 0;
       __syncthreads();
       for (int i = threadIdx.x; i < found; i += LT) {
         const unsigned long long me = hits[i];
-        int rank = 0;
-        for (int j = 0; j < found; ++j) rank += hits[j] > me;
+        const int rank = larger(hits, found, me);
         if (rank < n) best[rank] = me;
       }
     } else {
@@ -214,43 +310,44 @@ __global__ void __launch_bounds__(LT, TOP ? 2 : 3) logprobs_kernel(const Logprob
       }
     }
   }
-  // the cluster's CTAs meet in the first one
-  Sums all;
-  if (S > 1) {
-    cluster_sync_all();
-    if (c == 0) {
-      all = cta_sums;
-      for (int o = 1; o < S; ++o) {
-        const uint32_t at = cluster_at((uint32_t)__cvta_generic_to_shared(&cta_sums), o);
-        Sums other;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.m) : "r"(at) : "memory");
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.s) : "r"(at + 4) : "memory");
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.t) : "r"(at + 8) : "memory");
-        all = joined(all, other);
+  __syncthreads();
+  Sums all = gathered[0];
+  if (S > 1) {  // the others hand theirs to the first CTA, and are done
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (c) {
+      if (threadIdx.x == 0) {
+        const uint32_t to = cluster_at((uint32_t)__cvta_generic_to_shared(&gathered[c]), 0);
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(all.m) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(all.s) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(all.t) : "memory");
       }
       if constexpr (TOP) {
-        for (int i = threadIdx.x; i < S * a.n; i += LT) {
-          const uint32_t at = cluster_at((uint32_t)__cvta_generic_to_shared(&best[i % a.n]), i / a.n);
-          asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(hits[i]) : "r"(at) : "memory");
-        }
+        if ((int)threadIdx.x < a.n)
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_at((uint32_t)__cvta_generic_to_shared(&best[c * a.n + threadIdx.x]), 0)), "l"(best[threadIdx.x]) : "memory");
       }
+      __syncwarp();
     }
-    cluster_sync_all();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     if (c) return;
-    if constexpr (TOP) {
-      for (int i = threadIdx.x; i < a.n; i += LT) best[i] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < S * a.n; i += LT) {
-        const unsigned long long me = hits[i];
-        int rank = 0;
-        for (int j = 0; j < S * a.n; ++j) rank += hits[j] > me;
-        if (me && rank < a.n) best[rank] = me;
-      }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int o = 1; o < S; ++o) {
+      const float top = fmaxf(all.m, gathered[o].m);
+      const Sums other = moved(gathered[o], top);
+      all = moved(all, top);
+      all.s += other.s;
+      all.t += other.t;
     }
-    __syncthreads();
-  } else {
-    __syncthreads();
-    all = cta_sums;
+    if constexpr (TOP) {
+      const int each = S * a.n;  // an even number
+      for (int i = threadIdx.x; i < a.n; i += LT) chosen[i] = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < each; i += LT) {
+        const unsigned long long me = best[i];
+        const int rank = larger(best, each, me);
+        if (me && rank < a.n) chosen[rank] = me;
+      }
+      __syncthreads();
+    }
   }
   const float log_s = logf(all.s);
   const bool none = all.m == -INFINITY && !(all.s != all.s);  // no token has a probability
@@ -263,7 +360,7 @@ __global__ void __launch_bounds__(LT, TOP ? 2 : 3) logprobs_kernel(const Logprob
   }
   if constexpr (TOP) {
     for (int i = threadIdx.x; i < a.n; i += LT) {
-      const unsigned long long e = best[i];
+      const unsigned long long e = (S > 1 ? chosen : best)[i];
       a.out_top[(size_t)row * a.n + i] = e ? key_value((uint32_t)(e >> 32)) - all.m - log_s : -INFINITY;
       a.out_top_tokens[(size_t)row * a.n + i] = e ? (int)(0xffffffffu - (uint32_t)e) : -1;
     }
