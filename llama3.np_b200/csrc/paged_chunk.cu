@@ -2,11 +2,16 @@
 //   s_j = scale q_t . k_j,  o_t = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  lse_t = m + log sum_j e^(s_j - m),  m = max_j s_j
 // over the tokens j that row t sees, j <= its position.  paged_chunk.cuh says how the work is cut.
 //
-// This file: fp32 caches, the products as FFMA; and the join of what several CTAs have of an item.
-// A CTA's 256 threads hold 64 rows and walk their keys, 64 at a time.  Keys and values come row by row through the page table, 16 bytes a
-// copy, while the tile before is worked on; rows of no token become zeros.
-//   scores   a thread has 4 rows x 4 keys, summed as even and odd entries (pairs: fma2); rows padded to an odd number of 16-byte pieces
-//   output   a thread has 4 rows x HD / 16 columns, in pairs of rows; the weights arrive through shared memory, [key][row]
+// This file: fp32 caches; and the join of what several CTAs have of an item.  Products as three of TF32 numbers on the tensor cores (mma.sync): a number is
+// the nearest one of 11 bits and what that leaves, cut to 11 bits, and x y = xh yh + xh yl + xl yh is off by at most 2^-20 of it - where numbers'
+// second parts are not below fp32's normal ones, from 2^-115 on.  (With FFMA what shared memory delivers bounded the kernel, 3200 wavefronts a tile of
+// 64 x 64 with heads of 48 in place of 800: 64 prompts of up to 220 tokens, 6 heads of 48, 88 us, now 62.)
+// A CTA's four warps hold 16 rows each and walk their keys, 64 at a time.  Keys and values come row by row through the page table, 16 bytes a
+// copy, while the tile before is worked on; rows of no token become zeros.  Rows of tiles are padded to an odd number of 16-byte pieces: eight rows'
+// pieces (scores, ldmatrix), and eight columns of four rows two apart (output), lie on different banks.  The weights stay in registers: the lane that has
+// row g's keys 2 t and 2 t + 1 takes them for the product's t-th and t + 4-th, in whose place the values' rows are read.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "paged_chunk.cuh"
@@ -14,11 +19,12 @@
 
 namespace {
 using namespace chunk;
-constexpr int TR = 64, BK = 64, NT = 256;
-__host__ __device__ constexpr Split fma_split() { return Split{BK, 4, 8, TR, 3}; }
-constexpr int ctas_of_sm(int HD) { return HD > 64 ? 1 : HD > 48 ? 2 : 3; }  // as shared memory has room for
+constexpr int TR = 64, BK = 64, NT = 128;
+__host__ __device__ constexpr Split f32_split() { return Split{BK, 1, 4, TR, 2}; }
+// as registers and shared memory have room for; of heads of 48, where there is room for four, three: 61.9 : 62.9 us
+constexpr int ctas_of_sm(int HD) { return HD > 64 ? 2 : 3; }
 template <int HD> constexpr int row_ld() { return HD + 4; }
-template <int HD> constexpr size_t smem_bytes() { return (size_t)(2 * 64 * row_ld<HD>() + 64 * HD + 64 * (TR + 4)) * 4 + 2 * 2 * BK * 8 + 2 * 8 + 16; }
+template <int HD> constexpr size_t smem_bytes() { return (size_t)3 * 64 * row_ld<HD>() * 4 + 2 * 2 * BK * 8 + 2 * 8; }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {  // zeros where !take
@@ -26,41 +32,59 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the nearest number of 11 bits, and what that leaves, cut to 11 bits
+__device__ __forceinline__ void two_parts(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  hi = (x + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) & 0xffffe000u;
+}
+__device__ __forceinline__ void mma_parts(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t b0, uint32_t b1) {
+  uint32_t h0, l0, h1, l1;
+  two_parts(b0, h0, l0);
+  two_parts(b1, h1, l1);
+  mma_tf32(c, al, h0, h1);
+  mma_tf32(c, ah, l0, l1);
+  mma_tf32(c, ah, h0, h1);
+}
 
 template <int HD>
-__global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_fma_kernel(const ChunkArgs a) {
-  using T = float;
-  constexpr Split SPLIT = fma_split();
-  constexpr int LD = row_ld<HD>(), PL = TR + 4;
-  constexpr int CW = HD % 64 == 0 ? 4 : HD % 32 == 0 ? 2 : 1, NC = HD / (16 * CW);  // columns side by side, and how often
+__global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const ChunkArgs a) {
+  constexpr Split SPLIT = f32_split();
+  constexpr int LD = row_ld<HD>(), KS = HD / 8;
   extern __shared__ __align__(16) float sm[];
   float* sQ = sm;                     // [64][LD]
   float* sK = sQ + 64 * LD;           // [64][LD]
-  float* sV = sK + 64 * LD;           // [64][HD]
-  float* sP = sV + 64 * HD;           // [keys][rows]
-  long long* sOff = reinterpret_cast<long long*>(sP + 64 * PL);  // [turn][k, v][64]
+  float* sV = sK + 64 * LD;           // [64][LD]
+  long long* sOff = reinterpret_cast<long long*>(sV + 64 * LD);  // [turn][k, v][64]
   unsigned* sThere = reinterpret_cast<unsigned*>(sOff + 2 * 2 * BK);  // [turn][2] bits of keys that there are
   __shared__ long long room[NT / 32 + 1];
   __shared__ Place place;
   pdl_launch();
   pdl_wait();
-  clear_rest<T>(a, threadIdx.x, NT);
+  clear_rest<float>(a, threadIdx.x, NT);
   find_share<BK, NT>(a, SPLIT, room, &place);
   if (threadIdx.x == 0) leave_nothing(a, place);
   __syncthreads();
-  const int lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
   const float sc = a.scale * 1.4426950408889634f;
   auto token_of = [&](int f) { return a.R == 1 ? f : f / a.R; };
   Cursor<BK> c;
   if (!c.start(a, SPLIT, place)) return;
   do {
     const int* table = a.table + c.b * a.table_stride;
-    const int flat0 = c.tile * TR, flats = c.r.n * a.R;
+    const int flat0 = c.tile * TR, flats = c.r.n * a.R, row0 = flat0 + warp * 16;
     const int most = c.r.seen(token_of(min(flats, flat0 + TR) - 1));   // keys that any of the rows sees
+    const bool busy = row0 < flats;                                    // the warp has rows
     for (int i = threadIdx.x; i < TR * (HD / 4); i += NT) {  // the rows' queries
       const int r = i / (HD / 4), p = i - r * (HD / 4), f = flat0 + r, t = token_of(f);
       const bool in = f < flats;
-      cp16(smem_u32(sQ + r * LD + p * 4), in ? (const T*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh + p * 4 : (const T*)a.q, in);
+      cp16(smem_u32(sQ + r * LD + p * 4), in ? (const float*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh + p * 4 : (const float*)a.q, in);
     }
     auto offsets = [&](int j) {  // by the first 64 threads
       if (threadIdx.x >= BK) return;
@@ -72,33 +96,31 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_fma_kernel(const Chu
       sOff[turn * 2 * BK + threadIdx.x] = there ? page * a.k.sp + c.g * a.k.sh + in * a.k.st : -1;
       sOff[turn * 2 * BK + BK + threadIdx.x] = there ? page * a.v.sp + c.g * a.v.sh + in * a.v.st : -1;
       const unsigned bits = __ballot_sync(L3_FULL, there);
-      if (lane == 0) sThere[turn * 2 + (threadIdx.x >> 5)] = bits;
+      if (lane == 0) sThere[turn * 2 + warp] = bits;
     };
     auto copy = [&](int j, bool value) {
       const long long* off = sOff + (j & 1) * 2 * BK + (value ? BK : 0);
-      const T* pool = (const T*)(value ? a.v.p : a.k.p);
+      const float* pool = (const float*)(value ? a.v.p : a.k.p);
       float* dst = value ? sV : sK;
-      const int ld = value ? HD : LD;
       constexpr int PIECES = HD / 4;
       for (int i = threadIdx.x; i < BK * PIECES; i += NT) {
         const int r = i / PIECES, p = i - r * PIECES;
         const long long at = off[r];
-        cp16(smem_u32(dst + r * ld + p * 4), at >= 0 ? pool + at + p * 4 : pool, at >= 0);
+        cp16(smem_u32(dst + r * LD + p * 4), at >= 0 ? pool + at + p * 4 : pool, at >= 0);
       }
       cp_commit();
     };
-    int seen[4];
+    int seen[2];
+    float o[KS][4], m[2], l[2];   // of rows g and g + 8: columns 8 n + 2 t4, + 1
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int f = flat0 + ty * 4 + i;
-      seen[i] = f < flats ? c.r.seen(token_of(f)) : 0;
+    for (int i = 0; i < 2; ++i) {
+      const int f = row0 + g + 8 * i;
+      seen[i] = f < flats ? c.r.seen(token_of(f)) : INT_MAX;  // a row behind the last: what it has goes nowhere
+      m[i] = -INFINITY;
+      l[i] = 0.f;
     }
-    float2 o[2][NC * CW];   // pairs of rows
-    float m[4], l[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
-#pragma unroll
-    for (int x = 0; x < NC * CW; ++x) o[0][x] = o[1][x] = make_float2(0.f, 0.f);
+    for (int n = 0; n < KS; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     if (c.j0 < c.j1) {
       offsets(c.j0);
       __syncthreads();
@@ -109,85 +131,83 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_fma_kernel(const Chu
       if (j + 1 < c.j1) offsets(j + 1);
       cp_wait<1>();
       __syncthreads();   // the keys are there, and the next ones' places
-      float2 s2[4][4];
+      float s[8][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s2[i][k] = make_float2(0.f, 0.f);
+      for (int n = 0; n < 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      if (busy) {
+        // ldmatrix of 8 rows of 4 numbers: lane i has row i / 4's number i % 4
+        const uint32_t qa = smem_u32(sQ + (warp * 16 + (lane & 15)) * LD + (lane >> 4) * 4);
+        const uint32_t ka = smem_u32(sK + ((lane >> 4) * 8 + (lane & 7)) * LD + (lane >> 3 & 1) * 4);
 #pragma unroll 2
-      for (int d = 0; d < HD; d += 4) {
-        float4 q[4], k[4];
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t q[4], qh[4], ql[4];
+          ldsm_x4(qa + ks * 32, q);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(sQ + (ty * 4 + i) * LD + d);
+          for (int i = 0; i < 4; ++i) two_parts(q[i], qh[i], ql[i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const float4*>(sK + (tx + 16 * i) * LD + d);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s2[i][x] = fma2(make_float2(q[i].x, q[i].y), make_float2(k[x].x, k[x].y), s2[i][x]);
-            s2[i][x] = fma2(make_float2(q[i].z, q[i].w), make_float2(k[x].z, k[x].w), s2[i][x]);
+          for (int n = 0; n < 8; n += 2) {
+            uint32_t k[4];
+            ldsm_x4(ka + n * 8 * LD * 4 + ks * 32, k);
+            mma_parts(s[n], qh, ql, k[0], k[1]);
+            mma_parts(s[n + 1], qh, ql, k[2], k[3]);
           }
+        }
       }
-      const unsigned there0 = sThere[(j & 1) * 2], there1 = sThere[(j & 1) * 2 + 1];
+      const unsigned there[2] = {sThere[(j & 1) * 2], sThere[(j & 1) * 2 + 1]};
       __syncthreads();   // all have read the keys
       if (j + 1 < c.j1) copy(j + 1, false);
       else cp_commit();
-      float p[4][4], alpha[4];
+      if (busy) {
+        const bool masked = __any_sync(L3_FULL, min(seen[0], seen[1]) - j * BK < BK) || (there[0] & there[1]) != L3_FULL;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float mx = -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+          float mx = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int key = tx + 16 * x;
-          const bool in = j * BK + key < seen[i] && ((x < 2 ? there0 : there1) >> (key & 31) & 1);
-          p[i][x] = in ? (s2[i][x].x + s2[i][x].y) * sc : -INFINITY;
-          mx = fmaxf(mx, p[i][x]);
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = s[n][2 * i + e];
+              x *= sc;
+              if (masked) {
+                const int key = 8 * n + 2 * t4 + e;
+                if (!(j * BK + key < seen[i] && (there[n / 4] >> (key & 31) & 1))) x = -INFINITY;
+              }
+              mx = fmaxf(mx, x);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(L3_FULL, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(L3_FULL, mx, 2));
+          const float mn = fmaxf(m[i], mx), from = mn == -INFINITY ? 0.f : mn;
+          if (__any_sync(L3_FULL, mn > m[i])) {
+            const float alpha = ex2(m[i] - from);
+            l[i] *= alpha;
+#pragma unroll
+            for (int n = 0; n < KS; ++n) {
+              o[n][2 * i] *= alpha;
+              o[n][2 * i + 1] *= alpha;
+            }
+          }
+          m[i] = mn;
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) l[i] += s[n][2 * i + e] = ex2(s[n][2 * i + e] - from);
         }
-#pragma unroll
-        for (int w = 8; w; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(L3_FULL, mx, w));
-        const float mn = fmaxf(m[i], mx), from = mn == -INFINITY ? 0.f : mn;
-        alpha[i] = ex2(m[i] - from);
-        m[i] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) sum += p[i][x] = ex2(p[i][x] - from);
-#pragma unroll
-        for (int w = 8; w; w >>= 1) sum += __shfl_xor_sync(L3_FULL, sum, w);
-        l[i] = l[i] * alpha[i] + sum;
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) *reinterpret_cast<float4*>(sP + (tx + 16 * x) * PL + ty * 4) = make_float4(p[0][x], p[1][x], p[2][x], p[3][x]);
-#pragma unroll
-      for (int x = 0; x < NC * CW; ++x) {
-        o[0][x].x *= alpha[0]; o[0][x].y *= alpha[1];
-        o[1][x].x *= alpha[2]; o[1][x].y *= alpha[3];
       }
       cp_wait<1>();
-      __syncthreads();   // the values are there, and the weights
-#pragma unroll 2
-      for (int k = 0; k < BK; ++k) {
-        const float4 w = *reinterpret_cast<const float4*>(sP + k * PL + ty * 4);
-        const float2 w01 = make_float2(w.x, w.y), w23 = make_float2(w.z, w.w);
-        float v[NC * CW];
+      __syncthreads();   // the values are there
+      if (busy) {
+        const float* va = sV + 2 * t4 * LD + g;
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-          const float* at = sV + k * HD + n * 16 * CW + tx * CW;
-          if constexpr (CW == 4) {
-            const float4 x = *reinterpret_cast<const float4*>(at);
-            v[n * 4] = x.x; v[n * 4 + 1] = x.y; v[n * 4 + 2] = x.z; v[n * 4 + 3] = x.w;
-          } else if constexpr (CW == 2) {
-            const float2 x = *reinterpret_cast<const float2*>(at);
-            v[n * 2] = x.x; v[n * 2 + 1] = x.y;
-          } else v[n] = *at;
-        }
+        for (int n = 0; n < 8; ++n) {
+          const uint32_t p[4] = {__float_as_uint(s[n][0]), __float_as_uint(s[n][2]), __float_as_uint(s[n][1]), __float_as_uint(s[n][3])};
+          uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int x = 0; x < NC * CW; ++x) {
-          o[0][x] = fma2(w01, make_float2(v[x], v[x]), o[0][x]);
-          o[1][x] = fma2(w23, make_float2(v[x], v[x]), o[1][x]);
+          for (int i = 0; i < 4; ++i) two_parts(p[i], ph[i], pl[i]);
+#pragma unroll
+          for (int d = 0; d < KS; ++d) mma_parts(o[d], ph, pl, __float_as_uint(va[8 * n * LD + 8 * d]), __float_as_uint(va[(8 * n + 1) * LD + 8 * d]));
         }
       }
-      __syncthreads();   // all have read the values and the weights
+      __syncthreads();   // all have read the values
       if (j + 1 < c.j1) copy(j + 1, true);
       else cp_commit();
     }
@@ -198,30 +218,23 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_fma_kernel(const Chu
     float2* part_ml = whole ? nullptr : a.part_ml + (size_t)(2 * blockIdx.x + c.slot()) * TR;
     if (!whole && threadIdx.x == 0) left_of(a, blockIdx.x).part[c.slot()] = make_int4(c.b, c.tile, c.g, c.j1 == c.nb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int f = flat0 + ty * 4 + i;
-      float y[NC * CW];
+    for (int i = 0; i < 2; ++i) {
+      const int in_tile = warp * 16 + g + 8 * i, f = flat0 + in_tile;
+      l[i] += __shfl_xor_sync(L3_FULL, l[i], 1);
+      l[i] += __shfl_xor_sync(L3_FULL, l[i], 2);
       bool finite = l[i] < INFINITY;
 #pragma unroll
-      for (int x = 0; x < NC * CW; ++x) {
-        y[x] = i & 1 ? o[i / 2][x].y : o[i / 2][x].x;
-        finite = finite && fabsf(y[x]) < INFINITY;
-      }
+      for (int n = 0; n < KS; ++n) finite = finite && fabsf(o[n][2 * i]) < INFINITY && fabsf(o[n][2 * i + 1]) < INFINITY;
       if (f < flats) {
         if (!finite && whole) left_of(a, blockIdx.x).odd = 1;
         const int t = token_of(f);
         const long long at = (long long)(c.r.s0 + t) * a.H + c.g * a.R + f - t * a.R;
-        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+        const float by = !whole ? 1.f : l[i] == 0.f ? 0.f : 1.f / l[i];
+        float* to = whole ? (float*)a.out + at * HD : part_o + in_tile * HD;
 #pragma unroll
-        for (int n = 0; n < NC; ++n)
-#pragma unroll
-          for (int e = 0; e < CW; ++e) {
-            const int d = n * 16 * CW + tx * CW + e;
-            if (whole) ((T*)a.out)[at * HD + d] = down<T>(y[n * CW + e] * inv);
-            else part_o[(ty * 4 + i) * HD + d] = y[n * CW + e];
-          }
-        if (tx == 0) {
-          if (!whole) part_ml[ty * 4 + i] = make_float2(m[i], l[i]);
+        for (int n = 0; n < KS; ++n) *reinterpret_cast<float2*>(to + 8 * n + 2 * t4) = make_float2(o[n][2 * i] * by, o[n][2 * i + 1] * by);
+        if (t4 == 0) {
+          if (!whole) part_ml[in_tile] = make_float2(m[i], l[i]);
           else if (a.lse) a.lse[at] = (m[i] + log2f(l[i])) * 0.6931471805599453f;
         }
       }
@@ -336,10 +349,10 @@ template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
   a.part_o = (float*)a.ws;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * TR * HD);
   a.left = a.part_ml + (size_t)a.n_cta * 2 * TR;
-  cudaError_t e = allow_smem(chunk_fma_kernel<HD>, smem);
+  cudaError_t e = allow_smem(chunk_f32_kernel<HD>, smem);
   if (e != cudaSuccess) return e;
-  if ((e = launch_k(chunk_fma_kernel<HD>, dim3(a.n_cta), dim3(NT), smem, s, a)) != cudaSuccess) return e;
-  return join_t<float, BK>(a, fma_split(), s);
+  if ((e = launch_k(chunk_f32_kernel<HD>, dim3(a.n_cta), dim3(NT), smem, s, a)) != cudaSuccess) return e;
+  return join_t<float, BK>(a, f32_split(), s);
 }
 }  // namespace
 
@@ -350,10 +363,10 @@ cudaError_t launch_chunk_join_tc(const ChunkArgs& a, cudaStream_t s) {
 namespace {
 // Few rows over few keys as single tokens (paged.cu), which read their request's keys anew each.  us, so : as tiles, 32 heads over 8 kv heads of 128, one
 // request, by rows x keys and what is read: bf16 5 x 1505 29 MB 14.2 : 23.0, 16 x 1516 95 MB 23.0 : 23.4, 8 x 6008 188 MB 34.4 : 29.2, 2 x 60002 469 MB 88 : 63;
-// fp32 5 x 6005 235 MB 50 : 75, 8 x 6008 376 MB 72 : 78, 16 x 6016 752 MB 130 : 82.  (That path writes every row.)
+// fp32 5 x 1505 59 MB 22 : 32, 5 x 6005 235 MB 49 : 65, 16 x 316 40 MB 19 : 28, 16 x 1516 190 MB 43 : 34, 16 x 6016 752 MB 130 : 67.  (That path writes every row.)
 bool as_single_tokens(const ChunkArgs& a) {
   const long long size = a.dtype == L3_DTYPE_F32 ? 4 : 2, keys = (long long)a.max_pages << a.log_page;
-  return a.clear_rest && a.B > 0 && a.T <= 16 && a.T * keys * a.G * a.HD * 2 * size <= (size == 4 ? 384LL : 128LL) << 20;
+  return a.clear_rest && a.B > 0 && a.T <= 16 && a.T * keys * a.G * a.HD * 2 * size <= (size == 4 ? 256LL : 128LL) << 20;
 }
 PagedAttnArgs single_tokens(const ChunkArgs& a) {
   PagedAttnArgs p{};
