@@ -480,7 +480,7 @@ int l3_beam_select(const L3BeamSelect* a);
  * order, request by request, and go into its row of the table behind the pages of the tokens it had; where the list is used up they are -1,
  * and what the table has no column for is dropped.  A row's position is its token's number in its request, its slot the place
  * page * page_size + position % page_size; both are -1 for rows of no request, the slot also where there is no page.  out_used: pages that
- * were needed (more than n_free: too few were given). */
+ * were needed (more than n_free: too few were given).  No output shares memory with what is read. */
 typedef struct L3PagedExtend {
   int32_t device;
   int32_t batch, tokens, max_pages, page_size, n_free;
@@ -519,8 +519,8 @@ typedef struct L3Rotary {
 int l3_rotary(const L3Rotary* a);
 /* Attention of the rows of a packed step over their requests' pages: row t of request b, at position p = lengths[b] - (starts[b + 1] - starts[b])
  * + t, sees the tokens j <= p.  lengths count the rows' own tokens, whose keys and values are in their pages already.  Pages outside [0, pages) hold
- * no tokens, lengths are cut to [0, max_pages * page_size]; a row that sees no token gets 0 and lse -infinity.  Rows of no request are left as they
- * are, or set to 0 (lse -infinity) with clear_rest != 0.  A value that a row does not see has no part in its result, not even a NaN. */
+ * no tokens, lengths are cut to [0, max_pages * page_size]; a row that sees no token gets 0 and lse -infinity.  Rows of no request, ahead of starts[0]
+ * or from starts[batch] on: clear_rest 0: left as they are, 1: set to 0, lse -infinity, 2: lse alone.  A value that a row does not see has no part in its result, not even a NaN. */
 typedef struct L3PagedChunk {
   int32_t device;
   int32_t batch, tokens, heads, kv_heads, head_dim;  /* head_dim 16, 32, 48, 64, 96, 128 */

@@ -312,6 +312,7 @@ extern "C" int l3_paged_chunk_attention(const L3PagedChunk* a) {
   int rc = check_chunk(a->tokens, a->heads, a->kv_heads, a->head_dim, a->dtype);
   if (rc != L3_OK) return rc;
   REQ(a->batch >= 0, "bad batch");
+  REQ(a->clear_rest >= 0 && a->clear_rest <= 2, "clear_rest %d is not 0, 1 or 2", a->clear_rest);
   if ((rc = check_pages(a->pages, a->page_size, a->max_pages)) != L3_OK) return rc;
   if (a->tokens == 0 || (a->batch == 0 && !a->clear_rest)) return L3_OK;
   const int size = size_of(a->dtype);
@@ -330,7 +331,7 @@ extern "C" int l3_paged_chunk_attention(const L3PagedChunk* a) {
   p.k = pool_of(a->k, 1); p.v = pool_of(a->v, 1); p.n_pages = a->pages; p.log_page = log2_of(a->page_size);
   p.table = a->table; p.table_stride = a->table_stride; p.max_pages = a->max_pages; p.lengths = a->lengths; p.starts = a->starts;
   p.B = a->batch; p.T = a->tokens; p.H = a->heads; p.G = a->kv_heads; p.R = a->heads / a->kv_heads; p.HD = a->head_dim; p.dtype = a->dtype;
-  p.scale = a->scale; p.out = a->out; p.lse = a->lse; p.clear_rest = a->clear_rest != 0; p.ws = a->workspace;
+  p.scale = a->scale; p.out = a->out; p.lse = a->lse; p.clear_rest = a->clear_rest; p.ws = a->workspace;
   CKD(launch_paged_chunk(p, n_sm, (cudaStream_t)a->stream));
   return L3_OK;
 }

@@ -45,7 +45,7 @@ struct ChunkArgs {
   float scale;
   void* out;                         // [T, H, HD]
   float* lse;                        // [T, H] or null
-  bool clear_rest;
+  int clear_rest;                    // rows of no request: 0 as they are, 1: 0 (lse -infinity), 2: lse alone
   void* ws;                          // paged_chunk_workspace bytes, 16-byte aligned
   // set by the launcher
   int n_cta, tile_rows;              // CTAs, flat rows of an item

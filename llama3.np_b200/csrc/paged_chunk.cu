@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a, const
   } while (c.next(a, sp));
 }
 
-size_t partials(int n_cta, int rows, int HD) { return (size_t)n_cta * (2 * rows * ((size_t)HD * 4 + 8) + sizeof(Left)); }
+size_t partials(int n_cta, int rows, int HD) { return (size_t)n_cta * (2 * rows * ((size_t)HD * 4 + 8) + sizeof(Left)) + PART_ALIGN; }
 template <typename T, int BK> cudaError_t join_t(const ChunkArgs& a, const Split& sp, cudaStream_t s) {
   const dim3 grid(a.n_cta, a.tile_rows / JROWS), block(JT);
   g_l3_pdl_next = true;
@@ -346,7 +346,7 @@ template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
   constexpr size_t smem = smem_bytes<HD>();
   a.n_cta = ctas_of_sm(HD) * n_sm;
   a.tile_rows = TR;
-  a.part_o = (float*)a.ws;
+  a.part_o = part_begin(a.ws);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * TR * HD);
   a.left = a.part_ml + (size_t)a.n_cta * 2 * TR;
   cudaError_t e = allow_smem(chunk_f32_kernel<HD>, smem);
@@ -366,7 +366,7 @@ namespace {
 // fp32 5 x 1505 59 MB 22 : 32, 5 x 6005 235 MB 49 : 65, 16 x 316 40 MB 19 : 28, 16 x 1516 190 MB 43 : 34, 16 x 6016 752 MB 130 : 67.  (That path writes every row.)
 bool as_single_tokens(const ChunkArgs& a) {
   const long long size = a.dtype == L3_DTYPE_F32 ? 4 : 2, keys = (long long)a.max_pages << a.log_page;
-  return a.clear_rest && a.B > 0 && a.T <= 16 && a.T * keys * a.G * a.HD * 2 * size <= (size == 4 ? 256LL : 128LL) << 20;
+  return a.clear_rest == 1 && a.B > 0 && a.T <= 16 && a.T * keys * a.G * a.HD * 2 * size <= (size == 4 ? 256LL : 128LL) << 20;
 }
 PagedAttnArgs single_tokens(const ChunkArgs& a) {
   PagedAttnArgs p{};

@@ -176,45 +176,63 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // The values of a key that a row sees may be infinite or NaN, those of keys that it does not see have to be kept out even so, and tiles
-// multiply them by a weight of 0.  A row whose result is not finite is therefore taken once more, behind the join, by the formula alone: its keys one
-// at a time, by a warp; only what the row sees enters.  A weight is 0 for a score of -infinity only, however small, as its value may be infinite.
+// multiply them by a weight of 0.  A row whose result is not finite is therefore taken once more, behind the join, by the formula alone, by a warp:
+// scores with a lane a key, then the values a key at a time, four on their way; only what the row sees enters.  A weight is 0 for a score of
+// -infinity only, however small, as its value may be infinite.
 template <typename T, int HD> __device__ __forceinline__ void by_formula(const ChunkArgs& a, int b, int g, int row, int head, int seen) {
-  constexpr int N = (HD + 31) / 32;
+  constexpr int N = (HD + 31) / 32, E = 16 / sizeof(T);
+  struct alignas(16) Piece { T x[E]; };
   const int lane = threadIdx.x & 31;
   const int* table = a.table + b * a.table_stride;
   const T* q = (const T*)a.q + row * a.q_st + head * a.q_sh;
   const float sc = a.scale * 1.4426950408889634f;
-  auto row_of = [&](const PagedPool& p, int j, bool& there) {
-    const int page = table[j >> a.log_page];
-    there = (unsigned)page < (unsigned)a.n_pages;
-    return (const T*)p.p + page * p.sp + g * p.sh + (j & ((1 << a.log_page) - 1)) * p.st;
-  };
-  auto score = [&](int j, bool& there) {
-    const T* k = row_of(a.k, j, there);
-    if (!there) return -INFINITY;
+  auto row_of = [&](const PagedPool& p, int j, int page) { return (const T*)p.p + page * p.sp + g * p.sh + (j & ((1 << a.log_page) - 1)) * p.st; };
+  auto score = [&](int j, int& page) {  // of this lane's key; page -1: there is none
+    page = j < seen ? table[j >> a.log_page] : -1;
+    if ((unsigned)page >= (unsigned)a.n_pages) page = -1;
+    if (page < 0) return -INFINITY;
+    const T* k = row_of(a.k, j, page);
     float s = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < HD; i += E) {
+      const Piece x = *reinterpret_cast<const Piece*>(q + i), y = *reinterpret_cast<const Piece*>(k + i);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + 32 * i < HD) s += up(q[lane + 32 * i]) * up(k[lane + 32 * i]);
-    return warp_sum(s) * sc;
+      for (int e = 0; e < E; ++e) s += up(x.x[e]) * up(y.x[e]);
+    }
+    return s * sc;
   };
   float o[N], m = -INFINITY, l = 0.f;
-  bool there;
-  for (int j = 0; j < seen; ++j) m = fmaxf(m, score(j, there));
+  int page;
+  for (int j = 0; j < seen; j += 32) m = fmaxf(m, score(j + lane, page));
+  m = warp_max(m);
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   const float from = m == -INFINITY ? 0.f : m;
-  for (int j = 0; j < seen; ++j) {
-    const float s = score(j, there);
-    if (!there) continue;
-    const float x = s - from;
-    const float w = x < -149.f && s > -INFINITY ? 1.4e-45f : exp2f(x);
+  for (int j = 0; j < seen; j += 32) {
+    const float s = score(j + lane, page), x = s - from;
+    const float w = page < 0 ? 0.f : x < -149.f && s > -INFINITY ? 1.4e-45f : exp2f(x);
     l += w;
-    const T* v = row_of(a.v, j, there);
+    unsigned list = __ballot_sync(L3_FULL, page >= 0);
+    while (list) {
+      float wk[4], v[4][N];
+      int of[4];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + 32 * i < HD) o[i] += w * up(v[lane + 32 * i]);
+      for (int k = 0; k < 4; ++k) {
+        of[k] = __ffs(list) - 1;
+        list &= list - 1;
+        const int from_lane = max(of[k], 0), its = __shfl_sync(L3_FULL, page, from_lane);
+        wk[k] = __shfl_sync(L3_FULL, w, from_lane);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[k][i] = of[k] >= 0 && lane + 32 * i < HD ? up(row_of(a.v, j + from_lane, its)[lane + 32 * i]) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (of[k] >= 0) o[i] += wk[k] * v[k][i];
+    }
   }
+  l = warp_sum(l);
   const long long at = (long long)row * a.H + head;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -223,15 +241,16 @@ template <typename T, int HD> __device__ __forceinline__ void by_formula(const C
   if (lane == 0 && a.lse) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// rows of no request: as they are, or 0
+// rows of no request, ahead of the first and behind the last
 template <typename T> __device__ __forceinline__ void clear_rest(const ChunkArgs& a, int thread, int threads) {  // by some of a CTA's threads
   if (!a.clear_rest) return;
-  const int from = a.B ? min(max(a.starts[a.B], 0), a.T) : 0;
-  const long long n = (long long)(a.T - from) * a.H, at = (long long)from * a.H;
-  for (long long i = (long long)blockIdx.x * threads + thread; i < n * a.HD; i += (long long)gridDim.x * threads) {
-    ((T*)a.out)[at * a.HD + i] = down<T>(0.f);
-    if (a.lse && i < n) a.lse[at + i] = -INFINITY;
-  }
+  const int from = a.B ? min(max(a.starts[a.B], 0), a.T) : 0, ahead = a.B ? min(max(a.starts[0], 0), from) : 0;
+  const long long first = (long long)ahead * a.H, gap = (long long)(from - ahead) * a.H, n = (long long)a.T * a.H - gap;  // heads' rows; i-th: behind the gap from `first` on
+  const long long begin = (long long)blockIdx.x * threads + thread, step = (long long)gridDim.x * threads;
+  if (a.lse)
+    for (long long i = begin; i < n; i += step) a.lse[i < first ? i : i + gap] = -INFINITY;
+  if (a.clear_rest == 1)
+    for (long long i = begin; i < n * a.HD; i += step) ((T*)a.out)[i < first * a.HD ? i : i + gap * a.HD] = down<T>(0.f);
 }
 
 // What a CTA leaves for the join: its share, whether a result of an item that it has whole is not finite, and of its two partials - of the
@@ -242,6 +261,9 @@ struct Left {
   int odd, pad[3];
 };
 static_assert(sizeof(Left) % 16 == 0, "");
+// the partials begin on 32 bytes, as they are stored; a workspace need not
+constexpr size_t PART_ALIGN = 32;
+inline float* part_begin(void* ws) { return reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ws) + PART_ALIGN - 1) & ~(uintptr_t)(PART_ALIGN - 1)); }
 __device__ __forceinline__ Left& left_of(const ChunkArgs& a, int cta) { return reinterpret_cast<Left*>(a.left)[cta]; }
 __device__ __forceinline__ void leave_nothing(const ChunkArgs& a, const Place& place) {  // by one thread, ahead of all others' words
   Left& left = left_of(a, blockIdx.x);

@@ -741,7 +741,7 @@ template <typename T, int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaS
   using C = Cfg<T, HD>;
   a.n_cta = n_sm;
   a.tile_rows = rows_of_item(a, n_sm);
-  a.part_o = (float*)a.ws;
+  a.part_o = part_begin(a.ws);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * a.tile_rows * HD);
   a.left = a.part_ml + (size_t)a.n_cta * 2 * a.tile_rows;
   cudaError_t e = allow_smem(chunk_tc_kernel<T, HD>, C::SMEM);

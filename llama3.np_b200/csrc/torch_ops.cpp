@@ -572,7 +572,7 @@ PyObject* paged_rotary_write(PyObject*, PyObject* const* x, Py_ssize_t n) {
     NEED(o.sizes() == q.sizes(), "out must be ", q.sizes(), ", got ", o.sizes());
     last_is_dense(o, "out");
     no_overlap(o, "out");
-    NEED(!meets(o, q) || same_place(o, q), "out shares memory with q and is not q itself");
+    NEED(same_place(o, q) || !(meets(o, q) || meets(o, k) || meets(o, v)), "out shares memory with q, k or v and is not q itself");
   }
   OneDevice on;
   on.add(q, "q"); on.add(k, "k"); on.add(v, "v"); on.add(positions, "positions"); on.add(slots, "slots"); on.add(kp, "k_pages"); on.add(vp, "v_pages");
@@ -632,7 +632,7 @@ PyObject* paged_chunk_attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
   if (tokens) {
     a.device = on.index; a.batch = size32(batch, "batch"); a.tokens = size32(tokens, "tokens"); a.heads = size32(heads, "heads"); a.kv_heads = size32(G, "kv heads");
     a.head_dim = (int)dim; a.pages = size32(k.size(0), "pages"); a.page_size = (int)k.size(2); a.max_pages = size32(table.size(1), "page_table");
-    a.clear_rest = !given(x[8]);
+    a.clear_rest = given(x[8]) ? 2 : 1;  // lse is made here
     a.scale = given(x[6]) ? (float)real(x[6]) : (float)(1.0 / std::sqrt((double)dim));
     a.stream = on.stream();
     a.q = q.const_data_ptr(); a.q_token_stride = step_of(q, 0); a.q_head_stride = step_of(q, 1);

@@ -111,6 +111,16 @@ def test_rotary_write_refuses(change, text):
         paged_rotary_write(**_write(**change))
 
 
+def test_rotary_write_refuses_results_over_what_it_reads():
+    qkv = torch.zeros(7, 12, 64)
+    q, k, v = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
+    for a, out in [(_write(k=torch.zeros(7, 8, 64)[:, :2]), "k"), (_write(v=torch.zeros(7, 8, 64)[:, :2]), "v"), (_write(), "q")]:
+        with pytest.raises(ValueError, match="shares memory"):
+            paged_rotary_write(**a, out=a[out].as_strided((7, 8, 64), (512, 64, 1)) if out != "q" else a["q"].as_strided((7, 8, 64), (64, 448, 1)))
+    with pytest.raises(ValueError, match="CUDA device"):   # q itself, beside k and v in one tensor
+        paged_rotary_write(**_write(q=q, k=k, v=v), out=q)
+
+
 @pytest.mark.parametrize("args,kw,text", [
     ((torch.zeros(9), ints(1)), {}, "dimensions"), ((torch.zeros(2, 9).double(), ints(2)), {}, "type"), ((torch.zeros(2, 9), ints(3)), {}, "tokens"),
     ((torch.zeros(2, 9), ints(2, dtype=torch.int64)), {}, "type"), ((torch.zeros(9, 2).T, ints(2)), {}, "contiguous"),

@@ -1,10 +1,12 @@
 """GPU suite: attention of a packed step's rows over a cache in pages, against its formula in 64 bits."""
+import ctypes as C
 import math
+import threading
 
 import pytest
 import torch
 
-from llama3_np_b200 import paged_attention, paged_chunk_attention
+from llama3_np_b200 import _cabi, paged_attention, paged_chunk_attention
 
 pytestmark = pytest.mark.gpu
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
@@ -319,3 +321,98 @@ def test_pools_beyond_32_bits(kind):
     table = ids[torch.randperm(35, generator=torch.Generator().manual_seed(1))][None].cuda()
     q = torch.randn(90, 4, 64, device="cuda").to(dtype)
     check(q, k, v, table, torch.tensor([550], dtype=torch.int32, device="cuda"), torch.tensor([0, 90], dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("requests", [[(60, 9), (0, 0), (3, 1)], [(30, 70), (0, 0), (5, 17)]])
+def test_rows_ahead_of_the_first_request(kind, requests):
+    """Rows ahead of starts[0] belong to no request, either: 0, or as they are in `out`; what is made here is always set."""
+    ahead = 3
+    args = list(make(2, TYPES[kind], 8, 2, 64, 16, requests, rest=ahead + 2))
+    args[-1] = args[-1] + ahead
+    got = check(*args)
+    n = int(args[-1][-1])
+    out = torch.full_like(args[0], 7.0)
+    torch.full((1 << 16,), 5.0, device="cuda")   # what lse's memory may hold
+    again, lse = paged_chunk_attention(*args, out=out, return_lse=True)
+    none = torch.ones(len(out), dtype=torch.bool, device="cuda")
+    none[ahead:n] = False
+    assert torch.allclose(again[~none].float(), got[~none].float(), rtol=2e-2, atol=2e-2)
+    assert bool((again[none] == 7).all()) and bool((lse[none] == -math.inf).all()) and bool(lse[~none].isfinite().all())
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("how", ["pages of both", "one behind the other", "values first", "the same", "rows of both"])
+@pytest.mark.parametrize("page", [4, 16, 256])
+def test_pools_in_one_piece_of_memory(kind, how, page):
+    q, k, v, table, lens, starts = make(3, TYPES[kind], 8, 2, 64, page, [(300, 40), (0, 170), (77, 1)], garbage=math.nan)
+    if how == "pages of both":
+        k, v = torch.stack([k, v], 1).unbind(1)
+    elif how == "one behind the other":
+        k, v = torch.stack([k, v]).unbind(0)
+    elif how == "values first":
+        v, k = torch.stack([v, k]).unbind(0)
+    elif how == "rows of both":
+        v, k = torch.cat([v, k], -1).split(64, -1)
+    else:
+        v = k
+    check(q, k, v, table, lens, starts)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_a_table_without_columns(kind):
+    q, k, v, table, lens, starts = make(4, TYPES[kind], 8, 2, 64, 16, [(30, 20), (5, 7)])
+    out, lse = paged_chunk_attention(q, k, v, table[:, :0], lens, starts, return_lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [16, 64, 128])
+def test_results_on_16_bytes(kind, dim):
+    args = make(5, TYPES[kind], 8, 2, dim, 16, [(300, 140), (5, 7)])
+    want = check(*args)
+    out = torch.empty(want.numel() + 8, dtype=want.dtype, device="cuda")[8:].view_as(want)
+    assert torch.equal(paged_chunk_attention(*args, out=out), want)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_a_workspace_on_16_bytes(kind):
+    """As the C interface asks for it, and no byte around it is written."""
+    q, k, v, table, lens, starts = make(6, TYPES[kind], 8, 2, 64, 16, [(5000, 40), (0, 170)])
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    code = {"f32": _cabi.DTYPE_F32, "bf16": _cabi.DTYPE_BF16, "f16": _cabi.DTYPE_F16}[kind]
+    need = C.c_int64()
+    lib = _cabi.lib()
+    assert lib.l3_paged_chunk_workspace(0, len(q), 8, 2, 64, code, C.byref(need)) == 0
+    room = torch.full((need.value + 256,), 77, dtype=torch.uint8, device="cuda")
+    begin = 16 if room.data_ptr() % 32 == 0 else 0
+    a = _cabi.L3PagedChunk(device=0, batch=2, tokens=len(q), heads=8, kv_heads=2, head_dim=64, pages=len(k), page_size=16, max_pages=table.shape[1], dtype=code,
+                           clear_rest=1, scale=0.125, stream=torch.cuda.current_stream().cuda_stream, q=q.data_ptr(), q_token_stride=512, q_head_stride=64,
+                           k=_cabi.L3PagePool(k.data_ptr(), *k.stride()[:3]), v=_cabi.L3PagePool(v.data_ptr(), *v.stride()[:3]), table=table.data_ptr(),
+                           table_stride=table.stride(0), lengths=lens.data_ptr(), starts=starts.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
+                           workspace=room.data_ptr() + begin, workspace_bytes=need.value)
+    assert lib.l3_paged_chunk_attention(C.byref(a)) == 0
+    near(out, lse, formula(q, k, v, table, lens, starts))
+    assert bool((room[:begin] == 77).all()) and bool((room[begin + need.value:] == 77).all())
+
+
+def test_several_streams_and_threads_at_once():
+    cases = [make(20 + i, dtype, 8, 2, dim, 16, requests) for i, (dtype, dim, requests) in enumerate([
+        (torch.bfloat16, 128, [(900, 300), (0, 500)]), (torch.float16, 64, [(3000, 30)] * 4), (torch.float32, 48, [(100, 90)] * 6), (torch.bfloat16, 64, [(40, 5)])])]
+    want = [paged_chunk_attention(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got[i].append(paged_chunk_attention(*cases[i]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for w, all_of in zip(want, got):
+        assert len(all_of) == 50 and all(torch.equal(w, x) for x in all_of)
