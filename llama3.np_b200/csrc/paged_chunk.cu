@@ -5,7 +5,8 @@
 // This file: fp32 caches; and the join of what several CTAs have of an item.  Products as three of TF32 numbers on the tensor cores (mma.sync): a number is
 // the nearest one of 11 bits and what that leaves, cut to 11 bits, and x y = xh yh + xh yl + xl yh is off by at most 2^-20 of it - where numbers'
 // second parts are not below fp32's normal ones, from 2^-115 on.  (With FFMA what shared memory delivers bounded the kernel, 3200 wavefronts a tile of
-// 64 x 64 with heads of 48 in place of 800: 64 prompts of up to 220 tokens, 6 heads of 48, 88 us, now 62.)
+// 64 x 64 with heads of 48 in place of 800: 64 prompts of up to 220 tokens, 6 heads of 48, 88 us, now 56.  There
+// the tensor pipe is busy for a quarter of the time and 39 % of the issue slots are used: three warps a scheduler wait for one another's products.)
 // A CTA's four warps hold 16 rows each and walk their keys, 64 at a time.  Keys and values come row by row through the page table, 16 bytes a
 // copy, while the tile before is worked on; rows of no token become zeros.  Rows of tiles are padded to an odd number of 16-byte pieces: eight rows'
 // pieces (scores, ldmatrix), and eight columns of four rows two apart (output), lie on different banks.  The weights stay in registers: the lane that has
@@ -21,7 +22,7 @@ namespace {
 using namespace chunk;
 constexpr int TR = 64, BK = 64, NT = 128;
 __host__ __device__ constexpr Split f32_split() { return Split{BK, 1, 4, TR, 2}; }
-// as registers and shared memory have room for; of heads of 48, where there is room for four, three: 61.9 : 62.9 us
+// as registers and shared memory have room for; of heads of 48, three : four: 61.9 : 62.9 us (four's registers spill)
 constexpr int ctas_of_sm(int HD) { return HD > 64 ? 2 : 3; }
 template <int HD> constexpr int row_ld() { return HD + 4; }
 template <int HD> constexpr size_t smem_bytes() { return (size_t)3 * 64 * row_ld<HD>() * 4 + 2 * 2 * BK * 8 + 2 * 8; }
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const Chu
     const int* table = a.table + c.b * a.table_stride;
     const int flat0 = c.tile * TR, flats = c.r.n * a.R, row0 = flat0 + warp * 16;
     const int most = c.r.seen(token_of(min(flats, flat0 + TR) - 1));   // keys that any of the rows sees
-    const bool busy = row0 < flats;                                    // the warp has rows
+    const int ours = row0 < flats ? c.r.seen(token_of(min(flats, row0 + 16) - 1)) : 0;  // that any of this warp's rows sees
     for (int i = threadIdx.x; i < TR * (HD / 4); i += NT) {  // the rows' queries
       const int r = i / (HD / 4), p = i - r * (HD / 4), f = flat0 + r, t = token_of(f);
       const bool in = f < flats;
@@ -131,10 +132,11 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const Chu
       if (j + 1 < c.j1) offsets(j + 1);
       cp_wait<1>();
       __syncthreads();   // the keys are there, and the next ones' places
+      const int left = ours - j * BK;  // what lies behind is not multiplied (56 us for 60)
       float s[8][4];
 #pragma unroll
       for (int n = 0; n < 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      if (busy) {
+      if (left > 0) {
         // ldmatrix of 8 rows of 4 numbers: lane i has row i / 4's number i % 4
         const uint32_t qa = smem_u32(sQ + (warp * 16 + (lane & 15)) * LD + (lane >> 4) * 4);
         const uint32_t ka = smem_u32(sK + ((lane >> 4) * 8 + (lane & 7)) * LD + (lane >> 3 & 1) * 4);
@@ -146,6 +148,7 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const Chu
           for (int i = 0; i < 4; ++i) two_parts(q[i], qh[i], ql[i]);
 #pragma unroll
           for (int n = 0; n < 8; n += 2) {
+            if (8 * n >= left) break;
             uint32_t k[4];
             ldsm_x4(ka + n * 8 * LD * 4 + ks * 32, k);
             mma_parts(s[n], qh, ql, k[0], k[1]);
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const Chu
       __syncthreads();   // all have read the keys
       if (j + 1 < c.j1) copy(j + 1, false);
       else cp_commit();
-      if (busy) {
+      if (left > 0) {
         const bool masked = __any_sync(L3_FULL, min(seen[0], seen[1]) - j * BK < BK) || (there[0] & there[1]) != L3_FULL;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -195,10 +198,11 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const Chu
       }
       cp_wait<1>();
       __syncthreads();   // the values are there
-      if (busy) {
+      if (left > 0) {
         const float* va = sV + 2 * t4 * LD + g;
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
+          if (8 * n >= left) break;
           const uint32_t p[4] = {__float_as_uint(s[n][0]), __float_as_uint(s[n][2]), __float_as_uint(s[n][1]), __float_as_uint(s[n][3])};
           uint32_t ph[4], pl[4];
 #pragma unroll
