@@ -5,7 +5,7 @@
 // This file: fp32 caches; and the join of what several CTAs have of an item.  Products as three of TF32 numbers on the tensor cores (mma.sync): a number is
 // the nearest one of 11 bits and what that leaves, cut to 11 bits, and x y = xh yh + xh yl + xl yh is off by at most 2^-20 of it - where numbers'
 // second parts are not below fp32's normal ones, from 2^-115 on.  (With FFMA what shared memory delivers bounded the kernel, 3200 wavefronts a tile of
-// 64 x 64 with heads of 48 in place of 800: 64 prompts of up to 220 tokens, 6 heads of 48, 88 us, now 56.  There
+// 64 x 64 with heads of 48 in place of 800: 64 prompts of up to 220 tokens, 6 heads of 48, 88 us, now 54.  There
 // the tensor pipe is busy for a quarter of the time and 39 % of the issue slots are used: three warps a scheduler wait for one another's products.)
 // A CTA's four warps hold 16 rows each and walk their keys, 64 at a time.  Keys and values come row by row through the page table, 16 bytes a
 // copy, while the tile before is worked on; rows of no token become zeros.  Rows of tiles are padded to an odd number of 16-byte pieces: eight rows'
@@ -249,71 +249,85 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const Chu
 
 // ---------------------------------------------------------------------------------------------------------------- the join
 // Block (c, y) joins 16 rows of the item that CTA c began and others ended, o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, and looks after
-// the rows of all its items that are not finite.
-constexpr int JROWS = 16, JT = 256;
+// the rows of all its items that are not finite.  A thread has four columns of a row: most items are in two or three CTAs, and a warp a row took
+// four times as many instructions (48 requests over 8 kv heads of 64: 96 us for 100 in all).
+constexpr int JROWS = 16, JT = 256, MOST_CTAS = 1024;
+__device__ __forceinline__ void store4(float* to, const float (&o)[4]) { *reinterpret_cast<float4*>(to) = make_float4(o[0], o[1], o[2], o[3]); }
+template <typename T> __device__ __forceinline__ void store4(T* to, const float (&o)[4]) {
+  struct alignas(8) Four { T x[4]; } four{down<T>(o[0]), down<T>(o[1]), down<T>(o[2]), down<T>(o[3])};
+  *reinterpret_cast<Four*>(to) = four;
+}
 template <typename T, int HD, int BK>
 __global__ void __launch_bounds__(JT) chunk_join_kernel(const ChunkArgs a, const Split sp) {
+  constexpr int N = (HD + 31) / 32, UNITS = HD / 4;
+  __shared__ int list[MOST_CTAS];  // the item's partials, 2 CTA + slot, in the order of the keys
+  __shared__ int parts;
+  __shared__ unsigned odd_rows;
   pdl_launch();
   pdl_wait();
-  constexpr int N = (HD + 31) / 32;
   const int TR = a.tile_rows;
   const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Left& own = left_of(a, c0);
   const int4 first = own.part[1];
   if (first.x >= 0) {
     const Request r = request(a, first.x);
-    for (int i = warp; i < JROWS; i += JT / 32) {
-      const int in_tile = blockIdx.y * JROWS + i, f = first.y * TR + in_tile;
-      if (f >= r.n * a.R) break;
-      const int t = f / a.R, head = first.z * a.R + f - t * a.R;
-      const long long at = (long long)(r.s0 + t) * a.H + head;
-      float o[N], m, l;
-      const size_t p0 = (size_t)(2 * c0 + 1) * TR + in_tile;
-      m = a.part_ml[p0].x;
-      l = a.part_ml[p0].y;
-#pragma unroll
-      for (int x = 0; x < N; ++x) o[x] = lane + 32 * x < HD ? a.part_o[p0 * HD + lane + 32 * x] : 0.f;
-      // the CTAs behind, 32 at a time, a lane each; those that ended nothing and went on with nothing have no part
-      for (int c = c0 + 1;; c += 32) {
-        const int4 its = c + lane < a.n_cta ? left_of(a, c + lane).part[0] : make_int4(-1, 0, 0, 0);
-        const unsigned ends = __ballot_sync(L3_FULL, its.x >= 0 && its.w);
-        const bool part = its.x >= 0 && (!ends || lane < __ffs(ends));
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (part) ml = a.part_ml[(size_t)(2 * (c + lane)) * TR + in_tile];
-        const float mn = fmaxf(m, warp_max(ml.x)), from = mn == -INFINITY ? 0.f : mn;
-        const float f0 = exp2f(m - from), fp = exp2f(ml.x - from);
-        l = l * f0 + warp_sum(ml.y * fp);
-        m = mn;
-#pragma unroll
-        for (int x = 0; x < N; ++x) o[x] *= f0;
-        unsigned list = __ballot_sync(L3_FULL, part);
-        while (list) {
-          float f[4], y[4][N];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {  // four partials' rows on their way together
-            const int of = list ? __ffs(list) - 1 : -1;
-            list &= list - 1;
-            f[k] = __shfl_sync(L3_FULL, fp, max(of, 0));
-#pragma unroll
-            for (int x = 0; x < N; ++x)
-              y[k][x] = of >= 0 && lane + 32 * x < HD ? a.part_o[((size_t)(2 * (c + of)) * TR + in_tile) * HD + lane + 32 * x] : 0.f;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int x = 0; x < N; ++x) o[x] += y[k][x] * f[k];
+    const int row0 = blockIdx.y * JROWS, rows = min(JROWS, r.n * a.R - first.y * TR - row0);  // of the tile
+    if (rows > 0) {
+      if (warp == 0) {  // the CTAs behind, a lane each; those that ended nothing and went on with nothing have no part
+        int n = 1;
+        for (int c = c0 + 1; c < a.n_cta; c += 32) {
+          const int4 its = c + lane < a.n_cta ? left_of(a, c + lane).part[0] : make_int4(-1, 0, 0, 0);
+          const unsigned ends = __ballot_sync(L3_FULL, its.x >= 0 && its.w);
+          const unsigned has = __ballot_sync(L3_FULL, its.x >= 0 && (!ends || lane < __ffs(ends)));
+          if (has >> lane & 1) list[n + __popc(has & ((1u << lane) - 1))] = 2 * (c + lane);
+          n += __popc(has);
+          if (ends) break;
         }
-        if (ends || c + 32 >= a.n_cta) break;
+        if (lane == 0) {
+          list[0] = 2 * c0 + 1;
+          parts = n;
+          odd_rows = 0;
+        }
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      bool odd = !(l < INFINITY);
+      __syncthreads();
+      const int n = parts;
+      for (int u = threadIdx.x; u < rows * UNITS; u += JT) {
+        const int i = u / UNITS, d = (u - i * UNITS) * 4, in_tile = row0 + i, f = first.y * TR + in_tile;
+        const int t = f / a.R, head = first.z * a.R + f - t * a.R;
+        float o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) m = fmaxf(m, a.part_ml[(size_t)list[k] * TR + in_tile].x);
+        const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+          const size_t at = (size_t)list[k] * TR + in_tile;
+          const float2 ml = a.part_ml[at];
+          const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
+          const float by = ex2(ml.x - from);
+          l += ml.y * by;
+          o[0] += x.x * by;
+          o[1] += x.y * by;
+          o[2] += x.z * by;
+          o[3] += x.w * by;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bool odd = !(l < INFINITY);
 #pragma unroll
-      for (int x = 0; x < N; ++x) {
-        odd = odd || !(fabsf(o[x]) < INFINITY);
-        if (lane + 32 * x < HD) ((T*)a.out)[at * HD + lane + 32 * x] = down<T>(o[x] * inv);
+        for (int e = 0; e < 4; ++e) {
+          odd = odd || !(fabsf(o[e]) < INFINITY);
+          o[e] *= inv;
+        }
+        const long long at = (long long)(r.s0 + t) * a.H + head;
+        store4((T*)a.out + at * HD + d, o);
+        if (a.lse && d == 0) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
+        if (odd) atomicOr(&odd_rows, 1u << i);
       }
-      if (a.lse && lane == 0) a.lse[at] = (m + log2f(l)) * 0.6931471805599453f;
-      if (__any_sync(L3_FULL, odd)) by_formula<T, HD>(a, first.x, first.z, r.s0 + t, head, r.seen(t));
+      __syncthreads();
+      for (int i = warp; i < rows; i += JT / 32) {
+        if (!(odd_rows >> i & 1)) continue;
+        const int f = first.y * TR + row0 + i, t = f / a.R;
+        by_formula<T, HD>(a, first.x, first.z, r.s0 + t, first.z * a.R + f - t * a.R, r.seen(t));
+      }
     }
   }
   if (!own.odd) return;
@@ -348,7 +362,7 @@ template <typename T, int BK> cudaError_t join_t(const ChunkArgs& a, const Split
 }
 template <int HD> cudaError_t launch_hd(ChunkArgs a, int n_sm, cudaStream_t s) {
   constexpr size_t smem = smem_bytes<HD>();
-  a.n_cta = ctas_of_sm(HD) * n_sm;
+  a.n_cta = std::min(ctas_of_sm(HD) * n_sm, MOST_CTAS);
   a.tile_rows = TR;
   a.part_o = part_begin(a.ws);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)a.n_cta * 2 * TR * HD);
