@@ -7,6 +7,9 @@
 // bound the n-th largest logit from below, so only the few threads whose maximum passes the bound look at their logits
 // again (a warp together at one thread's, 32 pieces at a time), and what passes is ranked by counting.  Where more values pass than there is room
 // for, a better bound is found; where that does not help (many equal ones), the n are drawn one after the other.
+//
+// 2047 rows of 128256 in bf16 with entropy: 99 us, 5.3 TB/s (82 % of a copy's rate) at 74 % of the issue slots: an exponential and five other
+// instructions a logit.  48 rows in fp32 with entropy and 20 tokens: 16.5 us, 7.3 without the tokens, whose ranking is a chain of barriers.
 #include <float.h>
 #include <math.h>
 
@@ -367,7 +370,8 @@ __global__ void __launch_bounds__(LT, 2) logprobs_kernel(const LogprobsArgs a) {
   }
 }
 template <typename T, bool ENTROPY, bool TOP> cudaError_t launch_tt(const LogprobsArgs& a, int n_sm, cudaStream_t s) {
-  // a cluster's CTAs: as many as fill the SMs, if each has a piece for every thread
+  // a cluster's CTAs: as many as fill the SMs, if each has a piece for every thread.  us, rows of 128256 in fp32 with entropy and 20 tokens, by 1 : as chosen : by 8:
+  // 1 row 14.7 : 12.7 : 12.7 (8 chosen; calls differ by 0.5), 48 rows 19.3 : 16.5 : 24.5 (4), 148 rows 23.7 : 21.6 : 57.7 (2), 600 rows 100 : 100 : 225 (1)
   int S = 1;
   while (S < 8 && (long long)a.R * S * 2 <= 2LL * n_sm && (long long)a.V >= (long long)S * 2 * LT * Piece<T>::N) S *= 2;
   for (int row = 0; row < a.R; row += 65535) {
