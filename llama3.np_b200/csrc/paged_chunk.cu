@@ -21,7 +21,7 @@
 namespace {
 using namespace chunk;
 constexpr int TR = 64, BK = 64, NT = 128;
-__host__ __device__ constexpr Split f32_split() { return Split{BK, 1, 4, TR, 2}; }
+__host__ __device__ constexpr Split f32_split() { return Split{BK, 1, 16, 8, 8}; }
 // as registers and shared memory have room for; of heads of 48, three : four: 61.9 : 62.9 us (four's registers spill)
 constexpr int ctas_of_sm(int HD) { return HD > 64 ? 2 : 3; }
 template <int HD> constexpr int row_ld() { return HD + 4; }

@@ -40,14 +40,16 @@ template <int BK> __device__ __forceinline__ int blocks(const ChunkArgs& a, cons
   const int last = min(r.n * a.R, (tile + 1) * a.tile_rows) - 1;
   return (int)((unsigned)(r.seen(last / a.R) + BK - 1) / BK);
 }
-// An item's weight: `per` a block - 2, or 4 of a tile of more than rows_of_half rows - and `ends` for what begins and ends it.  Items of `whole` blocks or
+// An item's weight: 8 a block, or from `few` on of a tile of up to 128 rows, and `ends` for what begins and ends it.  Items of `whole` blocks or
 // fewer are not cut; `least`: the least weight of a share.
-struct Split { int block, whole, least, rows_of_half, ends; };
-// paged_chunk_tc.cu: one tile of rows has two blocks at a time, which takes half the time as long as the tiles' copies keep up.  us, half : three quarters :
-// all of a block's weight: heads of 64, 48 requests of up to 3001 tokens 125 : 131 : 141; of 128, six prompts of up to 4096 tokens 666 : 600 : 575
-__host__ __device__ constexpr Split tc_split(int HD) { return Split{TC_BK, 4, 4, HD <= 64 ? 128 : 0, 6}; }
+struct Split { int block, whole, least, few, ends; };
+// paged_chunk_tc.cu: one tile of rows has two blocks at a time, which takes half the time as long as the tiles' copies keep up: not in heads of 128, and in
+// smaller ones the sooner, the larger the copies.  us, few 4 : 5 : 6 of heads of 64, 48 requests of up to 3001 tokens in pages of 32 98.5 : 100.2 : 104.5, of
+// 16 113.5 : - : 106.9, of 8 142 : - : 120; six prompts of up to 4096 in pages of 32 374 : - : 356, of 16 447 : 414 : 381; heads of 128, pages of 16, 6 : 7 : 8
+// 508 : 467 : 458
+__host__ __device__ constexpr Split tc_split(int HD) { return Split{TC_BK, 4, 8, HD <= 64 ? 5 : 8, 12}; }
 __device__ __forceinline__ int per_block(const ChunkArgs& a, const Split& sp, const Request& r, int tile) {
-  return min(r.n * a.R - tile * a.tile_rows, a.tile_rows) > sp.rows_of_half ? 4 : 2;
+  return min(r.n * a.R - tile * a.tile_rows, a.tile_rows) > 128 ? 8 : min(sp.few + (a.log_page >= 5 ? 0 : a.log_page == 4 ? 1 : 3), 8);
 }
 // The blocks of an item of nb that lie ahead of weight x.
 __device__ __forceinline__ int ahead(long long x, int nb, int per, const Split& sp) {
