@@ -257,17 +257,23 @@ __global__ void __launch_bounds__(LT, 2) logprobs_kernel(const LogprobsArgs a) {
       }
       if (ends >= 0) offer(value(x0 + ends), ends);
     };
-    collect();
-    __syncthreads();
-    if (count > ROOM) {  // the best bound that the threads' maxima give: the largest key that n of them reach (its first 20 bits)
-      __syncthreads();
-      if (threadIdx.x == 0) count = 0;
+    auto refine = [&]() {  // the best bound that the threads' maxima give: the largest key that n of them reach (its first 20 bits)
       bound = 0;
       for (int bit = 31; bit >= 12; --bit) {
         const uint32_t with = bound | 1u << bit;
         if (__syncthreads_count(most > -INFINITY && mine >= with) >= n) bound = with;
       }
       bound = max(bound, NO_KEY + 1);
+    };
+    // a warp with too few bounds nothing: rows shorter than the threads' pieces, or banned tokens (2 rows of 3277 in bf16, 33 tokens: 7.3 us, 34 without this)
+    const bool weak = bound == NO_KEY + 1;
+    if (weak) refine();
+    collect();
+    __syncthreads();
+    if (!weak && count > ROOM) {
+      __syncthreads();
+      if (threadIdx.x == 0) count = 0;
+      refine();
       collect();
     }
     __syncthreads();

@@ -153,3 +153,13 @@ def test_captured_and_on_another_stream():
     want = check(x, t, 5)
     for a, b, c in zip(got, other, want):
         assert torch.equal(a, c) and torch.equal(b, c)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vocab", [100, 515, 3277, 4100, 9000])
+@pytest.mark.parametrize("top", [33, 64])
+@pytest.mark.parametrize("banned", [0.0, 0.97])
+def test_rows_with_too_few_logits_for_a_warps_bound(kind, vocab, top, banned):
+    x, t = logits(8, 5, vocab, kind)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    check(x.masked_fill(torch.rand(x.shape, generator=g, device="cuda") < banned, -math.inf), t, top)
