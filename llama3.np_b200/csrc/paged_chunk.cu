@@ -82,7 +82,8 @@ __global__ void __launch_bounds__(NT, ctas_of_sm(HD)) chunk_f32_kernel(const Chu
     const int flat0 = c.tile * TR, flats = c.r.n * a.R, row0 = flat0 + warp * 16;
     const int most = c.r.seen(token_of(min(flats, flat0 + TR) - 1));   // keys that any of the rows sees
     const int ours = row0 < flats ? c.r.seen(token_of(min(flats, row0 + 16) - 1)) : 0;  // that any of this warp's rows sees
-    for (int i = threadIdx.x; i < TR * (HD / 4); i += NT) {  // the rows' queries
+    // the rows' queries; not where there are no keys: such copies would be in no group, so that nothing waited for them, and the next item's go to the same place
+    for (int i = threadIdx.x; c.j0 < c.j1 && i < TR * (HD / 4); i += NT) {
       const int r = i / (HD / 4), p = i - r * (HD / 4), f = flat0 + r, t = token_of(f);
       const bool in = f < flats;
       cp16(smem_u32(sQ + r * LD + p * 4), in ? (const float*)a.q + (c.r.s0 + t) * a.q_st + (c.g * a.R + f - t * a.R) * a.q_sh + p * 4 : (const float*)a.q, in);
