@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from llama3_np_b200 import paged_chunk_attention
-from test_paged_chunk_gpu import TYPES, check, make
+from test_paged_chunk_gpu import TYPES, check, formula, make, near
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +21,44 @@ def test_requests_without_keys_between_others(kind, dim, heads, n, lengths):
     got = check(q, k, v, table, lens, starts)
     for _ in range(3):
         assert torch.equal(paged_chunk_attention(q, k, v, table, lens, starts, out=torch.full_like(q, 3.0)), got)
+
+
+def _place(table, b, p):
+    return int(table[b, p // 16]), p % 16
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [16, 64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_hidden_values_as_large_as_the_type_has_them(kind, dim, sign):
+    """Later tokens, keys of every residue modulo 8 among them: the rows ahead of them do not change."""
+    q, k, v, table, lens, starts = make(5, TYPES[kind], 8, 2, dim, 16, [(40, 100), (3000, 50), (0, 300)])
+    want = formula(q, k, v, table, lens, starts)
+    for b, first, last in ((0, 90, 140), (1, 3030, 3050), (2, 130, 300)):
+        for p in range(first, last):
+            page, at = _place(table, b, p)
+            v[page, :, at] = sign * torch.finfo(TYPES[kind]).max
+    got, lse = paged_chunk_attention(q, k, v, table, lens, starts, return_lse=True)
+    keep = torch.cat([torch.arange(50), torch.arange(100, 130), torch.arange(150, 280)]).cuda()
+    near(got[keep], lse[keep], [x[keep] for x in want])
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("large", [1e30, None])
+def test_keys_of_no_weight_under_large_values(kind, large):
+    """A score of -infinity is no weight, however large the value, whichever key of a block has it."""
+    q, k, v, table, lens, starts = make(6, TYPES[kind], 4, 2, 64, 16, [(700, 40), (0, 200)])
+    large = min(large or torch.finfo(TYPES[kind]).max, torch.finfo(TYPES[kind]).max)
+    q[..., 3] = q[..., 3].abs() + 0.01
+    for b, first in ((0, 300), (1, 17)):
+        for p in range(first, first + 11):
+            page, at = _place(table, b, p)
+            k[page, :, at, 3] = -float("inf")
+            v[page, :, at] = 0.0
+    want = formula(q, k, v, table, lens, starts)   # weights of 0: the values have no part in it
+    for b, first in ((0, 300), (1, 17)):
+        for p in range(first, first + 11):
+            page, at = _place(table, b, p)
+            v[page, :, at] = large
+    got, lse = paged_chunk_attention(q, k, v, table, lens, starts, return_lse=True)
+    near(got, lse, want)
