@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(ET) paged_extend_kernel(const PagedExtendArgs 
 // (a, b) -> (a cos - b sin, b cos + a sin).  Bound by the rows' bytes, in once and out once.  A CTA takes TOK rows with all their heads: the angles are
 // taken once for all heads, in 64 bits as parts of a whole turn - position * frequency / 2 pi less its nearest integer, so that far positions lose
 // nothing - and go as cosines and sines to shared memory; then a thread turns two pieces of E entries at a time.  8191 rows of 32 + 8 heads of 128 in bf16, keys
-// and values to their slots: 38.7 us, 5.2 TB/s (80 % of a copy's rate), 69 % of the issue slots.  A step's 32 rows: 3.5 us, latency.
+// and values to their slots: 39.2 us, 5.1 TB/s (79 % of a copy's rate), 69 % of the issue slots.  A step's 32 rows: 3.5 us, latency.
 constexpr int RT = 256;
 template <typename T> __device__ __forceinline__ float up(T x) { return to_f32(x); }
 template <> __device__ __forceinline__ float up<__half>(__half x) { return __half2float(x); }
@@ -141,6 +141,7 @@ template <typename T, int E> struct alignas(sizeof(T) * E) Entries { T v[E]; };
 template <typename T, int E, int TOK>
 __global__ void __launch_bounds__(RT) rotary_kernel(const RotaryArgs a) {
   extern __shared__ float2 turn[];   // [TOK][dims / 2]: cosine, sine
+  __shared__ int at[TOK];            // the rows' positions, if anything is turned
   using En = Entries<T, E>;
   const long long row0 = (long long)blockIdx.x * TOK, rows = (long long)a.B * a.L;
   const int half = a.dims / 2;
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(RT) rotary_kernel(const RotaryArgs a) {
       cs = make_float2(c * a.amplitude, (a.inverse ? -s : s) * a.amplitude);
     }
     turn[i] = cs;
+    if (p == 0) at[t] = position;
   }
   __syncthreads();
   const int turned = half / E, tail = (a.D - a.dims) / E, units = turned + (tail + 1) / 2;  // of a head: two pieces each, the last perhaps one
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(RT) rotary_kernel(const RotaryArgs a) {
     if (row >= rows) break;
     const T* from;
     T* to;
-    bool rotate = u < turned;
+    bool rotate = u < turned && at[t] >= 0;  // the others are copied: a product with 1 and 0 would make NaN of an infinite entry's partner
     if (head < a.H) {
       const long long b = row / a.L, l = row - b * a.L;
       from = (const T*)a.x + b * a.x_sb + l * a.x_st + head * a.x_sh;
