@@ -423,6 +423,18 @@ struct Together {
     return Tensor(std::move(impl));
   }
 };
+void no_overlap(const Tensor& t, const char* name) {
+  for (int64_t d = 0; d < t.dim(); ++d) NEED(t.size(d) <= 1 || t.stride(d) != 0, name, " is expanded, and would be written");
+}
+// whether the stretches of memory from the first entry to the last meet
+bool meets(const Tensor& a, const Tensor& b) {
+  auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (uintptr_t)t.const_data_ptr() + (last + 1) * t.element_size();
+  };
+  return a.numel() && b.numel() && (uintptr_t)a.const_data_ptr() < end(b) && (uintptr_t)b.const_data_ptr() < end(a);
+}
 int page_of(int64_t page) {
   NEED(page >= 1 && page <= 65536 && (page & (page - 1)) == 0, "page size ", page, " is not a power of two up to 65536");
   return (int)page;
@@ -448,6 +460,7 @@ PyObject* paged_extend(PyObject*, PyObject* const* x, Py_ssize_t n) {
   a.tokens = size32(tokens, "tokens");
   a.max_pages = size32(table.size(1), "page_table");
   NEED(batch <= 1 || table.size(1) == 0 || table.stride(0) >= table.size(1), "page_table is expanded, and would be written");
+  for (const Tensor* t : {&lengths, &counts, &pages}) NEED(!meets(table, *t), "page_table shares memory with lengths, counts or free_pages");
   OneDevice on;
   on.add(table, "page_table"); on.add(lengths, "lengths"); on.add(counts, "counts"); on.add(pages, "free_pages");
   const auto like = lengths.options();
@@ -482,18 +495,6 @@ void turn_of(L3Rotary& a, const Tensor& positions, PyObject* frequencies, PyObje
   a.inverse = inverse == Py_True;
   a.positions = positions.const_data_ptr<int32_t>();
   a.frequencies = f.const_data_ptr<double>();
-}
-void no_overlap(const Tensor& t, const char* name) {
-  for (int64_t d = 0; d < t.dim(); ++d) NEED(t.size(d) <= 1 || t.stride(d) != 0, name, " is expanded, and would be written");
-}
-// whether the stretches of memory from the first entry to the last meet
-bool meets(const Tensor& a, const Tensor& b) {
-  auto end = [](const Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return (uintptr_t)t.const_data_ptr() + (last + 1) * t.element_size();
-  };
-  return a.numel() && b.numel() && (uintptr_t)a.const_data_ptr() < end(b) && (uintptr_t)b.const_data_ptr() < end(a);
 }
 bool same_place(const Tensor& a, const Tensor& b) { return a.const_data_ptr() == b.const_data_ptr() && a.strides() == b.strides(); }
 
@@ -573,6 +574,7 @@ PyObject* paged_rotary_write(PyObject*, PyObject* const* x, Py_ssize_t n) {
     last_is_dense(o, "out");
     no_overlap(o, "out");
     NEED(same_place(o, q) || !(meets(o, q) || meets(o, k) || meets(o, v)), "out shares memory with q, k or v and is not q itself");
+    NEED(!meets(o, kp) && !meets(o, vp), "out shares memory with the pools");
   }
   OneDevice on;
   on.add(q, "q"); on.add(k, "k"); on.add(v, "v"); on.add(positions, "positions"); on.add(slots, "slots"); on.add(kp, "k_pages"); on.add(vp, "v_pages");
@@ -620,7 +622,7 @@ PyObject* paged_chunk_attention(PyObject*, PyObject* const* x, Py_ssize_t n) {
     typed(out, "out", q.scalar_type());
     NEED(out.sizes() == q.sizes() && out.is_contiguous() && (reinterpret_cast<uintptr_t>(out.const_data_ptr()) & 15) == 0,
          "out must be contiguous, of q's shape");
-    NEED(!meets(out, q), "out shares memory with q");
+    for (const Tensor* t : {&q, &k, &v, &table, &lengths, &starts}) NEED(!meets(out, *t), "out shares memory with what is read");
   }
   OneDevice on;
   on.add(q, "q"); on.add(k, "k_pages"); on.add(v, "v_pages"); on.add(table, "page_table"); on.add(lengths, "lengths"); on.add(starts, "starts");

@@ -120,7 +120,7 @@ def paged_rotary_write(q, k, v, positions, slots, k_pages, v_pages, frequencies,
     q            [tokens, heads, head size], k, v [tokens, kv heads, head size], of the pools' type
     slots        [tokens] int64, page * page size + token of the page, no two alike; one outside the pools: the row is written nowhere
     k_pages, v_pages   pools as `paged_attention` takes them
-    Returns the turned queries (written into `out` where given: q itself, or memory of its own).
+    Returns the turned queries (written into `out` where given: q itself, or memory of its own; never the pools').
     """
     return (paged._module or paged._ops()).paged_rotary_write(q, k, v, positions, slots, k_pages, v_pages, frequencies, layout, amplitude, out)
 
@@ -134,7 +134,7 @@ def paged_chunk_attention(q, k_pages, v_pages, page_table, lengths, starts, *, s
     lengths      [batch] int32: tokens of a request, the new ones among them
     starts       [batch + 1] int32: request b has the rows starts[b] .. starts[b + 1] - 1, its newest tokens; requests may have none
     scale        of q . k; 1 / sqrt(head size) by default
-    Returns [tokens, heads, head size] of q's type (written into `out` where given), and with `return_lse` also the log of the softmax's
+    Returns [tokens, heads, head size] of q's type (written into `out` where given: memory of its own), and with `return_lse` also the log of the softmax's
     denominator, [tokens, heads] fp32.  A row that sees no token has result 0 and lse -inf.  Rows of no request are left as they are in
     `out`, and 0 in a result that is made here.
     """
