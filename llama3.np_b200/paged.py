@@ -219,7 +219,8 @@ class PagedCache(PageTable):
     class View:
         """Sequences of a cache as its operators take them: `table` [n, pages], `lengths` and `start` [n], int32 on the device; the
         tokens from start on are the newest.  As rows of a packed step those of sequence i are the rows starts[i] .. starts[i + 1] - 1, with
-        `positions` and `slots`: made by `paged_extend` when first asked for."""
+        `positions` and `slots`: made by `paged_extend` when first asked for, which is before a capture.  All of them are there when the
+        host has them, so that any stream may use them."""
 
         def __init__(self, seqs, table, lengths, start, packed=None):
             self.seqs, self.table, self.lengths, self.start = seqs, table, lengths, start
@@ -228,7 +229,11 @@ class PagedCache(PageTable):
         def _rows(self):
             if self._step is None:
                 _need(self._packed is not None, "this view was not made by a cache")
-                self._step = self._packed()
+                with torch.cuda.device(self.table.device):
+                    _need(not torch.cuda.is_current_stream_capturing(), "a view's starts, positions and slots are uploads when first asked for: ask for one ahead of the capture")
+                    step = self._packed()
+                    torch.cuda.current_stream().synchronize()  # as the uploads of the view itself do
+                self._step = step
             return self._step
 
         starts = property(lambda self: self._rows().starts)
