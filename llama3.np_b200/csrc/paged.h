@@ -1,4 +1,4 @@
-// A key / value cache in pages: interface of paged.cu (attention of single tokens) and paged_rows.cu (writing, copying, reordering).
+// A key / value cache in pages: interface of paged.cu, paged_packed.cu (attention of single tokens) and paged_rows.cu (writing, copying, reordering).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -44,7 +44,8 @@ struct PagedAttnArgs {
 };
 size_t paged_attn_workspace(int H, int G, int HD, int n_sm);
 bool paged_attn_fits(PagedAttnArgs a);  // the pools' offsets fit 32 bits of the largest unit that divides their strides
-cudaError_t launch_paged_attention(PagedAttnArgs a, int n_sm, cudaStream_t s, int* launches = nullptr);  // launches: how many it made, 1 or 2
+cudaError_t launch_paged_attention(const PagedAttnArgs& a, int n_sm, cudaStream_t s, int* launches = nullptr);  // launches: how many it made, 1 or 2
+cudaError_t launch_paged_attention_step(const PagedAttnArgs& a, int n_sm, cudaStream_t s, int& launches);         // rows of a step (a.starts)
 
 struct PagedWriteArgs {
   const void *k, *v;                 // [B, L, G, HD]; strides in bytes

@@ -380,8 +380,8 @@ cudaError_t launch_chunk_join_tc(const ChunkArgs& a, cudaStream_t s) {
 }
 
 namespace {
-// Few rows over few keys as single tokens (paged.cu), which read their request's keys anew each.  us, so : as tiles, 32 heads over 8 kv heads of 128, one
-// request, by rows x keys and what is read: bf16 5 x 1505 29 MB 14.2 : 23.0, 16 x 1516 95 MB 23.0 : 23.4, 8 x 6008 188 MB 34.4 : 29.2, 2 x 60002 469 MB 88 : 63;
+// Few rows over few keys as single tokens (paged_packed.cu), which read their request's keys anew each.  us, so : as tiles, 32 heads over 8 kv heads of 128, one
+// request, by rows x keys and what is read: bf16 5 x 1505 29 MB 13.9 : 23.0, 16 x 1516 95 MB 23.0 : 23.4, 8 x 6008 188 MB 34.4 : 29.2, 2 x 60002 469 MB 88 : 63;
 // fp32 5 x 1505 59 MB 22 : 32, 5 x 6005 235 MB 49 : 65, 16 x 316 40 MB 19 : 28, 16 x 1516 190 MB 43 : 34, 16 x 6016 752 MB 130 : 67.  (That path writes every row.)
 bool as_single_tokens(const ChunkArgs& a) {
   const long long size = a.dtype == L3_DTYPE_F32 ? 4 : 2, keys = (long long)a.max_pages << a.log_page;
