@@ -495,7 +495,7 @@ typedef struct L3PagedExtend {
 int l3_paged_extend(const L3PagedExtend* a);
 /* Rotary positions: entries a and b of a pair become (a cos - b sin, b cos + a sin), each times `amplitude`, by the angle positions[row] *
  * frequencies[pair] (taken in 64 bits); inverse != 0: by the negative angle.  The first `dims` entries of a head are turned, the others and the
- * rows at negative positions are not.  layout 0: pairs (2 i, 2 i + 1) (llama3.py:41-76), 1: (i, i + dims / 2).  The rows are batch x tokens.
+ * rows at negative positions are not (bit for bit).  layout 0: pairs (2 i, 2 i + 1) (llama3.py:41-76), 1: (i, i + dims / 2).  The rows are batch x tokens.
  * With k and v (kv_heads > 0; batch 1) k is turned, too, and both go to their slots of the pools: slot page * page_size + place; a slot outside
  * the pool is none.  No two rows share a slot. */
 typedef struct L3Rotary {
@@ -520,7 +520,8 @@ int l3_rotary(const L3Rotary* a);
 /* Attention of the rows of a packed step over their requests' pages: row t of request b, at position p = lengths[b] - (starts[b + 1] - starts[b])
  * + t, sees the tokens j <= p.  lengths count the rows' own tokens, whose keys and values are in their pages already.  Pages outside [0, pages) hold
  * no tokens, lengths are cut to [0, max_pages * page_size]; a row that sees no token gets 0 and lse -infinity.  Rows of no request, ahead of starts[0]
- * or from starts[batch] on: clear_rest 0: left as they are, 1: set to 0, lse -infinity, 2: lse alone.  A value that a row does not see has no part in its result, not even a NaN. */
+ * or from starts[batch] on: clear_rest 0: left as they are, 1: set to 0, lse -infinity, 2: lse alone.  A value that a row does not see has no part in its result, not even a NaN.
+ * Sums of weighted values are held in fp32.  out and lse share no memory with what is read. */
 typedef struct L3PagedChunk {
   int32_t device;
   int32_t batch, tokens, heads, kv_heads, head_dim;  /* head_dim 16, 32, 48, 64, 96, 128 */

@@ -9,7 +9,7 @@
 // again (a warp together at one thread's, 32 pieces at a time), and what passes is ranked by counting.  Where more values pass than there is room
 // for, a better bound is found; where that does not help (many equal ones), the n are drawn one after the other.
 //
-// 2047 rows of 128256 in bf16 with entropy: 99.8 us, 5.3 TB/s (82 % of a copy's rate) at 74 % of the issue slots: an exponential and five other
+// 2047 rows of 128256 in bf16 with entropy: 99.8 us, 5.3 TB/s (81 % of a copy's rate) at 74 % of the issue slots: an exponential and five other
 // instructions a logit.  48 rows in fp32 with entropy and 20 tokens: 16.5 us, 7.3 without the tokens, whose ranking is a chain of barriers.
 #include <float.h>
 #include <math.h>

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(ET) paged_extend_kernel(const PagedExtendArgs 
 // (a, b) -> (a cos - b sin, b cos + a sin).  Bound by the rows' bytes, in once and out once.  A CTA takes TOK rows with all their heads: the angles are
 // taken once for all heads, in 64 bits as parts of a whole turn - position * frequency / 2 pi less its nearest integer, so that far positions lose
 // nothing - and go as cosines and sines to shared memory; then a thread turns two pieces of E entries at a time.  8191 rows of 32 + 8 heads of 128 in bf16, keys
-// and values to their slots: 39.2 us, 5.1 TB/s (79 % of a copy's rate), 69 % of the issue slots.  A step's 32 rows: 3.5 us, latency.
+// and values to their slots: 39.2 us, 5.1 TB/s (79 % of a copy's rate), 69 % of the issue slots.  A step's 32 rows: 3.6 us, latency.
 constexpr int RT = 256;
 template <typename T> __device__ __forceinline__ float up(T x) { return to_f32(x); }
 template <> __device__ __forceinline__ float up<__half>(__half x) { return __half2float(x); }
@@ -226,7 +226,7 @@ template <typename T, int E> cudaError_t rotary_e(const RotaryArgs& a, int n_sm,
   const long long rows = (long long)a.B * a.L;
   const size_t per = (size_t)a.dims / 2 * sizeof(float2);
   // rows of a CTA, us, one : four: 600 of 40 heads of 128 in bf16 5.9 : 7.8, 1000 9.2 : 8.1, 3000 17.2 : 16.3, 8000 38 : 34; 1001 of 16 fp32 heads of 96, 24 entries
-  // turned, 4.0 : 4.5
+  // turned, 4.0 : 4.5 (a row has few pieces there, which the rule does not look at)
   if (rows >= 6LL * n_sm) return launch_k(rotary_kernel<T, E, 4>, dim3((unsigned)((rows + 3) / 4)), dim3(RT), 4 * per, s, a);
   return launch_k(rotary_kernel<T, E, 1>, dim3((unsigned)rows), dim3(RT), per, s, a);
 }

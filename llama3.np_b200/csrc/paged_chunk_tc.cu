@@ -11,8 +11,8 @@
 // rows over the same keys, so that every key and value that arrives is used for 256 rows; with few rows they are one tile of rows over every other
 // block of keys, and meet at the end.
 //
-// Bound by the softmax: two score tiles over a block take 3.3 K cycles, their products 2.05 K (heads of 128; the tensor pipe is busy for 57 % of the time), an item's
-// beginning and end 5.5 K.  32 heads over 8 kv heads of 128 in bf16: 511 rows over 65000 tokens 465 - 481 us (1.14 - 1.17 PFLOP/s, 69 - 71 % of what a large
+// Bound by latency within the softmax: two score tiles over a block take 3.3 K cycles, their products 2.05 K (heads of 128; the tensor pipe is busy for 57 % of the time, the
+// issue slots for 40 %, the exponentials' units for less than half), an item's beginning and end 5.5 K.  32 heads over 8 kv heads of 128 in bf16: 511 rows over 65000 tokens 465 - 481 us (1.14 - 1.17 PFLOP/s, 69 - 71 % of what a large
 // product reaches), six prompts of up to 4096 454 - 462; of 64 in fp16, 48 requests of up to 3001 tokens in pages of 32, most with one row, 98 us, 177 MB.
 //
 // A weight enters the product rounded to the cache's type (half a step: bf16 2^-9 of it, as much as the result's own rounding; sums are of the unrounded
