@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(ET) paged_extend_kernel(const PagedExtendArgs 
 // (a, b) -> (a cos - b sin, b cos + a sin).  Bound by the rows' bytes, in once and out once.  A CTA takes TOK rows with all their heads: the angles are
 // taken once for all heads, in 64 bits as parts of a whole turn - position * frequency / 2 pi less its nearest integer, so that far positions lose
 // nothing - and go as cosines and sines to shared memory; then a thread turns two pieces of E entries at a time.  8191 rows of 32 + 8 heads of 128 in bf16, keys
-// and values to their slots: 39.2 us, 5.1 TB/s (79 % of a copy's rate), 69 % of the issue slots.  A step's 32 rows: 3.6 us, latency.
+// and values to their slots: 39.2 us, 5.1 TB/s (79 % of a copy's rate), 70 % of the issue slots.  A step's 32 rows: 3.6 us, latency.
 constexpr int RT = 256;
 template <typename T> __device__ __forceinline__ float up(T x) { return to_f32(x); }
 template <> __device__ __forceinline__ float up<__half>(__half x) { return __half2float(x); }
